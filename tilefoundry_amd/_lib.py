@@ -13,7 +13,7 @@ from pathlib import Path
 
 from .build import LIB
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 PRO_PLAIN, PRO_NORM = 0, 1
 EPI_STORE, EPI_RESID, EPI_SWIGLU, EPI_LOGITS, EPI_RESID_F32 = 0, 1, 2, 3, 4
@@ -63,6 +63,12 @@ P = c_void_p
 I = c_int
 F = c_float
 L = c_int64
+
+#: include/tf_mx4.h: activation types, router scores, elements that share a scale
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+ROUTE_MAX_EXPERTS = 512
+MX4_BLOCK = 32
 
 #: argtypes of every entry, in header order (restype is int unless named here)
 SIGNATURES: dict[str, list] = {
@@ -135,8 +141,19 @@ SIGNATURES: dict[str, list] = {
     "tfd_panel_gdn": [P, P],
     "tfd_panel_mamba": [P, P],
     "tfd_panel_gqa": [P, P],
+    # include/tf_mx4.h
+    "tfd_mx4_quantise": [P, L, I, L, I, P, L, P, L, P],
+    "tfd_mx4_dequantise": [P, L, P, L, L, I, P, L, I, P],
+    "tfd_mx4_packed_bytes": [L, I],
+    "tfd_mx4_pack": [P, P, P, P, L, I, P, P],
+    "tfd_mx4_gemm": [P, P],
+    "tfd_route_experts": [P, P],
+    "tfd_mx4_experts_work_bytes": [I, I, I, I, I],
+    "tfd_mx4_experts": [P, P],
 }
-RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c_int64}
+RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c_int64,
+            "tfd_mx4_packed_bytes": ctypes.c_int64,
+            "tfd_mx4_experts_work_bytes": ctypes.c_int64}
 UNCHECKED = {"tfd_abi_version", "tfd_decode_persistent_grid", "tfd_panel_gemm_slices",
              "tfd_panel_attn_rows"}
 
@@ -332,6 +349,34 @@ class TfdPanelGqaArgs(ctypes.Structure):
                 ("scale", c_float), ("eps", c_float),
                 *[(n, c_void_p) for n in ("q", "gate", "self_scores", "out")],
                 ("policy", c_int), ("err", c_void_p)]
+
+
+class TfdMx4GemmArgs(ctypes.Structure):
+    """``TfdMx4GemmArgs`` of include/tf_mx4.h, field for field."""
+
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("x_scales", c_void_p), ("ldxs", c_int64),
+                ("w", c_void_p), *[(n, c_int) for n in ("M", "K", "N")], ("out", c_void_p),
+                ("ldo", c_int64), ("out_type", c_int)]
+
+
+class TfdRouteArgs(ctypes.Structure):
+    """``TfdRouteArgs`` of include/tf_mx4.h, field for field."""
+
+    _fields_ = [("logits", c_void_p), ("ldl", c_int64), ("type", c_int), ("bias", c_void_p),
+                *[(n, c_int) for n in ("rows", "experts", "k", "score", "groups", "kept_groups",
+                                       "group_top", "shared", "renormalise")],
+                ("scale", c_float), ("weights", c_void_p), ("ids", c_void_p), ("ld", c_int)]
+
+
+class TfdMx4ExpertsArgs(ctypes.Structure):
+    """``TfdMx4ExpertsArgs`` of include/tf_mx4.h, field for field."""
+
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("ids", c_void_p), ("weights", c_void_p),
+                ("ld", c_int), ("w_gu", c_void_p), ("w_down", c_void_p),
+                *[(n, c_int) for n in ("rows", "k", "experts", "H", "I")], ("out", c_void_p),
+                ("ldo", c_int64), ("out_type", c_int), ("accumulate", c_int),
+                ("mult", c_float), ("work", c_void_p), ("work_bytes", c_int64),
+                ("err", c_void_p)]
 
 
 class TfdDecodeArgs(ctypes.Structure):

@@ -1,0 +1,899 @@
+// Products by microscaled 4-bit weights: a projection's, and the routed experts'.
+//
+// Weights are read as tfd_mx4_pack lays them out (mx4.h).  bf16 rows meet weights
+// converted to bf16 in registers, exactly, on the bf16 matrix instruction; rows that
+// are microscaled too go with the weights' codes into the scaled one.  Sums are f32
+// throughout, each output rounded once.  The weight is the A operand, so a lane ends
+// up with four consecutive outputs of one row.
+#include <type_traits>
+
+#include "host_common.h"
+#include "mx4.h"
+#include "tf_decode.h"
+#include "tf_mx4.h"
+
+using namespace tfd;
+using namespace tfd_host;
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+enum XKind { kXBf16 = 0, kXMx4 = 1 };
+enum Mode { kDense = 0, kHere = 1, kListed = 2 };   // rows: all; grouped in the block; before
+enum Epi { kBf16 = 0, kF32 = 1, kSwiglu = 2 };
+
+constexpr int kHereMax = 128;    // entries that a block groups itself
+constexpr int kHereRows = 16;    // rows of a fused step: its mix has a thread for each column
+
+struct Job {
+  const uint8_t* x;              // rows, bf16 or codes
+  int64_t ldx;                   // bytes
+  const uint8_t* xs;             // microscaled rows' scales
+  int64_t ldxs;
+  const uint8_t* w;              // packed weights
+  int64_t w_tiles;               // 16-row tiles of all of them
+  int K, kb, N;                  // N: outputs (of one expert)
+  int M;                         // dense: rows; experts: entries
+  void* out;
+  int64_t ldo;
+  int vec;                       // four outputs of a row may go in one store
+  // experts: entry i is place i % k of row i / k; its row of x is i / div
+  const int32_t* ids;
+  int ldi, k, div, E;
+  const int* groups;             // kListed: tiles, then the entries in their order
+  int32_t* err;
+};
+
+__device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, f32x4 c) {
+  const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+  const i32x8 y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+__device__ __forceinline__ u32x4 ld16(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) u32x4*)p;
+}
+__device__ __forceinline__ u32x4 ld16_stream(const uint8_t* p) {
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) u32x4*)p);
+}
+__device__ __forceinline__ uint32_t ld1(const uint8_t* p) {
+  return *(const __attribute__((address_space(1))) uint8_t*)p;
+}
+
+// ---------------------------------------------------------------------------
+// Entries (row, place) grouped by expert in tiles of up to 16, by the block that
+// uses them: up to kHereMax entries, each compared with those before it, which
+// costs less than a launch of its own.  Ids outside the experts make no entry; any
+// but -1 raises the error bit.
+// ---------------------------------------------------------------------------
+struct Tiles {
+  int n, first_wave;
+  int id[kHereMax], rank[kHereMax];
+  int expert[kHereMax], count[kHereMax];
+  uint8_t tile[kHereMax];
+  uint8_t entry[kHereMax][16];
+};
+
+__device__ void group_here(const Job& a, Tiles& s) {
+  const int i = threadIdx.x, lane = i & (kWave - 1);
+  int id = -1;
+  if (i < kHereMax) {
+    if (i < a.M) {
+      id = a.ids[(int64_t)(i / a.k) * a.ldi + i % a.k];
+      if (id < 0 || id >= a.E) {
+        if (id != -1 && blockIdx.x == 0 && a.err) raise_error(a.err, kErrTokenRange);
+        id = -1;
+      }
+    }
+    s.id[i] = id;
+    s.count[i] = 0;
+  }
+  __syncthreads();
+  int rank = 0, first = i;
+  if (id >= 0)
+    for (int j = i - 1; j >= 0; --j)
+      if (s.id[j] == id) {
+        ++rank;
+        first = j;
+      }
+  const bool leads = id >= 0 && (rank & 15) == 0;
+  const uint64_t before = __ballot(leads);
+  if (i < kHereMax) s.rank[i] = rank;
+  if (i == 0) s.first_wave = __popcll(before);
+  __syncthreads();
+  int t = 0;
+  if (i < kHereMax) {
+    const int base = i < kWave ? 0 : s.first_wave;
+    t = base + __popcll(before & ((1ull << lane) - 1));
+    if (leads) {
+      s.tile[i] = (uint8_t)t;
+      s.expert[t] = id;
+    }
+    if (i == kHereMax - 1) s.n = base + __popcll(before);
+  }
+  __syncthreads();
+  if (id >= 0) {
+    int lead = first;
+    if (rank >= 16)
+      for (lead = first; s.id[lead] != id || s.rank[lead] != (rank & ~15);) ++lead;
+    t = s.tile[lead];
+    s.entry[t][rank & 15] = (uint8_t)i;
+    atomicMax(&s.count[t], (rank & 15) + 1);
+  }
+  __syncthreads();
+}
+
+// The tile of expert rows that item `rt` works on.
+template <int kMode>
+struct RowTile {
+  int expert, count;
+  int first;                     // kDense: row; kListed: place in the order
+  __device__ __forceinline__ RowTile(const Job& a, const Tiles* s, int rt, int rows) {
+    if (kMode == kDense) {
+      expert = 0;
+      first = rt * rows;
+      count = min(rows, a.M - first);
+    } else if (kMode == kHere) {
+      expert = s->expert[rt];
+      first = rt;
+      count = s->count[rt];
+    } else {
+      const int* t = a.groups + 4 + rt * 4;
+      expert = t[0];
+      first = t[1];
+      count = t[2];
+    }
+  }
+  // the i-th row's place: a row of the dense product, or an entry (past the end: the last)
+  __device__ __forceinline__ int at(const Job& a, const Tiles* s, int i, int tiles) const {
+    i = min(i, count - 1);
+    if (kMode == kDense) return first + i;
+    if (kMode == kHere) return s->entry[first][i];
+    return a.groups[4 + tiles * 4 + first + i];
+  }
+};
+
+// The row tiles that fit a list's head: what group_listed wrote after them.
+__device__ __forceinline__ int listed_room(const Job& a) { return a.groups[1]; }
+
+template <int kEpi>
+__device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v) {
+  if (kEpi == kSwiglu) {
+    // (gate, up) pairs: the hidden value is the next product's operand, hence bf16
+    const float h0 = silu_f(v.x) * v.y, h1 = silu_f(v.z) * v.w;
+    *reinterpret_cast<uint32_t*>((bf16*)a.out + (int64_t)row * a.ldo + n / 2) = pack2(h0, h1);
+    return;
+  }
+  if (kEpi == kF32) {
+    float* o = (float*)a.out + (int64_t)row * a.ldo + n;
+    if (a.vec && n + 4 <= a.N) {
+      *reinterpret_cast<f32x4*>(o) = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < a.N) o[i] = v[i];
+    }
+    return;
+  }
+  bf16* o = (bf16*)a.out + (int64_t)row * a.ldo + n;
+  if (a.vec && n + 4 <= a.N) {
+    *reinterpret_cast<u32x2*>(o) = u32x2{pack2(v.x, v.y), pack2(v.z, v.w)};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) o[i] = f2bf(v[i]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the weights' stream bounds it.  An item is a tile of MT x 16 rows by TN
+// column tiles over all of K; items are dealt to the blocks in turn, and a block's
+// four waves split K and meet in LDS.  A wave has the next D steps' (128 k) weights,
+// scales and rows in flight across items, so the stream does not stop where an item
+// ends.  Rows come straight from memory (L2): each wave needs its own part of K, so
+// LDS would not save a read.
+// ---------------------------------------------------------------------------
+template <int kX, int MT, int TN, int D, int kMode, int kEpi>
+__global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
+  constexpr int kR = 16 * MT;
+  __shared__ f32x4 red[2][kWavesPerBlock][MT * TN][kWave];
+  __shared__ typename std::conditional<kMode == kHere, Tiles, int>::type group_s;
+  const Tiles* tiles = nullptr;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int nl = lane & 15, kq = lane >> 4;
+  int nT, room = 0;
+  if constexpr (kMode == kHere) {
+    group_here(a, group_s);
+    tiles = &group_s;
+    nT = group_s.n;
+  } else if (kMode == kListed) {
+    nT = a.groups[0];
+    room = listed_room(a);
+  } else {
+    nT = (a.M + kR - 1) / kR;
+  }
+  const int ntiles = (a.N + 15) / 16;
+  const int nC = (ntiles + TN - 1) / TN;
+  const int items = nT * nC, G = (int)gridDim.x, me = (int)blockIdx.x;
+  if (me >= items) return;
+  const int mine = (items - 1 - me) / G + 1;
+  const int ns = (a.kb + kWavesPerBlock - 1) / kWavesPerBlock;   // steps of a wave's part
+  const int k0 = wave * ns;
+  const int sg = mx4_scale_groups(a.kb);
+  const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
+
+  struct Item {
+    int64_t tile[TN];
+    const uint8_t *x[MT], *xs[MT];
+  };
+  auto decode = [&](int j) {
+    const int it = me + j * G, rt = it % nT, c = it / nT;
+    const RowTile<kMode> r(a, tiles, rt, kR);
+    Item d;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+      d.tile[t] = (int64_t)r.expert * ntiles + min(c * TN + t, ntiles - 1);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int at = r.at(a, tiles, m * 16 + nl, room);
+      const int64_t row = kMode == kDense ? at : at / a.div;
+      d.x[m] = a.x + row * a.ldx;
+      d.xs[m] = kX == kXMx4 ? a.xs + row * a.ldxs : nullptr;
+    }
+    return d;
+  };
+  u32x4 w[D][TN];
+  uint32_t ws[D][TN];
+  u32x4 x[D][MT][kX == kXMx4 ? 1 : 4];
+  uint32_t xs[D][MT];
+  Item nx = decode(0);
+  int jn = 0, sn = 0;
+  auto issue = [&](int u) {
+    const int b = min(k0 + sn, a.kb - 1);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      w[u][t] = ld16_stream(a.w + (nx.tile[t] * a.kb + b) * 1024 + lane * 16);
+      ws[u][t] = ld1(scales + (nx.tile[t] * sg + (b >> 2)) * 256 + lane * 4 + (b & 3));
+    }
+    // a lane's 32 k; those past K read the row's first and are cleared before use
+    const int k = b * kMx4K + 32 * kq, kk = k < a.K ? k : 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (kX == kXMx4) {
+        x[u][m][0] = ld16(nx.x[m] + (kk >> 1));
+        xs[u][m] = ld1(nx.xs[m] + (kk >> 5));
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) x[u][m][s] = ld16(nx.x[m] + 2 * kk + 16 * s);
+      }
+    }
+    if (++sn == ns && jn + 1 < mine) {
+      sn = 0;
+      nx = decode(++jn);
+    }
+  };
+  f32x4 c[TN][MT];
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  int jc = 0, sc = 0;
+  auto compute = [&](int u) {
+    const int b = k0 + sc;
+    if (b < a.kb) {
+      if (b == a.kb - 1 && b * kMx4K + 32 * kq >= a.K) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+          for (int s = 0; s < (kX == kXMx4 ? 1 : 4); ++s) x[u][m][s] = u32x4{0u, 0u, 0u, 0u};
+          xs[u][m] = 127;
+        }
+      }
+      if (kX == kXMx4) {
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            c[t][m] = mfma_mx4(w[u][t], ws[u][t], x[u][m][0], xs[u][m], c[t][m]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const float scale = mx4_scale(ws[u][t]);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            const u32x4 v = fp4x8_to_bf16(w[u][t][s], scale);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) c[t][m] = mfma(v, x[u][m][kX == kXMx4 ? 0 : s], c[t][m]);
+          }
+        }
+      }
+    }
+    if (++sc < ns) return;
+    // the item is done: the four parts of K meet in LDS (two buffers, so one barrier an
+    // item is enough) and the waves take turns to write
+    const int j = jc++;
+    sc = 0;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        red[j & 1][wave][t * MT + m][lane] = c[t][m];
+        c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    __syncthreads();
+    const int it = me + j * G, rt = it % nT, cc = it / nT;
+    const RowTile<kMode> r(a, tiles, rt, kR);
+#pragma unroll
+    for (int q = 0; q < TN * MT; ++q) {
+      if ((q + j) % kWavesPerBlock != wave) continue;
+      const int t = q / MT, m = q % MT;
+      f32x4 v = red[j & 1][0][q][lane];
+#pragma unroll
+      for (int p = 1; p < kWavesPerBlock; ++p) v += red[j & 1][p][q][lane];
+      const int n = (cc * TN + t) * 16 + 4 * kq;
+      if (m * 16 + nl < r.count && cc * TN + t < ntiles && n < a.N)
+        put<kEpi>(a, r.at(a, tiles, m * 16 + nl, room), n, v);
+    }
+  };
+  const int total = mine * ns;
+#pragma unroll
+  for (int u = 0; u < D; ++u) issue(u);
+  int q0 = 0;
+  for (; q0 + D < total; q0 += D) {
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      compute(u);
+      issue(u);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < D; ++u)
+    if (q0 + u < total) compute(u);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: the matrix cores bound it.  A block of four waves takes TM x 16 rows by
+// 4 x TN x 16 columns; its rows pass through LDS, 128 k at a time in two buffers, in
+// the order the matrix instruction takes them (a wave's read is 1 KiB in a row, and a
+// write's eight lanes are 128 bytes in a row: no bank conflicts); each wave's own
+// weights go straight to its registers, two steps ahead, and are converted there.
+// ---------------------------------------------------------------------------
+template <int kX, int TM, int TN, int kMode, int kEpi>
+__global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a, int nT_host) {
+  constexpr int kR = 16 * TM;
+  constexpr int kStep = TM * (kX == kXMx4 ? 1024 : 4096);   // LDS bytes of 128 k
+  constexpr int kPass = kX == kXMx4 ? (TM + 3) / 4 : TM;    // 16-byte pieces a thread stages
+  __shared__ __align__(16) uint8_t xs_s[2][kStep];
+  __shared__ uint8_t xsc_s[2][kX == kXMx4 ? TM * kWave : 1];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int nl = lane & 15, kq = lane >> 4;
+  const int nT = kMode == kListed ? a.groups[0] : nT_host;
+  const int room = kMode == kListed ? listed_room(a) : 0;
+  const int ntiles = (a.N + 15) / 16;
+  const int nC = (ntiles + 4 * TN - 1) / (4 * TN);
+  // consecutive items (eight row tiles by a few column blocks) on one XCD: what they
+  // share stays in its L2
+  const int total = nT * nC, per = (nT_host * nC + 7) / 8;
+  const int g = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || g >= total) return;
+  const int grp = g / (8 * nC), within = g % (8 * nC);
+  const int gm = min(8, nT - grp * 8);
+  const int rt = grp * 8 + within % gm, cb = within / gm;
+  const RowTile<kMode> r(a, nullptr, rt, kR);
+  const int sg = mx4_scale_groups(a.kb);
+  const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
+
+  // bf16: piece (tile m, row nl of it, k 32 wave + 8 kq); microscaled: (tile, row nl, k 32 kq)
+  // (row numbers, not pointers: a register each)
+  int xrow[kPass];
+#pragma unroll
+  for (int q = 0; q < kPass; ++q) {
+    const int m = kX == kXMx4 ? min(q * 4 + wave, TM - 1) : q;
+    const int at = r.at(a, nullptr, m * 16 + nl, room);
+    xrow[q] = kMode == kDense ? at : at / a.div;
+  }
+  u32x4 xr[kPass];
+  uint32_t xsr[kPass];
+  auto load_x = [&](int b) {
+    if (kX == kXMx4) {
+      const int k = b * kMx4K + 32 * kq;
+      const bool in = k < a.K;
+#pragma unroll
+      for (int q = 0; q < kPass; ++q) {
+        xr[q] = ld16(a.x + xrow[q] * a.ldx + (in ? k >> 1 : 0));
+        xsr[q] = ld1(a.xs + xrow[q] * a.ldxs + (in ? k >> 5 : 0));
+        if (!in) {
+          xr[q] = u32x4{0u, 0u, 0u, 0u};
+          xsr[q] = 127;
+        }
+      }
+    } else {
+      const int k = b * kMx4K + 32 * wave;
+      const bool in = k < a.K;                    // the wave's 32 k are in or out together
+#pragma unroll
+      for (int q = 0; q < kPass; ++q)
+        xr[q] = in ? ld16(a.x + xrow[q] * a.ldx + 2 * (k + 8 * kq)) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int q = 0; q < kPass; ++q) {
+      if (kX == kXMx4) {
+        const int m = q * 4 + wave;
+        if (m < TM) {
+          *reinterpret_cast<u32x4*>(&xs_s[buf][m * 1024 + lane * 16]) = xr[q];
+          xsc_s[buf][m * kWave + lane] = (uint8_t)xsr[q];
+        }
+      } else {
+        *reinterpret_cast<u32x4*>(&xs_s[buf][(q * 4 + kq) * 1024 + (nl + 16 * wave) * 16]) = xr[q];
+      }
+    }
+  };
+  int64_t wt[TN];
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+    wt[t] = (int64_t)r.expert * ntiles + min((cb * 4 + wave) * TN + t, ntiles - 1);
+  u32x4 w[2][TN];
+  uint32_t ws[2][TN];
+  auto load_w = [&](int u, int b) {
+    b = min(b, a.kb - 1);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      w[u][t] = ld16(a.w + (wt[t] * a.kb + b) * 1024 + lane * 16);
+      ws[u][t] = ld1(scales + (wt[t] * sg + (b >> 2)) * 256 + lane * 4 + (b & 3));
+    }
+  };
+  f32x4 c[TM][TN];
+#pragma unroll
+  for (int m = 0; m < TM; ++m)
+#pragma unroll
+    for (int t = 0; t < TN; ++t) c[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  load_x(0);
+  load_w(0, 0);
+  load_w(1, 1);
+  stage(0);
+  __syncthreads();
+  auto body = [&](auto slot, int b) {
+    constexpr int u = decltype(slot)::value;
+    const bool next = b + 1 < a.kb;
+    if (next) load_x(b + 1);
+    if (kX == kXMx4) {
+      u32x4 v[TM];
+      uint32_t vs[TM];
+#pragma unroll
+      for (int m = 0; m < TM; ++m) {
+        v[m] = *reinterpret_cast<const u32x4*>(&xs_s[u][m * 1024 + lane * 16]);
+        vs[m] = xsc_s[u][m * kWave + lane];
+      }
+#pragma unroll
+      for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int m = 0; m < TM; ++m) c[m][t] = mfma_mx4(w[u][t], ws[u][t], v[m], vs[m], c[m][t]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        u32x4 v[TM];
+#pragma unroll
+        for (int m = 0; m < TM; ++m)
+          v[m] = *reinterpret_cast<const u32x4*>(&xs_s[u][(m * 4 + s) * 1024 + lane * 16]);
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const u32x4 q = fp4x8_to_bf16(w[u][t][s], mx4_scale(ws[u][t]));
+#pragma unroll
+          for (int m = 0; m < TM; ++m) c[m][t] = mfma(q, v[m], c[m][t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    load_w(u, b + 2);
+    if (next) {
+      stage(1 - u);
+      __syncthreads();
+    }
+  };
+  for (int b = 0; b < a.kb; b += 2) {
+    body(std::integral_constant<int, 0>{}, b);
+    if (b + 1 < a.kb) body(std::integral_constant<int, 1>{}, b + 1);
+  }
+#pragma unroll
+  for (int m = 0; m < TM; ++m) {
+    const int i = m * 16 + nl;
+    if (i >= r.count) continue;
+    const int at = r.at(a, nullptr, i, room);
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      const int tile = (cb * 4 + wave) * TN + t, n = tile * 16 + 4 * kq;
+      if (tile < ntiles && n < a.N) put<kEpi>(a, at, n, c[m][t]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Down projection and mix of a step of few rows, in one launch: a block per column
+// tile holds every entry's 16 outputs, so the weighted sum needs no second pass over
+// memory.  A wave takes (row tile, part of K) units in turn, its next D steps in flight
+// across them; each unit's sums have a place of their own in LDS, and a row's places
+// are added in their order: the result does not depend on which wave ran when.
+// ---------------------------------------------------------------------------
+constexpr int kMixWaves = 8;
+constexpr int kMixParts = 256;   // (entry, part of K) places, 16 columns each
+
+template <int D>
+__global__ __launch_bounds__(kMixWaves * kWave) void k_mx4_down_mix(
+    Job a, const float* __restrict__ weights, int rows, float mult, int out_f32, int accumulate) {
+  __shared__ Tiles s;
+  __shared__ float part[kMixParts][16];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int nl = lane & 15, kq = lane >> 4;
+  const int ct = blockIdx.x, ntiles = a.N / 16;
+  group_here(a, s);
+  const int nT = s.n;
+  // with fewer tiles than waves a tile's K goes to several waves, as far as every entry's
+  // parts (empty places count) have room
+  const int parts = nT >= kMixWaves || nT == 0
+                        ? 1
+                        : min(min(a.kb, (kMixWaves + nT - 1) / nT), kMixParts / a.M);
+  const int ns = (a.kb + parts - 1) / parts;
+  const int units = nT * parts;
+  const int mine = wave < units ? (units - 1 - wave) / kMixWaves + 1 : 0;
+  const int sg = mx4_scale_groups(a.kb);
+  const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
+  u32x4 w[D], x[D][4];
+  uint32_t ws[D];
+  int64_t tile = 0;
+  const uint8_t* xp = a.x;
+  int k0 = 0, jn = 0, sn = 0;
+  auto decode = [&](int j) {
+    const int u = wave + j * kMixWaves, rt = u / parts;
+    k0 = u % parts * ns;
+    tile = (int64_t)s.expert[rt] * ntiles + ct;
+    xp = a.x + (int64_t)s.entry[rt][min(nl, s.count[rt] - 1)] * a.ldx;
+  };
+  auto issue = [&](int u) {
+    const int b = min(k0 + sn, a.kb - 1);
+    w[u] = ld16_stream(a.w + (tile * a.kb + b) * 1024 + lane * 16);
+    ws[u] = ld1(scales + (tile * sg + (b >> 2)) * 256 + lane * 4 + (b & 3));
+    const int k = b * kMx4K + 32 * kq, kk = k < a.K ? k : 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[u][q] = ld16(xp + 2 * kk + 16 * q);
+    if (++sn == ns && jn + 1 < mine) {
+      sn = 0;
+      decode(++jn);
+    }
+  };
+  f32x4 c = {0.f, 0.f, 0.f, 0.f};
+  int jc = 0, sc = 0;
+  auto compute = [&](int u) {
+    const int unit = wave + jc * kMixWaves, rt = unit / parts, p = unit % parts;
+    const int b = p * ns + sc;
+    if (b < a.kb) {
+      if (b == a.kb - 1 && b * kMx4K + 32 * kq >= a.K) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[u][q] = u32x4{0u, 0u, 0u, 0u};
+      }
+      const float scale = mx4_scale(ws[u]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) c = mfma(fp4x8_to_bf16(w[u][q], scale), x[u][q], c);
+    }
+    if (++sc < ns) return;
+    sc = 0;
+    ++jc;
+    if (nl < s.count[rt])
+      *reinterpret_cast<f32x4*>(&part[s.entry[rt][nl] * parts + p][4 * kq]) = c;
+    c = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  if (mine > 0) {
+    decode(0);
+    const int total = mine * ns;
+#pragma unroll
+    for (int u = 0; u < D; ++u) issue(u);
+    int q0 = 0;
+    for (; q0 + D < total; q0 += D) {
+#pragma unroll
+      for (int u = 0; u < D; ++u) {
+        compute(u);
+        issue(u);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < D; ++u)
+      if (q0 + u < total) compute(u);
+  }
+  __syncthreads();
+  const int r = threadIdx.x / 16, n = threadIdx.x % 16;
+  if (r >= rows) return;
+  float y = 0.f;
+  for (int j = 0; j < a.k; ++j) {
+    const int e = r * a.k + j;
+    if (s.id[e] < 0) continue;
+    float d = part[e * parts][n];
+    for (int p = 1; p < parts; ++p) d += part[e * parts + p][n];
+    y += weights[(int64_t)r * a.ldi + j] * d;
+  }
+  y *= mult;
+  const int64_t at = (int64_t)r * a.ldo + ct * 16 + n;
+  if (out_f32) {
+    float* o = (float*)a.out + at;
+    *o = accumulate ? *o + y : y;
+  } else {
+    bf16* o = (bf16*)a.out + at;
+    *o = f2bf(accumulate ? bf2f(*o) + y : y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Entries of many rows by expert: counts, places and the list of row tiles, by one
+// block.  The order of an expert's entries is free (each is computed by itself).
+// ---------------------------------------------------------------------------
+constexpr int kGroupThreads = 1024;
+
+__global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_rows, int room,
+                                                             int* __restrict__ groups) {
+  __shared__ int count[TFD_ROUTE_MAX_EXPERTS], first[2][TFD_ROUTE_MAX_EXPERTS],
+      tile[2][TFD_ROUTE_MAX_EXPERTS];
+  const int tid = threadIdx.x;
+  if (tid < TFD_ROUTE_MAX_EXPERTS) count[tid] = 0;
+  __syncthreads();
+  for (int i = tid; i < a.M; i += kGroupThreads) {
+    const int id = a.ids[(int64_t)(i / a.k) * a.ldi + i % a.k];
+    if ((unsigned)id < (unsigned)a.E) atomicAdd(&count[id], 1);
+    else if (id != -1 && a.err) raise_error(a.err, kErrTokenRange);
+  }
+  __syncthreads();
+  int mine = 0, tiles = 0;
+  if (tid < TFD_ROUTE_MAX_EXPERTS) {
+    mine = tid < a.E ? count[tid] : 0;
+    tiles = (mine + tile_rows - 1) / tile_rows;
+    first[0][tid] = mine;
+    tile[0][tid] = tiles;
+  }
+  int cur = 0;
+  for (int d = 1; d < TFD_ROUTE_MAX_EXPERTS; d *= 2) {
+    __syncthreads();
+    if (tid < TFD_ROUTE_MAX_EXPERTS) {
+      first[1 - cur][tid] = first[cur][tid] + (tid >= d ? first[cur][tid - d] : 0);
+      tile[1 - cur][tid] = tile[cur][tid] + (tid >= d ? tile[cur][tid - d] : 0);
+    }
+    cur = 1 - cur;
+  }
+  __syncthreads();
+  if (tid < a.E) {
+    const int f = first[cur][tid] - mine, t0 = tile[cur][tid] - tiles;
+    for (int t = 0; t < tiles; ++t) {
+      int* o = groups + 4 + (t0 + t) * 4;
+      o[0] = tid;
+      o[1] = f + t * tile_rows;
+      o[2] = min(tile_rows, mine - t * tile_rows);
+    }
+    count[tid] = f;
+  }
+  if (tid == 0) {
+    groups[0] = tile[cur][TFD_ROUTE_MAX_EXPERTS - 1];
+    groups[1] = room;
+  }
+  __syncthreads();
+  int* order = groups + 4 + room * 4;
+  for (int i = tid; i < a.M; i += kGroupThreads) {
+    const int id = a.ids[(int64_t)(i / a.k) * a.ldi + i % a.k];
+    if ((unsigned)id < (unsigned)a.E) order[atomicAdd(&count[id], 1)] = i;
+  }
+}
+
+// The weighted sum of a row's places, in their order; four columns a thread.
+__global__ __launch_bounds__(kBlock) void k_mx4_mix(const float* __restrict__ d,
+                                                    const int32_t* __restrict__ ids,
+                                                    const float* __restrict__ weights, int ldi,
+                                                    int k, int E, int H, float mult, int out_f32,
+                                                    int accumulate, void* __restrict__ out,
+                                                    int64_t ldo) {
+  const int r = blockIdx.y, n = (blockIdx.x * kBlock + threadIdx.x) * 4;
+  if (n >= H) return;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < k; ++j) {
+    const int id = ids[(int64_t)r * ldi + j];
+    if ((unsigned)id >= (unsigned)E) continue;
+    y += weights[(int64_t)r * ldi + j] *
+         *reinterpret_cast<const f32x4*>(d + ((int64_t)r * k + j) * H + n);
+  }
+  y *= mult;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = (int64_t)r * ldo + n + i;
+    if (out_f32) {
+      float* o = (float*)out + at;
+      *o = accumulate ? *o + y[i] : y[i];
+    } else {
+      bf16* o = (bf16*)out + at;
+      *o = f2bf(accumulate ? bf2f(*o) + y[i] : y[i]);
+    }
+  }
+}
+
+bool fused_step(int rows, int k) { return rows <= kHereRows && rows * k <= kHereMax; }
+
+struct Work {
+  int64_t hidden, d, groups, bytes;
+  int room;
+};
+Work experts_work(int rows, int k, int E, int H, int I) {
+  const int64_t n = (int64_t)rows * k;
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  Work w = {};
+  w.room = (int)(E + n / 16);
+  w.d = up(n * I * 2);
+  w.groups = w.d + (fused_step(rows, k) ? 0 : up(n * H * 4));
+  w.bytes = w.groups + (fused_step(rows, k) ? 0 : up((4 + 4 * (int64_t)w.room + n) * 4));
+  return w;
+}
+
+template <int TM, int TN>
+void launch_listed(const Job& gu, const Job& down, int tiles, hipStream_t s) {
+  auto grid = [&](const Job& j) {
+    const int64_t nC = ((j.N + 15) / 16 + 4 * TN - 1) / (4 * TN);
+    return (int)(8 * ((tiles * nC + 7) / 8));
+  };
+  k_mx4_many<kXBf16, TM, TN, kListed, kSwiglu><<<grid(gu), kBlock, 0, s>>>(gu, tiles);
+  k_mx4_many<kXBf16, TM, TN, kListed, kF32><<<grid(down), kBlock, 0, s>>>(down, tiles);
+}
+
+int job_checks(const char* what, int K, int64_t N) {
+  if (K <= 0 || K % 32 || K > (1 << 22) || N <= 0 || N > (1 << 24))
+    return fail(kBadShape, "%s: K=%d N=%lld (K a multiple of 32)", what, K, (long long)N);
+  return 0;
+}
+
+template <int kX, int kEpi>
+int launch_dense(const Job& a, hipStream_t s) {
+  const int cus = compute_units(), ntiles = (a.N + 15) / 16;
+  if (a.M <= 16) {
+    k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<min(ntiles, 4 * cus), kBlock, 0, s>>>(a);
+  } else if (a.M <= 64) {
+    const int items = (a.M + 31) / 32 * ntiles;
+    k_mx4_few<kX, 2, 1, 2, kDense, kEpi><<<min(items, 4 * cus), kBlock, 0, s>>>(a);
+  } else {
+    const int nT = (a.M + 127) / 128, nC = (ntiles + 15) / 16;
+    if ((int64_t)nT * nC > (1 << 30)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
+    k_mx4_many<kX, 8, 4, kDense, kEpi><<<8 * ((nT * nC + 7) / 8), kBlock, 0, s>>>(a, nT);
+  }
+  return launched("mx4_gemm");
+}
+
+}  // namespace
+
+extern "C" int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream) {
+  if (!args) return fail(kBadArg, "mx4_gemm: null args");
+  const TfdMx4GemmArgs& a = *args;
+  if (a.out_type != TFD_TYPE_F32 && a.out_type != TFD_TYPE_BF16)
+    return fail(kBadArg, "mx4_gemm: out_type %d", a.out_type);
+  if (const int rc = job_checks("mx4_gemm", a.K, a.N)) return rc;
+  if (a.M < 0 || a.M > (1 << 30)) return fail(kBadShape, "mx4_gemm: M=%d", a.M);
+  if (a.M == 0) return 0;
+  if (!a.x || !a.w || !a.out) return fail(kBadArg, "mx4_gemm: null pointer");
+  const bool mx = a.x_scales != nullptr;
+  const int64_t row = mx ? a.K / 2 : 2 * (int64_t)a.K, ld = mx ? a.ldx : 2 * a.ldx;
+  if ((uintptr_t)a.x % 16 || (uintptr_t)a.w % 16 || (a.M > 1 && (ld % 16 || ld < row)) ||
+      (mx && a.M > 1 && a.ldxs < a.K / 32) || a.ldo < a.N ||
+      (uintptr_t)a.out % (a.out_type == TFD_TYPE_F32 ? 4 : 2))
+    return fail(kBadArg, "mx4_gemm: ldx=%lld ldxs=%lld ldo=%lld or an alignment",
+                (long long)a.ldx, (long long)a.ldxs, (long long)a.ldo);
+  Job j = {};
+  j.x = (const uint8_t*)a.x;
+  j.ldx = ld;
+  j.xs = (const uint8_t*)a.x_scales;
+  j.ldxs = a.ldxs;
+  j.w = (const uint8_t*)a.w;
+  j.w_tiles = (a.N + 15) / 16;
+  j.K = a.K;
+  j.kb = mx4_blocks(a.K);
+  j.N = a.N;
+  j.M = a.M;
+  j.out = a.out;
+  j.ldo = a.ldo;
+  const int size = a.out_type == TFD_TYPE_F32 ? 4 : 2;
+  j.vec = a.ldo % 4 == 0 && (uintptr_t)a.out % (4 * size) == 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (mx) return a.out_type == TFD_TYPE_F32 ? launch_dense<kXMx4, kF32>(j, s)
+                                            : launch_dense<kXMx4, kBf16>(j, s);
+  return a.out_type == TFD_TYPE_F32 ? launch_dense<kXBf16, kF32>(j, s)
+                                    : launch_dense<kXBf16, kBf16>(j, s);
+}
+
+extern "C" {
+
+int64_t tfd_mx4_experts_work_bytes(int rows, int k, int experts, int H, int I) {
+  if (rows <= 0 || k <= 0 || experts <= 0 || H <= 0 || I <= 0) return 0;
+  return experts_work(rows, k, experts, H, I).bytes;
+}
+
+int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
+  if (!args) return fail(kBadArg, "mx4_experts: null args");
+  const TfdMx4ExpertsArgs& a = *args;
+  if (a.out_type != TFD_TYPE_F32 && a.out_type != TFD_TYPE_BF16)
+    return fail(kBadArg, "mx4_experts: out_type %d", a.out_type);
+  if (a.H <= 0 || a.I <= 0 || a.H % 32 || a.I % 32 || a.H > (1 << 20) || a.I > (1 << 20))
+    return fail(kBadShape, "mx4_experts: H=%d I=%d (multiples of 32)", a.H, a.I);
+  if (a.experts < 1 || a.experts > TFD_ROUTE_MAX_EXPERTS || a.k < 1 || a.k > 64 || a.rows < 0 ||
+      a.rows > 65535)
+    return fail(kBadShape, "mx4_experts: rows=%d k=%d experts=%d", a.rows, a.k, a.experts);
+  if (a.rows == 0) return 0;
+  if (!a.x || !a.ids || !a.weights || !a.w_gu || !a.w_down || !a.out || !a.work)
+    return fail(kBadArg, "mx4_experts: null pointer");
+  if ((uintptr_t)a.x % 16 || (uintptr_t)a.w_gu % 16 || (uintptr_t)a.w_down % 16 ||
+      (uintptr_t)a.work % 256 || (uintptr_t)a.ids % 4 || (uintptr_t)a.weights % 4 ||
+      (a.rows > 1 && (a.ldx % 8 || a.ldx < a.H)) || a.ld < a.k || a.ldo < a.H ||
+      (uintptr_t)a.out % (a.out_type == TFD_TYPE_F32 ? 4 : 2))
+    return fail(kBadArg, "mx4_experts: ldx=%lld ld=%d ldo=%lld or an alignment",
+                (long long)a.ldx, a.ld, (long long)a.ldo);
+  const Work wk = experts_work(a.rows, a.k, a.experts, a.H, a.I);
+  if (a.work_bytes < wk.bytes)
+    return fail(kBadArg, "mx4_experts: work of %lld bytes, %lld needed", (long long)a.work_bytes,
+                (long long)wk.bytes);
+  uint8_t* work = (uint8_t*)a.work;
+  const int n = a.rows * a.k;
+  Job gu = {};
+  gu.x = (const uint8_t*)a.x;
+  gu.ldx = 2 * a.ldx;
+  gu.w = (const uint8_t*)a.w_gu;
+  gu.w_tiles = (int64_t)a.experts * (a.I / 8);
+  gu.K = a.H;
+  gu.kb = mx4_blocks(a.H);
+  gu.N = 2 * a.I;
+  gu.M = n;
+  gu.out = work + wk.hidden;
+  gu.ldo = a.I;
+  gu.vec = 1;
+  gu.ids = a.ids;
+  gu.ldi = a.ld;
+  gu.k = gu.div = a.k;
+  gu.E = a.experts;
+  gu.err = a.err;
+  Job down = gu;
+  down.x = work + wk.hidden;
+  down.ldx = 2 * (int64_t)a.I;
+  down.w = (const uint8_t*)a.w_down;
+  down.w_tiles = (int64_t)a.experts * (a.H / 16);
+  down.K = a.I;
+  down.kb = mx4_blocks(a.I);
+  down.N = a.H;
+  down.div = 1;
+  down.err = nullptr;              // the first launch has raised it
+  hipStream_t s = (hipStream_t)stream;
+  const int cus = compute_units();
+  const int out_f32 = a.out_type == TFD_TYPE_F32;
+  if (fused_step(a.rows, a.k)) {
+    down.out = a.out;
+    down.ldo = a.ldo;
+    const int items = n * (a.I / 8);
+    k_mx4_few<kXBf16, 1, 1, 4, kHere, kSwiglu><<<min(items, 4 * cus), kBlock, 0, s>>>(gu);
+    k_mx4_down_mix<4><<<a.H / 16, kMixWaves * kWave, 0, s>>>(down, a.weights, a.rows, a.mult,
+                                                            out_f32, a.accumulate);
+    return launched("mx4_experts");
+  }
+  down.out = work + wk.d;
+  down.ldo = a.H;
+  int* groups = (int*)(work + wk.groups);
+  gu.groups = down.groups = groups;
+  // rows an expert has if all are picked alike; a tile is that and a bit
+  const int mean = n / a.experts;
+  const int tile_rows = mean <= 16 ? 16 : mean <= 48 ? 64 : 128;
+  const int tiles = a.experts + n / tile_rows;
+  k_mx4_group<<<1, kGroupThreads, 0, s>>>(gu, tile_rows, wk.room, groups);
+  if (tile_rows == 16) {
+    k_mx4_few<kXBf16, 1, 1, 4, kListed, kSwiglu><<<4 * cus, kBlock, 0, s>>>(gu);
+    k_mx4_few<kXBf16, 1, 1, 4, kListed, kF32><<<4 * cus, kBlock, 0, s>>>(down);
+  } else if (tile_rows == 64) {
+    launch_listed<4, 4>(gu, down, tiles, s);
+  } else {
+    launch_listed<8, 4>(gu, down, tiles, s);
+  }
+  k_mx4_mix<<<dim3((a.H / 4 + kBlock - 1) / kBlock, a.rows), kBlock, 0, s>>>(
+      (const float*)(work + wk.d), a.ids, a.weights, a.ld, a.k, a.experts, a.H, a.mult, out_f32,
+      a.accumulate, a.out, a.ldo);
+  return launched("mx4_experts");
+}
+
+}  // extern "C"

@@ -1,0 +1,293 @@
+"""Microscaled 4-bit tensors (OCP MXFP4) on the GPU: quantisation and its inverse.
+
+Along the last dimension 32 elements share a power-of-two scale (an e8m0 byte) and an
+element is an e2m1 code, two to a byte: 17 bytes where bf16 takes 64.  ``quantise`` gives
+codes and scales; ``Mx4.dequantise`` the values they stand for.  The kernels and their
+exact definitions are declared in ``include/tf_mx4.h``.  ``Linear`` multiplies by mx4
+weights, ``Experts`` runs a mixture's routed experts over them.
+
+Every call runs on its tensors' device and that device's current stream, allocates its
+outputs like any torch operation (so calls can be captured into a HIP graph and made from
+several streams) and computes no gradients.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import lib, ptr
+
+BLOCK = _lib.MX4_BLOCK
+U8 = torch.uint8
+TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16,
+         torch.float16: _lib.TYPE_F16}
+
+
+def stream_on(device) -> int:
+    """The device's current stream, as the C entries take it."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """Makes *device* the current one where it is not (a launch belongs to the current
+    device, a stream to its own)."""
+
+    __slots__ = ("index", "guard")
+
+    def __init__(self, device):
+        self.index, self.guard = device.index, None
+
+    def __enter__(self):
+        if self.index is not None and self.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def check_input(x, what: str, dtypes) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{what}: expected a tensor, got {type(x).__name__}")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{what}: dtype {x.dtype} is not one of "
+                         f"{', '.join(str(d) for d in dtypes)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: these operators compute no gradients; detach it or work "
+                         "under torch.no_grad()")
+
+
+def check_device(device, *others) -> None:
+    if device.type != "cuda":
+        raise ValueError(f"expected tensors on the GPU, got one on {device}")
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and on {t.device}")
+
+
+def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
+    """*x* as [rows][K] with unit stride along K, rows that do not overlap and, with
+    *align*, rows that start at multiples of that many bytes: a view where it is one."""
+    K = x.shape[-1]
+    x = x.reshape(-1, K)
+    size = x.element_size()
+    if (x.stride(1) != 1 and K > 1) or (x.shape[0] > 1 and (
+            x.stride(0) < K or x.stride(0) * size % align)) or x.data_ptr() % align:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def row_stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+@dataclass(frozen=True)
+class Mx4:
+    """Codes uint8 ``[..., K / 2]`` and scales uint8 ``[..., K / 32]`` of one tensor."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        c, s = self.codes, self.scales
+        if c.dtype != U8 or s.dtype != U8:
+            raise ValueError(f"mx4 codes and scales are uint8, got {c.dtype} and {s.dtype}")
+        if c.dim() < 1 or c.shape[:-1] != s.shape[:-1] or c.shape[-1] != 16 * s.shape[-1] or \
+                c.shape[-1] == 0:
+            raise ValueError(f"mx4 codes {tuple(c.shape)} and scales {tuple(s.shape)} are not "
+                             "[..., K / 2] and [..., K / 32] of one tensor")
+        if c.device != s.device:
+            raise ValueError(f"mx4 codes on {c.device}, scales on {s.device}")
+
+    @property
+    def shape(self) -> tuple[int, ...]:
+        """Shape of the values."""
+        return (*self.codes.shape[:-1], 2 * self.codes.shape[-1])
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def __getitem__(self, index) -> "Mx4":
+        """The tensors of some of the leading dimensions' entries."""
+        if self.codes.dim() < 2:
+            raise IndexError("mx4: an index takes whole rows, this is one row")
+        return Mx4(self.codes[index], self.scales[index])
+
+    def dequantise(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, exact in f32 and bf16 (f16 rounds what its range does not hold)."""
+        if dtype not in TYPES:
+            raise ValueError(f"dequantise: dtype {dtype} is not one of "
+                             f"{', '.join(str(d) for d in TYPES)}")
+        check_device(self.device)
+        codes, scales = rows_of(self.codes, 4), rows_of(self.scales)
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        with on_device(self.device):
+            lib().tfd_mx4_dequantise(ptr(codes), row_stride(codes), ptr(scales),
+                                     row_stride(scales), codes.shape[0], self.shape[-1],
+                                     ptr(out), self.shape[-1], TYPES[dtype],
+                                     stream_on(self.device))
+        return out
+
+
+def quantise(x: torch.Tensor) -> Mx4:
+    """Rows ``[..., K]`` (f32, bf16 or f16, K a multiple of 32) to mx4: for 32 values with
+    largest magnitude t the scale 2^(floor(log2 t) - 2), codes rounded to nearest even,
+    magnitudes past 6 scales as 6.  A block with a value that is not finite becomes NaN."""
+    check_input(x, "quantise", TYPES)
+    if x.dim() < 1 or x.shape[-1] % BLOCK or x.shape[-1] == 0:
+        raise ValueError(f"quantise: the last dimension must be a multiple of {BLOCK}, got "
+                         f"{tuple(x.shape)}")
+    check_device(x.device)
+    K, lead = x.shape[-1], x.shape[:-1]
+    codes = torch.empty(*lead, K // 2, dtype=U8, device=x.device)
+    scales = torch.empty(*lead, K // BLOCK, dtype=U8, device=x.device)
+    rows = rows_of(x)
+    with on_device(x.device):
+        lib().tfd_mx4_quantise(ptr(rows), row_stride(rows), TYPES[x.dtype], rows.shape[0], K,
+                               ptr(codes), K // 2, ptr(scales), K // BLOCK, stream_on(x.device))
+    return Mx4(codes, scales)
+
+
+def _pack(first: Mx4, second: Mx4 | None, what: str) -> torch.Tensor:
+    """Weights ``[..., N, K]`` (two of them alternating row by row) in the products'
+    layout, once, at load time."""
+    check_device(first.device, *(() if second is None else (second.codes,)))
+    K = first.shape[-1]
+    parts = [t.contiguous() for w in (first, second) if w is not None
+             for t in (w.codes, w.scales)]
+    for i in (0, 2):
+        if i < len(parts) and parts[i].data_ptr() % 16:
+            parts[i] = parts[i].clone()
+    rows = first.codes.numel() // (K // 2)
+    if rows == 0:
+        raise ValueError(f"{what}: no rows in weights of shape {first.shape}")
+    L = lib()
+    with on_device(first.device):
+        packed = torch.empty(L.tfd_mx4_packed_bytes(rows * (len(parts) // 2), K), dtype=U8,
+                             device=first.device)
+        L.tfd_mx4_pack(ptr(parts[0]), ptr(parts[1]),
+                       *((ptr(parts[2]), ptr(parts[3])) if second is not None else (None, None)),
+                       rows, K, ptr(packed), stream_on(first.device))
+    return packed
+
+
+OUT_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
+
+
+def _out_type(dtype, what: str) -> int:
+    if dtype not in OUT_TYPES:
+        raise ValueError(f"{what}: dtype {dtype} is neither float32 nor bfloat16")
+    return OUT_TYPES[dtype]
+
+
+class Linear:
+    """x -> x W^T by mx4 weights ``[N, K]``, kept in the layout the kernels read.
+
+    x: bf16 ``[..., K]`` (weights become bf16 on the way, exactly), or an ``Mx4`` of that
+    shape (both operands stay in 4 bits).  Sums are f32; the output is bf16 or f32."""
+
+    def __init__(self, weight: Mx4):
+        if len(weight.shape) != 2:
+            raise ValueError(f"Linear: weights must be [N, K], got {weight.shape}")
+        self.N, self.K = weight.shape
+        self.device = weight.device
+        self.packed = _pack(weight, None, "Linear")
+
+    def __call__(self, x, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        kind = _out_type(dtype, "Linear")
+        scales, ldxs = None, 0
+        if isinstance(x, Mx4):
+            lead, K, values = x.shape[:-1], x.shape[-1], x.codes
+        else:
+            check_input(x, "Linear", (torch.bfloat16,))
+            if x.dim() < 1:
+                raise ValueError("Linear: the input has no dimensions")
+            lead, K, values = x.shape[:-1], x.shape[-1], x
+        if K != self.K:
+            raise ValueError(f"Linear: input {tuple(x.shape)} for weights [{self.N}, {self.K}]")
+        if values.device != self.device:
+            raise ValueError(f"Linear: input on {values.device}, weights on {self.device}")
+        values = rows_of(values, 16)
+        if isinstance(x, Mx4):
+            scales = rows_of(x.scales)
+            ldxs = row_stride(scales)
+        out = torch.empty(*lead, self.N, dtype=dtype, device=self.device)
+        a = _lib.TfdMx4GemmArgs(ptr(values), row_stride(values), ptr(scales), ldxs,
+                                ptr(self.packed), values.shape[0], K, self.N, ptr(out), self.N,
+                                kind)
+        with on_device(self.device):
+            lib().tfd_mx4_gemm(ctypes.addressof(a), stream_on(self.device))
+        return out
+
+
+class Experts:
+    """The routed experts of a mixture by mx4 weights: gate and up ``[E, I, H]``, down
+    ``[E, H, I]``.  For each row of bf16 x ``[rows, H]``, with ids int32 and weights f32
+    ``[rows, k]`` (``routing.Routing`` gives both),
+
+        y = sum over the row's places of weight * down_e(silu(gate_e x) * (up_e x)).
+
+    The hidden values are rounded to bf16 (they are the down product's operands);
+    everything else is f32, the output rounded once to bf16 or f32.  Id -1 is an empty
+    place; any other id outside the experts is skipped and raises ``check_errors``.  An
+    expert may come twice in a row."""
+
+    def __init__(self, gate: Mx4, up: Mx4, down: Mx4):
+        if len(gate.shape) != 3 or gate.shape != up.shape or \
+                down.shape != (gate.shape[0], gate.shape[2], gate.shape[1]):
+            raise ValueError("Experts: gate and up must be [E, I, H] and down [E, H, I], got "
+                             f"{gate.shape}, {up.shape}, {down.shape}")
+        self.E, self.I, self.H = gate.shape
+        if not 1 <= self.E <= _lib.ROUTE_MAX_EXPERTS:
+            raise ValueError(f"Experts: 1 to {_lib.ROUTE_MAX_EXPERTS} experts, got {self.E}")
+        check_device(gate.device, up.codes, down.codes)
+        self.device = gate.device
+        self.w_gu = _pack(gate, up, "Experts")
+        self.w_down = _pack(down, None, "Experts")
+        self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+
+    def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
+                 dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        kind = _out_type(dtype, "Experts")
+        check_input(x, "x", (torch.bfloat16,))
+        check_input(ids, "ids", (torch.int32,))
+        check_input(weights, "weights", (torch.float32,))
+        if x.dim() != 2 or x.shape[1] != self.H:
+            raise ValueError(f"Experts: x must be [rows, {self.H}], got {tuple(x.shape)}")
+        rows = x.shape[0]
+        if ids.dim() != 2 or ids.shape != weights.shape or ids.shape[0] != rows or \
+                not 1 <= ids.shape[1] <= 64:
+            raise ValueError(f"Experts: ids {tuple(ids.shape)} and weights "
+                             f"{tuple(weights.shape)} must be [{rows}, 1..64]")
+        for t in (x, ids, weights):
+            if t.device != self.device:
+                raise ValueError(f"Experts: input on {t.device}, weights on {self.device}")
+        if rows > 65535:
+            raise ValueError(f"Experts: up to 65535 rows a call, got {rows}")
+        x = rows_of(x, 16)
+        ids, weights = ids.contiguous(), weights.contiguous()
+        out = torch.empty(rows, self.H, dtype=dtype, device=self.device)
+        L = lib()
+        need = L.tfd_mx4_experts_work_bytes(rows, ids.shape[1], self.E, self.H, self.I)
+        with on_device(self.device):
+            # of the stream that uses it, like the output: calls on several streams and
+            # captured graphs share nothing
+            work = torch.empty(need, dtype=U8, device=self.device)
+            a = _lib.TfdMx4ExpertsArgs(
+                ptr(x), row_stride(x), ptr(ids), ptr(weights), ids.shape[1], ptr(self.w_gu),
+                ptr(self.w_down), rows, ids.shape[1], self.E, self.H, self.I, ptr(out), self.H,
+                kind, 0, 1.0, ptr(work), need, ptr(self.err))
+            L.tfd_mx4_experts(ctypes.addressof(a), stream_on(self.device))
+        return out
+
+    def check_errors(self) -> None:
+        """Raises if a call since the last check met an id outside the experts (waits for
+        the device)."""
+        if int(self.err.item()):
+            self.err.zero_()
+            raise RuntimeError("mx4 experts: an id outside the experts (and not -1) was skipped")
