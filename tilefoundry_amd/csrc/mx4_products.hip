@@ -23,6 +23,7 @@ enum XKind { kXBf16 = 0, kXMx4 = 1 };
 enum Mode { kDense = 0, kHere = 1, kListed = 2 };   // rows: all; grouped in the block; before
 enum Epi { kBf16 = 0, kF32 = 1, kSwiglu = 2 };
 
+constexpr uint32_t kRange = 0x7fffffffu;   // of a row tile's descriptor: offsets up to 2 GiB
 constexpr int kHereMax = 128;    // entries that a block groups itself
 constexpr int kHereRows = 16;    // rows of a fused step: its mix has a thread for each column
 
@@ -45,10 +46,20 @@ struct Job {
   int32_t* err;
 };
 
+// The scaled product; a lane's scales are byte kA of sa and byte kB of sb.
+template <int kA, int kB>
 __device__ __forceinline__ f32x4 mfma_mx4(u32x4 a, uint32_t sa, u32x4 b, uint32_t sb, f32x4 c) {
   const i32x8 x = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
   const i32x8 y = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, (int)sa, 0, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, kA, (int)sa, kB, (int)sb);
+}
+// A compile-time loop: f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>).
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+  if constexpr (N > 0) {
+    unrolled<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
 }
 
 __device__ __forceinline__ u32x4 ld16(const uint8_t* p) {
@@ -124,7 +135,7 @@ __device__ void group_here(const Job& a, Tiles& s) {
   __syncthreads();
 }
 
-// The tile of expert rows that item `rt` works on.
+// The tile of expert rows that item `rt` works on (the same for a whole wave, and held so).
 template <int kMode>
 struct RowTile {
   int expert, count;
@@ -135,14 +146,14 @@ struct RowTile {
       first = rt * rows;
       count = min(rows, a.M - first);
     } else if (kMode == kHere) {
-      expert = s->expert[rt];
+      expert = __builtin_amdgcn_readfirstlane(s->expert[rt]);
       first = rt;
-      count = s->count[rt];
+      count = __builtin_amdgcn_readfirstlane(s->count[rt]);
     } else {
       const int* t = a.groups + 4 + rt * 4;
-      expert = t[0];
-      first = t[1];
-      count = t[2];
+      expert = __builtin_amdgcn_readfirstlane(t[0]);
+      first = __builtin_amdgcn_readfirstlane(t[1]);
+      count = __builtin_amdgcn_readfirstlane(t[2]);
     }
   }
   // the i-th row's place: a row of the dense product, or an entry (past the end: the last)
@@ -188,16 +199,17 @@ __device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v) {
 
 // ---------------------------------------------------------------------------
 // Few rows: the weights' stream bounds it.  An item is a tile of MT x 16 rows by TN
-// column tiles over all of K; items are dealt to the blocks in turn, and a block's
-// four waves split K and meet in LDS.  A wave has the next D steps' (128 k) weights,
-// scales and rows in flight across items, so the stream does not stop where an item
-// ends.  Rows come straight from memory (L2): each wave needs its own part of K, so
-// LDS would not save a read.
+// column tiles over all of K.  With kSplit items are dealt to the blocks in turn, and a
+// block's four waves split K and meet in LDS (few items, or a long K); without, each wave
+// takes items of its own.  A wave has the next D steps' (128 k) weights, scales and rows in
+// flight across items, so the stream does not stop where an item ends.  Rows come straight
+// from memory (L2), once for TN column tiles.
 // ---------------------------------------------------------------------------
-template <int kX, int MT, int TN, int D, int kMode, int kEpi>
+template <int kX, int MT, int TN, int D, int kMode, int kEpi, bool kSplit = true>
 __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
   constexpr int kR = 16 * MT;
-  __shared__ f32x4 red[2][kWavesPerBlock][MT * TN][kWave];
+  __shared__ f32x4 red[kSplit ? 2 : 1][kSplit ? kWavesPerBlock : 1][kSplit ? MT * TN : 1]
+                      [kSplit ? kWave : 1];
   __shared__ typename std::conditional<kMode == kHere, Tiles, int>::type group_s;
   const Tiles* tiles = nullptr;
   const int lane = threadIdx.x & (kWave - 1);
@@ -216,11 +228,14 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
   }
   const int ntiles = (a.N + 15) / 16;
   const int nC = (ntiles + TN - 1) / TN;
-  const int items = nT * nC, G = (int)gridDim.x, me = (int)blockIdx.x;
+  const int items = nT * nC;
+  const int G = (int)gridDim.x * (kSplit ? 1 : kWavesPerBlock);
+  const int me = kSplit ? (int)blockIdx.x : (int)blockIdx.x * kWavesPerBlock + wave;
   if (me >= items) return;
   const int mine = (items - 1 - me) / G + 1;
-  const int ns = (a.kb + kWavesPerBlock - 1) / kWavesPerBlock;   // steps of a wave's part
-  const int k0 = wave * ns;
+  // steps of a wave's part of K
+  const int ns = kSplit ? (a.kb + kWavesPerBlock - 1) / kWavesPerBlock : a.kb;
+  const int k0 = kSplit ? wave * ns : 0;
   const int sg = mx4_scale_groups(a.kb);
   const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
 
@@ -296,7 +311,7 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
         for (int t = 0; t < TN; ++t)
 #pragma unroll
           for (int m = 0; m < MT; ++m)
-            c[t][m] = mfma_mx4(w[u][t], ws[u][t], x[u][m][0], xs[u][m], c[t][m]);
+            c[t][m] = mfma_mx4<0, 0>(w[u][t], ws[u][t], x[u][m][0], xs[u][m], c[t][m]);
       } else {
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
@@ -315,23 +330,26 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
     // item is enough) and the waves take turns to write
     const int j = jc++;
     sc = 0;
+    if (kSplit) {
 #pragma unroll
-    for (int t = 0; t < TN; ++t)
+      for (int t = 0; t < TN; ++t)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        red[j & 1][wave][t * MT + m][lane] = c[t][m];
-        c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-    __syncthreads();
+        for (int m = 0; m < MT; ++m) red[j & 1][wave][t * MT + m][lane] = c[t][m];
+      __syncthreads();
+    }
     const int it = me + j * G, rt = it % nT, cc = it / nT;
     const RowTile<kMode> r(a, tiles, rt, kR);
 #pragma unroll
     for (int q = 0; q < TN * MT; ++q) {
-      if ((q + j) % kWavesPerBlock != wave) continue;
       const int t = q / MT, m = q % MT;
-      f32x4 v = red[j & 1][0][q][lane];
+      f32x4 v = c[t][m];
+      c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (kSplit) {
+        if ((q + j) % kWavesPerBlock != wave) continue;
+        v = red[j & 1][0][q][lane];
 #pragma unroll
-      for (int p = 1; p < kWavesPerBlock; ++p) v += red[j & 1][p][q][lane];
+        for (int p = 1; p < kWavesPerBlock; ++p) v += red[j & 1][p][q][lane];
+      }
       const int n = (cc * TN + t) * 16 + 4 * kq;
       if (m * 16 + nl < r.count && cc * TN + t < ntiles && n < a.N)
         put<kEpi>(a, r.at(a, tiles, m * 16 + nl, room), n, v);
@@ -354,81 +372,111 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: the matrix cores bound it.  A block of four waves takes TM x 16 rows by
-// 4 x TN x 16 columns; its rows pass through LDS, 128 k at a time in two buffers, in
-// the order the matrix instruction takes them (a wave's read is 1 KiB in a row, and a
-// write's eight lanes are 128 bytes in a row: no bank conflicts); each wave's own
-// weights go straight to its registers, two steps ahead, and are converted there.
+// Many rows: the matrix cores bound it.  A block of four waves takes up to TM x 16 rows
+// by 4 x TN x 16 columns.  Its rows pass through LDS, a stage (128 k of bf16, 256 k of
+// codes) at a time in two buffers, in the order the matrix instruction takes them (a
+// wave's read is 1 KiB in a row, and a write's eight lanes are 128 bytes in a row: no bank
+// conflicts); each wave's own weights go straight to its registers, two blocks of 128 k
+// ahead, and are converted there.  bf16 rows come in two halves, each loaded and written
+// beside the products of half a stage: with all in flight at once the kernel needs more
+// than the 256 registers at which two blocks share a compute unit.  (DMA into LDS needs
+// none, but every LDS read behind it waits for it.)
 // ---------------------------------------------------------------------------
+template <int kX, int TM>
+struct ManyLds {
+  static constexpr int kBlocks = kX == kXMx4 ? 2 : 1;               // of 128 k in a stage
+  static constexpr int kBytes = TM * (kX == kXMx4 ? 1024 : 4096);   // of a block
+  // a lane's scales of all row tiles and blocks side by side: one read gives them all
+  static constexpr int kScPad = kBlocks * TM;
+  static constexpr int kScales = kX == kXMx4 ? kScPad * kWave : 0;
+  static constexpr int kTotal = 2 * (kBlocks * kBytes + kScales);   // rows, then scales
+};
+
+// One item: a row tile `r` of at most TM x 16 rows and column block `cb`.
 template <int kX, int TM, int TN, int kMode, int kEpi>
-__global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a, int nT_host) {
-  constexpr int kR = 16 * TM;
-  constexpr int kStep = TM * (kX == kXMx4 ? 1024 : 4096);   // LDS bytes of 128 k
-  constexpr int kPass = kX == kXMx4 ? (TM + 3) / 4 : TM;    // 16-byte pieces a thread stages
-  __shared__ __align__(16) uint8_t xs_s[2][kStep];
-  __shared__ uint8_t xsc_s[2][kX == kXMx4 ? TM * kWave : 1];
+__device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r, int room, int cb,
+                                          uint8_t* lds) {
+  constexpr bool kMx = kX == kXMx4;
+  using Lds = ManyLds<kX, TM>;
+  constexpr int KC = Lds::kBlocks, kScPad = Lds::kScPad;
+  static_assert(!kMx || kScPad == 16, "a lane's scales of a stage are one 16-byte read");
+  constexpr int kPieces = kMx ? (KC * TM + 3) / 4 : (TM + 1) / 2;   // loads in flight a thread
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  auto xs_s = [&](int buf) { return lds + buf * (KC * Lds::kBytes); };
+  auto xsc_s = [&](int buf) { return lds + 2 * KC * Lds::kBytes + buf * Lds::kScales; };
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int nl = lane & 15, kq = lane >> 4;
-  const int nT = kMode == kListed ? a.groups[0] : nT_host;
-  const int room = kMode == kListed ? listed_room(a) : 0;
   const int ntiles = (a.N + 15) / 16;
-  const int nC = (ntiles + 4 * TN - 1) / (4 * TN);
-  // consecutive items (eight row tiles by a few column blocks) on one XCD: what they
-  // share stays in its L2
-  const int total = nT * nC, per = (nT_host * nC + 7) / 8;
-  const int g = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || g >= total) return;
-  const int grp = g / (8 * nC), within = g % (8 * nC);
-  const int gm = min(8, nT - grp * 8);
-  const int rt = grp * 8 + within % gm, cb = within / gm;
-  const RowTile<kMode> r(a, nullptr, rt, kR);
   const int sg = mx4_scale_groups(a.kb);
   const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
 
-  // bf16: piece (tile m, row nl of it, k 32 wave + 8 kq); microscaled: (tile, row nl, k 32 kq)
-  // (row numbers, not pointers: a register each)
-  int xrow[kPass];
+  // Eight lanes of a load take 128 bytes of one row, a whole cache line: rows a power of two
+  // apart share a set of the L1, which keeps no line until another wave wants its other half
+  // (64 bytes of 16 rows: 203 us for 4,001 x 2048 x 12288, 171 on padded rows).  bf16: of row
+  // tile m, rows 8 (wave % 2) + lane / 8, k 64 (wave / 2) + 8 (lane % 8); codes: piece q
+  // is rows 8 (i % 2) + lane / 8 of row tile i / 2, i = 4 q + wave, both blocks of a stage.
+  // 32-bit offsets from a base that all lanes share (the entries check that they fit).
+  const uint8_t* xb = a.x + (kMode == kDense ? r.first * a.ldx : 0);
+  const uint8_t* xsb = kMx ? a.xs + (kMode == kDense ? r.first * a.ldxs : 0) : nullptr;
+  auto offset = [&](int i, int64_t ld) {
+    const int at = r.at(a, nullptr, i, room);
+    return (uint32_t)(kMode == kDense ? at - r.first : at / a.div) * (uint32_t)ld;
+  };
+  const int lr = lane >> 3, lp = lane & 7;
+  uint32_t xo[kMx ? kPieces : TM], xso[kMx ? kPieces : 1];
 #pragma unroll
-  for (int q = 0; q < kPass; ++q) {
-    const int m = kX == kXMx4 ? min(q * 4 + wave, TM - 1) : q;
-    const int at = r.at(a, nullptr, m * 16 + nl, room);
-    xrow[q] = kMode == kDense ? at : at / a.div;
+  for (int q = 0; q < (kMx ? kPieces : TM); ++q) {
+    const int i = kMx ? min(q * 4 + wave, 2 * TM - 1) : 2 * q + (wave & 1);
+    xo[q] = offset(i * 8 + lr, a.ldx) + 16 * lp + (kMx ? 0 : 128 * (wave >> 1));
+    if (kMx) xso[q] = offset(min(q * 4 + wave, KC * TM - 1) % TM * 16 + nl, a.ldxs);
   }
-  u32x4 xr[kPass];
-  uint32_t xsr[kPass];
-  auto load_x = [&](int b) {
-    if (kX == kXMx4) {
-      const int k = b * kMx4K + 32 * kq;
-      const bool in = k < a.K;
+  u32x4 xr[kPieces];
+  uint32_t xsr[kMx ? kPieces : 1];
+  // pieces past K, and past the last block, are out of the descriptors' range: zeros (a zero
+  // scale byte is 2^-127) without a branch between a load and its use
+  const auto xrs = rsrc_bounded(xb, kRange);
+  const auto xsrs = rsrc_bounded(xsb, kRange);
+  auto load_x = [&](int half, int b0) {
+    if (kMx) {
+      const bool in = b0 * kMx4K + 32 * lp < a.K;
 #pragma unroll
-      for (int q = 0; q < kPass; ++q) {
-        xr[q] = ld16(a.x + xrow[q] * a.ldx + (in ? k >> 1 : 0));
-        xsr[q] = ld1(a.xs + xrow[q] * a.ldxs + (in ? k >> 5 : 0));
-        if (!in) {
-          xr[q] = u32x4{0u, 0u, 0u, 0u};
-          xsr[q] = 127;
-        }
+      for (int q = 0; q < kPieces; ++q) {
+        const int k = (b0 + (q * 4 + wave) / TM) * kMx4K + 32 * kq;
+        xr[q] = __builtin_amdgcn_raw_buffer_load_b128(xrs, in ? xo[q] : kOutOfRange, b0 * 64, 0);
+        xsr[q] = __builtin_amdgcn_raw_buffer_load_b8(
+            xsrs, k < a.K ? xso[q] + (k >> 5) : kOutOfRange, 0, 0);
       }
     } else {
-      const int k = b * kMx4K + 32 * wave;
-      const bool in = k < a.K;                    // the wave's 32 k are in or out together
+      const bool in = b0 * kMx4K + 64 * (wave >> 1) + 8 * lp < a.K;
 #pragma unroll
-      for (int q = 0; q < kPass; ++q)
-        xr[q] = in ? ld16(a.x + xrow[q] * a.ldx + 2 * (k + 8 * kq)) : u32x4{0u, 0u, 0u, 0u};
+      for (int q = 0; q < kPieces; ++q) {
+        const int m = half * kPieces + q;
+        if (m < TM)
+          xr[q] = __builtin_amdgcn_raw_buffer_load_b128(xrs, in ? xo[m] : kOutOfRange,
+                                                        2 * b0 * kMx4K, 0);
+      }
     }
   };
-  auto stage = [&](int buf) {
+  // Where 16 bytes lie in LDS: 1 KiB for the 64 lanes of an operand, lane (row, 32 k group)
+  // at row ^ f + 16 group, f running over 0..7 among the eight lanes that write one row's
+  // pieces (which go to eight operands or groups): no bank conflicts, nor for the reads.
+  auto operand = [&](int buf, int i, int row, int group, int f) {
+    return &xs_s(buf)[i * 1024 + ((row ^ f) + 16 * group) * 16];
+  };
+  auto stage = [&](int half, int buf) {
 #pragma unroll
-    for (int q = 0; q < kPass; ++q) {
-      if (kX == kXMx4) {
-        const int m = q * 4 + wave;
-        if (m < TM) {
-          *reinterpret_cast<u32x4*>(&xs_s[buf][m * 1024 + lane * 16]) = xr[q];
-          xsc_s[buf][m * kWave + lane] = (uint8_t)xsr[q];
-        }
+    for (int q = 0; q < kPieces; ++q) {
+      if (kMx) {
+        const int i = q * 4 + wave;
+        if (i < 2 * TM)
+          *reinterpret_cast<u32x4*>(operand(buf, (lp >> 2) * TM + (i >> 1), 8 * (i & 1) + lr,
+                                            lp & 3, lp)) = xr[q];
+        if (i < KC * TM) xsc_s(buf)[lane * kScPad + i] = (uint8_t)xsr[q];
       } else {
-        *reinterpret_cast<u32x4*>(&xs_s[buf][(q * 4 + kq) * 1024 + (nl + 16 * wave) * 16]) = xr[q];
+        const int m = half * kPieces + q, group = 2 * (wave >> 1) + (lp >> 2);
+        if (m < TM)
+          *reinterpret_cast<u32x4*>(operand(buf, m * 4 + (lp & 3), 8 * (wave & 1) + lr, group,
+                                            (lp & 3) + 4 * (group & 1))) = xr[q];
       }
     }
   };
@@ -436,67 +484,105 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
 #pragma unroll
   for (int t = 0; t < TN; ++t)
     wt[t] = (int64_t)r.expert * ntiles + min((cb * 4 + wave) * TN + t, ntiles - 1);
+  // two blocks' codes ahead; the scales of four blocks are one dword
   u32x4 w[2][TN];
-  uint32_t ws[2][TN];
+  uint32_t ws[TN], ws_next[TN];
   auto load_w = [&](int u, int b) {
-    b = min(b, a.kb - 1);
+    const int64_t at = min(b, a.kb - 1);
 #pragma unroll
-    for (int t = 0; t < TN; ++t) {
-      w[u][t] = ld16(a.w + (wt[t] * a.kb + b) * 1024 + lane * 16);
-      ws[u][t] = ld1(scales + (wt[t] * sg + (b >> 2)) * 256 + lane * 4 + (b & 3));
-    }
+    for (int t = 0; t < TN; ++t)
+      w[u][t] = ld16(a.w + (wt[t] * a.kb + at) * 1024 + lane * 16);
+  };
+  auto load_ws = [&](int q) {
+    const int64_t at = min(q, sg - 1);
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+      ws_next[t] = *(const __attribute__((address_space(1))) uint32_t*)(
+          scales + (wt[t] * sg + at) * 256 + lane * 4);
   };
   f32x4 c[TM][TN];
 #pragma unroll
   for (int m = 0; m < TM; ++m)
 #pragma unroll
     for (int t = 0; t < TN; ++t) c[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load_x(0);
+  load_x(0, 0);
+  load_ws(0);
   load_w(0, 0);
   load_w(1, 1);
-  stage(0);
+  stage(0, 0);
+  if (!kMx) {
+    load_x(1, 0);
+    stage(1, 0);
+  }
   __syncthreads();
-  auto body = [&](auto slot, int b) {
-    constexpr int u = decltype(slot)::value;
-    const bool next = b + 1 < a.kb;
-    if (next) load_x(b + 1);
-    if (kX == kXMx4) {
+  int buf = 0;
+  u32x4 vs = {0u, 0u, 0u, 0u};
+  // the 128 k of block b, the j-th of its four: weights in slot j % 2, rows in the current
+  // buffer; the slot is refilled behind its use
+  auto products = [&](auto jth, int b) {
+    constexpr int j = decltype(jth)::value, u = j % 2;
+    if constexpr (kMx) {
       u32x4 v[TM];
-      uint32_t vs[TM];
 #pragma unroll
-      for (int m = 0; m < TM; ++m) {
-        v[m] = *reinterpret_cast<const u32x4*>(&xs_s[u][m * 1024 + lane * 16]);
-        vs[m] = xsc_s[u][m * kWave + lane];
-      }
-#pragma unroll
-      for (int t = 0; t < TN; ++t)
-#pragma unroll
-        for (int m = 0; m < TM; ++m) c[m][t] = mfma_mx4(w[u][t], ws[u][t], v[m], vs[m], c[m][t]);
+      for (int m = 0; m < TM; ++m)
+        v[m] = *reinterpret_cast<const u32x4*>(operand(buf, u * TM + m, nl, kq, kq + 4 * u));
+      unrolled<TN>([&](auto t) {
+        unrolled<TM>([&](auto m) {
+          constexpr int i = u * TM + m.value;
+          c[m.value][t.value] = mfma_mx4<j, i % 4>(w[u][t.value], ws[t.value], v[m.value],
+                                                   vs[i / 4], c[m.value][t.value]);
+        });
+      });
     } else {
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
+        if (s % 2 == 0) load_x(s / 2, b + 1);
         u32x4 v[TM];
 #pragma unroll
         for (int m = 0; m < TM; ++m)
-          v[m] = *reinterpret_cast<const u32x4*>(&xs_s[u][(m * 4 + s) * 1024 + lane * 16]);
+          v[m] = *reinterpret_cast<const u32x4*>(
+              operand(buf, m * 4 + s, nl, kq, s + 4 * (kq & 1)));
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
-          const u32x4 q = fp4x8_to_bf16(w[u][t][s], mx4_scale(ws[u][t]));
+          const u32x4 q = fp4x8_to_bf16(w[u][t][s], mx4_scale((ws[t] >> (8 * j)) & 0xffu));
 #pragma unroll
           for (int m = 0; m < TM; ++m) c[m][t] = mfma(q, v[m], c[m][t]);
         }
         __builtin_amdgcn_sched_barrier(0);
+        if (s % 2 == 1) stage(s / 2, 1 - buf);
+        // keeps the next step's LDS reads from being gathered here: registers
+        asm volatile("" ::: "memory");
       }
     }
     load_w(u, b + 2);
-    if (next) {
-      stage(1 - u);
-      __syncthreads();
-    }
+    __builtin_amdgcn_sched_barrier(0);
   };
-  for (int b = 0; b < a.kb; b += 2) {
-    body(std::integral_constant<int, 0>{}, b);
-    if (b + 1 < a.kb) body(std::integral_constant<int, 1>{}, b + 1);
+  auto turn = [&] {
+    __syncthreads();
+    buf = 1 - buf;
+  };
+  // blocks b and b + 1, the j-th two of four
+  auto two = [&](auto jth, int b) {
+    constexpr int j = decltype(jth)::value;
+    if (kMx) {
+      load_x(0, b + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      vs = *reinterpret_cast<const u32x4*>(&xsc_s(buf)[lane * kScPad]);
+    }
+    products(std::integral_constant<int, 2 * j>{}, b);
+    if (b + 1 < a.kb) {
+      if (!kMx) turn();
+      products(std::integral_constant<int, 2 * j + 1>{}, b + 1);
+    }
+    if (kMx) stage(0, 1 - buf);
+    turn();
+  };
+  for (int q = 0; q < sg; ++q) {
+#pragma unroll
+    for (int t = 0; t < TN; ++t) ws[t] = ws_next[t];
+    load_ws(q + 1);
+    two(std::integral_constant<int, 0>{}, 4 * q);
+    if (4 * q + 2 < a.kb) two(std::integral_constant<int, 1>{}, 4 * q + 2);
   }
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
@@ -509,6 +595,33 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
       if (tile < ntiles && n < a.N) put<kEpi>(a, at, n, c[m][t]);
     }
   }
+}
+
+template <int kX, int TM, int TN, int kMode, int kEpi>
+__global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a, int nT_host) {
+  __shared__ __align__(16) uint8_t lds[ManyLds<kX, TM>::kTotal];
+  const int nT = kMode == kListed ? a.groups[0] : nT_host;
+  const int room = kMode == kListed ? listed_room(a) : 0;
+  const int ntiles = (a.N + 15) / 16;
+  const int nC = (ntiles + 4 * TN - 1) / (4 * TN);
+  // consecutive items (eight row tiles by a few column blocks) on one XCD: what they
+  // share stays in its L2
+  const int total = nT * nC, per = (total + 7) / 8;
+  const int g = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || g >= total) return;
+  const int grp = g / (8 * nC), within = g % (8 * nC);
+  const int gm = min(8, nT - grp * 8);
+  const int rt = grp * 8 + within % gm, cb = within / gm;
+  const RowTile<kMode> r(a, nullptr, rt, 16 * TM);
+  // a list's tile may hold fewer rows: it runs as the smallest tile that holds them
+  const int used = (r.count + 15) >> 4;
+  if constexpr (kMode == kListed && TM == 8) {
+    if (used <= 2) return many_item<kX, 2, TN, kMode, kEpi>(a, r, room, cb, lds);
+    if (used <= 4) return many_item<kX, 4, TN, kMode, kEpi>(a, r, room, cb, lds);
+    if (used == 5) return many_item<kX, 5, TN, kMode, kEpi>(a, r, room, cb, lds);
+    if (used == 6) return many_item<kX, 6, TN, kMode, kEpi>(a, r, room, cb, lds);
+  }
+  many_item<kX, TM, TN, kMode, kEpi>(a, r, room, cb, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -633,51 +746,76 @@ constexpr int kGroupThreads = 1024;
 
 __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_rows, int room,
                                                              int* __restrict__ groups) {
-  __shared__ int count[TFD_ROUTE_MAX_EXPERTS], first[2][TFD_ROUTE_MAX_EXPERTS],
-      tile[2][TFD_ROUTE_MAX_EXPERTS];
-  const int tid = threadIdx.x;
-  if (tid < TFD_ROUTE_MAX_EXPERTS) count[tid] = 0;
+  constexpr int kE = TFD_ROUTE_MAX_EXPERTS, kKeep = 16;
+  __shared__ int count[kE], wave_rows[kE / kWave], wave_tiles[kE / kWave];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  if (tid < kE) count[tid] = 0;
+  // a thread's first ids stay in registers for the second pass
+  auto id_at = [&](int i) {
+    if (i >= a.M) return -1;
+    const int id = a.ids[a.ldi == a.k ? i : (int64_t)(i / a.k) * a.ldi + i % a.k];
+    if ((unsigned)id < (unsigned)a.E) return id;
+    if (id != -1 && a.err) raise_error(a.err, kErrTokenRange);
+    return -1;
+  };
+  int kept[kKeep];
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j) kept[j] = id_at(tid + j * kGroupThreads);
   __syncthreads();
-  for (int i = tid; i < a.M; i += kGroupThreads) {
-    const int id = a.ids[(int64_t)(i / a.k) * a.ldi + i % a.k];
-    if ((unsigned)id < (unsigned)a.E) atomicAdd(&count[id], 1);
-    else if (id != -1 && a.err) raise_error(a.err, kErrTokenRange);
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (kept[j] >= 0) atomicAdd(&count[kept[j]], 1);
+  for (int i = tid + kKeep * kGroupThreads; i < a.M; i += kGroupThreads) {
+    const int id = id_at(i);
+    if (id >= 0) atomicAdd(&count[id], 1);
   }
   __syncthreads();
-  int mine = 0, tiles = 0;
-  if (tid < TFD_ROUTE_MAX_EXPERTS) {
-    mine = tid < a.E ? count[tid] : 0;
-    tiles = (mine + tile_rows - 1) / tile_rows;
-    first[0][tid] = mine;
-    tile[0][tid] = tiles;
+  // rows and tiles before each expert: a scan by waves, then over the waves
+  const int mine = tid < a.E ? count[tid] : 0;
+  const int tiles = (mine + tile_rows - 1) / tile_rows;
+  int rows_to = mine, tiles_to = tiles;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const int r = __shfl_up(rows_to, d, kWave), t = __shfl_up(tiles_to, d, kWave);
+    rows_to += lane >= d ? r : 0;
+    tiles_to += lane >= d ? t : 0;
   }
-  int cur = 0;
-  for (int d = 1; d < TFD_ROUTE_MAX_EXPERTS; d *= 2) {
-    __syncthreads();
-    if (tid < TFD_ROUTE_MAX_EXPERTS) {
-      first[1 - cur][tid] = first[cur][tid] + (tid >= d ? first[cur][tid - d] : 0);
-      tile[1 - cur][tid] = tile[cur][tid] + (tid >= d ? tile[cur][tid - d] : 0);
+  if (tid < kE && lane == kWave - 1) {
+    wave_rows[wave] = rows_to;
+    wave_tiles[wave] = tiles_to;
+  }
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int v = 0; v < kE / kWave; ++v) {
+    if (v < wave) {
+      rows_to += wave_rows[v];
+      tiles_to += wave_tiles[v];
     }
-    cur = 1 - cur;
+    all += wave_tiles[v];
   }
-  __syncthreads();
   if (tid < a.E) {
-    const int f = first[cur][tid] - mine, t0 = tile[cur][tid] - tiles;
+    // an expert's rows spread evenly over its tiles, in sixteens: a tile costs by those
+    const int f = rows_to - mine, t0 = tiles_to - tiles;
+    const int even = tiles ? ((mine + tiles - 1) / tiles + 15) / 16 * 16 : 0;
     for (int t = 0; t < tiles; ++t) {
       int* o = groups + 4 + (t0 + t) * 4;
       o[0] = tid;
-      o[1] = f + t * tile_rows;
-      o[2] = min(tile_rows, mine - t * tile_rows);
+      o[1] = f + t * even;
+      o[2] = min(even, mine - t * even);
     }
     count[tid] = f;
   }
   if (tid == 0) {
-    groups[0] = tile[cur][TFD_ROUTE_MAX_EXPERTS - 1];
+    groups[0] = all;
     groups[1] = room;
   }
   __syncthreads();
   int* order = groups + 4 + room * 4;
-  for (int i = tid; i < a.M; i += kGroupThreads) {
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    if (kept[j] >= 0) order[atomicAdd(&count[kept[j]], 1)] = tid + j * kGroupThreads;
+  for (int i = tid + kKeep * kGroupThreads; i < a.M; i += kGroupThreads) {
     const int id = a.ids[(int64_t)(i / a.k) * a.ldi + i % a.k];
     if ((unsigned)id < (unsigned)a.E) order[atomicAdd(&count[id], 1)] = i;
   }
@@ -756,7 +894,7 @@ int launch_dense(const Job& a, hipStream_t s) {
     k_mx4_few<kX, 2, 1, 2, kDense, kEpi><<<min(items, 4 * cus), kBlock, 0, s>>>(a);
   } else {
     const int nT = (a.M + 127) / 128, nC = (ntiles + 15) / 16;
-    if ((int64_t)nT * nC > (1 << 30)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
+    if ((int64_t)nT * nC > (1 << 28)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
     k_mx4_many<kX, 8, 4, kDense, kEpi><<<8 * ((nT * nC + 7) / 8), kBlock, 0, s>>>(a, nT);
   }
   return launched("mx4_gemm");
@@ -770,7 +908,9 @@ extern "C" int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream) {
   if (a.out_type != TFD_TYPE_F32 && a.out_type != TFD_TYPE_BF16)
     return fail(kBadArg, "mx4_gemm: out_type %d", a.out_type);
   if (const int rc = job_checks("mx4_gemm", a.K, a.N)) return rc;
-  if (a.M < 0 || a.M > (1 << 30)) return fail(kBadShape, "mx4_gemm: M=%d", a.M);
+  if (a.M < 0 || a.M > (1 << 30) || a.ldx > (1 << 23) || a.ldxs > (1 << 23))
+    return fail(kBadShape, "mx4_gemm: M=%d ldx=%lld ldxs=%lld", a.M, (long long)a.ldx,
+                (long long)a.ldxs);
   if (a.M == 0) return 0;
   if (!a.x || !a.w || !a.out) return fail(kBadArg, "mx4_gemm: null pointer");
   const bool mx = a.x_scales != nullptr;
@@ -822,6 +962,11 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
   if (a.rows == 0) return 0;
   if (!a.x || !a.ids || !a.weights || !a.w_gu || !a.w_down || !a.out || !a.work)
     return fail(kBadArg, "mx4_experts: null pointer");
+  // rows are read at 31-bit offsets from their first
+  if (((int64_t)a.rows * (a.rows > 1 ? a.ldx : a.H)) >> 30 ||
+      ((int64_t)a.rows * a.k * a.I) >> 30)
+    return fail(kBadShape, "mx4_experts: rows=%d of %lld, or %d x %d hidden values, pass 2 GiB",
+                a.rows, (long long)a.ldx, a.rows * a.k, a.I);
   if ((uintptr_t)a.x % 16 || (uintptr_t)a.w_gu % 16 || (uintptr_t)a.w_down % 16 ||
       (uintptr_t)a.work % 256 || (uintptr_t)a.ids % 4 || (uintptr_t)a.weights % 4 ||
       (a.rows > 1 && (a.ldx % 8 || a.ldx < a.H)) || a.ld < a.k || a.ldo < a.H ||
@@ -883,8 +1028,8 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
   const int tiles = a.experts + n / tile_rows;
   k_mx4_group<<<1, kGroupThreads, 0, s>>>(gu, tile_rows, wk.room, groups);
   if (tile_rows == 16) {
-    k_mx4_few<kXBf16, 1, 1, 4, kListed, kSwiglu><<<4 * cus, kBlock, 0, s>>>(gu);
-    k_mx4_few<kXBf16, 1, 1, 4, kListed, kF32><<<4 * cus, kBlock, 0, s>>>(down);
+    k_mx4_few<kXBf16, 1, 4, 2, kListed, kSwiglu, false><<<3 * cus, kBlock, 0, s>>>(gu);
+    k_mx4_few<kXBf16, 1, 4, 2, kListed, kF32, false><<<3 * cus, kBlock, 0, s>>>(down);
   } else if (tile_rows == 64) {
     launch_listed<4, 4>(gu, down, tiles, s);
   } else {
