@@ -456,6 +456,7 @@ class _Checked:
                 raise TFDError(name, rc, self.last_error())
             return rc
 
+        setattr(self, name, call)            # found at once from the second use on
         return call
 
 

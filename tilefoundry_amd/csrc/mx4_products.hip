@@ -200,15 +200,15 @@ __device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v) {
 // ---------------------------------------------------------------------------
 // Few rows: the weights' stream bounds it.  An item is a tile of MT x 16 rows by TN
 // column tiles over all of K.  With kSplit items are dealt to the blocks in turn, and a
-// block's four waves split K and meet in LDS (few items, or a long K); without, each wave
-// takes items of its own.  A wave has the next D steps' (128 k) weights, scales and rows in
+// block's waves split K and meet in LDS (few items, or a long K); without, each wave takes
+// items of its own.  A wave has the next D steps' (128 k) weights, scales and rows in
 // flight across items, so the stream does not stop where an item ends.  Rows come straight
 // from memory (L2), once for TN column tiles.
 // ---------------------------------------------------------------------------
-template <int kX, int MT, int TN, int D, int kMode, int kEpi, bool kSplit = true>
-__global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
+template <int kX, int MT, int TN, int D, int kMode, int kEpi, int kWaves = 4, bool kSplit = true>
+__global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   constexpr int kR = 16 * MT;
-  __shared__ f32x4 red[kSplit ? 2 : 1][kSplit ? kWavesPerBlock : 1][kSplit ? MT * TN : 1]
+  __shared__ f32x4 red[kSplit ? 2 : 1][kSplit ? kWaves : 1][kSplit ? MT * TN : 1]
                       [kSplit ? kWave : 1];
   __shared__ typename std::conditional<kMode == kHere, Tiles, int>::type group_s;
   const Tiles* tiles = nullptr;
@@ -229,12 +229,12 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
   const int ntiles = (a.N + 15) / 16;
   const int nC = (ntiles + TN - 1) / TN;
   const int items = nT * nC;
-  const int G = (int)gridDim.x * (kSplit ? 1 : kWavesPerBlock);
-  const int me = kSplit ? (int)blockIdx.x : (int)blockIdx.x * kWavesPerBlock + wave;
+  const int G = (int)gridDim.x * (kSplit ? 1 : kWaves);
+  const int me = kSplit ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave;
   if (me >= items) return;
   const int mine = (items - 1 - me) / G + 1;
   // steps of a wave's part of K
-  const int ns = kSplit ? (a.kb + kWavesPerBlock - 1) / kWavesPerBlock : a.kb;
+  const int ns = kSplit ? (a.kb + kWaves - 1) / kWaves : a.kb;
   const int k0 = kSplit ? wave * ns : 0;
   const int sg = mx4_scale_groups(a.kb);
   const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
@@ -272,7 +272,9 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
       w[u][t] = ld16_stream(a.w + (nx.tile[t] * a.kb + b) * 1024 + lane * 16);
       ws[u][t] = ld1(scales + (nx.tile[t] * sg + (b >> 2)) * 256 + lane * 4 + (b & 3));
     }
-    // a lane's 32 k; those past K read the row's first and are cleared before use
+    // a lane's 32 k; those past K read the row's first and are cleared before use.  (Loads of
+    // 64 bytes of a row by four lanes, transposed by lane swaps, measured no faster: 19 rows
+    // 10.6 us for 10.4, eight rows' experts 52 for 48.)
     const int k = b * kMx4K + 32 * kq, kk = k < a.K ? k : 0;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -326,7 +328,7 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
       }
     }
     if (++sc < ns) return;
-    // the item is done: the four parts of K meet in LDS (two buffers, so one barrier an
+    // the item is done: the parts of K meet in LDS (two buffers, so one barrier an
     // item is enough) and the waves take turns to write
     const int j = jc++;
     sc = 0;
@@ -345,10 +347,10 @@ __global__ __launch_bounds__(kBlock) void k_mx4_few(Job a) {
       f32x4 v = c[t][m];
       c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (kSplit) {
-        if ((q + j) % kWavesPerBlock != wave) continue;
+        if ((q + j) % kWaves != wave) continue;
         v = red[j & 1][0][q][lane];
 #pragma unroll
-        for (int p = 1; p < kWavesPerBlock; ++p) v += red[j & 1][p][q][lane];
+        for (int p = 1; p < kWaves; ++p) v += red[j & 1][p][q][lane];
       }
       const int n = (cc * TN + t) * 16 + 4 * kq;
       if (m * 16 + nl < r.count && cc * TN + t < ntiles && n < a.N)
@@ -604,14 +606,24 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
   const int room = kMode == kListed ? listed_room(a) : 0;
   const int ntiles = (a.N + 15) / 16;
   const int nC = (ntiles + 4 * TN - 1) / (4 * TN);
-  // consecutive items (eight row tiles by a few column blocks) on one XCD: what they
-  // share stays in its L2
-  const int total = nT * nC, per = (total + 7) / 8;
-  const int g = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per || g >= total) return;
-  const int grp = g / (8 * nC), within = g % (8 * nC);
-  const int gm = min(8, nT - grp * 8);
-  const int rt = grp * 8 + within % gm, cb = within / gm;
+  // Blocks go to the XCDs in turn, and what an XCD's blocks share stays in its L2.  Dense:
+  // an XCD has a run of items, eight row tiles by a few column blocks at a time.  Lists: an
+  // XCD has every eighth row tile with all its columns, so that all get their part of the
+  // large ones.
+  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+  int rt, cb;
+  if (kMode == kListed) {
+    rt = local / nC * 8 + xcd;
+    cb = local % nC;
+    if (rt >= nT) return;
+  } else {
+    const int total = nT * nC, per = (total + 7) / 8, g = xcd * per + local;
+    if (local >= per || g >= total) return;
+    const int grp = g / (8 * nC), within = g % (8 * nC);
+    const int gm = min(8, nT - grp * 8);
+    rt = grp * 8 + within % gm;
+    cb = within / gm;
+  }
   const RowTile<kMode> r(a, nullptr, rt, 16 * TM);
   // a list's tile may hold fewer rows: it runs as the smallest tile that holds them
   const int used = (r.count + 15) >> 4;
@@ -747,9 +759,11 @@ constexpr int kGroupThreads = 1024;
 __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_rows, int room,
                                                              int* __restrict__ groups) {
   constexpr int kE = TFD_ROUTE_MAX_EXPERTS, kKeep = 16;
-  __shared__ int count[kE], wave_rows[kE / kWave], wave_tiles[kE / kWave];
+  constexpr int kSizes = 8;              // of a tile, in sixteens
+  __shared__ int count[kE], wave_rows[kE / kWave], size_s[kSizes];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   if (tid < kE) count[tid] = 0;
+  if (tid < kSizes) size_s[tid] = 0;
   // a thread's first ids stay in registers for the second pass
   auto id_at = [&](int i) {
     if (i >= a.M) return -1;
@@ -770,45 +784,44 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
     if (id >= 0) atomicAdd(&count[id], 1);
   }
   __syncthreads();
-  // rows and tiles before each expert: a scan by waves, then over the waves
+  // an expert's rows spread evenly over its tiles, in sixteens: a tile costs by those.  The
+  // list has the largest tiles first: the last to start are then the shortest.
   const int mine = tid < a.E ? count[tid] : 0;
   const int tiles = (mine + tile_rows - 1) / tile_rows;
-  int rows_to = mine, tiles_to = tiles;
+  const int even = tiles ? ((mine + tiles - 1) / tiles + 15) / 16 : 0;
+  if (tiles) atomicAdd(&size_s[kSizes - even], tiles);
+  int rows_to = mine;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
-    const int r = __shfl_up(rows_to, d, kWave), t = __shfl_up(tiles_to, d, kWave);
+    const int r = __shfl_up(rows_to, d, kWave);
     rows_to += lane >= d ? r : 0;
-    tiles_to += lane >= d ? t : 0;
   }
-  if (tid < kE && lane == kWave - 1) {
-    wave_rows[wave] = rows_to;
-    wave_tiles[wave] = tiles_to;
+  if (tid < kE && lane == kWave - 1) wave_rows[wave] = rows_to;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < kE / kWave; ++v)
+    if (v < wave) rows_to += wave_rows[v];
+  if (tid == 0) {
+    int all = 0;
+#pragma unroll
+    for (int v = 0; v < kSizes; ++v) {
+      const int n = size_s[v];
+      size_s[v] = all;
+      all += n;
+    }
+    groups[0] = all;
+    groups[1] = room;
   }
   __syncthreads();
-  int all = 0;
-#pragma unroll
-  for (int v = 0; v < kE / kWave; ++v) {
-    if (v < wave) {
-      rows_to += wave_rows[v];
-      tiles_to += wave_tiles[v];
-    }
-    all += wave_tiles[v];
-  }
-  if (tid < a.E) {
-    // an expert's rows spread evenly over its tiles, in sixteens: a tile costs by those
-    const int f = rows_to - mine, t0 = tiles_to - tiles;
-    const int even = tiles ? ((mine + tiles - 1) / tiles + 15) / 16 * 16 : 0;
+  if (tiles) {
+    const int f = rows_to - mine, t0 = atomicAdd(&size_s[kSizes - even], tiles);
     for (int t = 0; t < tiles; ++t) {
       int* o = groups + 4 + (t0 + t) * 4;
       o[0] = tid;
-      o[1] = f + t * even;
-      o[2] = min(even, mine - t * even);
+      o[1] = f + t * even * 16;
+      o[2] = min(even * 16, mine - t * even * 16);
     }
     count[tid] = f;
-  }
-  if (tid == 0) {
-    groups[0] = all;
-    groups[1] = room;
   }
   __syncthreads();
   int* order = groups + 4 + room * 4;
@@ -872,7 +885,7 @@ template <int TM, int TN>
 void launch_listed(const Job& gu, const Job& down, int tiles, hipStream_t s) {
   auto grid = [&](const Job& j) {
     const int64_t nC = ((j.N + 15) / 16 + 4 * TN - 1) / (4 * TN);
-    return (int)(8 * ((tiles * nC + 7) / 8));
+    return (int)((tiles + 7) / 8 * 8 * nC);
   };
   k_mx4_many<kXBf16, TM, TN, kListed, kSwiglu><<<grid(gu), kBlock, 0, s>>>(gu, tiles);
   k_mx4_many<kXBf16, TM, TN, kListed, kF32><<<grid(down), kBlock, 0, s>>>(down, tiles);
@@ -1012,9 +1025,15 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
   if (fused_step(a.rows, a.k)) {
     down.out = a.out;
     down.ldo = a.ldo;
-    const int items = n * (a.I / 8);
-    k_mx4_few<kXBf16, 1, 1, 4, kHere, kSwiglu><<<min(items, 4 * cus), kBlock, 0, s>>>(gu);
-    k_mx4_down_mix<4><<<a.H / 16, kMixWaves * kWave, 0, s>>>(down, a.weights, a.rows, a.mult,
+    // column tiles of an item, which share its rows' loads: four where the items still go
+    // round (eight Granite rows: gate/up and down 48 us; one tile an item 58), else one (a
+    // Qwen3.5 row: 11.5 us; four 12.2)
+    const int wide = n * ((a.I / 8 + 3) / 4);
+    if (wide >= 4 * cus)
+      k_mx4_few<kXBf16, 1, 4, 2, kHere, kSwiglu><<<4 * cus, kBlock, 0, s>>>(gu);
+    else
+      k_mx4_few<kXBf16, 1, 1, 4, kHere, kSwiglu><<<min(n * (a.I / 8), 4 * cus), kBlock, 0, s>>>(gu);
+    k_mx4_down_mix<6><<<a.H / 16, kMixWaves * kWave, 0, s>>>(down, a.weights, a.rows, a.mult,
                                                             out_f32, a.accumulate);
     return launched("mx4_experts");
   }
@@ -1028,8 +1047,8 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
   const int tiles = a.experts + n / tile_rows;
   k_mx4_group<<<1, kGroupThreads, 0, s>>>(gu, tile_rows, wk.room, groups);
   if (tile_rows == 16) {
-    k_mx4_few<kXBf16, 1, 4, 2, kListed, kSwiglu, false><<<3 * cus, kBlock, 0, s>>>(gu);
-    k_mx4_few<kXBf16, 1, 4, 2, kListed, kF32, false><<<3 * cus, kBlock, 0, s>>>(down);
+    k_mx4_few<kXBf16, 1, 4, 2, kListed, kSwiglu, 4, false><<<3 * cus, kBlock, 0, s>>>(gu);
+    k_mx4_few<kXBf16, 1, 4, 2, kListed, kF32, 4, false><<<3 * cus, kBlock, 0, s>>>(down);
   } else if (tile_rows == 64) {
     launch_listed<4, 4>(gu, down, tiles, s);
   } else {

@@ -13,24 +13,67 @@ namespace {
 // 64-bit: biased scores of different experts lie as close as an f32 rounding often
 // enough to settle a choice by it.  Groups: a power of two of lanes per group walks
 // it for its two best choices; a group's rank is the number of groups before it.
-// Picks: k rounds of a wave's best (value, then lower index).
-// Bound: at one row the chain of k wave reductions, at thousands of rows the
-// 64-bit exponentials and reductions' VALU operations; the logits themselves are
-// read once.
+// Picks: k rounds of a wave's best (value, then lower index), on the choices as
+// integers in their order: the upper halves' maximum almost always leaves one lane,
+// the lower halves and the index settle the rest.  Reductions stay in registers
+// (DPP and lane swaps).
+// Bound: at one row the launch and the chain of k wave maxima, at thousands of rows the
+// 64-bit exponentials' and the rounds' VALU operations; the logits are read once.
 // ---------------------------------------------------------------------------
 constexpr double kNone = -__builtin_huge_val();
 
-__device__ __forceinline__ double xor_d(double v, int mask) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __shfl_xor((uint32_t)b, mask, kWave);
-  const uint32_t hi = __shfl_xor((uint32_t)(b >> 32), mask, kWave);
+__device__ __forceinline__ uint32_t lo32(double v) {
+  return (uint32_t)__builtin_bit_cast(uint64_t, v);
+}
+__device__ __forceinline__ uint32_t hi32(double v) {
+  return (uint32_t)(__builtin_bit_cast(uint64_t, v) >> 32);
+}
+__device__ __forceinline__ double both(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 __device__ __forceinline__ double from_lane_d(double v, int lane) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, lane);
-  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), lane);
-  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+  return both(__builtin_amdgcn_readlane(lo32(v), lane), __builtin_amdgcn_readlane(hi32(v), lane));
+}
+
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
+  v = max(v, dpp_u<kDppXor1>(v));
+  v = max(v, dpp_u<kDppXor2>(v));
+  v = max(v, dpp_u<kDppHalfMirror>(v));
+  v = max(v, dpp_u<kDppMirror>(v));
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+template <int kCtrl>
+__device__ __forceinline__ double dpp_d(double v) {
+  return both(dpp_u<kCtrl>(lo32(v)), dpp_u<kCtrl>(hi32(v)));
+}
+__device__ __forceinline__ double wave_sum_d(double v) {
+  v += dpp_d<kDppXor1>(v);
+  v += dpp_d<kDppXor2>(v);
+  v += dpp_d<kDppHalfMirror>(v);
+  v += dpp_d<kDppMirror>(v);
+  const auto l = __builtin_amdgcn_permlane16_swap(lo32(v), lo32(v), false, false);
+  const auto h = __builtin_amdgcn_permlane16_swap(hi32(v), hi32(v), false, false);
+  v = both(l[0], h[0]) + both(l[1], h[1]);
+  const auto m = __builtin_amdgcn_permlane32_swap(lo32(v), lo32(v), false, false);
+  const auto n = __builtin_amdgcn_permlane32_swap(hi32(v), hi32(v), false, false);
+  return both(m[0], n[0]) + both(m[1], n[1]);
+}
+__device__ __forceinline__ double xor_d(double v, int mask) {
+  return both(__shfl_xor(lo32(v), mask, kWave), __shfl_xor(hi32(v), mask, kWave));
+}
+
+// A double as an integer in the doubles' order (no NaN comes here; -0 before +0 is put
+// right by adding a zero).
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
+  return b >> 63 ? ~b : b | (1ull << 63);
 }
 
 __device__ __forceinline__ float logit(const TfdRouteArgs& a, int64_t at) {
@@ -48,17 +91,16 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
   if (row >= a.rows) return;
   const int E = a.experts;
   double l[kPer], s[kPer], c[kPer];
-  double m = kNone;
+  float top = -__builtin_huge_valf();
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const int e = lane + kWave * j;
     const float v = e < E ? logit(a, (int64_t)row * a.ldl + e) : -__builtin_huge_valf();
     l[j] = v != v ? kNone : (double)v;               // NaN: as masked
-    m = fmax(m, l[j]);
+    top = fmaxf(top, (float)l[j]);
   }
   if (a.score == TFD_SCORE_SOFTMAX) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) m = fmax(m, xor_d(m, d));
+    const double m = (double)wave_max(top);
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -66,8 +108,7 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
       s[j] = l[j] == kNone ? 0.0 : l[j] == m ? 1.0 : exp(l[j] - m);
       sum += s[j];
     }
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) sum += xor_d(sum, d);
+    sum = wave_sum_d(sum);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) s[j] = sum > 0.0 ? s[j] / sum : 0.0;
   } else {
@@ -115,41 +156,51 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
       if (e < E && !((kept >> (e / per * L)) & 1)) c[j] = kNone;
     }
   }
+  uint64_t key[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) key[j] = ordered(c[j]);
+  const uint64_t none = ordered(kNone);
   double my_s = 0.0, total = 0.0;
   int my_id = -1;
   for (int r = 0; r < a.k; ++r) {
-    // this lane's best, then the wave's: the larger choice, equal ones the lower id
-    double bc = c[0], bs = s[0];
-    int bi = lane;
+    // this lane's best (ids grow with j: a tie keeps the first), then the wave's
+    uint64_t best = key[0];
+    double bs = s[0];
+    int bj = 0;
 #pragma unroll
     for (int j = 1; j < kPer; ++j)
-      if (c[j] > bc) {
-        bc = c[j];
+      if (key[j] > best) {
+        best = key[j];
         bs = s[j];
-        bi = lane + kWave * j;
+        bj = j;
       }
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const double oc = xor_d(bc, d);
-      const int oi = __shfl_xor(bi, d, kWave);
-      if (oc > bc || (oc == bc && oi < bi)) {
-        bc = oc;
-        bi = oi;
+    const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
+    const uint32_t mh = wave_max_u(hi);
+    uint64_t who = __ballot(hi == mh);
+    if (__popcll(who) > 1) {
+      const uint32_t ml = wave_max_u(hi == mh ? lo : 0u);
+      who = __ballot(hi == mh && lo == ml);
+      if (__popcll(who) > 1) {
+        // the same value: the lowest id (as the largest of complements)
+        const bool in = (who >> lane) & 1;
+        const uint32_t id = ~(uint32_t)(lane + kWave * bj);
+        const uint32_t mi = wave_max_u(in ? id : 0u);
+        who = __ballot(in && id == mi);
       }
     }
-    if (bc == kNone) break;                          // nothing left that can be chosen
-    const int owner = bi & (kWave - 1);
+    const int owner = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(who));
+    if (__builtin_amdgcn_readlane(lo, owner) == (uint32_t)none &&
+        __builtin_amdgcn_readlane(hi, owner) == (uint32_t)(none >> 32))
+      break;                                         // nothing left that can be chosen
+    const double ps = from_lane_d(bs, owner);
+    const int id = owner + kWave * __builtin_amdgcn_readlane(bj, owner);
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (bi == lane + kWave * j) {
-        bs = s[j];
-        c[j] = kNone;
-      }
-    bs = from_lane_d(bs, __builtin_amdgcn_readfirstlane(owner));
-    total += bs;
+      if (id == lane + kWave * j) key[j] = none;
+    total += ps;
     if (lane == r) {
-      my_s = bs;
-      my_id = bi;
+      my_s = ps;
+      my_id = id;
     }
   }
   if (lane < a.k + a.shared) {

@@ -13,7 +13,6 @@ several streams) and computes no gradients.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
 
 import torch
 
@@ -26,28 +25,20 @@ TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16,
          torch.float16: _lib.TYPE_F16}
 
 
-def stream_on(device) -> int:
-    """The device's current stream, as the C entries take it."""
-    return torch.cuda.current_stream(device).cuda_stream
+_current_device = torch.cuda.current_device
+# the handle that torch.cuda.current_stream(device).cuda_stream gives, without the object
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-class on_device:
-    """Makes *device* the current one where it is not (a launch belongs to the current
-    device, a stream to its own)."""
-
-    __slots__ = ("index", "guard")
-
-    def __init__(self, device):
-        self.index, self.guard = device.index, None
-
-    def __enter__(self):
-        if self.index is not None and self.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def launch(device, entry, *args) -> None:
+    """Calls a C entry on *device*'s current stream, with the device the current one (a
+    launch belongs to the current device, a stream to its own)."""
+    i = device.index
+    if i == _current_device():
+        entry(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            entry(*args, _raw_stream(i))
 
 
 def check_input(x, what: str, dtypes) -> None:
@@ -70,8 +61,12 @@ def check_device(device, *others) -> None:
 
 
 def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
-    """*x* as [rows][K] with unit stride along K, rows that do not overlap and, with
-    *align*, rows that start at multiples of that many bytes: a view where it is one."""
+    """*x* as rows of its last dimension with unit stride, rows that do not overlap and,
+    with *align*, that start at multiples of that many bytes: *x* itself where it is that
+    (contiguous in any number of dimensions), else a two-dimensional view or a copy."""
+    if x.is_contiguous() and not x.data_ptr() % align and (
+            not x.shape[-1] * x.element_size() % align or x.numel() == x.shape[-1]):
+        return x
     K = x.shape[-1]
     x = x.reshape(-1, K)
     size = x.element_size()
@@ -82,18 +77,16 @@ def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
 
 
 def row_stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    return x.stride(-2) if x.dim() > 1 and x.shape[-2] > 1 else x.shape[-1]
 
 
-@dataclass(frozen=True)
 class Mx4:
     """Codes uint8 ``[..., K / 2]`` and scales uint8 ``[..., K / 32]`` of one tensor."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("codes", "scales")
 
-    def __post_init__(self):
-        c, s = self.codes, self.scales
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        c, s = codes, scales
         if c.dtype != U8 or s.dtype != U8:
             raise ValueError(f"mx4 codes and scales are uint8, got {c.dtype} and {s.dtype}")
         if c.dim() < 1 or c.shape[:-1] != s.shape[:-1] or c.shape[-1] != 16 * s.shape[-1] or \
@@ -102,6 +95,17 @@ class Mx4:
                              "[..., K / 2] and [..., K / 32] of one tensor")
         if c.device != s.device:
             raise ValueError(f"mx4 codes on {c.device}, scales on {s.device}")
+        self.codes, self.scales = c, s
+
+    @classmethod
+    def _of(cls, codes, scales) -> "Mx4":
+        """Of tensors made for each other."""
+        t = cls.__new__(cls)
+        t.codes, t.scales = codes, scales
+        return t
+
+    def __repr__(self) -> str:
+        return f"Mx4(shape={self.shape}, device={self.device})"
 
     @property
     def shape(self) -> tuple[int, ...]:
@@ -125,12 +129,11 @@ class Mx4:
                              f"{', '.join(str(d) for d in TYPES)}")
         check_device(self.device)
         codes, scales = rows_of(self.codes, 4), rows_of(self.scales)
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with on_device(self.device):
-            lib().tfd_mx4_dequantise(ptr(codes), row_stride(codes), ptr(scales),
-                                     row_stride(scales), codes.shape[0], self.shape[-1],
-                                     ptr(out), self.shape[-1], TYPES[dtype],
-                                     stream_on(self.device))
+        device, shape = self.codes.device, self.shape
+        out = torch.empty(shape, dtype=dtype, device=device)
+        K = shape[-1]
+        launch(device, lib().tfd_mx4_dequantise, ptr(codes), row_stride(codes), ptr(scales),
+               row_stride(scales), out.numel() // K, K, ptr(out), K, TYPES[dtype])
         return out
 
 
@@ -143,14 +146,13 @@ def quantise(x: torch.Tensor) -> Mx4:
         raise ValueError(f"quantise: the last dimension must be a multiple of {BLOCK}, got "
                          f"{tuple(x.shape)}")
     check_device(x.device)
-    K, lead = x.shape[-1], x.shape[:-1]
-    codes = torch.empty(*lead, K // 2, dtype=U8, device=x.device)
-    scales = torch.empty(*lead, K // BLOCK, dtype=U8, device=x.device)
+    K, lead, device = x.shape[-1], x.shape[:-1], x.device
+    codes = torch.empty((*lead, K // 2), dtype=U8, device=device)
+    scales = torch.empty((*lead, K // BLOCK), dtype=U8, device=device)
     rows = rows_of(x)
-    with on_device(x.device):
-        lib().tfd_mx4_quantise(ptr(rows), row_stride(rows), TYPES[x.dtype], rows.shape[0], K,
-                               ptr(codes), K // 2, ptr(scales), K // BLOCK, stream_on(x.device))
-    return Mx4(codes, scales)
+    launch(device, lib().tfd_mx4_quantise, ptr(rows), row_stride(rows), TYPES[x.dtype],
+           x.numel() // K, K, ptr(codes), K // 2, ptr(scales), K // BLOCK)
+    return Mx4._of(codes, scales)
 
 
 def _pack(first: Mx4, second: Mx4 | None, what: str) -> torch.Tensor:
@@ -167,15 +169,15 @@ def _pack(first: Mx4, second: Mx4 | None, what: str) -> torch.Tensor:
     if rows == 0:
         raise ValueError(f"{what}: no rows in weights of shape {first.shape}")
     L = lib()
-    with on_device(first.device):
-        packed = torch.empty(L.tfd_mx4_packed_bytes(rows * (len(parts) // 2), K), dtype=U8,
-                             device=first.device)
-        L.tfd_mx4_pack(ptr(parts[0]), ptr(parts[1]),
-                       *((ptr(parts[2]), ptr(parts[3])) if second is not None else (None, None)),
-                       rows, K, ptr(packed), stream_on(first.device))
+    packed = torch.empty(L.tfd_mx4_packed_bytes(rows * (len(parts) // 2), K), dtype=U8,
+                         device=first.device)
+    parts += [None] * (4 - len(parts))
+    launch(first.device, L.tfd_mx4_pack, *(ptr(t) for t in parts), rows, K, ptr(packed))
     return packed
 
 
+BF16, INT32, FLOAT32 = (torch.bfloat16,), (torch.int32,), (torch.float32,)
+MAX_ROWS = 1 << 30
 OUT_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
 
 
@@ -204,7 +206,7 @@ class Linear:
         if isinstance(x, Mx4):
             lead, K, values = x.shape[:-1], x.shape[-1], x.codes
         else:
-            check_input(x, "Linear", (torch.bfloat16,))
+            check_input(x, "Linear", BF16)
             if x.dim() < 1:
                 raise ValueError("Linear: the input has no dimensions")
             lead, K, values = x.shape[:-1], x.shape[-1], x
@@ -216,12 +218,13 @@ class Linear:
         if isinstance(x, Mx4):
             scales = rows_of(x.scales)
             ldxs = row_stride(scales)
-        out = torch.empty(*lead, self.N, dtype=dtype, device=self.device)
+        out = torch.empty((*lead, self.N), dtype=dtype, device=self.device)
+        rows = out.numel() // self.N
+        if rows > MAX_ROWS:
+            raise ValueError(f"Linear: up to {MAX_ROWS} rows a call, got {rows}")
         a = _lib.TfdMx4GemmArgs(ptr(values), row_stride(values), ptr(scales), ldxs,
-                                ptr(self.packed), values.shape[0], K, self.N, ptr(out), self.N,
-                                kind)
-        with on_device(self.device):
-            lib().tfd_mx4_gemm(ctypes.addressof(a), stream_on(self.device))
+                                ptr(self.packed), rows, K, self.N, ptr(out), self.N, kind)
+        launch(self.device, lib().tfd_mx4_gemm, ctypes.addressof(a))
         return out
 
 
@@ -254,9 +257,9 @@ class Experts:
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
                  dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         kind = _out_type(dtype, "Experts")
-        check_input(x, "x", (torch.bfloat16,))
-        check_input(ids, "ids", (torch.int32,))
-        check_input(weights, "weights", (torch.float32,))
+        check_input(x, "x", BF16)
+        check_input(ids, "ids", INT32)
+        check_input(weights, "weights", FLOAT32)
         if x.dim() != 2 or x.shape[1] != self.H:
             raise ValueError(f"Experts: x must be [rows, {self.H}], got {tuple(x.shape)}")
         rows = x.shape[0]
@@ -271,18 +274,17 @@ class Experts:
             raise ValueError(f"Experts: up to 65535 rows a call, got {rows}")
         x = rows_of(x, 16)
         ids, weights = ids.contiguous(), weights.contiguous()
-        out = torch.empty(rows, self.H, dtype=dtype, device=self.device)
-        L = lib()
-        need = L.tfd_mx4_experts_work_bytes(rows, ids.shape[1], self.E, self.H, self.I)
-        with on_device(self.device):
-            # of the stream that uses it, like the output: calls on several streams and
-            # captured graphs share nothing
-            work = torch.empty(need, dtype=U8, device=self.device)
-            a = _lib.TfdMx4ExpertsArgs(
-                ptr(x), row_stride(x), ptr(ids), ptr(weights), ids.shape[1], ptr(self.w_gu),
-                ptr(self.w_down), rows, ids.shape[1], self.E, self.H, self.I, ptr(out), self.H,
-                kind, 0, 1.0, ptr(work), need, ptr(self.err))
-            L.tfd_mx4_experts(ctypes.addressof(a), stream_on(self.device))
+        k, device, L = ids.shape[1], self.device, lib()
+        out = torch.empty((rows, self.H), dtype=dtype, device=device)
+        need = L.tfd_mx4_experts_work_bytes(rows, k, self.E, self.H, self.I)
+        # of the stream that uses it, like the output: calls on several streams and captured
+        # graphs share nothing
+        work = torch.empty(need, dtype=U8, device=device)
+        a = _lib.TfdMx4ExpertsArgs(
+            ptr(x), row_stride(x), ptr(ids), ptr(weights), k, ptr(self.w_gu), ptr(self.w_down),
+            rows, k, self.E, self.H, self.I, ptr(out), self.H, kind, 0, 1.0, ptr(work), need,
+            ptr(self.err))
+        launch(device, L.tfd_mx4_experts, ctypes.addressof(a))
         return out
 
     def check_errors(self) -> None:

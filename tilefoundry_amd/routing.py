@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import lib, ptr
-from .mx4 import TYPES, check_device, check_input, on_device, row_stride, rows_of, stream_on
+from .mx4 import FLOAT32, TYPES, check_device, check_input, launch, row_stride, rows_of
 
 SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
@@ -73,19 +73,19 @@ class Routing:
             raise ValueError(f"top_k {self.top_k} of {self.kept_groups} groups of "
                              f"{experts // self.groups} experts")
         if bias is not None:
-            check_input(bias, "bias", (torch.float32,))
+            check_input(bias, "bias", FLOAT32)
             if bias.shape != (experts,):
                 raise ValueError(f"bias must be [{experts}], got {tuple(bias.shape)}")
             bias = bias.contiguous()
         check_device(logits.device, bias)
         logits = rows_of(logits)
         n = self.top_k + self.shared
-        weights = torch.empty(rows, n, dtype=torch.float32, device=logits.device)
-        ids = torch.empty(rows, n, dtype=torch.int32, device=logits.device)
+        device = logits.device
+        weights = torch.empty((rows, n), dtype=torch.float32, device=device)
+        ids = torch.empty((rows, n), dtype=torch.int32, device=device)
         a = _lib.TfdRouteArgs(
             ptr(logits), row_stride(logits), TYPES[logits.dtype], ptr(bias), rows, experts,
             self.top_k, SCORES[self.score], self.groups, self.kept_groups, self.group_top,
             self.shared, int(self.renormalise), self.scale, ptr(weights), ptr(ids), n)
-        with on_device(logits.device):
-            lib().tfd_route_experts(ctypes.addressof(a), stream_on(logits.device))
+        launch(device, lib().tfd_route_experts, ctypes.addressof(a))
         return weights, ids
