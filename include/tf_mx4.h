@@ -103,7 +103,8 @@ int tfd_route_experts(const TfdRouteArgs* args, void* stream);
 
 /* The routed experts over mx4 weights, given the routing: for row r
  *   y = mult * sum over places j of weights[r][j] * Wdown_e (silu(Wgate_e x_r) * (Wup_e x_r)),
- *   e = ids[r][j]; the hidden values rounded to bf16, f32 otherwise;
+ *   e = ids[r][j]; f32 sums; the hidden values (the down product's operands) rounded to bf16,
+ *   or in calls of up to 16 rows and 128 places kept as sums of two bf16 (2^-17);
  * out = y, or with accumulate out + y (a residual stream), rounded once to out_type.  Entries
  * are grouped by expert, so a picked expert's weights are read once for all its rows (many
  * rows: once for each 16 to 128).  The 4-bit counterpart of tfd_moe_experts* / tfd_panel_moe;

@@ -21,7 +21,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 enum XKind { kXBf16 = 0, kXMx4 = 1 };
 enum Mode { kDense = 0, kHere = 1, kListed = 2 };   // rows: all; grouped in the block; before
-enum Epi { kBf16 = 0, kF32 = 1, kSwiglu = 2 };
+enum Epi { kBf16 = 0, kF32 = 1, kSwiglu = 2, kSwigluTwo = 3 };
 
 constexpr uint32_t kRange = 0x7fffffffu;   // of a row tile's descriptor: offsets up to 2 GiB
 constexpr int kHereMax = 128;    // entries that a block groups itself
@@ -39,6 +39,7 @@ struct Job {
   void* out;
   int64_t ldo;
   int vec;                       // four outputs of a row may go in one store
+  int64_t second;                // kSwigluTwo: bytes from a hidden row to its second part
   // experts: entry i is place i % k of row i / k; its row of x is i / div
   const int32_t* ids;
   int ldi, k, div, E;
@@ -73,10 +74,10 @@ __device__ __forceinline__ uint32_t ld1(const uint8_t* p) {
 }
 
 // ---------------------------------------------------------------------------
-// Entries (row, place) grouped by expert in tiles of up to 16, by the block that
-// uses them: up to kHereMax entries, each compared with those before it, which
-// costs less than a launch of its own.  Ids outside the experts make no entry; any
-// but -1 raises the error bit.
+// Entries (row, place) grouped by expert in tiles of kWidth, by the block that uses
+// them: up to kHereMax entries, each compared with those before it, which costs less
+// than a launch of its own.  Ids outside the experts make no entry; any but -1 raises
+// the error bit.
 // ---------------------------------------------------------------------------
 struct Tiles {
   int n, first_wave;
@@ -86,6 +87,7 @@ struct Tiles {
   uint8_t entry[kHereMax][16];
 };
 
+template <int kWidth>              // entries of a tile at most
 __device__ void group_here(const Job& a, Tiles& s) {
   const int i = threadIdx.x, lane = i & (kWave - 1);
   int id = -1;
@@ -108,7 +110,7 @@ __device__ void group_here(const Job& a, Tiles& s) {
         ++rank;
         first = j;
       }
-  const bool leads = id >= 0 && (rank & 15) == 0;
+  const bool leads = id >= 0 && rank % kWidth == 0;
   const uint64_t before = __ballot(leads);
   if (i < kHereMax) s.rank[i] = rank;
   if (i == 0) s.first_wave = __popcll(before);
@@ -126,11 +128,11 @@ __device__ void group_here(const Job& a, Tiles& s) {
   __syncthreads();
   if (id >= 0) {
     int lead = first;
-    if (rank >= 16)
-      for (lead = first; s.id[lead] != id || s.rank[lead] != (rank & ~15);) ++lead;
+    if (rank >= kWidth)
+      for (lead = first; s.id[lead] != id || s.rank[lead] != rank - rank % kWidth;) ++lead;
     t = s.tile[lead];
-    s.entry[t][rank & 15] = (uint8_t)i;
-    atomicMax(&s.count[t], (rank & 15) + 1);
+    s.entry[t][rank % kWidth] = (uint8_t)i;
+    atomicMax(&s.count[t], rank % kWidth + 1);
   }
   __syncthreads();
 }
@@ -170,10 +172,20 @@ __device__ __forceinline__ int listed_room(const Job& a) { return a.groups[1]; }
 
 template <int kEpi>
 __device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v) {
-  if (kEpi == kSwiglu) {
-    // (gate, up) pairs: the hidden value is the next product's operand, hence bf16
+  if (kEpi == kSwiglu || kEpi == kSwigluTwo) {
+    // (gate, up) pairs.  The hidden value is the next product's operand, hence bf16, or in a
+    // step of few rows the sum of two bf16 (2^-17): its matrix tiles have rows to spare, so
+    // the only rounding to bf16 that counts is the output's.  An infinity has no second part.
     const float h0 = silu_f(v.x) * v.y, h1 = silu_f(v.z) * v.w;
-    *reinterpret_cast<uint32_t*>((bf16*)a.out + (int64_t)row * a.ldo + n / 2) = pack2(h0, h1);
+    bf16* o = (bf16*)a.out + (int64_t)row * a.ldo + n / 2;
+    const uint32_t first = pack2(h0, h1);
+    *reinterpret_cast<uint32_t*>(o) = first;
+    if (kEpi == kSwigluTwo) {
+      const float f0 = bf_lo(first), f1 = bf_hi(first);
+      const float r0 = fabsf(f0) < __builtin_huge_valf() ? h0 - f0 : 0.f;
+      const float r1 = fabsf(f1) < __builtin_huge_valf() ? h1 - f1 : 0.f;
+      *reinterpret_cast<uint32_t*>((uint8_t*)o + a.second) = pack2(r0, r1);
+    }
     return;
   }
   if (kEpi == kF32) {
@@ -217,7 +229,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   const int nl = lane & 15, kq = lane >> 4;
   int nT, room = 0;
   if constexpr (kMode == kHere) {
-    group_here(a, group_s);
+    group_here<16>(a, group_s);
     tiles = &group_s;
     nT = group_s.n;
   } else if (kMode == kListed) {
@@ -261,7 +273,8 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   };
   u32x4 w[D][TN];
   uint32_t ws[D][TN];
-  u32x4 x[D][MT][kX == kXMx4 ? 1 : 4];
+  constexpr int kXr = kX == kXMx4 ? 1 : 4;      // 16-byte registers of a row's step
+  u32x4 x[D][MT][kXr];
   uint32_t xs[D][MT];
   Item nx = decode(0);
   int jn = 0, sn = 0;
@@ -283,7 +296,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
         xs[u][m] = ld1(nx.xs[m] + (kk >> 5));
       } else {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) x[u][m][s] = ld16(nx.x[m] + 2 * kk + 16 * s);
+        for (int s = 0; s < kXr; ++s) x[u][m][s] = ld16(nx.x[m] + 2 * kk + 16 * s);
       }
     }
     if (++sn == ns && jn + 1 < mine) {
@@ -304,7 +317,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
 #pragma unroll
-          for (int s = 0; s < (kX == kXMx4 ? 1 : 4); ++s) x[u][m][s] = u32x4{0u, 0u, 0u, 0u};
+          for (int s = 0; s < kXr; ++s) x[u][m][s] = u32x4{0u, 0u, 0u, 0u};
           xs[u][m] = 127;
         }
       }
@@ -639,11 +652,16 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
 // ---------------------------------------------------------------------------
 // Down projection and mix of a step of few rows, in one launch: a block per column
 // tile holds every entry's 16 outputs, so the weighted sum needs no second pass over
-// memory.  A wave takes (row tile, part of K) units in turn, its next D steps in flight
-// across them; each unit's sums have a place of their own in LDS, and a row's places
-// are added in their order: the result does not depend on which wave ran when.
+// memory.  Tiles hold eight entries, whose second halves of the hidden values are the
+// matrix tile's other eight rows: both products for the price of one.  A wave takes (row
+// tile, part of K) units in turn, its next D steps in flight across them; each unit's sums
+// have a place of their own in LDS, and a row's places are added in their order: the result
+// does not depend on which wave ran when.
+// Bound: the weights' stream; eight Granite rows 51 us for both launches (about 250 MB, 4.9
+// TB/s), D 3 to 8 within 2%.
 // ---------------------------------------------------------------------------
 constexpr int kMixWaves = 8;
+constexpr int kDppRotate8 = 0x128;   // lane i <- lane (i + 8) % 16 of its sixteen
 constexpr int kMixParts = 256;   // (entry, part of K) places, 16 columns each
 
 template <int D>
@@ -655,7 +673,7 @@ __global__ __launch_bounds__(kMixWaves * kWave) void k_mx4_down_mix(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int nl = lane & 15, kq = lane >> 4;
   const int ct = blockIdx.x, ntiles = a.N / 16;
-  group_here(a, s);
+  group_here<8>(a, s);
   const int nT = s.n;
   // with fewer tiles than waves a tile's K goes to several waves, as far as every entry's
   // parts (empty places count) have room
@@ -676,7 +694,7 @@ __global__ __launch_bounds__(kMixWaves * kWave) void k_mx4_down_mix(
     const int u = wave + j * kMixWaves, rt = u / parts;
     k0 = u % parts * ns;
     tile = (int64_t)s.expert[rt] * ntiles + ct;
-    xp = a.x + (int64_t)s.entry[rt][min(nl, s.count[rt] - 1)] * a.ldx;
+    xp = a.x + (int64_t)s.entry[rt][min(nl & 7, s.count[rt] - 1)] * a.ldx + (nl & 8 ? a.second : 0);
   };
   auto issue = [&](int u) {
     const int b = min(k0 + sn, a.kb - 1);
@@ -707,6 +725,9 @@ __global__ __launch_bounds__(kMixWaves * kWave) void k_mx4_down_mix(
     if (++sc < ns) return;
     sc = 0;
     ++jc;
+    // an entry's two halves of the hidden values are columns nl and nl + 8
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] += dpp_f<kDppRotate8>(c[i]);
     if (nl < s.count[rt])
       *reinterpret_cast<f32x4*>(&part[s.entry[rt][nl] * parts + p][4 * kq]) = c;
     c = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -864,21 +885,27 @@ __global__ __launch_bounds__(kBlock) void k_mx4_mix(const float* __restrict__ d,
   }
 }
 
-bool fused_step(int rows, int k) { return rows <= kHereRows && rows * k <= kHereMax; }
-
-struct Work {
-  int64_t hidden, d, groups, bytes;
-  int room;
+// How a call runs, and what of `work` it uses.
+struct Plan {
+  bool fused;                    // grouped in the blocks, the mix in the down launch, hidden
+                                 // values as two bf16
+  int tile_rows, room;
+  int64_t second, d, groups, bytes;
 };
-Work experts_work(int rows, int k, int E, int H, int I) {
+Plan experts_plan(int rows, int k, int E, int H, int I) {
   const int64_t n = (int64_t)rows * k;
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-  Work w = {};
-  w.room = (int)(E + n / 16);
-  w.d = up(n * I * 2);
-  w.groups = w.d + (fused_step(rows, k) ? 0 : up(n * H * 4));
-  w.bytes = w.groups + (fused_step(rows, k) ? 0 : up((4 + 4 * (int64_t)w.room + n) * 4));
-  return w;
+  Plan p = {};
+  p.fused = rows <= kHereRows && n <= kHereMax;
+  // rows an expert has if all are picked alike; a tile holds that and a bit
+  const int64_t mean = n / E;
+  p.tile_rows = mean <= 16 ? 16 : mean <= 48 ? 64 : 128;
+  p.room = (int)(E + n / p.tile_rows);
+  p.second = up(n * I * 2);
+  p.d = p.second * (p.fused ? 2 : 1);
+  p.groups = p.d + (p.fused ? 0 : up(n * H * 4));
+  p.bytes = p.groups + (p.fused ? 0 : up((4 + 4 * (int64_t)p.room + n) * 4));
+  return p;
 }
 
 template <int TM, int TN>
@@ -959,7 +986,7 @@ extern "C" {
 
 int64_t tfd_mx4_experts_work_bytes(int rows, int k, int experts, int H, int I) {
   if (rows <= 0 || k <= 0 || experts <= 0 || H <= 0 || I <= 0) return 0;
-  return experts_work(rows, k, experts, H, I).bytes;
+  return experts_plan(rows, k, experts, H, I).bytes;
 }
 
 int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
@@ -986,10 +1013,10 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
       (uintptr_t)a.out % (a.out_type == TFD_TYPE_F32 ? 4 : 2))
     return fail(kBadArg, "mx4_experts: ldx=%lld ld=%d ldo=%lld or an alignment",
                 (long long)a.ldx, a.ld, (long long)a.ldo);
-  const Work wk = experts_work(a.rows, a.k, a.experts, a.H, a.I);
-  if (a.work_bytes < wk.bytes)
+  const Plan plan = experts_plan(a.rows, a.k, a.experts, a.H, a.I);
+  if (a.work_bytes < plan.bytes)
     return fail(kBadArg, "mx4_experts: work of %lld bytes, %lld needed", (long long)a.work_bytes,
-                (long long)wk.bytes);
+                (long long)plan.bytes);
   uint8_t* work = (uint8_t*)a.work;
   const int n = a.rows * a.k;
   Job gu = {};
@@ -1001,16 +1028,17 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
   gu.kb = mx4_blocks(a.H);
   gu.N = 2 * a.I;
   gu.M = n;
-  gu.out = work + wk.hidden;
+  gu.out = work;
   gu.ldo = a.I;
   gu.vec = 1;
+  gu.second = plan.second;
   gu.ids = a.ids;
   gu.ldi = a.ld;
   gu.k = gu.div = a.k;
   gu.E = a.experts;
   gu.err = a.err;
   Job down = gu;
-  down.x = work + wk.hidden;
+  down.x = work;
   down.ldx = 2 * (int64_t)a.I;
   down.w = (const uint8_t*)a.w_down;
   down.w_tiles = (int64_t)a.experts * (a.H / 16);
@@ -1022,7 +1050,7 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   const int cus = compute_units();
   const int out_f32 = a.out_type == TFD_TYPE_F32;
-  if (fused_step(a.rows, a.k)) {
+  if (plan.fused) {
     down.out = a.out;
     down.ldo = a.ldo;
     // column tiles of an item, which share its rows' loads: four where the items still go
@@ -1030,22 +1058,19 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
     // Qwen3.5 row: 11.5 us; four 12.2)
     const int wide = n * ((a.I / 8 + 3) / 4);
     if (wide >= 4 * cus)
-      k_mx4_few<kXBf16, 1, 4, 2, kHere, kSwiglu><<<4 * cus, kBlock, 0, s>>>(gu);
+      k_mx4_few<kXBf16, 1, 4, 2, kHere, kSwigluTwo><<<4 * cus, kBlock, 0, s>>>(gu);
     else
-      k_mx4_few<kXBf16, 1, 1, 4, kHere, kSwiglu><<<min(n * (a.I / 8), 4 * cus), kBlock, 0, s>>>(gu);
-    k_mx4_down_mix<6><<<a.H / 16, kMixWaves * kWave, 0, s>>>(down, a.weights, a.rows, a.mult,
+      k_mx4_few<kXBf16, 1, 1, 4, kHere, kSwigluTwo><<<min(n * (a.I / 8), 4 * cus), kBlock, 0, s>>>(gu);
+    k_mx4_down_mix<4><<<a.H / 16, kMixWaves * kWave, 0, s>>>(down, a.weights, a.rows, a.mult,
                                                             out_f32, a.accumulate);
     return launched("mx4_experts");
   }
-  down.out = work + wk.d;
+  down.out = work + plan.d;
   down.ldo = a.H;
-  int* groups = (int*)(work + wk.groups);
+  int* groups = (int*)(work + plan.groups);
   gu.groups = down.groups = groups;
-  // rows an expert has if all are picked alike; a tile is that and a bit
-  const int mean = n / a.experts;
-  const int tile_rows = mean <= 16 ? 16 : mean <= 48 ? 64 : 128;
-  const int tiles = a.experts + n / tile_rows;
-  k_mx4_group<<<1, kGroupThreads, 0, s>>>(gu, tile_rows, wk.room, groups);
+  const int tile_rows = plan.tile_rows, tiles = a.experts + n / tile_rows;
+  k_mx4_group<<<1, kGroupThreads, 0, s>>>(gu, tile_rows, plan.room, groups);
   if (tile_rows == 16) {
     k_mx4_few<kXBf16, 1, 4, 2, kListed, kSwiglu, 4, false><<<3 * cus, kBlock, 0, s>>>(gu);
     k_mx4_few<kXBf16, 1, 4, 2, kListed, kF32, 4, false><<<3 * cus, kBlock, 0, s>>>(down);
@@ -1055,7 +1080,7 @@ int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
     launch_listed<8, 4>(gu, down, tiles, s);
   }
   k_mx4_mix<<<dim3((a.H / 4 + kBlock - 1) / kBlock, a.rows), kBlock, 0, s>>>(
-      (const float*)(work + wk.d), a.ids, a.weights, a.ld, a.k, a.experts, a.H, a.mult, out_f32,
+      (const float*)(work + plan.d), a.ids, a.weights, a.ld, a.k, a.experts, a.H, a.mult, out_f32,
       a.accumulate, a.out, a.ldo);
   return launched("mx4_experts");
 }

@@ -235,8 +235,9 @@ class Experts:
 
         y = sum over the row's places of weight * down_e(silu(gate_e x) * (up_e x)).
 
-    The hidden values are rounded to bf16 (they are the down product's operands);
-    everything else is f32, the output rounded once to bf16 or f32.  Id -1 is an empty
+    Sums are f32, the output rounded once to bf16 or f32.  The hidden values are the down
+    product's operands: rounded to bf16, or in calls of up to 16 rows and 128 places kept as
+    sums of two bf16 (2^-17).  Id -1 is an empty
     place; any other id outside the experts is skipped and raises ``check_errors``.  An
     expert may come twice in a row."""
 
