@@ -191,9 +191,12 @@ def build(args, model: str, device: str):
             w = synthetic_weights(cfg, seed=args.seed, device=device)
         engine_cls = GraniteEngine
 
+    more = {"experts": "mx4"} if args.experts == "mx4" else {}
+
     def make(prompt_len):
         return engine_cls(cfg, w, rows=1, device=device,
-                          max_steps=prompt_len + args.max_new_tokens + 8, sampling=sampling)
+                          max_steps=prompt_len + args.max_new_tokens + 8, sampling=sampling,
+                          **more)
 
     def run(eng, prompt):
         t0 = perf_counter()
@@ -227,6 +230,9 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--prefill", action="store_true",
                     help="Qwen3: fill the prompt's cache in batched passes (up to 4,096 "
                          "positions each) instead of walking it one decode step per token")
+    ap.add_argument("--experts", choices=("fp8", "mx4"), default=None,
+                    help="Granite: the experts' weights in 8 bits (default) or quantised to "
+                         "microscaled 4 bits at load")
     ap.add_argument("--sample", action="store_true",
                     help="draw tokens instead of taking the largest logit (the model's "
                          "reference defaults unless the flags below say otherwise)")
@@ -245,6 +251,8 @@ def main(argv: list[str] | None = None) -> int:
     if args.synthetic in ("c4", "c5"):
         args.model = args.model or {"c4": "qwen3_5", "c5": "granite"}[args.synthetic]
     model = model_of(args)
+    if args.experts is not None and model != "granite":
+        raise SystemExit("--experts is for granite")
 
     tokenizer = None
     if args.ckpt is not None and args.prompt is not None:

@@ -276,3 +276,11 @@ def test_structs_match_c_layout(tmp_path):
     for name in ("TYPE_F32", "TYPE_BF16", "TYPE_F16", "SCORE_SOFTMAX", "SCORE_SIGMOID",
                  "ROUTE_MAX_EXPERTS"):
         assert f"#define TFD_{name} {getattr(_lib, name)}\n" in text
+
+
+def test_run_takes_4_bit_experts_for_granite_alone():
+    import run
+
+    for synthetic in ("c1", "c2", "c4"):
+        with pytest.raises(SystemExit, match="granite"):
+            run.main(["--synthetic", synthetic, "--random-prompt", "4", "--experts", "mx4"])

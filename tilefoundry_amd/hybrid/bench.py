@@ -446,19 +446,21 @@ def bench_c4_step(rows: int, steps: int, prompt: int = 32, small: bool | None = 
     return out
 
 
-def bench_c5_step(rows: int, steps: int, ctx: int = 8192, context: str = "drawn") -> dict:
+def bench_c5_step(rows: int, steps: int, ctx: int = 8192, context: str = "drawn",
+                  experts: str = "fp8") -> dict:
     """Whole C5 decode steps (Granite-4.0-H-style, 40 layers, fp8 weights, batch
     `rows`) after a `ctx`-token context per sequence: drawn at random into the
     caches and states (GraniteEngine.synthetic_context: the work of each later
     step is that of a real context of that length), or with *context* "walk"
     built from a random prompt by GraniteEngine.prefill (ctx - 1 decode steps,
-    untimed)."""
+    untimed).  *experts*: "fp8", or "mx4" for 4-bit experts and shared MLP."""
     from .granite import GraniteConfig, GraniteEngine, synthetic_weights
 
     cfg = GraniteConfig()
     t0 = time.perf_counter()
     w = synthetic_weights(cfg, seed=0, device=DEV)
-    eng = GraniteEngine(cfg, w, rows=rows, device=DEV, max_steps=ctx + steps + 32)
+    eng = GraniteEngine(cfg, w, rows=rows, device=DEV, max_steps=ctx + steps + 32,
+                        experts=experts)
     if context == "walk":
         g = torch.Generator().manual_seed(5)
         eng.prefill([torch.randint(0, cfg.vocab, (ctx + 1,), generator=g).tolist()
@@ -476,12 +478,12 @@ def bench_c5_step(rows: int, steps: int, ctx: int = 8192, context: str = "drawn"
     torch.cuda.synchronize()
     seconds = time.perf_counter() - t1
     eng.check_errors()
-    touched = len(set(eng.ridx.reshape(-1).tolist()))
+    touched = len(set(eng.ridx[:, :cfg.top_k].reshape(-1).tolist()))
     wbytes = eng.weight_bytes_per_step(touched)
     positions = range(ctx + 4, ctx + 4 + steps)
     sbytes = sum(eng.state_bytes_per_step([p] * rows) for p in positions) / steps
     step_s = seconds / steps
-    out = {"config": f"c5 step b{rows} ctx{ctx}", "context": context,
+    out = {"config": f"c5 step b{rows} ctx{ctx}", "context": context, "experts": experts,
            "tok_s": round(rows * steps / seconds, 1),
            "ms_per_step": round(step_s * 1e3, 4), "steps": steps,
            "bytes_per_step": int(wbytes + sbytes), "experts_touched_sample": touched,
@@ -502,6 +504,8 @@ def main(argv=None) -> int:
     ap.add_argument("--context", choices=("drawn", "walk"), default="drawn",
                     help="c5-step: the contexts drawn into the caches and states (default) or "
                          "built by prefill from random prompts")
+    ap.add_argument("--experts", choices=("fp8", "mx4"), default="fp8",
+                    help="c5-step: the experts' and shared MLP's weights")
     ap.add_argument("--ctx", type=int, default=8192, help="c5-step: context length")
     ap.add_argument("--path", choices=("auto", "small", "mfma"), default="auto",
                     help="c4-step: the small-batch kernels (rows <= 4, the default there) or "
@@ -514,7 +518,8 @@ def main(argv=None) -> int:
                       small=None if args.path == "auto" else args.path == "small")
         return 0
     if args.config == "c5-step":
-        bench_c5_step(args.rows, args.steps, ctx=args.ctx, context=args.context)
+        bench_c5_step(args.rows, args.steps, ctx=args.ctx, context=args.context,
+                      experts=args.experts)
         return 0
     if args.config == "gemm":
         run_gemm(args.reps)

@@ -22,6 +22,11 @@ then the final norm, the head over the tied table divided by ``logits_scaling``
 next token's embedding times ``embedding_multiplier``.  Sequences (up to 32) step
 together; a step is recorded into two HIP graphs (the conv windows ping-pong).
 Weights are synthetic (random init on the device).
+
+``experts="mx4"`` holds the experts and the shared MLP in microscaled 4 bits instead
+(``tilefoundry_amd.mx4``; quantised from the fp8 weights at load): the shared MLP's columns
+become experts that every row picks, ``tfd_route_experts`` routes and ``tfd_mx4_experts``
+adds their output into the stream, with f32 weights and one rounding.
 """
 from __future__ import annotations
 
@@ -32,6 +37,7 @@ import torch
 
 from .. import _lib
 from .._lib import lib, ptr
+from ..mx4 import Experts, Mx4, quantise
 from ..sampling import Picker, Sampling
 from .prefill import GranitePass, prefill
 from .qwen3_5 import attention_splits, ctypes_addr
@@ -190,6 +196,20 @@ def validate(cfg: GraniteConfig, weights: dict[str, torch.Tensor]) -> None:
             raise ValueError(f"weight {name!r}: declared dtype {dt}, got {t.dtype}")
 
 
+def mx4_shared(cfg: GraniteConfig) -> int:
+    """Experts that the shared MLP makes beside the routed ones in 4 bits (``ValueError``
+    where it does not divide into experts of the routed width, or the kernels' limits)."""
+    E, I, IS = cfg.experts, cfg.moe_inter, cfg.shared_inter
+    if I % 32 or cfg.hidden % 32 or IS % I:
+        raise ValueError(f"4-bit experts: hidden {cfg.hidden} and width {I} must be multiples of "
+                         f"32, the shared width {IS} one of {I}")
+    n = IS // I
+    if E + n > _lib.ROUTE_MAX_EXPERTS or cfg.top_k + n > 64:
+        raise ValueError(f"4-bit experts: {E} + {n} experts, {cfg.top_k} + {n} a row exceed "
+                         f"{_lib.ROUTE_MAX_EXPERTS} and 64")
+    return n
+
+
 class GraniteEngine:
     """A Granite-style hybrid decoder stepping `rows` sequences together.
 
@@ -199,9 +219,14 @@ class GraniteEngine:
     def __init__(self, cfg: GraniteConfig, weights: dict[str, torch.Tensor], *, rows: int,
                  device: str = "cuda:0", max_steps: int = 1024, page_seed: int = 0,
                  split_len: int | None = None, graph: bool = True, record_routes: bool = False,
-                 sampling: Sampling | None = None):
+                 sampling: Sampling | None = None, experts: str = "fp8"):
         if not 1 <= rows <= 32:
             raise ValueError("rows: 1..32 sequences")
+        if experts not in ("fp8", "mx4"):
+            raise ValueError(f"experts must be 'fp8' or 'mx4', got {experts!r}")
+        self.mx4 = experts == "mx4"
+        self.shared = mx4_shared(cfg) if self.mx4 else 0    # experts that every row picks
+        self.picks = cfg.top_k + self.shared                # places of a row
         self.cfg, self.B, self.device = cfg, rows, device
         self._lib = lib()
         self.sampling = sampling                # the token choice (None: greedy)
@@ -212,8 +237,8 @@ class GraniteEngine:
         # more: row-major, the lane-sum kernels.  (At C4's bf16 widths the
         # lane-sum kernels already stream at 0.75-0.8 of HBM, and the pair's down
         # has only hidden / 16 = 128 blocks there: that engine keeps them.)
-        self.moe_packed = _lib.moe_packed_fits(rows, cfg.top_k, cfg.hidden, cfg.moe_inter,
-                                               cfg.shared_inter)
+        self.moe_packed = not self.mx4 and _lib.moe_packed_fits(
+            rows, cfg.top_k, cfg.hidden, cfg.moe_inter, cfg.shared_inter)
         # up to 8 sequences at the 4,096 hidden size: the router with the post
         # norm as its prologue (tfd_proj8_norm; 7.5 us against 9.7 for the norm
         # launch and the skinny GEMM, the same bits)
@@ -251,6 +276,8 @@ class GraniteEngine:
             d = {k[len(p):]: v for k, v in w.items() if k.startswith(p)}
             for name in ("w_in", "w_out", "w_router"):
                 d[name] = self._packed8(d[name])
+            if self.mx4:
+                d["experts"] = self._mx4_experts(d)
             if self.moe_packed:
                 for name in ("w_gate", "w_up", "w_down", "w_shared_in", "w_shared_out"):
                     d[name] = self._packed8(d[name])
@@ -261,6 +288,27 @@ class GraniteEngine:
         self.head = torch.empty(-(-N // 16) * 16 * K, dtype=BF, device=self.device)
         self._lib.tfd_pack_skinny_bf16(ptr(self.embed), K, N, K, ptr(self.head), self._stream())
         torch.cuda.synchronize(self.device)
+
+    def _mx4_experts(self, d) -> Experts:
+        """The layer's experts, and its shared MLP as further ones, in 4 bits; their fp8
+        weights leave *d*."""
+        cfg, n = self.cfg, self.shared
+        E, I, H = cfg.experts, cfg.moe_inter, cfg.hidden
+
+        def values(name, scale):
+            return d.pop(name).view(torch.float8_e4m3fn).float() * d.pop(scale).unsqueeze(1)
+
+        def stack(parts, *shape):
+            q = [quantise(w) for w in parts]
+            return Mx4(torch.cat([t.codes for t in q]).view(E + n, *shape[:-1], shape[-1] // 2),
+                       torch.cat([t.scales for t in q]).view(E + n, *shape[:-1], shape[-1] // 32))
+
+        gate, up = values("w_shared_in", "w_shared_in_scale").split(n * I)
+        down = values("w_shared_out", "w_shared_out_scale")
+        down = down.view(H, n, I).transpose(0, 1).reshape(n * H, I)
+        return Experts(stack([values("w_gate", "s_gate"), gate], I, H),
+                       stack([values("w_up", "s_up"), up], I, H),
+                       stack([values("w_down", "s_down"), down], H, I))
 
     def _buffers(self, page_seed):
         cfg, B, dev = self.cfg, self.B, self.device
@@ -278,8 +326,12 @@ class GraniteEngine:
         self.proj = z(B, self.nproj, dtype=BF)
         self.mix = z(32 * max(cfg.d_inner, cfg.heads * cfg.head_dim), dtype=BF)
         self.rlog = z(B, cfg.experts)
-        self.rw = z(B, k)
-        self.ridx = z(B, k, dtype=I32)
+        self.rw = z(B, self.picks)
+        self.ridx = z(B, self.picks, dtype=I32)
+        if self.mx4:
+            self.mx4_bytes = self._lib.tfd_mx4_experts_work_bytes(
+                B, self.picks, cfg.experts + self.shared, H, cfg.moe_inter)
+            self.mx4_work = z(self.mx4_bytes, dtype=U8)
         ld = max(cfg.moe_inter, cfg.shared_inter)
         self.moe_hidden = z(B, k + 1, ld, dtype=BF)
         self.moe_sscale = z(B)
@@ -368,8 +420,26 @@ class GraniteEngine:
         a.out, a.policy, a.err = ptr(self.mix), _lib.POLICY_BF16, ptr(self.err)
         self._lib.tfd_gqa_decode(ctypes_addr(a), s)
 
+    def mx4_moe(self, w, rows, x, logits, weights, ids, stream_rows, work, nbytes, s):
+        """Routing and experts of *rows* rows in 4 bits, added into *stream_rows*."""
+        cfg, n, ex = self.cfg, self.picks, w["experts"]
+        E, H = cfg.experts, cfg.hidden
+        r = _lib.TfdRouteArgs(ptr(logits), E, _lib.TYPE_F32, None, rows, E, cfg.top_k,
+                              _lib.SCORE_SOFTMAX, 1, 1, 2, self.shared, 1, 1.0, ptr(weights),
+                              ptr(ids), n)
+        self._lib.tfd_route_experts(ctypes_addr(r), s)
+        a = _lib.TfdMx4ExpertsArgs(
+            ptr(x), H, ptr(ids), ptr(weights), n, ptr(ex.w_gu), ptr(ex.w_down), rows, n, ex.E, H,
+            cfg.moe_inter, ptr(stream_rows), H, _lib.TYPE_BF16, 1, cfg.residual_multiplier,
+            ptr(work), nbytes, ptr(self.err))
+        self._lib.tfd_mx4_experts(ctypes_addr(a), s)
+
     def _moe(self, w, s):
         cfg = self.cfg
+        if self.mx4:
+            self.mx4_moe(w, self.B, self.xm, self.rlog, self.rw, self.ridx, self.hidden,
+                         self.mx4_work, self.mx4_bytes, s)
+            return
         a = _lib.TfdMoeArgs()
         a.x, a.weights, a.idx = ptr(self.xm), ptr(self.rw), ptr(self.ridx)
         a.w_gate, a.w_up, a.w_down = ptr(w["w_gate"]), ptr(w["w_up"]), ptr(w["w_down"])
@@ -423,7 +493,7 @@ class GraniteEngine:
                         _lib.EPI_LOGITS, self.rlog, cfg.experts, s)
         self._moe(w, s)                    # routes inside the call, adds into the stream
         if self.routes is not None:
-            self.routes[i].copy_(self.ridx)
+            self.routes[i].copy_(self.ridx[:, :cfg.top_k])
 
     def _step(self, cur):
         s = self._stream()
@@ -571,12 +641,15 @@ class GraniteEngine:
 
     # ------------------------------------------------------------ accounting
     def weight_bytes_per_step(self, experts_touched: float) -> float:
-        """fp8 weights (1 byte each, 4 bytes per row scale) once, the experts picked
-        (their union per layer) once, the bf16 head table once."""
+        """fp8 weights (1 byte each, 4 bytes per row scale; 4-bit experts 17/32 byte) once,
+        the experts picked (their union per layer) once, the bf16 head table once."""
         cfg, H = self.cfg, self.cfg.hidden
 
         def lin(n, k):
             return n * k + 4 * n
+
+        def expert(n, k):
+            return n * k * 17 // 32 if self.mx4 else lin(n, k)
 
         total = 2 * cfg.vocab * H + 2 * H
         for i in range(cfg.layers):
@@ -587,8 +660,8 @@ class GraniteEngine:
                           2 * (cfg.conv_dim * (cfg.conv_kernel + 1) + 3 * cfg.mamba_heads +
                                cfg.d_inner))
             total += 2 * 2 * H + lin(cfg.experts, H)
-            total += lin(2 * cfg.shared_inter, H) + lin(H, cfg.shared_inter)
-            total += experts_touched * (2 * lin(cfg.moe_inter, H) + lin(H, cfg.moe_inter))
+            total += expert(2 * cfg.shared_inter, H) + expert(H, cfg.shared_inter)
+            total += experts_touched * (2 * expert(cfg.moe_inter, H) + expert(H, cfg.moe_inter))
         return total
 
     def state_bytes_per_step(self, positions) -> float:

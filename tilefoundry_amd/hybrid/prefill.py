@@ -51,6 +51,7 @@ class _Pass:
         # the engine holds this pass: a strong reference back would keep both, and
         # their device memory, until a garbage collection
         self._eng, self.cfg, self._lib = weakref.ref(eng), eng.cfg, lib()
+        self.mx4 = getattr(eng, "mx4", False)
         self.B, self.H, self.k = eng.B, eng.cfg.hidden, eng.cfg.top_k
         self.dev = eng.device
         self.layers = [self._weights(w) for w in eng.layers]
@@ -72,8 +73,9 @@ class _Pass:
             wait_for_work(self.dev)
         self.rows = 0                       # until every buffer below holds R rows
         c, H, k = self.cfg, self.H, self.k
-        shapes = [(H, self.in_rows), (self.out_k, H), (H, c.experts), (H, 2 * c.shared_inter),
-                  (c.shared_inter, H)]
+        shapes = [(H, self.in_rows), (self.out_k, H), (H, c.experts)]
+        if not self.mx4:
+            shapes += [(H, 2 * c.shared_inter), (c.shared_inter, H)]
         if self.attn_k:
             shapes += [(self.attn_k, H), (H, c.attn_in)]
         part = max(self._lib.tfd_panel_gemm_slices(m, K, N) * m * N
@@ -86,11 +88,19 @@ class _Pass:
         self.part = z(part, dtype=F32)
         self.emb, self.xm, self.xn = z(R, H), z(R, H), z(R * H)
         self.proj, self.mix = z(R, self.nproj), z(R * max(self.out_k, self.attn_k))
-        self.rlog, self.rw = z(R, c.experts, dtype=F32), z(R, k, dtype=F32)
-        self.ridx = z(R, k, dtype=I32)
-        self.groups = z(_lib.panel_moe_words(c.experts, R * k), dtype=I32)
-        self.moe_hidden, self.d = z(R * k, c.moe_inter), z(R * k, H)
-        self.shared = z(R * c.shared_inter)
+        self.rlog = z(R, c.experts, dtype=F32)
+        n = self.e.picks if self.mx4 else k
+        self.rw, self.ridx = z(R, n, dtype=F32), z(R, n, dtype=I32)
+        if self.mx4:
+            E = c.experts + self.e.shared
+            # a call of fewer rows may run in another way, which needs less for each row
+            self.mx4_bytes = max(self._lib.tfd_mx4_experts_work_bytes(m, n, E, H, c.moe_inter)
+                                 for m in {min(R, 16), R})
+            self.mx4_work = z(self.mx4_bytes, dtype=torch.uint8)
+        else:
+            self.groups = z(_lib.panel_moe_words(c.experts, R * k), dtype=I32)
+            self.moe_hidden, self.d = z(R * k, c.moe_inter), z(R * k, H)
+            self.shared = z(R * c.shared_inter)
         self._mixer_buffers(R, z)
         self.rows = R
 
@@ -132,10 +142,14 @@ class _Pass:
 
     def _moe(self, w, M, s):
         """The routed experts' outputs in ``d`` and the shared expert's sums in
-        ``part`` -> their slices."""
+        ``part`` -> their slices.  (4-bit experts: all added into the stream, 0 slices.)"""
         c, L, H = self.cfg, self._lib, self.H
         sl = self._gemm(self.xn, w["w_router"], w.get("w_router_scale"), M, H, c.experts, s)
         L.tfd_panel_sum(ptr(self.part), sl, M, c.experts, ptr(self.rlog), c.experts, 1, s)
+        if self.mx4:
+            self.e.mx4_moe(w, M, self.xm, self.rlog, self.rw, self.ridx, self.stream,
+                           self.mx4_work, self.mx4_bytes, s)
+            return 0
         L.tfd_route_topk(ptr(self.rlog), c.experts, M, c.experts, self.k, self.route,
                          ptr(self.rw), ptr(self.ridx), s)
         a = _lib.TfdPanelMoeArgs()
@@ -168,7 +182,7 @@ class _Pass:
                         self.attn_k if full else self.out_k, self.H, s)
         self._update(M, sl, w["gamma_post"], s, rows=True)
         sl = self._moe(w, M, s)
-        self._update(M, sl, self.layers[i + 1]["gamma_in"], s, moe=w)
+        self._update(M, sl, self.layers[i + 1]["gamma_in"], s, moe=None if self.mx4 else w)
 
     def run(self, prompts: list[list[int]]):
         """Positions 0 .. n - 2 of every sequence (prompts of one length n), from the
@@ -295,7 +309,7 @@ class GranitePass(_Pass):
         """Whether the kernels of a pass cover this engine's sizes and weights."""
         c = eng.cfg
         ks = (c.hidden, c.d_inner, c.heads * c.head_dim, c.shared_inter)
-        return (eng.moe_packed and c.mamba_head_dim == 64 and c.d_state == 128 and
+        return ((eng.moe_packed or eng.mx4) and c.mamba_head_dim == 64 and c.d_state == 128 and
                 c.conv_kernel == 4 and all(k % 256 == 0 for k in ks) and c.hidden <= 8192 and
                 c.d_inner <= 8192 and c.moe_inter % 128 == 0 and c.experts <= 256 and
                 c.experts % 4 == 0 and c.mamba_in % 4 == 0 and c.head_dim == 128 and
@@ -303,7 +317,8 @@ class GranitePass(_Pass):
 
     def _weights(self, w):
         w = dict(w)
-        w["p_shared_in"], w["p_shared_out"] = w["w_shared_in"], w["w_shared_out"]
+        if not self.mx4:
+            w["p_shared_in"], w["p_shared_out"] = w["w_shared_in"], w["w_shared_out"]
         return w
 
     def _is_full(self, i):
