@@ -53,7 +53,10 @@ int tfd_mx4_pack(const void* codes, const void* scales, const void* codes2, cons
  * (out_type).  W packed by tfd_mx4_pack ([N][K]).  x: bf16 [M][ldx], or mx4 with x_scales
  * set (codes [M][ldx bytes], scales [M][ldxs]); rows 16-byte aligned.  The 4-bit
  * counterpart of tfd_gemm_skinny_bf16 / tfd_panel_gemm_bf16 for any M, N and K a multiple of
- * 32, on plain rows; no work buffer. */
+ * 32, on plain rows.  work (may be NULL): with tfd_mx4_gemm_work_bytes of it, 16-byte
+ * aligned and contents free, products of few blocks split K over more of them and add the
+ * parts in a second launch, always in the same order; without, the same product in one
+ * launch.  One call's at a time. */
 typedef struct {
   const void* x;
   int64_t ldx;
@@ -64,7 +67,10 @@ typedef struct {
   void* out;
   int64_t ldo;
   int out_type;
+  void* work;
+  int64_t work_bytes;
 } TfdMx4GemmArgs;
+int64_t tfd_mx4_gemm_work_bytes(int M, int K, int N);
 int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream);
 
 /* The choice of experts after the router's projection.  Replaces the two fixed routers of

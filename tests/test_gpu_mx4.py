@@ -467,3 +467,36 @@ def test_serving_chain(gpu_device):
             assert torch.equal(out[3], y) and torch.equal(out[2], ids)
             static.zero_()
     ex.check_errors()
+
+
+@pytest.mark.parametrize("M,K,N", [(17, 6144, 40), (33, 2080, 300), (64, 4096, 129),
+                                   (65, 1184, 130), (128, 6144, 260), (500, 544, 70),
+                                   (260, 4128, 513)])
+@pytest.mark.parametrize("both", [False, True])
+def test_linear_parts_of_k(gpu_device, M, K, N, both):
+    """Products of few blocks add parts of K in a second launch: right with the work they ask
+    for and, in one launch, without; the same bits on every call."""
+    import ctypes
+
+    from tilefoundry_amd import _lib
+    from tilefoundry_amd._lib import lib, ptr
+
+    w = mx4.quantise((torch.randn(N, K, generator=_gen(K)) * 0.05).to(gpu_device))
+    x = torch.randn(M, K, generator=_gen(M)).to(BF).to(gpu_device)
+    given = mx4.quantise(x) if both else x
+    x64 = (given.dequantise() if both else x).double().cpu()
+    w64 = w.dequantise().double().cpu()
+    lin = mx4.Linear(w)
+    if K >= 4096:
+        assert lib().tfd_mx4_gemm_work_bytes(M, K, N) > 0
+    for dtype, kind in ((BF, _lib.TYPE_BF16), (F32, _lib.TYPE_F32)):
+        got = lin(given, dtype=dtype)
+        _check_product(got, x64, w64)
+        assert torch.equal(got, lin(given, dtype=dtype))
+        out = torch.full((M + 1, N + 3), 7.0, dtype=dtype, device=gpu_device)
+        rows, scales = (given.codes, given.scales) if both else (x, None)
+        a = _lib.TfdMx4GemmArgs(ptr(rows), rows.shape[1], ptr(scales), K // 32 if both else 0,
+                                ptr(lin.packed), M, K, N, ptr(out), N + 3, kind, None, 0)
+        lib().tfd_mx4_gemm(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream)
+        _check_product(out[:M, :N], x64, w64)
+        assert (out[M:] == 7).all() and (out[:, N:] == 7).all()

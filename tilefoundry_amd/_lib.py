@@ -146,6 +146,7 @@ SIGNATURES: dict[str, list] = {
     "tfd_mx4_dequantise": [P, L, P, L, L, I, P, L, I, P],
     "tfd_mx4_packed_bytes": [L, I],
     "tfd_mx4_pack": [P, P, P, P, L, I, P, P],
+    "tfd_mx4_gemm_work_bytes": [I, I, I],
     "tfd_mx4_gemm": [P, P],
     "tfd_route_experts": [P, P],
     "tfd_mx4_experts_work_bytes": [I, I, I, I, I],
@@ -153,6 +154,7 @@ SIGNATURES: dict[str, list] = {
 }
 RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c_int64,
             "tfd_mx4_packed_bytes": ctypes.c_int64,
+            "tfd_mx4_gemm_work_bytes": ctypes.c_int64,
             "tfd_mx4_experts_work_bytes": ctypes.c_int64}
 UNCHECKED = {"tfd_abi_version", "tfd_decode_persistent_grid", "tfd_panel_gemm_slices",
              "tfd_panel_attn_rows"}
@@ -356,7 +358,8 @@ class TfdMx4GemmArgs(ctypes.Structure):
 
     _fields_ = [("x", c_void_p), ("ldx", c_int64), ("x_scales", c_void_p), ("ldxs", c_int64),
                 ("w", c_void_p), *[(n, c_int) for n in ("M", "K", "N")], ("out", c_void_p),
-                ("ldo", c_int64), ("out_type", c_int)]
+                ("ldo", c_int64), ("out_type", c_int), ("work", c_void_p),
+                ("work_bytes", c_int64)]
 
 
 class TfdRouteArgs(ctypes.Structure):

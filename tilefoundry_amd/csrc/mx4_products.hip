@@ -39,6 +39,8 @@ struct Job {
   void* out;
   int64_t ldo;
   int vec;                       // four outputs of a row may go in one store
+  int slices;                    // dense: parts of K, each with its own f32 rows in out
+  int64_t slice;                 // floats from one's rows to the next one's
   int64_t second;                // kSwigluTwo: bytes from a hidden row to its second part
   // experts: entry i is place i % k of row i / k; its row of x is i / div
   const int32_t* ids;
@@ -171,7 +173,7 @@ struct RowTile {
 __device__ __forceinline__ int listed_room(const Job& a) { return a.groups[1]; }
 
 template <int kEpi>
-__device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v) {
+__device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v, int slice = 0) {
   if (kEpi == kSwiglu || kEpi == kSwigluTwo) {
     // (gate, up) pairs.  The hidden value is the next product's operand, hence bf16, or in a
     // step of few rows the sum of two bf16 (2^-17): its matrix tiles have rows to spare, so
@@ -189,7 +191,7 @@ __device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v) {
     return;
   }
   if (kEpi == kF32) {
-    float* o = (float*)a.out + (int64_t)row * a.ldo + n;
+    float* o = (float*)a.out + slice * a.slice + (int64_t)row * a.ldo + n;
     if (a.vec && n + 4 <= a.N) {
       *reinterpret_cast<f32x4*>(o) = v;
     } else {
@@ -240,25 +242,29 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   }
   const int ntiles = (a.N + 15) / 16;
   const int nC = (ntiles + TN - 1) / TN;
-  const int items = nT * nC;
+  const int slices = kMode == kDense ? a.slices : 1, per_slice = nT * nC;
+  const int items = per_slice * slices;
   const int G = (int)gridDim.x * (kSplit ? 1 : kWaves);
   const int me = kSplit ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave;
   if (me >= items) return;
   const int mine = (items - 1 - me) / G + 1;
   // steps of a wave's part of K
-  const int ns = kSplit ? (a.kb + kWaves - 1) / kWaves : a.kb;
-  const int k0 = kSplit ? wave * ns : 0;
+  const int parts = kSplit ? kWaves * slices : 1;
+  const int ns = (a.kb + parts - 1) / parts;
+  auto first_of = [&](int it) { return kSplit ? (it / per_slice * kWaves + wave) * ns : 0; };
   const int sg = mx4_scale_groups(a.kb);
   const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
 
   struct Item {
     int64_t tile[TN];
     const uint8_t *x[MT], *xs[MT];
+    int k0;
   };
   auto decode = [&](int j) {
-    const int it = me + j * G, rt = it % nT, c = it / nT;
+    const int it = me + j * G, in = it % per_slice, rt = in % nT, c = in / nT;
     const RowTile<kMode> r(a, tiles, rt, kR);
     Item d;
+    d.k0 = first_of(it);
 #pragma unroll
     for (int t = 0; t < TN; ++t)
       d.tile[t] = (int64_t)r.expert * ntiles + min(c * TN + t, ntiles - 1);
@@ -279,7 +285,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   Item nx = decode(0);
   int jn = 0, sn = 0;
   auto issue = [&](int u) {
-    const int b = min(k0 + sn, a.kb - 1);
+    const int b = min(nx.k0 + sn, a.kb - 1);
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
       w[u][t] = ld16_stream(a.w + (nx.tile[t] * a.kb + b) * 1024 + lane * 16);
@@ -309,9 +315,9 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   for (int t = 0; t < TN; ++t)
 #pragma unroll
     for (int m = 0; m < MT; ++m) c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int jc = 0, sc = 0;
+  int jc = 0, sc = 0, kc = first_of(me);
   auto compute = [&](int u) {
-    const int b = k0 + sc;
+    const int b = kc + sc;
     if (b < a.kb) {
       if (b == a.kb - 1 && b * kMx4K + 32 * kq >= a.K) {
 #pragma unroll
@@ -345,6 +351,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
     // item is enough) and the waves take turns to write
     const int j = jc++;
     sc = 0;
+    kc = first_of(me + jc * G);
     if (kSplit) {
 #pragma unroll
       for (int t = 0; t < TN; ++t)
@@ -352,7 +359,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
         for (int m = 0; m < MT; ++m) red[j & 1][wave][t * MT + m][lane] = c[t][m];
       __syncthreads();
     }
-    const int it = me + j * G, rt = it % nT, cc = it / nT;
+    const int it = me + j * G, in = it % per_slice, rt = in % nT, cc = in / nT;
     const RowTile<kMode> r(a, tiles, rt, kR);
 #pragma unroll
     for (int q = 0; q < TN * MT; ++q) {
@@ -367,7 +374,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
       }
       const int n = (cc * TN + t) * 16 + 4 * kq;
       if (m * 16 + nl < r.count && cc * TN + t < ntiles && n < a.N)
-        put<kEpi>(a, r.at(a, tiles, m * 16 + nl, room), n, v);
+        put<kEpi>(a, r.at(a, tiles, m * 16 + nl, room), n, v, it / per_slice);
     }
   };
   const int total = mine * ns;
@@ -407,14 +414,18 @@ struct ManyLds {
   static constexpr int kTotal = 2 * (kBlocks * kBytes + kScales);   // rows, then scales
 };
 
-// One item: a row tile `r` of at most TM x 16 rows and column block `cb`.
+// One item: a row tile `r` of at most TM x 16 rows, column block `cb` and, of a dense product
+// of few blocks, part `slice` of K (whole fours of 128 k).
 template <int kX, int TM, int TN, int kMode, int kEpi>
 __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r, int room, int cb,
-                                          uint8_t* lds) {
+                                          int slice, uint8_t* lds) {
   constexpr bool kMx = kX == kXMx4;
   using Lds = ManyLds<kX, TM>;
   constexpr int KC = Lds::kBlocks, kScPad = Lds::kScPad;
-  static_assert(!kMx || kScPad == 16, "a lane's scales of a stage are one 16-byte read");
+  static_assert(!kMx || kScPad % 8 == 0, "whole pieces, and a lane's scales of a stage one read");
+  const int quads = mx4_scale_groups(a.kb), slices = kMode == kDense ? a.slices : 1;
+  const int q_first = quads * slice / slices, q_last = quads * (slice + 1) / slices;
+  const int b_last = min(4 * q_last, a.kb);
   constexpr int kPieces = kMx ? (KC * TM + 3) / 4 : (TM + 1) / 2;   // loads in flight a thread
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   auto xs_s = [&](int buf) { return lds + buf * (KC * Lds::kBytes); };
@@ -438,12 +449,14 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
     return (uint32_t)(kMode == kDense ? at - r.first : at / a.div) * (uint32_t)ld;
   };
   const int lr = lane >> 3, lp = lane & 7;
-  uint32_t xo[kMx ? kPieces : TM], xso[kMx ? kPieces : 1];
+  // scale bytes: of row tile (4 q + wave) % TM, row nl, 32 k group kq of block (4 q + wave) / TM
+  constexpr int kScTiles = kMx ? TM / 4 : 1;
+  uint32_t xo[kMx ? kPieces : TM], xso[kScTiles];
 #pragma unroll
   for (int q = 0; q < (kMx ? kPieces : TM); ++q) {
-    const int i = kMx ? min(q * 4 + wave, 2 * TM - 1) : 2 * q + (wave & 1);
+    const int i = kMx ? q * 4 + wave : 2 * q + (wave & 1);
     xo[q] = offset(i * 8 + lr, a.ldx) + 16 * lp + (kMx ? 0 : 128 * (wave >> 1));
-    if (kMx) xso[q] = offset(min(q * 4 + wave, KC * TM - 1) % TM * 16 + nl, a.ldxs);
+    if (kMx && q < kScTiles) xso[q] = offset(i * 16 + nl, a.ldxs);
   }
   u32x4 xr[kPieces];
   uint32_t xsr[kMx ? kPieces : 1];
@@ -459,7 +472,7 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
         const int k = (b0 + (q * 4 + wave) / TM) * kMx4K + 32 * kq;
         xr[q] = __builtin_amdgcn_raw_buffer_load_b128(xrs, in ? xo[q] : kOutOfRange, b0 * 64, 0);
         xsr[q] = __builtin_amdgcn_raw_buffer_load_b8(
-            xsrs, k < a.K ? xso[q] + (k >> 5) : kOutOfRange, 0, 0);
+            xsrs, k < a.K ? xso[q % kScTiles] + (k >> 5) : kOutOfRange, 0, 0);
       }
     } else {
       const bool in = b0 * kMx4K + 64 * (wave >> 1) + 8 * lp < a.K;
@@ -483,10 +496,9 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
     for (int q = 0; q < kPieces; ++q) {
       if (kMx) {
         const int i = q * 4 + wave;
-        if (i < 2 * TM)
-          *reinterpret_cast<u32x4*>(operand(buf, (lp >> 2) * TM + (i >> 1), 8 * (i & 1) + lr,
-                                            lp & 3, lp)) = xr[q];
-        if (i < KC * TM) xsc_s(buf)[lane * kScPad + i] = (uint8_t)xsr[q];
+        *reinterpret_cast<u32x4*>(operand(buf, (lp >> 2) * TM + (i >> 1), 8 * (i & 1) + lr,
+                                          lp & 3, lp)) = xr[q];
+        xsc_s(buf)[lane * kScPad + i] = (uint8_t)xsr[q];
       } else {
         const int m = half * kPieces + q, group = 2 * (wave >> 1) + (lp >> 2);
         if (m < TM)
@@ -503,13 +515,13 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
   u32x4 w[2][TN];
   uint32_t ws[TN], ws_next[TN];
   auto load_w = [&](int u, int b) {
-    const int64_t at = min(b, a.kb - 1);
+    const int64_t at = min(b, b_last - 1);
 #pragma unroll
     for (int t = 0; t < TN; ++t)
       w[u][t] = ld16(a.w + (wt[t] * a.kb + at) * 1024 + lane * 16);
   };
   auto load_ws = [&](int q) {
-    const int64_t at = min(q, sg - 1);
+    const int64_t at = min(q, q_last - 1);
 #pragma unroll
     for (int t = 0; t < TN; ++t)
       ws_next[t] = *(const __attribute__((address_space(1))) uint32_t*)(
@@ -520,18 +532,18 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
   for (int m = 0; m < TM; ++m)
 #pragma unroll
     for (int t = 0; t < TN; ++t) c[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load_x(0, 0);
-  load_ws(0);
-  load_w(0, 0);
-  load_w(1, 1);
+  load_x(0, 4 * q_first);
+  load_ws(q_first);
+  load_w(0, 4 * q_first);
+  load_w(1, 4 * q_first + 1);
   stage(0, 0);
   if (!kMx) {
-    load_x(1, 0);
+    load_x(1, 4 * q_first);
     stage(1, 0);
   }
   __syncthreads();
   int buf = 0;
-  u32x4 vs = {0u, 0u, 0u, 0u};
+  uint32_t vs[kScPad > 8 ? kScPad / 4 : 2];
   // the 128 k of block b, the j-th of its four: weights in slot j % 2, rows in the current
   // buffer; the slot is refilled behind its use
   auto products = [&](auto jth, int b) {
@@ -579,25 +591,31 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
   // blocks b and b + 1, the j-th two of four
   auto two = [&](auto jth, int b) {
     constexpr int j = decltype(jth)::value;
-    if (kMx) {
+    if constexpr (kMx) {
       load_x(0, b + 2);
       __builtin_amdgcn_sched_barrier(0);
-      vs = *reinterpret_cast<const u32x4*>(&xsc_s(buf)[lane * kScPad]);
+      if constexpr (kScPad == 16) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(&xsc_s(buf)[lane * kScPad]);
+        vs[0] = v.x, vs[1] = v.y, vs[2] = v.z, vs[3] = v.w;
+      } else {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(&xsc_s(buf)[lane * kScPad]);
+        vs[0] = v.x, vs[1] = v.y;
+      }
     }
     products(std::integral_constant<int, 2 * j>{}, b);
-    if (b + 1 < a.kb) {
+    if (b + 1 < b_last) {
       if (!kMx) turn();
       products(std::integral_constant<int, 2 * j + 1>{}, b + 1);
     }
     if (kMx) stage(0, 1 - buf);
     turn();
   };
-  for (int q = 0; q < sg; ++q) {
+  for (int q = q_first; q < q_last; ++q) {
 #pragma unroll
     for (int t = 0; t < TN; ++t) ws[t] = ws_next[t];
     load_ws(q + 1);
     two(std::integral_constant<int, 0>{}, 4 * q);
-    if (4 * q + 2 < a.kb) two(std::integral_constant<int, 1>{}, 4 * q + 2);
+    if (4 * q + 2 < b_last) two(std::integral_constant<int, 1>{}, 4 * q + 2);
   }
 #pragma unroll
   for (int m = 0; m < TM; ++m) {
@@ -607,7 +625,7 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
       const int tile = (cb * 4 + wave) * TN + t, n = tile * 16 + 4 * kq;
-      if (tile < ntiles && n < a.N) put<kEpi>(a, at, n, c[m][t]);
+      if (tile < ntiles && n < a.N) put<kEpi>(a, at, n, c[m][t], slice);
     }
   }
 }
@@ -624,14 +642,17 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
   // XCD has every eighth row tile with all its columns, so that all get their part of the
   // large ones.
   const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-  int rt, cb;
+  int rt, cb, slice = 0;
   if (kMode == kListed) {
     rt = local / nC * 8 + xcd;
     cb = local % nC;
     if (rt >= nT) return;
   } else {
-    const int total = nT * nC, per = (total + 7) / 8, g = xcd * per + local;
+    const int total = nT * nC * a.slices, per = (total + 7) / 8;
+    int g = xcd * per + local;
     if (local >= per || g >= total) return;
+    slice = g / (nT * nC);
+    g %= nT * nC;
     const int grp = g / (8 * nC), within = g % (8 * nC);
     const int gm = min(8, nT - grp * 8);
     rt = grp * 8 + within % gm;
@@ -640,13 +661,17 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
   const RowTile<kMode> r(a, nullptr, rt, 16 * TM);
   // a list's tile may hold fewer rows: it runs as the smallest tile that holds them
   const int used = (r.count + 15) >> 4;
-  if constexpr (kMode == kListed && TM == 8) {
-    if (used <= 2) return many_item<kX, 2, TN, kMode, kEpi>(a, r, room, cb, lds);
-    if (used <= 4) return many_item<kX, 4, TN, kMode, kEpi>(a, r, room, cb, lds);
-    if (used == 5) return many_item<kX, 5, TN, kMode, kEpi>(a, r, room, cb, lds);
-    if (used == 6) return many_item<kX, 6, TN, kMode, kEpi>(a, r, room, cb, lds);
+  if constexpr (kMode == kListed && TM == 4) {
+    if (used <= 2) return many_item<kX, 2, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
+    if (used == 3) return many_item<kX, 3, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
   }
-  many_item<kX, TM, TN, kMode, kEpi>(a, r, room, cb, lds);
+  if constexpr (kMode == kListed && TM == 8) {
+    if (used <= 2) return many_item<kX, 2, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
+    if (used <= 4) return many_item<kX, 4, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
+    if (used == 5) return many_item<kX, 5, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
+    if (used == 6) return many_item<kX, 6, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
+  }
+  many_item<kX, TM, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -785,23 +810,27 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   if (tid < kE) count[tid] = 0;
   if (tid < kSizes) size_s[tid] = 0;
-  // a thread's first ids stay in registers for the second pass
-  auto id_at = [&](int i) {
-    if (i >= a.M) return -1;
-    const int id = a.ids[a.ldi == a.k ? i : (int64_t)(i / a.k) * a.ldi + i % a.k];
+  auto at = [&](int i) {
+    return a.ids[a.ldi == a.k ? i : (int64_t)(i / a.k) * a.ldi + i % a.k];
+  };
+  auto valid = [&](int id) {
     if ((unsigned)id < (unsigned)a.E) return id;
     if (id != -1 && a.err) raise_error(a.err, kErrTokenRange);
     return -1;
   };
+  // a thread's first ids stay in registers for the second pass (all loads before a use)
   int kept[kKeep];
 #pragma unroll
-  for (int j = 0; j < kKeep; ++j) kept[j] = id_at(tid + j * kGroupThreads);
+  for (int j = 0; j < kKeep; ++j) kept[j] = at(min(tid + j * kGroupThreads, a.M - 1));
+#pragma unroll
+  for (int j = 0; j < kKeep; ++j)
+    kept[j] = tid + j * kGroupThreads < a.M ? valid(kept[j]) : -1;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
     if (kept[j] >= 0) atomicAdd(&count[kept[j]], 1);
   for (int i = tid + kKeep * kGroupThreads; i < a.M; i += kGroupThreads) {
-    const int id = id_at(i);
+    const int id = valid(at(i));
     if (id >= 0) atomicAdd(&count[id], 1);
   }
   __syncthreads();
@@ -850,7 +879,7 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
   for (int j = 0; j < kKeep; ++j)
     if (kept[j] >= 0) order[atomicAdd(&count[kept[j]], 1)] = tid + j * kGroupThreads;
   for (int i = tid + kKeep * kGroupThreads; i < a.M; i += kGroupThreads) {
-    const int id = a.ids[(int64_t)(i / a.k) * a.ldi + i % a.k];
+    const int id = at(i);
     if ((unsigned)id < (unsigned)a.E) order[atomicAdd(&count[id], 1)] = i;
   }
 }
@@ -897,9 +926,13 @@ Plan experts_plan(int rows, int k, int E, int H, int I) {
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   Plan p = {};
   p.fused = rows <= kHereRows && n <= kHereMax;
-  // rows an expert has if all are picked alike; a tile holds that and a bit
+  // By the rows an expert has if all are picked alike: items of 16 rows by the stream's
+  // kernel for few (32 Granite rows, 4 an expert: 81 us; tiles of 64 89), where a longer K
+  // leaves it ahead for longer (64 Qwen3.5 rows, 2 an expert: 68; 61); tiles of up to 64
+  // (250 Qwen3.5 rows: 81; 16-row items 101; 512 Granite rows: 168, tiles of 128 185); of up
+  // to 128 past as many (1,024 Granite rows: 277; 64 281).
   const int64_t mean = n / E;
-  p.tile_rows = mean <= 16 ? 16 : mean <= 48 ? 64 : 128;
+  p.tile_rows = mean * 2048 * 2048 <= (int64_t)H * H ? 16 : mean <= 128 ? 64 : 128;
   p.room = (int)(E + n / p.tile_rows);
   p.second = up(n * I * 2);
   p.d = p.second * (p.fused ? 2 : 1);
@@ -924,23 +957,102 @@ int job_checks(const char* what, int K, int64_t N) {
   return 0;
 }
 
-template <int kX, int kEpi>
-int launch_dense(const Job& a, hipStream_t s) {
-  const int cus = compute_units(), ntiles = (a.N + 15) / 16;
-  if (a.M <= 16) {
-    k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<min(ntiles, 4 * cus), kBlock, 0, s>>>(a);
-  } else if (a.M <= 64) {
-    const int items = (a.M + 31) / 32 * ntiles;
-    k_mx4_few<kX, 2, 1, 2, kDense, kEpi><<<min(items, 4 * cus), kBlock, 0, s>>>(a);
-  } else {
-    const int nT = (a.M + 127) / 128, nC = (ntiles + 15) / 16;
-    if ((int64_t)nT * nC > (1 << 28)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
-    k_mx4_many<kX, 8, 4, kDense, kEpi><<<8 * ((nT * nC + 7) / 8), kBlock, 0, s>>>(a, nT);
+// The parts of K of a product, added in their order; four columns a thread.
+__global__ __launch_bounds__(kBlock) void k_mx4_sum(const float* __restrict__ part, int slices,
+                                                    int64_t slice, int N, int ldp, void* out,
+                                                    int64_t ldo, int out_f32, int vec) {
+  const int n = (blockIdx.x * kBlock + threadIdx.x) * 4;
+  if (n >= N) return;
+  const float* p = part + (int64_t)blockIdx.y * ldp + n;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < slices; ++s) y += *reinterpret_cast<const f32x4*>(p + s * slice);
+  Job a = {};
+  a.out = out;
+  a.ldo = ldo;
+  a.N = N;
+  a.vec = vec;
+  if (out_f32) put<kF32>(a, blockIdx.y, n, y);
+  else put<kBf16>(a, blockIdx.y, n, y);
+}
+
+// How a dense product runs.
+//   rows <= 16     items of a column tile
+//   17 .. 64       items of 32 rows by four column tiles, which share the rows' loads, where
+//                  they occupy half the compute units (17 x 4096 x 8512: 11 us; one tile an
+//                  item 18); else one tile an item (17 x 6144 x 2048 in 4 bits: 6.8 us; four
+//                  9.5), for a long K of bf16 two tiles and parts of K (9.4 us; 10.0 whole)
+//   more           blocks of 128 x 256, or of 64 x 128 where the large ones leave compute
+//                  units idle, and parts of K where that is estimated to pay: a block of 64 x
+//                  128 takes about 0.8 us for 128 k of bf16 and 0.36 of 4 bits; adding parts
+//                  takes 3.5 us and their f32 rows' way to memory and back at 5 TB/s (65 x
+//                  6144 x 2048: 31 us whole, 15 in 12 parts; 1,000 rows 50 and 35; 65 x 2048 x
+//                  12288 13 and 16, not taken)
+struct DensePlan {
+  int rows, cols, slices;        // of an item; parts of K
+  int64_t items;
+};
+DensePlan dense_plan(bool mx, int M, int K, int N) {
+  const int cus = compute_units(), kb = mx4_blocks(K), quads = mx4_scale_groups(kb);
+  DensePlan p = {16, 16, 1, (N + 15) / 16};
+  auto shape = [&](int rows, int cols) {
+    p.rows = rows;
+    p.cols = cols;
+    p.items = (int64_t)((M + rows - 1) / rows) * ((N + cols - 1) / cols);
+  };
+  auto room = [&](int most) {    // parts that two blocks a compute unit have room for
+    return (int)max((int64_t)1, min((int64_t)most, 2 * cus / p.items));
+  };
+  if (M <= 16) return p;
+  if (M <= 64) {
+    shape(32, 64);
+    if (p.items >= cus / 2) return p;
+    shape(32, mx || kb < 24 ? 16 : 32);
+    if (p.cols == 32) p.slices = room(kb / kWavesPerBlock);
+    return p;
   }
+  shape(128, 256);
+  if (p.items >= cus) return p;
+  shape(64, 128);
+  const double whole = (mx ? 0.36 : 0.8) * kb;
+  double best = 0.8 * whole;     // the estimate has to save a fifth
+  for (int s = 2; s <= room(quads); ++s) {
+    const double us = whole / s + 3.5 + s * (double)M * N * 8 / 5e6;
+    if (us < best) {
+      best = us;
+      p.slices = s;
+    }
+  }
+  return p;
+}
+
+template <int kX, int kEpi>
+int launch_dense(const Job& a, const DensePlan& p, hipStream_t s) {
+  const int cus = compute_units();
+  const int64_t items = p.items * a.slices;
+  if (items > (1 << 28)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
+  const int few = (int)min(items, (int64_t)4 * cus), many = 8 * (((int)items + 7) / 8);
+  const int nT = (a.M + p.rows - 1) / p.rows;
+  if (p.rows == 16) k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
+  else if (p.rows == 32 && p.cols == 64)
+    k_mx4_few<kX, 2, 4, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
+  else if (p.rows == 32 && p.cols == 16)
+    k_mx4_few<kX, 2, 1, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
+  else if (p.rows == 32)         // bf16 rows alone
+    k_mx4_few<kXBf16, 2, 2, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
+  else if (p.rows == 64)
+    k_mx4_many<kX, 4, 2, kDense, kEpi><<<many, kBlock, 0, s>>>(a, nT);
+  else
+    k_mx4_many<kX, 8, 4, kDense, kEpi><<<many, kBlock, 0, s>>>(a, nT);
   return launched("mx4_gemm");
 }
 
 }  // namespace
+
+extern "C" int64_t tfd_mx4_gemm_work_bytes(int M, int K, int N) {
+  if (M <= 0 || K <= 0 || K % 32 || N <= 0) return 0;
+  const int s = max(dense_plan(false, M, K, N).slices, dense_plan(true, M, K, N).slices);
+  return s > 1 ? (int64_t)s * M * ((N + 3) / 4 * 4) * 4 : 0;
+}
 
 extern "C" int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream) {
   if (!args) return fail(kBadArg, "mx4_gemm: null args");
@@ -976,10 +1088,26 @@ extern "C" int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream) {
   const int size = a.out_type == TFD_TYPE_F32 ? 4 : 2;
   j.vec = a.ldo % 4 == 0 && (uintptr_t)a.out % (4 * size) == 0;
   hipStream_t s = (hipStream_t)stream;
-  if (mx) return a.out_type == TFD_TYPE_F32 ? launch_dense<kXMx4, kF32>(j, s)
-                                            : launch_dense<kXMx4, kBf16>(j, s);
-  return a.out_type == TFD_TYPE_F32 ? launch_dense<kXBf16, kF32>(j, s)
-                                    : launch_dense<kXBf16, kBf16>(j, s);
+  const DensePlan p = dense_plan(mx, a.M, a.K, a.N);
+  const int ldp = (a.N + 3) / 4 * 4;
+  const bool f32 = a.out_type == TFD_TYPE_F32;
+  const bool parts = p.slices > 1 && a.work && (uintptr_t)a.work % 16 == 0 &&
+                     a.work_bytes >= (int64_t)p.slices * a.M * ldp * 4;
+  j.slices = parts ? p.slices : 1;
+  if (!parts) {
+    if (mx) return f32 ? launch_dense<kXMx4, kF32>(j, p, s) : launch_dense<kXMx4, kBf16>(j, p, s);
+    return f32 ? launch_dense<kXBf16, kF32>(j, p, s) : launch_dense<kXBf16, kBf16>(j, p, s);
+  }
+  const int vec = j.vec;
+  j.out = a.work;
+  j.ldo = ldp;
+  j.slice = (int64_t)a.M * ldp;
+  j.vec = 1;
+  const int rc = mx ? launch_dense<kXMx4, kF32>(j, p, s) : launch_dense<kXBf16, kF32>(j, p, s);
+  if (rc) return rc;
+  k_mx4_sum<<<dim3((ldp / 4 + kBlock - 1) / kBlock, a.M), kBlock, 0, s>>>(
+      (const float*)a.work, j.slices, j.slice, a.N, ldp, a.out, a.ldo, f32, vec);
+  return launched("mx4_gemm");
 }
 
 extern "C" {

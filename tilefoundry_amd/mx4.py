@@ -222,9 +222,15 @@ class Linear:
         rows = out.numel() // self.N
         if rows > MAX_ROWS:
             raise ValueError(f"Linear: up to {MAX_ROWS} rows a call, got {rows}")
+        L = lib()
+        work, need = None, 0
+        if rows > 16:                        # (fewer never split K)
+            need = L.tfd_mx4_gemm_work_bytes(rows, K, self.N)
+            work = torch.empty(need, dtype=U8, device=self.device) if need else None
         a = _lib.TfdMx4GemmArgs(ptr(values), row_stride(values), ptr(scales), ldxs,
-                                ptr(self.packed), rows, K, self.N, ptr(out), self.N, kind)
-        launch(self.device, lib().tfd_mx4_gemm, ctypes.addressof(a))
+                                ptr(self.packed), rows, K, self.N, ptr(out), self.N, kind,
+                                ptr(work), need)
+        launch(self.device, L.tfd_mx4_gemm, ctypes.addressof(a))
         return out
 
 
