@@ -211,7 +211,9 @@ def test_linear_repeats_and_replays(gpu_device, M):
 
 
 @pytest.mark.parametrize("M,K,N,both", [(1, 6144, 12288, False), (48, 4096, 8512, False),
-                                        (1000, 2048, 6144, False), (700, 4096, 2048, True)])
+                                        (1000, 2048, 6144, False), (700, 4096, 2048, True),
+                                        (1024, 1056, 8512, False), (1024, 1056, 8512, True),
+                                        (4001, 544, 8500, False), (4001, 544, 8500, True)])
 def test_linear_at_model_sizes(gpu_device, M, K, N, both):
     """Every output against 64-bit products on the GPU."""
     w = mx4.quantise((torch.randn(N, K, generator=_gen(8)) * 0.02).to(gpu_device))

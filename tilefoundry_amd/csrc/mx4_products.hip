@@ -986,7 +986,10 @@ __global__ __launch_bounds__(kBlock) void k_mx4_sum(const float* __restrict__ pa
 //                  128 takes about 0.8 us for 128 k of bf16 and 0.36 of 4 bits; adding parts
 //                  takes 3.5 us and their f32 rows' way to memory and back at 5 TB/s (65 x
 //                  6144 x 2048: 31 us whole, 15 in 12 parts; 1,000 rows 50 and 35; 65 x 2048 x
-//                  12288 13 and 16, not taken)
+//                  12288 13 and 16, not taken).  Blocks of 128 x 192, which read 15% more for
+//                  a product, where 256 columns leave compute units with one block behind the
+//                  last pair, or a second one (1,024 x 4096 x 8512: 86 us, 72; 2,000 rows 136,
+//                  115; 4,001 rows 230, 239, not taken)
 struct DensePlan {
   int rows, cols, slices;        // of an item; parts of K
   int64_t items;
@@ -1010,8 +1013,18 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
     if (p.cols == 32) p.slices = room(kb / kWavesPerBlock);
     return p;
   }
+  shape(128, 192);
+  const int64_t narrow = p.items;
   shape(128, 256);
-  if (p.items >= cus) return p;
+  if (p.items >= cus) {
+    // the fullest compute unit's blocks, two at a time; one alone takes 0.6 of a pair's time
+    auto rounds = [&](int64_t items) {
+      const int64_t n = (items + cus - 1) / cus;
+      return n / 2 + (n % 2) * 0.6;
+    };
+    if (rounds(narrow) * 3 * 1.15 < 0.9 * rounds(p.items) * 4) shape(128, 192);
+    return p;
+  }
   shape(64, 128);
   const double whole = (mx ? 0.36 : 0.8) * kb;
   double best = 0.8 * whole;     // the estimate has to save a fifth
@@ -1041,6 +1054,8 @@ int launch_dense(const Job& a, const DensePlan& p, hipStream_t s) {
     k_mx4_few<kXBf16, 2, 2, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
   else if (p.rows == 64)
     k_mx4_many<kX, 4, 2, kDense, kEpi><<<many, kBlock, 0, s>>>(a, nT);
+  else if (p.cols == 192)
+    k_mx4_many<kX, 8, 3, kDense, kEpi><<<many, kBlock, 0, s>>>(a, nT);
   else
     k_mx4_many<kX, 8, 4, kDense, kEpi><<<many, kBlock, 0, s>>>(a, nT);
   return launched("mx4_gemm");
