@@ -476,8 +476,8 @@ def test_serving_chain(gpu_device):
                                    (260, 4128, 513)])
 @pytest.mark.parametrize("both", [False, True])
 def test_linear_parts_of_k(gpu_device, M, K, N, both):
-    """Products of few blocks add parts of K in a second launch: right with the work they ask
-    for and, in one launch, without; the same bits on every call."""
+    """Products of more than 64 rows but few blocks add parts of K in a second launch: right
+    with the work they ask for and, in one launch, without; the same bits on every call."""
     import ctypes
 
     from tilefoundry_amd import _lib
@@ -490,7 +490,7 @@ def test_linear_parts_of_k(gpu_device, M, K, N, both):
     w64 = w.dequantise().double().cpu()
     lin = mx4.Linear(w)
     if K >= 4096:
-        assert lib().tfd_mx4_gemm_work_bytes(M, K, N) > 0
+        assert M <= 64 or lib().tfd_mx4_gemm_work_bytes(M, K, N) > 0
     for dtype, kind in ((BF, _lib.TYPE_BF16), (F32, _lib.TYPE_F32)):
         got = lin(given, dtype=dtype)
         _check_product(got, x64, w64)

@@ -151,13 +151,13 @@ class _NoGpu:
     @staticmethod
     def linear(N, K):
         lin = object.__new__(mx4.Linear)
-        lin.N, lin.K, lin.device, lin.packed = N, K, torch.device("cuda:0"), None
+        lin.N, lin.K, lin.device, lin.index, lin.packed = N, K, torch.device("cuda:0"), 0, None
         return lin
 
     @staticmethod
     def experts(E, H, I):
         ex = object.__new__(mx4.Experts)
-        ex.E, ex.H, ex.I, ex.device = E, H, I, torch.device("cuda:0")
+        ex.E, ex.H, ex.I, ex.device, ex.index = E, H, I, torch.device("cuda:0"), 0
         return ex
 
 
@@ -245,6 +245,8 @@ def test_product_entries_refuse():
     # a step of few rows needs the hidden values alone, as two bf16
     assert lib().tfd_mx4_experts_work_bytes(16, 8, 4, 64, 32) == 16 * 8 * 32 * 4
     assert lib().tfd_mx4_experts_work_bytes(0, 8, 4, 64, 32) == 0
+    # a list: 51 hidden rows, 51 f32 outputs, 4 words, 8 tiles of 4 words and the order
+    assert lib().tfd_mx4_experts_work_bytes(17, 3, 8, 64, 64) == 6656 + 13056 + 512
 
 
 def test_structs_match_c_layout(tmp_path):

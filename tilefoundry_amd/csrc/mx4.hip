@@ -15,7 +15,8 @@ namespace {
 // gfx950's scaled conversion, which divides by a power of two, rounds to the
 // nearest even code and saturates at 6 -- the definition, in one instruction for
 // two values (checked against it over grids of ties).
-// Bound: memory; a thread reads 32 or 16 bytes and writes four.
+// Bound: memory; a thread reads 32 or 16 bytes and writes four.  12,288 x 2048 f32 17 us
+// (6.7 TB/s, partly from the last-level cache), back to bf16 11.4 us (5.5 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kPerLane = 8;
 

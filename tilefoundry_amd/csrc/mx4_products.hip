@@ -218,6 +218,8 @@ __device__ __forceinline__ void put(const Job& a, int row, int n, f32x4 v, int s
 // items of its own.  A wave has the next D steps' (128 k) weights, scales and rows in
 // flight across items, so the stream does not stop where an item ends.  Rows come straight
 // from memory (L2), once for TN column tiles.
+// Measured: one row x 2048 x 12288 5.5 us (2.4 TB/s: the launch and one round of loads), the
+// gate/up of eight Granite rows 26.7 us (170 MB, 6.3 TB/s from the last-level cache).
 // ---------------------------------------------------------------------------
 template <int kX, int MT, int TN, int D, int kMode, int kEpi, int kWaves = 4, bool kSplit = true>
 __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
@@ -242,29 +244,25 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   }
   const int ntiles = (a.N + 15) / 16;
   const int nC = (ntiles + TN - 1) / TN;
-  const int slices = kMode == kDense ? a.slices : 1, per_slice = nT * nC;
-  const int items = per_slice * slices;
+  const int items = nT * nC;
   const int G = (int)gridDim.x * (kSplit ? 1 : kWaves);
   const int me = kSplit ? (int)blockIdx.x : (int)blockIdx.x * kWaves + wave;
   if (me >= items) return;
   const int mine = (items - 1 - me) / G + 1;
   // steps of a wave's part of K
-  const int parts = kSplit ? kWaves * slices : 1;
-  const int ns = (a.kb + parts - 1) / parts;
-  auto first_of = [&](int it) { return kSplit ? (it / per_slice * kWaves + wave) * ns : 0; };
+  const int ns = kSplit ? (a.kb + kWaves - 1) / kWaves : a.kb;
+  const int k0 = kSplit ? wave * ns : 0;
   const int sg = mx4_scale_groups(a.kb);
   const uint8_t* scales = a.w + a.w_tiles * a.kb * 1024;
 
   struct Item {
     int64_t tile[TN];
     const uint8_t *x[MT], *xs[MT];
-    int k0;
   };
   auto decode = [&](int j) {
-    const int it = me + j * G, in = it % per_slice, rt = in % nT, c = in / nT;
+    const int it = me + j * G, rt = it % nT, c = it / nT;
     const RowTile<kMode> r(a, tiles, rt, kR);
     Item d;
-    d.k0 = first_of(it);
 #pragma unroll
     for (int t = 0; t < TN; ++t)
       d.tile[t] = (int64_t)r.expert * ntiles + min(c * TN + t, ntiles - 1);
@@ -285,7 +283,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   Item nx = decode(0);
   int jn = 0, sn = 0;
   auto issue = [&](int u) {
-    const int b = min(nx.k0 + sn, a.kb - 1);
+    const int b = min(k0 + sn, a.kb - 1);
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
       w[u][t] = ld16_stream(a.w + (nx.tile[t] * a.kb + b) * 1024 + lane * 16);
@@ -315,9 +313,9 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
   for (int t = 0; t < TN; ++t)
 #pragma unroll
     for (int m = 0; m < MT; ++m) c[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int jc = 0, sc = 0, kc = first_of(me);
+  int jc = 0, sc = 0;
   auto compute = [&](int u) {
-    const int b = kc + sc;
+    const int b = k0 + sc;
     if (b < a.kb) {
       if (b == a.kb - 1 && b * kMx4K + 32 * kq >= a.K) {
 #pragma unroll
@@ -351,7 +349,6 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
     // item is enough) and the waves take turns to write
     const int j = jc++;
     sc = 0;
-    kc = first_of(me + jc * G);
     if (kSplit) {
 #pragma unroll
       for (int t = 0; t < TN; ++t)
@@ -359,7 +356,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
         for (int m = 0; m < MT; ++m) red[j & 1][wave][t * MT + m][lane] = c[t][m];
       __syncthreads();
     }
-    const int it = me + j * G, in = it % per_slice, rt = in % nT, cc = in / nT;
+    const int it = me + j * G, rt = it % nT, cc = it / nT;
     const RowTile<kMode> r(a, tiles, rt, kR);
 #pragma unroll
     for (int q = 0; q < TN * MT; ++q) {
@@ -374,7 +371,7 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
       }
       const int n = (cc * TN + t) * 16 + 4 * kq;
       if (m * 16 + nl < r.count && cc * TN + t < ntiles && n < a.N)
-        put<kEpi>(a, r.at(a, tiles, m * 16 + nl, room), n, v, it / per_slice);
+        put<kEpi>(a, r.at(a, tiles, m * 16 + nl, room), n, v);
     }
   };
   const int total = mine * ns;
@@ -403,6 +400,10 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
 // beside the products of half a stage: with all in flight at once the kernel needs more
 // than the 256 registers at which two blocks share a compute unit.  (DMA into LDS needs
 // none, but every LDS read behind it waits for it.)
+// Measured: 4,001 x 2048 x 12288 of bf16 157 us (1,280 TFLOP/s; a large library product of
+// bf16 reaches 1,413 here), 4,001 x 4096 x 8512 of codes 103 us (2,700 TFLOP/s): there the
+// matrix instructions fill a quarter of the time, and the operands' way from L2 bounds it
+// (narrower blocks, which read more, are slower in proportion).
 // ---------------------------------------------------------------------------
 template <int kX, int TM>
 struct ManyLds {
@@ -926,13 +927,13 @@ Plan experts_plan(int rows, int k, int E, int H, int I) {
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   Plan p = {};
   p.fused = rows <= kHereRows && n <= kHereMax;
-  // By the rows an expert has if all are picked alike: items of 16 rows by the stream's
-  // kernel for few (32 Granite rows, 4 an expert: 81 us; tiles of 64 89), where a longer K
-  // leaves it ahead for longer (64 Qwen3.5 rows, 2 an expert: 68; 61); tiles of up to 64
-  // (250 Qwen3.5 rows: 81; 16-row items 101; 512 Granite rows: 168, tiles of 128 185); of up
-  // to 128 past as many (1,024 Granite rows: 277; 64 281).
+  // By the rows an expert has if all are picked alike (us, weights from memory): items of 16
+  // rows by the stream's kernel for few, the longer K the more (64 Granite rows, 9 an expert:
+  // 95; tiles of 64 103; 128 rows 134 and 110; 64 Qwen3.5 rows, 2 an expert, 69 and 72; 250
+  // rows, 8, 109 and 105); tiles of up to 64 (512 Granite rows 167; tiles of 128 184); of up
+  // to 128 past as many (1,024 Granite rows 278; 64 286).
   const int64_t mean = n / E;
-  p.tile_rows = mean * 2048 * 2048 <= (int64_t)H * H ? 16 : mean <= 128 ? 64 : 128;
+  p.tile_rows = mean * 400 <= H ? 16 : mean <= 128 ? 64 : 128;
   p.room = (int)(E + n / p.tile_rows);
   p.second = up(n * I * 2);
   p.d = p.second * (p.fused ? 2 : 1);
@@ -979,8 +980,8 @@ __global__ __launch_bounds__(kBlock) void k_mx4_sum(const float* __restrict__ pa
 //   rows <= 16     items of a column tile
 //   17 .. 64       items of 32 rows by four column tiles, which share the rows' loads, where
 //                  they occupy half the compute units (17 x 4096 x 8512: 11 us; one tile an
-//                  item 18); else one tile an item (17 x 6144 x 2048 in 4 bits: 6.8 us; four
-//                  9.5), for a long K of bf16 two tiles and parts of K (9.4 us; 10.0 whole)
+//                  item 18); else one tile an item (17 x 6144 x 2048: 10.0 us; four 12.7, four
+//                  in 12 parts of K and a second launch 11.6)
 //   more           blocks of 128 x 256, or of 64 x 128 where the large ones leave compute
 //                  units idle, and parts of K where that is estimated to pay: a block of 64 x
 //                  128 takes about 0.8 us for 128 k of bf16 and 0.36 of 4 bits; adding parts
@@ -1002,15 +1003,10 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
     p.cols = cols;
     p.items = (int64_t)((M + rows - 1) / rows) * ((N + cols - 1) / cols);
   };
-  auto room = [&](int most) {    // parts that two blocks a compute unit have room for
-    return (int)max((int64_t)1, min((int64_t)most, 2 * cus / p.items));
-  };
   if (M <= 16) return p;
   if (M <= 64) {
     shape(32, 64);
-    if (p.items >= cus / 2) return p;
-    shape(32, mx || kb < 24 ? 16 : 32);
-    if (p.cols == 32) p.slices = room(kb / kWavesPerBlock);
+    if (p.items < cus / 2) shape(32, 16);
     return p;
   }
   shape(128, 192);
@@ -1028,7 +1024,8 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
   shape(64, 128);
   const double whole = (mx ? 0.36 : 0.8) * kb;
   double best = 0.8 * whole;     // the estimate has to save a fifth
-  for (int s = 2; s <= room(quads); ++s) {
+  // at most two blocks a compute unit, and four of 128 k a part
+  for (int s = 2; s <= quads && s * p.items <= 2 * cus; ++s) {
     const double us = whole / s + 3.5 + s * (double)M * N * 8 / 5e6;
     if (us < best) {
       best = us;
@@ -1048,10 +1045,8 @@ int launch_dense(const Job& a, const DensePlan& p, hipStream_t s) {
   if (p.rows == 16) k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
   else if (p.rows == 32 && p.cols == 64)
     k_mx4_few<kX, 2, 4, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
-  else if (p.rows == 32 && p.cols == 16)
+  else if (p.rows == 32)
     k_mx4_few<kX, 2, 1, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
-  else if (p.rows == 32)         // bf16 rows alone
-    k_mx4_few<kXBf16, 2, 2, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
   else if (p.rows == 64)
     k_mx4_many<kX, 4, 2, kDense, kEpi><<<many, kBlock, 0, s>>>(a, nT);
   else if (p.cols == 192)

@@ -30,10 +30,9 @@ _current_device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def launch(device, entry, *args) -> None:
-    """Calls a C entry on *device*'s current stream, with the device the current one (a
-    launch belongs to the current device, a stream to its own)."""
-    i = device.index
+def launch(i: int, entry, *args) -> None:
+    """Calls a C entry on the current stream of device *i*, with the device the current one
+    (a launch belongs to the current device, a stream to its own)."""
     if i == _current_device():
         entry(*args, _raw_stream(i))
     else:
@@ -64,8 +63,8 @@ def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
     """*x* as rows of its last dimension with unit stride, rows that do not overlap and,
     with *align*, that start at multiples of that many bytes: *x* itself where it is that
     (contiguous in any number of dimensions), else a two-dimensional view or a copy."""
-    if x.is_contiguous() and not x.data_ptr() % align and (
-            not x.shape[-1] * x.element_size() % align or x.numel() == x.shape[-1]):
+    if x.is_contiguous() and (align == 1 or not x.data_ptr() % align and (
+            not x.shape[-1] * x.element_size() % align or x.numel() == x.shape[-1])):
         return x
     K = x.shape[-1]
     x = x.reshape(-1, K)
@@ -77,7 +76,8 @@ def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
 
 
 def row_stride(x: torch.Tensor) -> int:
-    return x.stride(-2) if x.dim() > 1 and x.shape[-2] > 1 else x.shape[-1]
+    """Elements from one row of ``rows_of`` to the next."""
+    return x.shape[-1] if x.is_contiguous() else x.stride(-2)
 
 
 class Mx4:
@@ -127,12 +127,13 @@ class Mx4:
         if dtype not in TYPES:
             raise ValueError(f"dequantise: dtype {dtype} is not one of "
                              f"{', '.join(str(d) for d in TYPES)}")
-        check_device(self.device)
         codes, scales = rows_of(self.codes, 4), rows_of(self.scales)
-        device, shape = self.codes.device, self.shape
-        out = torch.empty(shape, dtype=dtype, device=device)
+        if not codes.is_cuda:
+            check_device(codes.device)
+        shape = self.shape
+        out = codes.new_empty(shape, dtype=dtype)
         K = shape[-1]
-        launch(device, lib().tfd_mx4_dequantise, ptr(codes), row_stride(codes), ptr(scales),
+        launch(codes.get_device(), lib().tfd_mx4_dequantise, ptr(codes), row_stride(codes), ptr(scales),
                row_stride(scales), out.numel() // K, K, ptr(out), K, TYPES[dtype])
         return out
 
@@ -142,15 +143,16 @@ def quantise(x: torch.Tensor) -> Mx4:
     largest magnitude t the scale 2^(floor(log2 t) - 2), codes rounded to nearest even,
     magnitudes past 6 scales as 6.  A block with a value that is not finite becomes NaN."""
     check_input(x, "quantise", TYPES)
-    if x.dim() < 1 or x.shape[-1] % BLOCK or x.shape[-1] == 0:
+    *lead, K = x.shape if x.dim() else (0,)
+    if K % BLOCK or K == 0:
         raise ValueError(f"quantise: the last dimension must be a multiple of {BLOCK}, got "
                          f"{tuple(x.shape)}")
-    check_device(x.device)
-    K, lead, device = x.shape[-1], x.shape[:-1], x.device
-    codes = torch.empty((*lead, K // 2), dtype=U8, device=device)
-    scales = torch.empty((*lead, K // BLOCK), dtype=U8, device=device)
+    if not x.is_cuda:
+        check_device(x.device)
+    codes = x.new_empty((*lead, K // 2), dtype=U8)
+    scales = x.new_empty((*lead, K // BLOCK), dtype=U8)
     rows = rows_of(x)
-    launch(device, lib().tfd_mx4_quantise, ptr(rows), row_stride(rows), TYPES[x.dtype],
+    launch(x.get_device(), lib().tfd_mx4_quantise, ptr(rows), row_stride(rows), TYPES[x.dtype],
            x.numel() // K, K, ptr(codes), K // 2, ptr(scales), K // BLOCK)
     return Mx4._of(codes, scales)
 
@@ -172,7 +174,7 @@ def _pack(first: Mx4, second: Mx4 | None, what: str) -> torch.Tensor:
     packed = torch.empty(L.tfd_mx4_packed_bytes(rows * (len(parts) // 2), K), dtype=U8,
                          device=first.device)
     parts += [None] * (4 - len(parts))
-    launch(first.device, L.tfd_mx4_pack, *(ptr(t) for t in parts), rows, K, ptr(packed))
+    launch(first.codes.get_device(), L.tfd_mx4_pack, *(ptr(t) for t in parts), rows, K, ptr(packed))
     return packed
 
 
@@ -199,6 +201,7 @@ class Linear:
         self.N, self.K = weight.shape
         self.device = weight.device
         self.packed = _pack(weight, None, "Linear")
+        self.index = self.packed.get_device()
 
     def __call__(self, x, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         kind = _out_type(dtype, "Linear")
@@ -212,25 +215,25 @@ class Linear:
             lead, K, values = x.shape[:-1], x.shape[-1], x
         if K != self.K:
             raise ValueError(f"Linear: input {tuple(x.shape)} for weights [{self.N}, {self.K}]")
-        if values.device != self.device:
+        if values.get_device() != self.index:
             raise ValueError(f"Linear: input on {values.device}, weights on {self.device}")
         values = rows_of(values, 16)
         if isinstance(x, Mx4):
             scales = rows_of(x.scales)
             ldxs = row_stride(scales)
-        out = torch.empty((*lead, self.N), dtype=dtype, device=self.device)
+        out = values.new_empty((*lead, self.N), dtype=dtype)
         rows = out.numel() // self.N
         if rows > MAX_ROWS:
             raise ValueError(f"Linear: up to {MAX_ROWS} rows a call, got {rows}")
         L = lib()
         work, need = None, 0
-        if rows > 16:                        # (fewer never split K)
+        if rows > 64:                        # (fewer never split K)
             need = L.tfd_mx4_gemm_work_bytes(rows, K, self.N)
-            work = torch.empty(need, dtype=U8, device=self.device) if need else None
+            work = values.new_empty(need, dtype=U8) if need else None
         a = _lib.TfdMx4GemmArgs(ptr(values), row_stride(values), ptr(scales), ldxs,
                                 ptr(self.packed), rows, K, self.N, ptr(out), self.N, kind,
                                 ptr(work), need)
-        launch(self.device, L.tfd_mx4_gemm, ctypes.addressof(a))
+        launch(self.index, L.tfd_mx4_gemm, ctypes.addressof(a))
         return out
 
 
@@ -259,6 +262,7 @@ class Experts:
         self.device = gate.device
         self.w_gu = _pack(gate, up, "Experts")
         self.w_down = _pack(down, None, "Experts")
+        self.index = self.w_gu.get_device()
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
@@ -275,23 +279,23 @@ class Experts:
             raise ValueError(f"Experts: ids {tuple(ids.shape)} and weights "
                              f"{tuple(weights.shape)} must be [{rows}, 1..64]")
         for t in (x, ids, weights):
-            if t.device != self.device:
+            if t.get_device() != self.index:
                 raise ValueError(f"Experts: input on {t.device}, weights on {self.device}")
         if rows > 65535:
             raise ValueError(f"Experts: up to 65535 rows a call, got {rows}")
         x = rows_of(x, 16)
         ids, weights = ids.contiguous(), weights.contiguous()
-        k, device, L = ids.shape[1], self.device, lib()
-        out = torch.empty((rows, self.H), dtype=dtype, device=device)
+        k, L = ids.shape[1], lib()
+        out = x.new_empty((rows, self.H), dtype=dtype)
         need = L.tfd_mx4_experts_work_bytes(rows, k, self.E, self.H, self.I)
         # of the stream that uses it, like the output: calls on several streams and captured
         # graphs share nothing
-        work = torch.empty(need, dtype=U8, device=device)
+        work = x.new_empty(need, dtype=U8)
         a = _lib.TfdMx4ExpertsArgs(
             ptr(x), row_stride(x), ptr(ids), ptr(weights), k, ptr(self.w_gu), ptr(self.w_down),
             rows, k, self.E, self.H, self.I, ptr(out), self.H, kind, 0, 1.0, ptr(work), need,
             ptr(self.err))
-        launch(device, L.tfd_mx4_experts, ctypes.addressof(a))
+        launch(self.index, L.tfd_mx4_experts, ctypes.addressof(a))
         return out
 
     def check_errors(self) -> None:

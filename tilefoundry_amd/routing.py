@@ -77,15 +77,16 @@ class Routing:
             if bias.shape != (experts,):
                 raise ValueError(f"bias must be [{experts}], got {tuple(bias.shape)}")
             bias = bias.contiguous()
-        check_device(logits.device, bias)
+            check_device(logits.device, bias)
+        elif not logits.is_cuda:
+            check_device(logits.device)
         logits = rows_of(logits)
         n = self.top_k + self.shared
-        device = logits.device
-        weights = torch.empty((rows, n), dtype=torch.float32, device=device)
-        ids = torch.empty((rows, n), dtype=torch.int32, device=device)
+        weights = logits.new_empty((rows, n), dtype=torch.float32)
+        ids = logits.new_empty((rows, n), dtype=torch.int32)
         a = _lib.TfdRouteArgs(
             ptr(logits), row_stride(logits), TYPES[logits.dtype], ptr(bias), rows, experts,
             self.top_k, SCORES[self.score], self.groups, self.kept_groups, self.group_top,
             self.shared, int(self.renormalise), self.scale, ptr(weights), ptr(ids), n)
-        launch(device, lib().tfd_route_experts, ctypes.addressof(a))
+        launch(logits.get_device(), lib().tfd_route_experts, ctypes.addressof(a))
         return weights, ids
