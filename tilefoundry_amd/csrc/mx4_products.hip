@@ -440,8 +440,8 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
   // Eight lanes of a load take 128 bytes of one row, a whole cache line: rows a power of two
   // apart share a set of the L1, which keeps no line until another wave wants its other half
   // (64 bytes of 16 rows: 203 us for 4,001 x 2048 x 12288, 171 on padded rows).  bf16: of row
-  // tile m, rows 8 (wave % 2) + lane / 8, k 64 (wave / 2) + 8 (lane % 8); codes: piece q
-  // is rows 8 (i % 2) + lane / 8 of row tile i / 2, i = 4 q + wave, both blocks of a stage.
+  // tile m, rows 2 (lane / 8) + wave % 2, k 64 (wave / 2) + 8 (lane % 8); codes: piece q
+  // is rows 2 (lane / 8) + i % 2 of row tile i / 2, i = 4 q + wave, both blocks of a stage.
   // 32-bit offsets from a base that all lanes share (the entries check that they fit).
   const uint8_t* xb = a.x + (kMode == kDense ? r.first * a.ldx : 0);
   const uint8_t* xsb = kMx ? a.xs + (kMode == kDense ? r.first * a.ldxs : 0) : nullptr;
@@ -456,7 +456,8 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
 #pragma unroll
   for (int q = 0; q < (kMx ? kPieces : TM); ++q) {
     const int i = kMx ? q * 4 + wave : 2 * q + (wave & 1);
-    xo[q] = offset(i * 8 + lr, a.ldx) + 16 * lp + (kMx ? 0 : 128 * (wave >> 1));
+    xo[q] = offset((i >> 1) * 16 + 2 * lr + (i & 1), a.ldx) + 16 * lp +
+            (kMx ? 0 : 128 * (wave >> 1));
     if (kMx && q < kScTiles) xso[q] = offset(i * 16 + nl, a.ldxs);
   }
   u32x4 xr[kPieces];
@@ -487,8 +488,11 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
     }
   };
   // Where 16 bytes lie in LDS: 1 KiB for the 64 lanes of an operand, lane (row, 32 k group)
-  // at row ^ f + 16 group, f running over 0..7 among the eight lanes that write one row's
-  // pieces (which go to eight operands or groups): no bank conflicts, nor for the reads.
+  // at row ^ f + 16 group.  A 16-byte access is served for lanes 0-3, 12-15, 20-23 and 24-27
+  // of 32 together, then the others, without conflict where their places differ mod 16.  A
+  // row's eight pieces go to four operands (or groups) times two groups (or blocks) of f 0..3
+  // and 12 apart: with even or odd rows in a load those lanes' places differ, and a read,
+  // whose lanes' f differ by 0..3 or 12 only, takes them as rows in a row would lie.
   auto operand = [&](int buf, int i, int row, int group, int f) {
     return &xs_s(buf)[i * 1024 + ((row ^ f) + 16 * group) * 16];
   };
@@ -497,14 +501,14 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
     for (int q = 0; q < kPieces; ++q) {
       if (kMx) {
         const int i = q * 4 + wave;
-        *reinterpret_cast<u32x4*>(operand(buf, (lp >> 2) * TM + (i >> 1), 8 * (i & 1) + lr,
-                                          lp & 3, lp)) = xr[q];
+        *reinterpret_cast<u32x4*>(operand(buf, (lp >> 2) * TM + (i >> 1), 2 * lr + (i & 1),
+                                          lp & 3, (lp & 3) + 12 * (lp >> 2))) = xr[q];
         xsc_s(buf)[lane * kScPad + i] = (uint8_t)xsr[q];
       } else {
         const int m = half * kPieces + q, group = 2 * (wave >> 1) + (lp >> 2);
         if (m < TM)
-          *reinterpret_cast<u32x4*>(operand(buf, m * 4 + (lp & 3), 8 * (wave & 1) + lr, group,
-                                            (lp & 3) + 4 * (group & 1))) = xr[q];
+          *reinterpret_cast<u32x4*>(operand(buf, m * 4 + (lp & 3), 2 * lr + (wave & 1), group,
+                                            (lp & 3) + 12 * (group & 1))) = xr[q];
       }
     }
   };
@@ -553,7 +557,7 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
       u32x4 v[TM];
 #pragma unroll
       for (int m = 0; m < TM; ++m)
-        v[m] = *reinterpret_cast<const u32x4*>(operand(buf, u * TM + m, nl, kq, kq + 4 * u));
+        v[m] = *reinterpret_cast<const u32x4*>(operand(buf, u * TM + m, nl, kq, kq + 12 * u));
       unrolled<TN>([&](auto t) {
         unrolled<TM>([&](auto m) {
           constexpr int i = u * TM + m.value;
@@ -569,7 +573,7 @@ __device__ __forceinline__ void many_item(const Job& a, const RowTile<kMode>& r,
 #pragma unroll
         for (int m = 0; m < TM; ++m)
           v[m] = *reinterpret_cast<const u32x4*>(
-              operand(buf, m * 4 + s, nl, kq, s + 4 * (kq & 1)));
+              operand(buf, m * 4 + s, nl, kq, s + 12 * (kq & 1)));
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
           const u32x4 q = fp4x8_to_bf16(w[u][t][s], mx4_scale((ws[t] >> (8 * j)) & 0xffu));
