@@ -27,7 +27,8 @@ extern "C" {
 /* Rows to mx4.  For a block with largest magnitude t: e = clamp(floor(log2 t) - 2, -127,
  * 125) (-127 for t = 0), scale byte e + 127, codes round-to-nearest-even of x / 2^e,
  * magnitudes past 6 as 6.  A block with a value that is not finite gets scale byte 255 and
- * zero codes: it stands for NaN.  x: f32, bf16 or f16 [rows][ldx]; any alignment of its
+ * zero codes: it stands for NaN.  Up to 2^35 - 2048 values a call (2^35: 64 GiB of bf16);
+ * the inverse too.  x: f32, bf16 or f16 [rows][ldx]; any alignment of its
  * element size (16-byte aligned rows are read faster).  codes [rows][ldc], ldc % 4 == 0,
  * 4-byte aligned; scales [rows][lds]. */
 int tfd_mx4_quantise(const void* x, int64_t ldx, int type, int64_t rows, int K, void* codes,
@@ -51,9 +52,9 @@ int tfd_mx4_pack(const void* codes, const void* scales, const void* codes2, cons
 
 /* out[m][n] = sum_k x[m][k] W[n][k], f32 sums, each output rounded once to f32 or bf16
  * (out_type).  W packed by tfd_mx4_pack ([N][K]).  x: bf16 [M][ldx], or mx4 with x_scales
- * set (codes [M][ldx bytes], scales [M][ldxs]); rows 16-byte aligned.  The 4-bit
- * counterpart of tfd_gemm_skinny_bf16 / tfd_panel_gemm_bf16 for any M, N and K a multiple of
- * 32, on plain rows.  work (may be NULL): with tfd_mx4_gemm_work_bytes of it, 16-byte
+ * set (codes [M][ldx bytes], scales [M][ldxs]); rows 16-byte aligned, ldx and ldxs up to
+ * 2^23.  The 4-bit counterpart of tfd_gemm_skinny_bf16 / tfd_panel_gemm_bf16 for any M, N
+ * and K a multiple of 32, on plain rows.  work (may be NULL): with tfd_mx4_gemm_work_bytes of it, 16-byte
  * aligned and contents free, products of few blocks split K over more of them and add the
  * parts in a second launch, always in the same order; without, the same product in one
  * launch.  One call's at a time. */
@@ -117,7 +118,7 @@ int tfd_route_experts(const TfdRouteArgs* args, void* stream);
  * shared experts are experts that every row picks (tfd_route_experts appends them).
  * x bf16 [rows][ldx], rows 16-byte aligned; ids / weights [rows][ld]; w_gu = tfd_mx4_pack of
  * gate [E I][H] with up [E I][H] as its second matrix, w_down of [E H][I]; H and I multiples
- * of 32, experts <= 512, k <= 64, rows <= 65535.  Id -1 is an empty place; another id outside
+ * of 32, experts <= 512, k <= 64, rows <= 65535, rows * ldx and rows * k * I below 2^30.  Id -1 is an empty place; another id outside
  * the experts is skipped and raises TFD_ERR_TOKEN_RANGE in err (NULL: nothing).  An expert
  * may come twice in a row.  work: tfd_mx4_experts_work_bytes, 256-byte aligned, contents
  * free, one call's at a time. */

@@ -502,3 +502,71 @@ def test_linear_parts_of_k(gpu_device, M, K, N, both):
         lib().tfd_mx4_gemm(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream)
         _check_product(out[:M, :N], x64, w64)
         assert (out[M:] == 7).all() and (out[:, N:] == 7).all()
+
+
+# ----------------------------------------------------------- offsets past 32 bits
+def test_rows_past_4_gib(gpu_device):
+    """Rows whose bytes start past 2^32: quantised, back, and multiplied, with 16, 100 and
+    all rows a call; a strided view too."""
+    M, K, N = (1 << 22) + 37, 512, 32
+    x = torch.zeros(M, K, dtype=BF, device=gpu_device)
+    tail = torch.randn(100, K, generator=_gen(40)).to(BF)
+    x[-100:] = tail.to(gpu_device)
+    q = mx4.quantise(x)
+    codes, scales = R.quantise(tail)
+    assert torch.equal(q.codes[-100:].cpu(), codes) and torch.equal(q.scales[-100:].cpu(), scales)
+    assert not q.codes[:-100].any()
+    back = q[-100:].dequantise()
+    assert torch.equal(q.dequantise(BF)[-100:].float(), back)
+    w = _weights(N, K, 41)
+    lin = mx4.Linear(_to(w, gpu_device))
+    w64 = R.values(w.codes, w.scales).to(F64)
+    for rows in (16, 100, M):
+        for t, t64 in ((x, tail.to(F64)), (q, back.cpu().to(F64))):
+            n = min(rows, 100)
+            _check_product(lin(t[-rows:], dtype=F32)[-n:], t64[-n:], w64)
+    # every 65,536th row: rows 64 MiB apart, the last one 4 GiB behind the first
+    step = x[M - 1 - (64 << 16)::1 << 16]
+    got = lin(step, dtype=F32)
+    _check_product(got[-1:], tail[-1:].to(F64), w64)
+    assert not got[:-1].any()
+    assert torch.equal(mx4.quantise(step).codes[-1], q.codes[-1])
+
+
+def test_weights_past_4_gib(gpu_device):
+    """Packed weights whose last tiles lie past 2^32 bytes, few rows and many."""
+    N, K = (1 << 21) + (1 << 14) + 5, 4096
+    codes = torch.zeros(N, K // 2, dtype=torch.uint8, device=gpu_device)
+    scales = torch.full((N, K // 32), 120, dtype=torch.uint8, device=gpu_device)
+    last = _weights(40, K, 42)
+    codes[-40:], scales[-40:] = last.codes.to(gpu_device), last.scales.to(gpu_device)
+    lin = mx4.Linear(mx4.Mx4(codes, scales))
+    del codes, scales
+    w64 = R.values(last.codes, last.scales).to(F64)
+    for rows in (1, 20, 70):
+        x = torch.randn(rows, K, generator=_gen(43)).to(BF)
+        got = lin(x.to(gpu_device), dtype=F32)
+        _check_product(got[:, -40:], x.to(F64), w64)
+        assert not got[:, :-40].any()
+
+
+def test_experts_of_the_most_rows(gpu_device):
+    """65,535 rows, whose f32 outputs before the mix pass 4 GiB."""
+    rows, E, k, H, I = 65535, 3, 4, 4096, 32
+    ex, values = _experts(E, H, I, 44, gpu_device)
+    x = torch.randn(rows, H, generator=_gen(45)).to(BF).to(gpu_device)
+    ids, weights = _choice(rows, E, k, 46, gpu_device, repeat=True)
+    got = ex(x, ids, weights)
+    for part in (slice(0, 50), slice(rows - 50, rows)):
+        _check_experts(got[part], x[part], ids[part], weights[part], values)
+
+
+@pytest.mark.parametrize("rows", [4, 60, 300])
+def test_experts_strided_rows(gpu_device, rows):
+    """Rows, ids and weights taken out of wider tensors, reversed or every second one."""
+    E, k, H, I = 7, 3, 96, 64
+    ex, values = _experts(E, H, I, 47, gpu_device)
+    wide = torch.randn(rows, H + 40, generator=_gen(48)).to(BF).to(gpu_device)
+    ids, weights = _choice(2 * rows, E, k, 49, gpu_device)
+    for x in (wide[:, 8:8 + H], wide[:, 3:3 + H], wide.flip(0)[:, :H], wide[:1, :H].expand(rows, H)):
+        _check_experts(ex(x, ids[::2], weights[::2]), x.contiguous(), ids[::2], weights[::2], values)

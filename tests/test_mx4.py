@@ -123,6 +123,24 @@ def test_quantise_entries_refuse():
     assert L.tfd_mx4_packed_bytes(0, 160) == 0 and L.tfd_mx4_packed_bytes(16, 33) == 0
 
 
+@pytest.mark.parametrize("K", [32, 64, 8192])
+def test_quantise_entries_refuse_launches_of_too_many_threads(K):
+    """A thread has eight values, and a launch's threads, in whole blocks of 256, 32 bits."""
+    L = lib()
+    first = (2 ** 32 - 256) // (K // 8) + 1
+    for rows in (first, 2 ** 32 // (K // 8), 2 ** 40):
+        with pytest.raises(TFDError, match="mx4_quantise"):
+            L.tfd_mx4_quantise(PTR, K, 1, rows, K, PTR, K // 2, PTR, K // 32, None)
+        with pytest.raises(TFDError, match="mx4_dequantise"):
+            L.tfd_mx4_dequantise(PTR, K // 2, PTR, K // 32, rows, K, PTR, K, 1, None)
+    tiles = (2 ** 32 - 256) // (-(-K // 512) * 256) + 1
+    for N in (tiles * 16, 2 ** 62):
+        with pytest.raises(TFDError, match="mx4_pack"):
+            L.tfd_mx4_pack(PTR, PTR, None, None, N, K, PTR, None)
+        with pytest.raises(TFDError, match="mx4_pack"):
+            L.tfd_mx4_pack(PTR, PTR, PTR, PTR, N, K, PTR, None)
+
+
 def test_route_entry_refuses():
     def call(**over):
         f = dict(logits=PTR, ldl=32, type=0, bias=None, rows=2, experts=32, k=4, score=0,

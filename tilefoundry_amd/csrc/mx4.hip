@@ -152,6 +152,9 @@ __global__ __launch_bounds__(kBlock) void k_pack(const uint8_t* __restrict__ cod
   packed[tiles * kb * 1024 + (tile * groups + (b >> 2)) * 256 + lane * 4 + (b & 3)] = s;
 }
 
+// Threads of one launch: their number, rounded up to blocks, has 32 bits.
+constexpr int64_t kMaxThreads = ((int64_t)1 << 32) - kBlock;
+
 int blocks_for(int64_t threads) { return (int)((threads + kBlock - 1) / kBlock); }
 
 }  // namespace
@@ -172,8 +175,8 @@ int tfd_mx4_quantise(const void* x, int64_t ldx, int type, int64_t rows, int K, 
     return fail(kBadArg, "mx4_quantise: ldx=%lld ldc=%lld lds=%lld or an alignment", (long long)ldx,
                 (long long)ldc, (long long)lds);
   const int per_row = K / kPerLane;
-  if (rows > (int64_t)INT32_MAX * kBlock / per_row)
-    return fail(kBadShape, "mx4_quantise: rows=%lld", (long long)rows);
+  if (rows > kMaxThreads / per_row)
+    return fail(kBadShape, "mx4_quantise: %lld rows of %d pass 2^35 values", (long long)rows, K);
   const int64_t pieces = rows * per_row;
   const bool vec = (uintptr_t)x % 16 == 0 && (rows == 1 || ldx * size % 16 == 0);
   const dim3 grid(blocks_for(pieces));
@@ -206,8 +209,9 @@ int tfd_mx4_dequantise(const void* codes, int64_t ldc, const void* scales, int64
     return fail(kBadArg, "mx4_dequantise: ldc=%lld lds=%lld ldo=%lld or an alignment",
                 (long long)ldc, (long long)lds, (long long)ldo);
   const int per_row = K / kPerLane;
-  if (rows > (int64_t)INT32_MAX * kBlock / per_row)
-    return fail(kBadShape, "mx4_dequantise: rows=%lld", (long long)rows);
+  if (rows > kMaxThreads / per_row)
+    return fail(kBadShape, "mx4_dequantise: %lld rows of %d pass 2^35 values", (long long)rows,
+                K);
   const int64_t pieces = rows * per_row;
   const dim3 grid(blocks_for(pieces));
   hipStream_t s = (hipStream_t)stream;
@@ -235,10 +239,11 @@ int tfd_mx4_pack(const void* codes, const void* scales, const void* codes2, cons
     return fail(kBadShape, "mx4_pack: N=%lld K=%d (K a multiple of 32)", (long long)N, K);
   if ((uintptr_t)codes % 16 || (uintptr_t)codes2 % 16 || (uintptr_t)packed % 16)
     return fail(kBadArg, "mx4_pack: codes or packed not 16-byte aligned");
-  const int64_t rows = codes2 ? 2 * N : N;
-  const int64_t threads = (rows + 15) / 16 * mx4_scale_groups(mx4_blocks(K)) * 4 * kWave;
-  if (threads > (int64_t)INT32_MAX * kBlock)
+  const int64_t per_tile = (int64_t)mx4_scale_groups(mx4_blocks(K)) * 4 * kWave;
+  const int64_t rows = N > kMaxThreads ? N : codes2 ? 2 * N : N;
+  if (rows / 16 + 1 > kMaxThreads / per_tile)
     return fail(kBadShape, "mx4_pack: N=%lld K=%d", (long long)N, K);
+  const int64_t threads = (rows + 15) / 16 * per_tile;
   k_pack<<<blocks_for(threads), kBlock, 0, (hipStream_t)stream>>>(
       (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)codes2,
       (const uint8_t*)scales2, rows, K, (uint8_t*)packed);

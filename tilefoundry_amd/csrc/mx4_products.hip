@@ -1043,7 +1043,7 @@ template <int kX, int kEpi>
 int launch_dense(const Job& a, const DensePlan& p, hipStream_t s) {
   const int cus = compute_units();
   const int64_t items = p.items * a.slices;
-  if (items > (1 << 28)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
+  if (items > (1 << 23)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
   const int few = (int)min(items, (int64_t)4 * cus), many = 8 * (((int)items + 7) / 8);
   const int nT = (a.M + p.rows - 1) / p.rows;
   if (p.rows == 16) k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<few, kBlock, 0, s>>>(a);

@@ -59,10 +59,14 @@ def check_device(device, *others) -> None:
             raise ValueError(f"tensors on {device} and on {t.device}")
 
 
-def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
+WIDEST = 1 << 23                             # elements between rows that a product takes
+
+
+def rows_of(x: torch.Tensor, align: int = 1, widest: int = 1 << 62) -> torch.Tensor:
     """*x* as rows of its last dimension with unit stride, rows that do not overlap and,
     with *align*, that start at multiples of that many bytes: *x* itself where it is that
-    (contiguous in any number of dimensions), else a two-dimensional view or a copy."""
+    (contiguous in any number of dimensions), else a two-dimensional view or, where its rows
+    lie otherwise or more than *widest* elements apart, a copy."""
     if x.is_contiguous() and (align == 1 or not x.data_ptr() % align and (
             not x.shape[-1] * x.element_size() % align or x.numel() == x.shape[-1])):
         return x
@@ -70,7 +74,7 @@ def rows_of(x: torch.Tensor, align: int = 1) -> torch.Tensor:
     x = x.reshape(-1, K)
     size = x.element_size()
     if (x.stride(1) != 1 and K > 1) or (x.shape[0] > 1 and (
-            x.stride(0) < K or x.stride(0) * size % align)) or x.data_ptr() % align:
+            not K <= x.stride(0) <= widest or x.stride(0) * size % align)) or x.data_ptr() % align:
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -141,7 +145,8 @@ class Mx4:
 def quantise(x: torch.Tensor) -> Mx4:
     """Rows ``[..., K]`` (f32, bf16 or f16, K a multiple of 32) to mx4: for 32 values with
     largest magnitude t the scale 2^(floor(log2 t) - 2), codes rounded to nearest even,
-    magnitudes past 6 scales as 6.  A block with a value that is not finite becomes NaN."""
+    magnitudes past 6 scales as 6.  A block with a value that is not finite becomes NaN.
+    Up to 2^35 - 2048 values a call."""
     check_input(x, "quantise", TYPES)
     *lead, K = x.shape if x.dim() else (0,)
     if K % BLOCK or K == 0:
@@ -217,9 +222,9 @@ class Linear:
             raise ValueError(f"Linear: input {tuple(x.shape)} for weights [{self.N}, {self.K}]")
         if values.get_device() != self.index:
             raise ValueError(f"Linear: input on {values.device}, weights on {self.device}")
-        values = rows_of(values, 16)
+        values = rows_of(values, 16, WIDEST)
         if isinstance(x, Mx4):
-            scales = rows_of(x.scales)
+            scales = rows_of(x.scales, 1, WIDEST)
             ldxs = row_stride(scales)
         out = values.new_empty((*lead, self.N), dtype=dtype)
         rows = out.numel() // self.N
@@ -248,7 +253,8 @@ class Experts:
     product's operands: rounded to bf16, or in calls of up to 16 rows and 128 places kept as
     sums of two bf16 (2^-17).  Id -1 is an empty
     place; any other id outside the experts is skipped and raises ``check_errors``.  An
-    expert may come twice in a row."""
+    expert may come twice in a row.  A call takes up to 65,535 rows, whose x and hidden
+    values are each below 2 GiB."""
 
     def __init__(self, gate: Mx4, up: Mx4, down: Mx4):
         if len(gate.shape) != 3 or gate.shape != up.shape or \
@@ -283,7 +289,7 @@ class Experts:
                 raise ValueError(f"Experts: input on {t.device}, weights on {self.device}")
         if rows > 65535:
             raise ValueError(f"Experts: up to 65535 rows a call, got {rows}")
-        x = rows_of(x, 16)
+        x = rows_of(x, 16, ((1 << 30) - 1) // max(rows, 1))
         ids, weights = ids.contiguous(), weights.contiguous()
         k, L = ids.shape[1], lib()
         out = x.new_empty((rows, self.H), dtype=dtype)
