@@ -570,3 +570,24 @@ def test_experts_strided_rows(gpu_device, rows):
     ids, weights = _choice(2 * rows, E, k, 49, gpu_device)
     for x in (wide[:, 8:8 + H], wide[:, 3:3 + H], wide.flip(0)[:, :H], wide[:1, :H].expand(rows, H)):
         _check_experts(ex(x, ids[::2], weights[::2]), x.contiguous(), ids[::2], weights[::2], values)
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("M,K,N", [(2050, 96, 4100), (4001, 160, 8512), (1900, 544, 4500),
+                                   (2048, 128, 4097)])
+def test_linear_last_blocks(gpu_device, M, K, N, both):
+    """Products of a few blocks more than the compute units hold at a time, whose last
+    blocks run in parts: every row and column, with rows and columns that end in each part."""
+    g = torch.Generator(device=gpu_device).manual_seed(M)
+    w = mx4.quantise(torch.randn(N, K, generator=g, device=gpu_device) * 0.05)
+    x = torch.randn(M, K, generator=g, device=gpu_device).to(BF)
+    x64 = x.double()
+    if both:
+        x = mx4.quantise(x)
+        x64 = x.dequantise().double()
+    wt = w.dequantise().double().t().contiguous()
+    want, size = x64 @ wt, x64.abs() @ wt.abs()
+    for dtype in (F32, BF):
+        got = mx4.Linear(w)(x, dtype=dtype).double()
+        bound = torch.finfo(dtype).eps / 2 * want.abs() + 2 * K * 2.0 ** -24 * size
+        assert ((got - want).abs() <= bound * 1.01).all()

@@ -39,6 +39,7 @@ struct Job {
   void* out;
   int64_t ldo;
   int vec;                       // four outputs of a row may go in one store
+  int whole;                     // dense: items before those that run in quarters
   int slices;                    // dense: parts of K, each with its own f32 rows in out
   int64_t slice;                 // floats from one's rows to the next one's
   int64_t second;                // kSwigluTwo: bytes from a hidden row to its second part
@@ -643,25 +644,43 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
   const int ntiles = (a.N + 15) / 16;
   const int nC = (ntiles + 4 * TN - 1) / (4 * TN);
   // Blocks go to the XCDs in turn, and what an XCD's blocks share stays in its L2.  Dense:
-  // an XCD has a run of items, eight row tiles by a few column blocks at a time.  Lists: an
+  // an XCD has a run of items, eight row tiles by a few column blocks at a time, then its
+  // part of the items that run in quarters (64 rows by half the columns).  Lists: an
   // XCD has every eighth row tile with all its columns, so that all get their part of the
   // large ones.
   const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-  int rt, cb, slice = 0;
+  int rt, cb, slice = 0, quarter = -1;
   if (kMode == kListed) {
     rt = local / nC * 8 + xcd;
     cb = local % nC;
     if (rt >= nT) return;
   } else {
-    const int total = nT * nC * a.slices, per = (total + 7) / 8;
+    const int total = nT * nC * a.slices, per = (a.whole + 7) / 8;
     int g = xcd * per + local;
-    if (local >= per || g >= total) return;
+    if (local >= per) {
+      const int parts = 4 * (total - a.whole), part = xcd * ((parts + 7) / 8) + local - per;
+      if (local - per >= (parts + 7) / 8 || part >= parts) return;
+      g = a.whole + part / 4;
+      quarter = part % 4;
+    } else if (g >= a.whole) {
+      return;
+    }
     slice = g / (nT * nC);
     g %= nT * nC;
     const int grp = g / (8 * nC), within = g % (8 * nC);
     const int gm = min(8, nT - grp * 8);
     rt = grp * 8 + within % gm;
     cb = within / gm;
+  }
+  if constexpr (kMode == kDense && TM == 8 && TN == 4) {
+    if (quarter >= 0) {
+      rt = 2 * rt + (quarter & 1);
+      cb = 2 * cb + (quarter >> 1);
+      const RowTile<kMode> r(a, nullptr, rt, 64);
+      if (r.count > 0 && cb * 8 < ntiles)
+        many_item<kX, 4, 2, kMode, kEpi>(a, r, room, cb, slice, lds);
+      return;
+    }
   }
   const RowTile<kMode> r(a, nullptr, rt, 16 * TM);
   // a list's tile may hold fewer rows: it runs as the smallest tile that holds them
@@ -991,17 +1010,22 @@ __global__ __launch_bounds__(kBlock) void k_mx4_sum(const float* __restrict__ pa
 //                  128 takes about 0.8 us for 128 k of bf16 and 0.36 of 4 bits; adding parts
 //                  takes 3.5 us and their f32 rows' way to memory and back at 5 TB/s (65 x
 //                  6144 x 2048: 31 us whole, 15 in 12 parts; 1,000 rows 50 and 35; 65 x 2048 x
-//                  12288 13 and 16, not taken).  Blocks of 128 x 192, which read 15% more for
-//                  a product, where 256 columns leave compute units with one block behind the
-//                  last pair, or a second one (1,024 x 4096 x 8512: 86 us, 72; 2,000 rows 136,
-//                  115; 4,001 rows 230, 239, not taken)
+//                  12288 13 and 16, not taken).  Of blocks of 128 x 256 a few that would run
+//                  behind all others run as quarters, on four times the compute units: up to
+//                  2 / 5 of those behind whole pairs, 1 / 5 behind single blocks, whose second
+//                  place was free (4,001 x 4096 x 8512, 64 behind 1,024: 218 us, 197 in
+//                  quarters, codes 100 and 92; 1,024 rows, 16 behind 256: 86 and 60; 84 behind
+//                  256: 91 in quarters, not taken).  Else blocks of 128 x 192, which read 15%
+//                  more for a product, where 256 columns leave compute units with one block
+//                  behind the last pair, or a second one (1,280 x 4096 x 8512: 76 us)
 struct DensePlan {
   int rows, cols, slices;        // of an item; parts of K
   int64_t items;
+  int rest;                      // the last items, which run in quarters
 };
 DensePlan dense_plan(bool mx, int M, int K, int N) {
   const int cus = compute_units(), kb = mx4_blocks(K), quads = mx4_scale_groups(kb);
-  DensePlan p = {16, 16, 1, (N + 15) / 16};
+  DensePlan p = {16, 16, 1, (N + 15) / 16, 0};
   auto shape = [&](int rows, int cols) {
     p.rows = rows;
     p.cols = cols;
@@ -1022,7 +1046,10 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
       const int64_t n = (items + cus - 1) / cus;
       return n / 2 + (n % 2) * 0.6;
     };
-    if (rounds(narrow) * 3 * 1.15 < 0.9 * rounds(p.items) * 4) shape(128, 192);
+    const int rest = p.items % cus;
+    const bool pairs = p.items / cus % 2 == 0;
+    if (rest * 5 <= cus * (pairs ? 2 : 1)) p.rest = rest;
+    else if (rounds(narrow) * 3 * 1.15 < 0.9 * rounds(p.items) * 4) shape(128, 192);
     return p;
   }
   shape(64, 128);
@@ -1040,11 +1067,13 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
 }
 
 template <int kX, int kEpi>
-int launch_dense(const Job& a, const DensePlan& p, hipStream_t s) {
+int launch_dense(Job a, const DensePlan& p, hipStream_t s) {
   const int cus = compute_units();
   const int64_t items = p.items * a.slices;
   if (items > (1 << 23)) return fail(kBadShape, "mx4_gemm: M=%d N=%d", a.M, a.N);
-  const int few = (int)min(items, (int64_t)4 * cus), many = 8 * (((int)items + 7) / 8);
+  const int few = (int)min(items, (int64_t)4 * cus), rest = (int)p.rest;
+  a.whole = (int)items - rest;
+  const int many = 8 * ((a.whole + 7) / 8 + (4 * rest + 7) / 8);
   const int nT = (a.M + p.rows - 1) / p.rows;
   if (p.rows == 16) k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
   else if (p.rows == 32 && p.cols == 64)
