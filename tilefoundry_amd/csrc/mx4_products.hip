@@ -830,9 +830,10 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
                                                              int* __restrict__ groups) {
   constexpr int kE = TFD_ROUTE_MAX_EXPERTS, kKeep = 16;
   constexpr int kSizes = 8;              // of a tile, in sixteens
-  __shared__ int count[kE], wave_rows[kE / kWave], size_s[kSizes];
+  __shared__ int count[kE], more[kE], wave_rows[kE / kWave], size_s[kSizes];
+  __shared__ uint16_t order_s[kKeep * kGroupThreads];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  if (tid < kE) count[tid] = 0;
+  if (tid < kE) count[tid] = more[tid] = 0;
   if (tid < kSizes) size_s[tid] = 0;
   auto at = [&](int i) {
     return a.ids[a.ldi == a.k ? i : (int64_t)(i / a.k) * a.ldi + i % a.k];
@@ -842,8 +843,9 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
     if (id != -1 && a.err) raise_error(a.err, kErrTokenRange);
     return -1;
   };
-  // a thread's first ids stay in registers for the second pass (all loads before a use)
-  int kept[kKeep];
+  // a thread's first ids, and their places among their expert's, stay in registers for the
+  // second pass (all loads before a use); the others are counted apart, behind them
+  int kept[kKeep], rank[kKeep];
 #pragma unroll
   for (int j = 0; j < kKeep; ++j) kept[j] = at(min(tid + j * kGroupThreads, a.M - 1));
 #pragma unroll
@@ -852,15 +854,15 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
-    if (kept[j] >= 0) atomicAdd(&count[kept[j]], 1);
+    if (kept[j] >= 0) rank[j] = atomicAdd(&count[kept[j]], 1);
   for (int i = tid + kKeep * kGroupThreads; i < a.M; i += kGroupThreads) {
     const int id = valid(at(i));
-    if (id >= 0) atomicAdd(&count[id], 1);
+    if (id >= 0) atomicAdd(&more[id], 1);
   }
   __syncthreads();
   // an expert's rows spread evenly over its tiles, in sixteens: a tile costs by those.  The
   // list has the largest tiles first: the last to start are then the shortest.
-  const int mine = tid < a.E ? count[tid] : 0;
+  const int mine = tid < a.E ? count[tid] + more[tid] : 0;
   const int tiles = (mine + tile_rows - 1) / tile_rows;
   const int even = tiles ? ((mine + tiles - 1) / tiles + 15) / 16 : 0;
   if (tiles) atomicAdd(&size_s[kSizes - even], tiles);
@@ -895,16 +897,28 @@ __global__ __launch_bounds__(kGroupThreads) void k_mx4_group(Job a, int tile_row
       o[1] = f + t * even * 16;
       o[2] = min(even * 16, mine - t * even * 16);
     }
+    more[tid] = f + count[tid];
     count[tid] = f;
   }
+  if (tid == kE - 1) wave_rows[0] = rows_to;
   __syncthreads();
   int* order = groups + 4 + room * 4;
+  // by way of LDS where all are kept: a store to 64 lines takes as many cycles
+  if (a.M <= kKeep * kGroupThreads) {
+    const int entries = wave_rows[0];
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (kept[j] >= 0) order_s[count[kept[j]] + rank[j]] = (uint16_t)(tid + j * kGroupThreads);
+    __syncthreads();
+    for (int i = tid; i < entries; i += kGroupThreads) order[i] = order_s[i];
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < kKeep; ++j)
-    if (kept[j] >= 0) order[atomicAdd(&count[kept[j]], 1)] = tid + j * kGroupThreads;
+    if (kept[j] >= 0) order[count[kept[j]] + rank[j]] = tid + j * kGroupThreads;
   for (int i = tid + kKeep * kGroupThreads; i < a.M; i += kGroupThreads) {
     const int id = at(i);
-    if ((unsigned)id < (unsigned)a.E) order[atomicAdd(&count[id], 1)] = i;
+    if ((unsigned)id < (unsigned)a.E) order[atomicAdd(&more[id], 1)] = i;
   }
 }
 
