@@ -401,10 +401,11 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
 // beside the products of half a stage: with all in flight at once the kernel needs more
 // than the 256 registers at which two blocks share a compute unit.  (DMA into LDS needs
 // none, but every LDS read behind it waits for it.)
-// Measured: 4,001 x 2048 x 12288 of bf16 157 us (1,280 TFLOP/s; a large library product of
-// bf16 reaches 1,413 here), 4,001 x 4096 x 8512 of codes 103 us (2,700 TFLOP/s): there the
-// matrix instructions fill a quarter of the time, and the operands' way from L2 bounds it
-// (narrower blocks, which read more, are slower in proportion).
+// Measured: 4,001 x 2048 x 12288 of bf16 146 to 157 us (1,280 to 1,380 TFLOP/s; 4,096 x 8192 x
+// 8192 1,550; a large library product of bf16 reaches 1,413 here), 4,001 x 4096 x 8512 of
+// codes 92 us (3,000 TFLOP/s): there the matrix instructions fill a third of the time, and
+// the operands' way from L2 bounds it (narrower blocks, which read more, are slower in
+// proportion).
 // ---------------------------------------------------------------------------
 template <int kX, int TM>
 struct ManyLds {
