@@ -695,6 +695,7 @@ __global__ __launch_bounds__(kBlock, TM * TN > 16 ? 2 : 3) void k_mx4_many(Job a
     if (used <= 4) return many_item<kX, 4, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
     if (used == 5) return many_item<kX, 5, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
     if (used == 6) return many_item<kX, 6, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
+    if (used == 7) return many_item<kX, 7, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
   }
   many_item<kX, TM, TN, kMode, kEpi>(a, r, room, cb, slice, lds);
 }
