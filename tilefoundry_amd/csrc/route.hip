@@ -13,13 +13,13 @@ namespace {
 // 64-bit: biased scores of different experts lie as close as an f32 rounding often
 // enough to settle a choice by it.  Groups: a power of two of lanes per group walks
 // it for its two best choices; a group's rank is the number of groups before it.
-// Picks: k rounds of a wave's best (value, then lower index), on the choices as
-// integers in their order: the upper halves' maximum almost always leaves one lane,
-// the lower halves and the index settle the rest.  Reductions stay in registers
+// Picks: k rounds of a wave's best (value, then lower index) of the lanes' sorted
+// choices, as integers in their order: the upper halves' maximum almost always leaves
+// one lane, the lower halves and the index settle the rest.  Reductions stay in registers
 // (DPP and lane swaps).
 // Bound: at one row the launch and the chain of k wave maxima, at thousands of rows the
 // 64-bit exponentials' and the rounds' VALU operations; the logits are read once.  256
-// experts, 8 picks: one row 4.4 us, 4,001 rows in 8 groups 11.6 us.
+// experts, 8 picks: one row 4.1 us, 4,001 rows in 8 groups 9.5 us.
 // ---------------------------------------------------------------------------
 constexpr double kNone = -__builtin_huge_val();
 
@@ -77,13 +77,6 @@ __device__ __forceinline__ uint64_t ordered(double v) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-__device__ __forceinline__ float logit(const TfdRouteArgs& a, int64_t at) {
-  if (a.type == TFD_TYPE_F32) return ((const float*)a.logits)[at];
-  const uint16_t b = ((const uint16_t*)a.logits)[at];
-  if (a.type == TFD_TYPE_BF16) return bf2f(b);
-  return (float)__builtin_bit_cast(_Float16, b);
-}
-
 template <int kPer>
 __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
   __shared__ double c_s[kWavesPerBlock][kPer * kWave];
@@ -92,12 +85,34 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
   if (row >= a.rows) return;
   const int E = a.experts;
   double l[kPer], s[kPer], c[kPer];
+  // every load before a use (past the experts: the last one again)
+  float v[kPer], bias[kPer];
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) bias[j] = a.bias[min(lane + kWave * j, E - 1)];
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) bias[j] = 0.f;
+  }
+  const int64_t first = (int64_t)row * a.ldl;
+  if (a.type == TFD_TYPE_F32) {
+    const float* p = (const float*)a.logits + first;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = p[min(lane + kWave * j, E - 1)];
+  } else {
+    const uint16_t* p = (const uint16_t*)a.logits + first;
+    uint16_t h[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) h[j] = p[min(lane + kWave * j, E - 1)];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      v[j] = a.type == TFD_TYPE_BF16 ? bf2f(h[j]) : (float)__builtin_bit_cast(_Float16, h[j]);
+  }
   float top = -__builtin_huge_valf();
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    const int e = lane + kWave * j;
-    const float v = e < E ? logit(a, (int64_t)row * a.ldl + e) : -__builtin_huge_valf();
-    l[j] = v != v ? kNone : (double)v;               // NaN: as masked
+    const bool in = lane + kWave * j < E && v[j] == v[j];
+    l[j] = in ? (double)v[j] : kNone;                // NaN: as masked
     top = fmaxf(top, (float)l[j]);
   }
   if (a.score == TFD_SCORE_SOFTMAX) {
@@ -109,17 +124,17 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
       s[j] = l[j] == kNone ? 0.0 : l[j] == m ? 1.0 : exp(l[j] - m);
       sum += s[j];
     }
-    sum = wave_sum_d(sum);
+    // (the largest's is one: a sum of zero has nothing to share)
+    const double all = wave_sum_d(sum), inv = all > 0.0 ? 1.0 / all : 0.0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) s[j] = sum > 0.0 ? s[j] / sum : 0.0;
+    for (int j = 0; j < kPer; ++j) s[j] *= inv;
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) s[j] = 1.0 / (1.0 + exp(-l[j]));
   }
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    const int e = lane + kWave * j;
-    const double b = a.bias && e < E ? (double)a.bias[e] : 0.0;
+    const double b = (double)bias[j];
     c[j] = l[j] == kNone || b != b ? kNone : s[j] + b;
   }
   if (a.kept_groups < a.groups) {
@@ -128,12 +143,12 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     const int per = E / a.groups;
-    int L = 1;                                       // lanes per group
-    while (2 * L * a.groups <= kWave) L *= 2;
-    const int g = lane / L;
+    int sh = 0;                                      // of lanes per group
+    while ((2 << sh) * a.groups <= kWave) ++sh;
+    const int L = 1 << sh, g = lane >> sh;
     double b1 = kNone, b2 = kNone;
     if (g < a.groups)
-      for (int i = lane % L; i < per; i += L) {
+      for (int i = lane & (L - 1); i < per; i += L) {
         const double v = c_s[wave][g * per + i];
         b2 = fmax(b2, fmin(b1, v));
         b1 = fmax(b1, v);
@@ -147,36 +162,46 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
     const double best = a.group_top == 2 && b2 != kNone ? b1 + b2 : b1;
     int rank = 0;
     for (int h = 0; h < a.groups; ++h) {
-      const double v = from_lane_d(best, h * L);
+      const double v = from_lane_d(best, h << sh);
       rank += v > best || (v == best && h < g);
     }
     const uint64_t kept = __ballot(g < a.groups && rank < a.kept_groups);
+    // an expert's group: e + 1/2 over `per` lies at least 1/1024 from a whole number, and f32's
+    // error under 512 * 2^-22
+    const float inv = __builtin_amdgcn_rcpf((float)per);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const int e = lane + kWave * j;
-      if (e < E && !((kept >> (e / per * L)) & 1)) c[j] = kNone;
+      const int e = lane + kWave * j, group = (int)(((float)e + 0.5f) * inv);
+      if (e < E && !((kept >> (group << sh)) & 1)) c[j] = kNone;
     }
   }
+  // each lane's keys, largest first (neighbours change places only where the second is
+  // larger: equal ones stay by their ids); the scores wait in LDS for the picks
   uint64_t key[kPer];
+  int id[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) key[j] = ordered(c[j]);
+  for (int j = 0; j < kPer; ++j) {
+    key[j] = ordered(c[j]);
+    id[j] = lane + kWave * j;
+    c_s[wave][id[j]] = s[j];
+  }
+#pragma unroll
+  for (int i = kPer - 1; i > 0; --i)
+#pragma unroll
+    for (int j = 0; j < i; ++j) {
+      const bool swap = key[j + 1] > key[j];
+      const uint64_t k0 = key[j], k1 = key[j + 1];
+      const int i0 = id[j], i1 = id[j + 1];
+      key[j] = swap ? k1 : k0, key[j + 1] = swap ? k0 : k1;
+      id[j] = swap ? i1 : i0, id[j + 1] = swap ? i0 : i1;
+    }
   const uint64_t none = ordered(kNone);
-  double my_s = 0.0, total = 0.0;
   int my_id = -1;
   for (int r = 0; r < a.k; ++r) {
-    // this lane's best (ids grow with j: a tie keeps the first), then the wave's
-    uint64_t best = key[0];
-    double bs = s[0];
-    int bj = 0;
-#pragma unroll
-    for (int j = 1; j < kPer; ++j)
-      if (key[j] > best) {
-        best = key[j];
-        bs = s[j];
-        bj = j;
-      }
-    const uint32_t hi = (uint32_t)(best >> 32), lo = (uint32_t)best;
-    const uint32_t mh = wave_max_u(hi);
+    const uint32_t hi = (uint32_t)(key[0] >> 32), lo = (uint32_t)key[0];
+    const uint32_t mh = __builtin_amdgcn_readfirstlane(wave_max_u(hi));
+    // nothing left that can be chosen (no finite value shares this half)
+    if (mh == (uint32_t)(none >> 32)) break;
     uint64_t who = __ballot(hi == mh);
     if (__popcll(who) > 1) {
       const uint32_t ml = wave_max_u(hi == mh ? lo : 0u);
@@ -184,26 +209,24 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
       if (__popcll(who) > 1) {
         // the same value: the lowest id (as the largest of complements)
         const bool in = (who >> lane) & 1;
-        const uint32_t id = ~(uint32_t)(lane + kWave * bj);
-        const uint32_t mi = wave_max_u(in ? id : 0u);
-        who = __ballot(in && id == mi);
+        const uint32_t other = ~(uint32_t)id[0];
+        const uint32_t mi = wave_max_u(in ? other : 0u);
+        who = __ballot(in && other == mi);
       }
     }
     const int owner = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(who));
-    if (__builtin_amdgcn_readlane(lo, owner) == (uint32_t)none &&
-        __builtin_amdgcn_readlane(hi, owner) == (uint32_t)(none >> 32))
-      break;                                         // nothing left that can be chosen
-    const double ps = from_lane_d(bs, owner);
-    const int id = owner + kWave * __builtin_amdgcn_readlane(bj, owner);
+    const int pick = __builtin_amdgcn_readlane(id[0], owner);
+    if (lane == owner) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (id == lane + kWave * j) key[j] = none;
-    total += ps;
-    if (lane == r) {
-      my_s = ps;
-      my_id = id;
+      for (int j = 0; j + 1 < kPer; ++j) key[j] = key[j + 1], id[j] = id[j + 1];
+      key[kPer - 1] = none;
     }
+    if (lane == r) my_id = pick;
   }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const double my_s = my_id >= 0 ? c_s[wave][my_id] : 0.0;
+  const double total = wave_sum_d(my_s);
   if (lane < a.k + a.shared) {
     double w = my_s * (double)a.scale;
     if (a.renormalise) w = total > 0.0 ? my_s / total * (double)a.scale : 0.0;
