@@ -970,7 +970,7 @@ Plan experts_plan(int rows, int k, int E, int H, int I) {
   // rows by the stream's kernel for few, the longer K the more (64 Granite rows, 9 an expert:
   // 95; tiles of 64 103; 128 rows 134 and 110; 64 Qwen3.5 rows, 2 an expert, 69 and 72; 250
   // rows, 8, 109 and 105); tiles of up to 64 (512 Granite rows 167; tiles of 128 184); of up
-  // to 128 past as many (1,024 Granite rows 278; 64 286).
+  // to 128 past as many (1,024 Granite rows 272; 64 286).
   const int64_t mean = n / E;
   p.tile_rows = mean * 400 <= H ? 16 : mean <= 128 ? 64 : 128;
   p.room = (int)(E + n / p.tile_rows);
