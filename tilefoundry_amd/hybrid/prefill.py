@@ -41,6 +41,7 @@ class _Pass:
 
     policy: int
     fp8: bool
+    mx4 = False                 # 4-bit experts: one call routes, runs and adds them
 
     @staticmethod
     def step_positions(seqs: int) -> int:
