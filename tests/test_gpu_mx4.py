@@ -591,3 +591,21 @@ def test_linear_last_blocks(gpu_device, M, K, N, both):
         got = mx4.Linear(w)(x, dtype=dtype).double()
         bound = torch.finfo(dtype).eps / 2 * want.abs() + 2 * K * 2.0 ** -24 * size
         assert ((got - want).abs() <= bound * 1.01).all()
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1, 2048, 40), (7, 2080, 1000), (16, 2272, 4096), (17, 2048, 33),
+                                   (32, 4128, 2048), (33, 2048, 1360), (33, 2048, 1370),
+                                   (64, 2176, 500)])
+def test_linear_of_few_long_rows(gpu_device, M, K, N, both):
+    """Few rows and columns of a long K: a block of eight waves each, rows in sixteens."""
+    w = _weights(N, K, M + N)
+    x = torch.randn(M, K, generator=_gen(K + M)).to(BF)
+    x64 = x.to(F64)
+    x = x.to(gpu_device)
+    if both:
+        x = mx4.quantise(x)
+        x64 = x.dequantise().cpu().to(F64)
+    lin = mx4.Linear(_to(w, gpu_device))
+    for dtype in (BF, F32):
+        _check_product(lin(x, dtype=dtype), x64, R.values(w.codes, w.scales).to(F64))

@@ -1016,11 +1016,15 @@ __global__ __launch_bounds__(kBlock) void k_mx4_sum(const float* __restrict__ pa
 }
 
 // How a dense product runs.
-//   rows <= 16     items of a column tile
+//   rows <= 16     items of a column tile; where a compute unit has one at most, by eight waves
+//                  (1 x 6144 x 2048 6.4 us by four, 5.6; 16 rows 9.4, 9.0; from a K of 2,048 on:
+//                  1 x 1024 x 2048 3.0, 3.1)
 //   17 .. 64       items of 32 rows by four column tiles, which share the rows' loads, where
 //                  they occupy half the compute units (17 x 4096 x 8512: 11 us; one tile an
-//                  item 18); else one tile an item (17 x 6144 x 2048: 10.0 us; four 12.7, four
-//                  in 12 parts of K and a second launch 11.6)
+//                  item 18); else 16 rows by a column tile, as above, where a compute unit has
+//                  one at most (32 x 6144 x 2048: 9.3 us; 32 rows an item 13.8, four column
+//                  tiles in 12 parts of K and a second launch 11.6); else 32 rows by a column
+//                  tile (40 x 6144 x 2048: 14.3 us; 16 rows 15.8)
 //   more           blocks of 128 x 256, or of 64 x 128 where the large ones leave compute
 //                  units idle, and parts of K where that is estimated to pay: a block of 64 x
 //                  128 takes about 0.8 us for 128 k of bf16 and 0.36 of 4 bits; adding parts
@@ -1051,6 +1055,7 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
   if (M <= 64) {
     shape(32, 64);
     if (p.items < cus / 2) shape(32, 16);
+    if (p.cols == 16 && K >= 2048 && (M + 15) / 16 * ((N + 15) / 16) <= cus) shape(16, 16);
     return p;
   }
   shape(128, 192);
@@ -1091,7 +1096,10 @@ int launch_dense(Job a, const DensePlan& p, hipStream_t s) {
   a.whole = (int)items - rest;
   const int many = 8 * ((a.whole + 7) / 8 + (4 * rest + 7) / 8);
   const int nT = (a.M + p.rows - 1) / p.rows;
-  if (p.rows == 16) k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
+  if (p.rows == 16 && items <= cus && a.K >= 2048)
+    k_mx4_few<kX, 1, 1, 2, kDense, kEpi, 8><<<few, 8 * kWave, 0, s>>>(a);
+  else if (p.rows == 16)
+    k_mx4_few<kX, 1, 1, 4, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
   else if (p.rows == 32 && p.cols == 64)
     k_mx4_few<kX, 2, 4, 2, kDense, kEpi><<<few, kBlock, 0, s>>>(a);
   else if (p.rows == 32)
