@@ -120,8 +120,9 @@ int tfd_route_experts(const TfdRouteArgs* args, void* stream);
  * gate [E I][H] with up [E I][H] as its second matrix, w_down of [E H][I]; H and I multiples
  * of 32, experts <= 512, k <= 64, rows <= 65535, rows * ldx and rows * k * I below 2^30.  Id -1 is an empty place; another id outside
  * the experts is skipped and raises TFD_ERR_TOKEN_RANGE in err (NULL: nothing).  An expert
- * may come twice in a row.  work: tfd_mx4_experts_work_bytes, 256-byte aligned, contents
- * free, one call's at a time. */
+ * may come twice in a row.  work: tfd_mx4_experts_work_bytes, which never falls as rows grow
+ * (one buffer serves its rows and all fewer), 256-byte aligned, contents free, one call's at a
+ * time. */
 typedef struct {
   const void* x;
   int64_t ldx;

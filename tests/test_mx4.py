@@ -304,3 +304,15 @@ def test_run_takes_4_bit_experts_for_granite_alone():
     for synthetic in ("c1", "c2", "c4"):
         with pytest.raises(SystemExit, match="granite"):
             run.main(["--synthetic", synthetic, "--random-prompt", "4", "--experts", "mx4"])
+
+
+@pytest.mark.parametrize("E,k,H,I", [(72, 12, 4096, 768), (256, 8, 2048, 512),
+                                     (14, 12, 1024, 4096), (8, 4, 64, 512), (512, 2, 32, 32),
+                                     (512, 1, 32, 32), (3, 64, 32, 4096), (1, 1, 4096, 32)])
+def test_experts_workspace_covers_fewer_rows(E, k, H, I):
+    """A workspace of `rows` rows serves every call of fewer, which may run in another way:
+    what the entry asks for never falls as rows grow.  (The prompt passes keep one for their
+    largest.)"""
+    need = lib().tfd_mx4_experts_work_bytes
+    sizes = [need(m, k, E, H, I) for m in range(1, 65536)]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))

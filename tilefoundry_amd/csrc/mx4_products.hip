@@ -980,6 +980,16 @@ Plan experts_plan(int rows, int k, int E, int H, int I) {
   p.bytes = p.groups + (p.fused ? 0 : up((4 + 4 * (int64_t)p.room + n) * 4));
   return p;
 }
+// Bytes for `rows` and for every smaller call, which may run in another way and need more:
+// the most rows that run fused hold two hidden parts, and tiles of 16 the longest list.
+int64_t experts_work(int rows, int k, int E, int H, int I) {
+  const int64_t fused = experts_plan(min(min(rows, kHereRows), kHereMax / k), k, E, H, I).bytes;
+  const Plan p = experts_plan(rows, k, E, H, I);
+  if (p.fused) return fused;
+  const int64_t n = (int64_t)rows * k, list = (4 + 4 * (E + n / 16) + n) * 4;
+  const int64_t listed = p.groups + (list + 255) / 256 * 256;
+  return fused > listed ? fused : listed;          // (the host's max takes ints)
+}
 
 template <int TM, int TN>
 void launch_listed(const Job& gu, const Job& down, int tiles, hipStream_t s) {
@@ -1181,7 +1191,7 @@ extern "C" {
 
 int64_t tfd_mx4_experts_work_bytes(int rows, int k, int experts, int H, int I) {
   if (rows <= 0 || k <= 0 || experts <= 0 || H <= 0 || I <= 0) return 0;
-  return experts_plan(rows, k, experts, H, I).bytes;
+  return experts_work(rows, k, experts, H, I);
 }
 
 int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {

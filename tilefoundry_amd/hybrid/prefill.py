@@ -94,9 +94,7 @@ class _Pass:
         self.rw, self.ridx = z(R, n, dtype=F32), z(R, n, dtype=I32)
         if self.mx4:
             E = c.experts + self.e.shared
-            # a call of fewer rows may run in another way, which needs less for each row
-            self.mx4_bytes = max(self._lib.tfd_mx4_experts_work_bytes(m, n, E, H, c.moe_inter)
-                                 for m in {min(R, 16), R})
+            self.mx4_bytes = self._lib.tfd_mx4_experts_work_bytes(R, n, E, H, c.moe_inter)
             self.mx4_work = z(self.mx4_bytes, dtype=torch.uint8)
         else:
             self.groups = z(_lib.panel_moe_words(c.experts, R * k), dtype=I32)
