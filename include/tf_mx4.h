@@ -51,7 +51,7 @@ int tfd_mx4_pack(const void* codes, const void* scales, const void* codes2, cons
                  int64_t N, int K, void* packed, void* stream);
 
 /* out[m][n] = sum_k x[m][k] W[n][k], f32 sums, each output rounded once to f32 or bf16
- * (out_type).  W packed by tfd_mx4_pack ([N][K]).  x: bf16 [M][ldx], or mx4 with x_scales
+ * (out_type).  W packed by tfd_mx4_pack ([N][K], N up to 2^24, K up to 2^22).  x: bf16 [M][ldx], or mx4 with x_scales
  * set (codes [M][ldx bytes], scales [M][ldxs]); rows 16-byte aligned, ldx and ldxs up to
  * 2^23.  The 4-bit counterpart of tfd_gemm_skinny_bf16 / tfd_panel_gemm_bf16 for any M, N
  * and K a multiple of 32, on plain rows.  work (may be NULL): with tfd_mx4_gemm_work_bytes of it, 16-byte
@@ -118,7 +118,7 @@ int tfd_route_experts(const TfdRouteArgs* args, void* stream);
  * shared experts are experts that every row picks (tfd_route_experts appends them).
  * x bf16 [rows][ldx], rows 16-byte aligned; ids / weights [rows][ld]; w_gu = tfd_mx4_pack of
  * gate [E I][H] with up [E I][H] as its second matrix, w_down of [E H][I]; H and I multiples
- * of 32, experts <= 512, k <= 64, rows <= 65535, rows * ldx and rows * k * I below 2^30.  Id -1 is an empty place; another id outside
+ * of 32 up to 2^20, experts <= 512, k <= 64, rows <= 65535, rows * ldx and rows * k * I below 2^30.  Id -1 is an empty place; another id outside
  * the experts is skipped and raises TFD_ERR_TOKEN_RANGE in err (NULL: nothing).  An expert
  * may come twice in a row.  work: tfd_mx4_experts_work_bytes, which never falls as rows grow
  * (one buffer serves its rows and all fewer), 256-byte aligned, contents free, one call's at a

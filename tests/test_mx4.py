@@ -316,3 +316,33 @@ def test_experts_workspace_covers_fewer_rows(E, k, H, I):
     need = lib().tfd_mx4_experts_work_bytes
     sizes = [need(m, k, E, H, I) for m in range(1, 65536)]
     assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
+def _far(*shape, dtype=torch.float32):
+    """One element seen as a tensor of that shape: sizes without the memory."""
+    return torch.zeros(1, dtype=dtype).expand(*shape)
+
+
+PAST = 2 ** 32 + 32                 # 32 where 32 bits are kept
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Dimensions that the C entries take as 32-bit integers: cut to those they would name a
+    smaller tensor, of which the kernels would compute a part and leave the rest unwritten."""
+    u8 = torch.uint8
+
+    def far(*shape):
+        return mx4.Mx4(_far(*shape[:-1], shape[-1] // 2, dtype=u8),
+                       _far(*shape[:-1], shape[-1] // 32, dtype=u8))
+
+    for K in (2 ** 31, PAST):
+        with pytest.raises(ValueError, match="last dimension"):
+            mx4.quantise(_far(1, K))
+        with pytest.raises(ValueError, match="last dimension"):
+            far(1, K).dequantise()
+    for N, K in ((16, PAST), (PAST, 32), (2 ** 24 + 1, 32), (16, 2 ** 22 + 32)):
+        with pytest.raises(ValueError, match="Linear: weights of up to"):
+            mx4.Linear(far(N, K))
+    for H, I in ((PAST, 32), (32, PAST), (2 ** 20 + 32, 32), (32, 2 ** 20 + 32)):
+        with pytest.raises(ValueError, match="Experts: hidden and width"):
+            mx4.Experts(far(2, I, H), far(2, I, H), far(2, H, I))

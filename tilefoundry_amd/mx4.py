@@ -59,6 +59,17 @@ def check_device(device, *others) -> None:
             raise ValueError(f"tensors on {device} and on {t.device}")
 
 
+# what the C entries take as 32-bit integers (ctypes would cut a larger one to its low bits)
+LONGEST = (1 << 31) - 1                      # values of a row
+MAX_K, MAX_N = 1 << 22, 1 << 24              # of a product
+MAX_EXPERT = 1 << 20                         # hidden columns, an expert's width
+
+
+def check_row(K: int, what: str) -> None:
+    if K > LONGEST:
+        raise ValueError(f"{what}: the last dimension must be below 2^31, got {K}")
+
+
 WIDEST = 1 << 23                             # elements between rows that a product takes
 
 
@@ -131,10 +142,11 @@ class Mx4:
         if dtype not in TYPES:
             raise ValueError(f"dequantise: dtype {dtype} is not one of "
                              f"{', '.join(str(d) for d in TYPES)}")
+        shape = self.shape
+        check_row(shape[-1], "dequantise")
         codes, scales = rows_of(self.codes, 4), rows_of(self.scales)
         if not codes.is_cuda:
             check_device(codes.device)
-        shape = self.shape
         out = codes.new_empty(shape, dtype=dtype)
         K = shape[-1]
         launch(codes.get_device(), lib().tfd_mx4_dequantise, ptr(codes), row_stride(codes), ptr(scales),
@@ -146,12 +158,13 @@ def quantise(x: torch.Tensor) -> Mx4:
     """Rows ``[..., K]`` (f32, bf16 or f16, K a multiple of 32) to mx4: for 32 values with
     largest magnitude t the scale 2^(floor(log2 t) - 2), codes rounded to nearest even,
     magnitudes past 6 scales as 6.  A block with a value that is not finite becomes NaN.
-    Up to 2^35 - 2048 values a call."""
+    Up to 2^35 - 2048 values a call, rows below 2^31."""
     check_input(x, "quantise", TYPES)
     *lead, K = x.shape if x.dim() else (0,)
     if K % BLOCK or K == 0:
         raise ValueError(f"quantise: the last dimension must be a multiple of {BLOCK}, got "
                          f"{tuple(x.shape)}")
+    check_row(K, "quantise")
     if not x.is_cuda:
         check_device(x.device)
     codes = x.new_empty((*lead, K // 2), dtype=U8)
@@ -204,6 +217,8 @@ class Linear:
         if len(weight.shape) != 2:
             raise ValueError(f"Linear: weights must be [N, K], got {weight.shape}")
         self.N, self.K = weight.shape
+        if self.N > MAX_N or self.K > MAX_K:
+            raise ValueError(f"Linear: weights of up to {MAX_N} x {MAX_K}, got {weight.shape}")
         self.device = weight.device
         self.packed = _pack(weight, None, "Linear")
         self.index = self.packed.get_device()
@@ -264,6 +279,9 @@ class Experts:
         self.E, self.I, self.H = gate.shape
         if not 1 <= self.E <= _lib.ROUTE_MAX_EXPERTS:
             raise ValueError(f"Experts: 1 to {_lib.ROUTE_MAX_EXPERTS} experts, got {self.E}")
+        if self.H > MAX_EXPERT or self.I > MAX_EXPERT:
+            raise ValueError(f"Experts: hidden and width up to {MAX_EXPERT}, got {self.H} and "
+                             f"{self.I}")
         check_device(gate.device, up.codes, down.codes)
         self.device = gate.device
         self.w_gu = _pack(gate, up, "Experts")
