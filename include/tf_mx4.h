@@ -90,8 +90,8 @@ int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream);
  * of zero gives weights of zero.  `shared` places follow each row's picks: ids experts,
  * experts + 1, ..., weight 1 (tfd_mx4_experts then adds the shared experts with the rest).
  * logits f32, bf16 or f16 [rows][ldl]; weights f32 and ids int32 [rows][ld], ld >= k + shared.
- * experts <= 512, groups <= 64 and a divisor of experts, k + shared <= 64, k <= kept_groups *
- * experts / groups. */
+ * rows <= 67,108,860, experts <= 512, groups <= 64 and a divisor of experts, k + shared <= 64,
+ * k <= kept_groups * experts / groups. */
 #define TFD_SCORE_SOFTMAX 0
 #define TFD_SCORE_SIGMOID 1
 #define TFD_ROUTE_MAX_EXPERTS 512

@@ -346,3 +346,20 @@ def test_sizes_past_32_bits_are_refused():
     for H, I in ((PAST, 32), (32, PAST), (2 ** 20 + 32, 32), (32, 2 ** 20 + 32)):
         with pytest.raises(ValueError, match="Experts: hidden and width"):
             mx4.Experts(far(2, I, H), far(2, I, H), far(2, H, I))
+
+
+def test_routing_refuses_rows_past_a_launch():
+    """Four rows a block of 256 threads, and a launch's threads have 32 bits; from 2^32 rows
+    on an integer of the entry would hold the rest of them."""
+    most = 4 * ((2 ** 32 - 256) // 256)
+    rule = routing.Routing(top_k=1)
+    for rows in (most + 1, 2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match=f"up to {most} rows"):
+            rule(_far(rows, 2))
+    with pytest.raises(ValueError, match="GPU"):
+        rule(_far(most, 2))
+    for rows in (most + 1, 2 ** 31 - 1):
+        a = _lib.TfdRouteArgs(logits=PTR, ldl=2, rows=rows, experts=2, k=1, groups=1,
+                              kept_groups=1, group_top=2, scale=1.0, weights=PTR, ids=PTR, ld=1)
+        with pytest.raises(TFDError, match="rows="):
+            lib().tfd_route_experts(ctypes.addressof(a), None)

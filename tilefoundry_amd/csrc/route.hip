@@ -236,6 +236,9 @@ __global__ __launch_bounds__(kBlock) void k_route_experts(TfdRouteArgs a) {
   }
 }
 
+// Threads of one launch, in whole blocks, have 32 bits.
+constexpr int kMaxRows = kWavesPerBlock * (int)((((int64_t)1 << 32) - kBlock) / kBlock);
+
 }  // namespace
 
 extern "C" int tfd_route_experts(const TfdRouteArgs* args, void* stream) {
@@ -245,9 +248,9 @@ extern "C" int tfd_route_experts(const TfdRouteArgs* args, void* stream) {
     return fail(kBadArg, "route_experts: type %d", a.type);
   if (a.score != TFD_SCORE_SOFTMAX && a.score != TFD_SCORE_SIGMOID)
     return fail(kBadArg, "route_experts: score %d", a.score);
-  if (a.experts < 1 || a.experts > TFD_ROUTE_MAX_EXPERTS || a.rows < 0)
-    return fail(kBadShape, "route_experts: rows=%d experts=%d (1..%d)", a.rows, a.experts,
-                TFD_ROUTE_MAX_EXPERTS);
+  if (a.experts < 1 || a.experts > TFD_ROUTE_MAX_EXPERTS || a.rows < 0 || a.rows > kMaxRows)
+    return fail(kBadShape, "route_experts: rows=%d (0..%d) experts=%d (1..%d)", a.rows, kMaxRows,
+                a.experts, TFD_ROUTE_MAX_EXPERTS);
   if (a.groups < 1 || a.groups > kWave || a.experts % a.groups || a.kept_groups < 1 ||
       a.kept_groups > a.groups || (a.group_top != 1 && a.group_top != 2))
     return fail(kBadShape, "route_experts: %d experts in %d groups, %d kept by their best %d",

@@ -22,6 +22,7 @@ from . import _lib
 from ._lib import lib, ptr
 from .mx4 import FLOAT32, TYPES, check_device, check_input, launch, row_stride, rows_of
 
+MAX_ROWS = 4 * ((1 << 24) - 1)          # blocks of four rows, 32 bits of threads in a launch
 SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
 
@@ -66,6 +67,8 @@ class Routing:
         if logits.dim() != 2:
             raise ValueError(f"logits must be [rows, experts], got {tuple(logits.shape)}")
         rows, experts = logits.shape
+        if rows > MAX_ROWS:
+            raise ValueError(f"routing: up to {MAX_ROWS} rows a call, got {rows}")
         if not 1 <= experts <= _lib.ROUTE_MAX_EXPERTS or experts % self.groups:
             raise ValueError(f"{experts} experts: 1 to {_lib.ROUTE_MAX_EXPERTS}, a multiple of "
                              f"{self.groups} groups")
