@@ -363,3 +363,30 @@ def test_routing_refuses_rows_past_a_launch():
                               kept_groups=1, group_top=2, scale=1.0, weights=PTR, ids=PTR, ld=1)
         with pytest.raises(TFDError, match="rows="):
             lib().tfd_route_experts(ctypes.addressof(a), None)
+
+
+def test_forward_mode_inputs_are_refused():
+    """A tangent would be dropped without a word; a detached input, or no_grad with a plain
+    one, is taken as far as the device's check."""
+    from torch.autograd import forward_ad
+
+    rule = routing.Routing(top_k=2)
+    ex, ids = _NoGpu.experts(4, 64, 32), torch.zeros(3, 2, dtype=torch.int32)
+    x, w = torch.zeros(3, 64), torch.zeros(3, 2)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in [lambda: mx4.quantise(dual(x)), lambda: _NoGpu.linear(3, 64)(dual(x.to(BF))),
+                     lambda: rule(dual(x)), lambda: rule(x, dual(torch.zeros(64))),
+                     lambda: ex(dual(x.to(BF)), ids, w), lambda: ex(x.to(BF), ids, dual(w))]:
+            with pytest.raises(ValueError, match="gradients"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="gradients"):
+                call()
+        with pytest.raises(ValueError, match="GPU"):
+            mx4.quantise(dual(x).detach())
+        with pytest.raises(ValueError, match="GPU"):
+            mx4.quantise(x)
+    with pytest.raises(ValueError, match="gradients"):
+        torch.func.jvp(mx4.quantise, (x,), (x,))

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import lib, ptr
@@ -49,6 +50,9 @@ def check_input(x, what: str, dtypes) -> None:
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: these operators compute no gradients; detach it or work "
                          "under torch.no_grad()")
+    # (a dual tensor keeps its tangent under no_grad too; without a level there is none)
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"{what}: these operators compute no gradients; detach it")
 
 
 def check_device(device, *others) -> None:
