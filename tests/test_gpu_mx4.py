@@ -609,3 +609,29 @@ def test_linear_of_few_long_rows(gpu_device, M, K, N, both):
     lin = mx4.Linear(_to(w, gpu_device))
     for dtype in (BF, F32):
         _check_product(lin(x, dtype=dtype), x64, R.values(w.codes, w.scales).to(F64))
+
+
+# -------------------------------------------------------------- other streams
+def _busy(dev):
+    """Work of some 100 ms on the current stream."""
+    a = torch.ones(8192, 8192, device=dev)
+    for _ in range(16):
+        torch.mm(a, a)
+
+
+def test_experts_errors_of_another_stream(gpu_device):
+    """check_errors waits for calls of every stream, not for the current one's alone."""
+    ex, _ = _experts(4, 64, 32, 60, gpu_device)
+    x = torch.randn(5, 64, generator=_gen(61)).to(BF).to(gpu_device)
+    ids, weights = _choice(5, 4, 3, 62, gpu_device)
+    ids[2, 1] = 4
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        _busy(gpu_device)
+        y = ex(x, ids, weights)
+    with pytest.raises(RuntimeError, match="id outside"):
+        ex.check_errors()
+    assert side.query()
+    ex.check_errors()
+    assert y.isfinite().all()

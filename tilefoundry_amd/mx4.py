@@ -328,7 +328,8 @@ class Experts:
 
     def check_errors(self) -> None:
         """Raises if a call since the last check met an id outside the experts (waits for
-        the device)."""
+        the device: calls may be on any stream)."""
+        torch.cuda.synchronize(self.device)
         if int(self.err.item()):
             self.err.zero_()
             raise RuntimeError("mx4 experts: an id outside the experts (and not -1) was skipped")
