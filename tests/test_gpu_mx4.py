@@ -635,3 +635,25 @@ def test_experts_errors_of_another_stream(gpu_device):
     assert side.query()
     ex.check_errors()
     assert y.isfinite().all()
+
+
+def test_handles_made_on_another_stream(gpu_device):
+    """A handle's weights are laid out once it is there, whichever stream calls it first."""
+    parts = [mx4.quantise((torch.randn(6, *s, generator=_gen(63)) * 0.1).to(gpu_device))
+             for s in [(96, 256), (96, 256), (256, 96)]]
+    w = mx4.quantise((torch.randn(700, 256, generator=_gen(64)) * 0.1).to(gpu_device))
+    x = torch.randn(40, 256, generator=_gen(65)).to(BF).to(gpu_device)
+    ids, weights = _choice(40, 6, 3, 66, gpu_device)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for make, args in ((lambda: mx4.Linear(w), (x,)),
+                       (lambda: mx4.Experts(*parts), (x, ids, weights))):
+        with torch.cuda.stream(side):
+            _busy(gpu_device)
+            handle = make()
+        got.append(handle(*args))
+        torch.cuda.synchronize()
+        assert torch.equal(got[-1], handle(*args))
+    _check_experts(got[1], x, ids, weights, [p.dequantise().double() for p in parts])
+    _check_product(got[0], x.cpu().to(F64), w.dequantise().double().cpu())

@@ -200,6 +200,14 @@ def _pack(first: Mx4, second: Mx4 | None, what: str) -> torch.Tensor:
     return packed
 
 
+def _settle(device) -> None:
+    """Waits, at load time, for what the current stream makes of a handle: its first call may
+    be on another one.  (A handle made inside a capture is that graph's.)"""
+    with torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream().synchronize()
+
+
 BF16, INT32, FLOAT32 = (torch.bfloat16,), (torch.int32,), (torch.float32,)
 MAX_ROWS = 1 << 30
 OUT_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16}
@@ -226,6 +234,7 @@ class Linear:
         self.device = weight.device
         self.packed = _pack(weight, None, "Linear")
         self.index = self.packed.get_device()
+        _settle(self.device)
 
     def __call__(self, x, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         kind = _out_type(dtype, "Linear")
@@ -292,6 +301,7 @@ class Experts:
         self.w_down = _pack(down, None, "Experts")
         self.index = self.w_gu.get_device()
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        _settle(self.device)
 
     def __call__(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
                  dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
