@@ -72,6 +72,10 @@ typedef struct {
   int64_t work_bytes;
 } TfdMx4GemmArgs;
 int64_t tfd_mx4_gemm_work_bytes(int M, int K, int N);
+/* How a product of these sizes runs on the current device, for tests and measurements: form =
+ * rows and columns of a block's outputs, parts of K (with work), and the last blocks that run
+ * in quarters.  x_mx4 != 0: microscaled rows. */
+int tfd_mx4_gemm_form(int x_mx4, int M, int K, int N, int32_t form[4]);
 int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream);
 
 /* The choice of experts after the router's projection.  Replaces the two fixed routers of
@@ -141,6 +145,9 @@ typedef struct {
   int32_t* err;
 } TfdMx4ExpertsArgs;
 int64_t tfd_mx4_experts_work_bytes(int rows, int k, int experts, int H, int I);
+/* How a call runs, for tests and measurements: an expert's rows in tiles of up to 16, 64 or
+ * 128, or 0 for the two launches of few rows (sizes as tfd_mx4_experts takes them, else -1). */
+int tfd_mx4_experts_tile_rows(int rows, int k, int experts, int H, int I);
 int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream);
 
 #ifdef __cplusplus

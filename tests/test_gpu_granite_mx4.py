@@ -91,3 +91,47 @@ def test_mx4_engine_refuses():
         with pytest.raises(ValueError, match="4-bit experts"):
             mx4_shared(GraniteConfig(**bad))
     assert mx4_shared(GraniteConfig()) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,tile", [(9, 0), (24, 16), (100, 64), (400, 128)])
+def test_mx4_moe_of_a_step_and_of_passes(gpu_device, M, tile):
+    """The engine's routing and experts added into a stream, in each way that a call may run,
+    against 64 bits from the engine's own fp8 weights, with the shared MLP as one."""
+    from tests import _mx4_ref as R
+    from tests.test_gpu_mx4 import _check_experts
+
+    cfg = GraniteConfig(experts=12, top_k=4, layers=2, attention_layers=(1,), vocab=4096)
+    w = _weights(cfg, 11, gpu_device)
+    eng = GraniteEngine(cfg, w, rows=1, device=gpu_device, max_steps=32, graph=False,
+                        experts="mx4")
+    E, n, k, H, I = cfg.experts, eng.shared, eng.picks, cfg.hidden, cfg.moe_inter
+    assert (n, k) == (2, 6)
+    assert eng._lib.tfd_mx4_experts_tile_rows(M, k, E + n, H, I) == tile
+
+    def f64(name, scale):
+        return w[f"layer0.{name}"].view(torch.float8_e4m3fn).double() * \
+            w[f"layer0.{scale}"].double().unsqueeze(1)
+
+    gate_s, up_s = f64("w_shared_in", "w_shared_in_scale").split(n * I)
+    down_s = f64("w_shared_out", "w_shared_out_scale")
+    values = [torch.cat((f64("w_gate", "s_gate").view(E, I, H), gate_s.view(n, I, H))),
+              torch.cat((f64("w_up", "s_up").view(E, I, H), up_s.view(n, I, H))),
+              torch.cat((f64("w_down", "s_down").view(E, H, I),
+                         torch.stack(down_s.split(I, dim=1))))]
+    g = torch.Generator(device=gpu_device).manual_seed(M)
+
+    def draw(*shape):
+        return torch.randn(*shape, generator=g, device=gpu_device)
+
+    x, logits, stream = draw(M, H).bfloat16(), draw(M, E), draw(M, H).bfloat16()
+    before, weights = stream.clone(), torch.empty(M, k, device=gpu_device)
+    ids = torch.empty(M, k, dtype=torch.int32, device=gpu_device)
+    need = eng._lib.tfd_mx4_experts_work_bytes(M, k, E + n, H, I)
+    work = torch.empty(need, dtype=torch.uint8, device=gpu_device)
+    eng.mx4_moe(eng.layers[0], M, x, logits, weights, ids, stream, work, need, eng._stream())
+    eng.check_errors()
+    want_w, want_i = R.route(logits, None, k=cfg.top_k, score="softmax", shared=n)
+    assert torch.equal(ids.cpu(), want_i)
+    assert ((weights.cpu().double() - want_w).abs() <= want_w * 2.0 ** -23).all()
+    _check_experts(stream, x, ids, weights, values, mult=cfg.residual_multiplier, start=before)

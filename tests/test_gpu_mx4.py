@@ -657,3 +657,255 @@ def test_handles_made_on_another_stream(gpu_device):
         assert torch.equal(got[-1], handle(*args))
     _check_experts(got[1], x, ids, weights, [p.dequantise().double() for p in parts])
     _check_product(got[0], x.cpu().to(F64), w.dequantise().double().cpu())
+
+
+# --------------------------------------- forms that few of the sizes above choose
+def _form(M, K, N, both):
+    """Rows and columns of a block, parts of K, blocks that run in quarters."""
+    import ctypes
+
+    from tilefoundry_amd._lib import lib
+
+    form = (ctypes.c_int32 * 4)()
+    lib().tfd_mx4_gemm_form(int(both), M, K, N, form)
+    return list(form)
+
+
+def _tile_rows(rows, E, k, H, I):
+    from tilefoundry_amd._lib import lib
+
+    return lib().tfd_mx4_experts_tile_rows(rows, k, E, H, I)
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("M,K,N", [(1270, 544, 8500), (1200, 288, 8300), (1152, 96, 9600),
+                                   (1153, 1312, 8449)])
+def test_linear_of_192_columns(gpu_device, M, K, N, both):
+    """Blocks of 128 x 192: the last column block part full, rows that end inside a tile, K that
+    is no multiple of a block; every output."""
+    assert _form(M, K, N, both) == [128, 192, 1, 0]
+    g = torch.Generator(device=gpu_device).manual_seed(M)
+    w = mx4.quantise(torch.randn(N, K, generator=g, device=gpu_device) * 0.05)
+    x = torch.randn(M, K, generator=g, device=gpu_device).to(BF)
+    x64 = x.double()
+    if both:
+        x = mx4.quantise(x)
+        x64 = x.dequantise().double()
+    wt = w.dequantise().double().t().contiguous()
+    want, size = x64 @ wt, x64.abs() @ wt.abs()
+    lin = mx4.Linear(w)
+    for dtype in (F32, BF):
+        got = lin(x, dtype=dtype)
+        bound = torch.finfo(dtype).eps / 2 * want.abs() + 2 * K * 2.0 ** -24 * size
+        assert ((got.double() - want).abs() <= bound * 1.01).all()
+        assert torch.equal(got, lin(x, dtype=dtype))
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("M,K,N", [(66, 2176, 70), (128, 6144, 260), (300, 4128, 513)])
+def test_linear_in_parts(gpu_device, M, K, N, both):
+    """Products that do split K, with their work and without."""
+    import ctypes
+
+    from tilefoundry_amd import _lib
+    from tilefoundry_amd._lib import lib, ptr
+
+    assert _form(M, K, N, both)[2] > 1
+    w = mx4.quantise((torch.randn(N, K, generator=_gen(K)) * 0.05).to(gpu_device))
+    x = torch.randn(M, K, generator=_gen(M)).to(BF).to(gpu_device)
+    given = mx4.quantise(x) if both else x
+    x64 = (given.dequantise() if both else x).double().cpu()
+    w64 = w.dequantise().double().cpu()
+    lin = mx4.Linear(w)
+    need = lib().tfd_mx4_gemm_work_bytes(M, K, N)
+    rows, scales = (given.codes, given.scales) if both else (x, None)
+    for size in (need, 0):
+        work = torch.full((need + 64,), 255, dtype=torch.uint8, device=gpu_device)
+        out = torch.full((M + 1, N + 3), 7.0, device=gpu_device)
+        a = _lib.TfdMx4GemmArgs(ptr(rows), rows.shape[1], ptr(scales), K // 32 if both else 0,
+                                ptr(lin.packed), M, K, N, ptr(out), N + 3, _lib.TYPE_F32,
+                                ptr(work) if size else None, size)
+        lib().tfd_mx4_gemm(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream)
+        _check_product(out[:M, :N], x64, w64)
+        assert (out[M:] == 7).all() and (out[:, N:] == 7).all()
+        assert (work[need:] == 255).all()
+        if size:
+            assert torch.equal(lin(given, dtype=F32), out[:M, :N])
+
+
+# lists in tiles of 16: many experts, few rows each; H and I end inside a block of 128
+LISTS = [(40, 64, 4, 1056, 96), (64, 72, 10, 4096, 160), (100, 300, 3, 416, 32)]
+
+
+def _crowded(ids):
+    """Some experts with more rows than a tile of 16: the first place of 17 rows, the second
+    of 33."""
+    ids = ids.clone()
+    ids[:17, 0], ids[:33, 1] = 3, 5
+    return ids
+
+
+@pytest.mark.parametrize("rows,E,k,H,I", LISTS)
+def test_experts_in_lists_of_16(gpu_device, rows, E, k, H, I):
+    assert _tile_rows(rows, E, k, H, I) == 16
+    ex, values = _experts(E, H, I, 70, gpu_device)
+    x = torch.randn(rows, H, generator=_gen(71)).to(BF).to(gpu_device)
+    ids, weights = _choice(rows, E, k, 72, gpu_device)
+    ids = _crowded(ids)
+    for dtype in (BF, F32):
+        got = ex(x, ids, weights, dtype=dtype)
+        _check_experts(got, x, ids, weights, values)
+        assert torch.equal(got, ex(x, ids, weights, dtype=dtype))
+    # against the definition, row by row, of which _check_experts is another writing.  `size` is
+    # the sum with every magnitude in it: as t <= 2 silu(t) for t >= 0, |h| is at most twice its
+    # hidden value.  Both sides round h to bf16, next to a border to either side: 2 * 2^-8 of h.
+    # Sums' roundings: 2 H 2^-24 of the magnitudes in a (slope of the SiLU up to 1.1) and in b,
+    # 2 I 2^-24 of those in y, under 8 (H + I) 2^-24 of 2 size together
+    pick = torch.tensor([0, 16, 32, rows - 1], device=gpu_device)
+    got = ex(x, ids, weights, dtype=F32)[pick].cpu().double()
+    v = [t.cpu() for t in values]
+    want = R.experts(x[pick], ids[pick], weights[pick], *v)
+    size = R.experts(x[pick].abs(), ids[pick], weights[pick].abs(), *[t.abs() for t in v],
+                     hidden_dtype=None)
+    assert ((got - want).abs() <= 2 * size * (2.0 ** -7 + 8 * (H + I) * 2.0 ** -24)).all()
+    # empty places, rows of nothing else, an expert several times in a row, one for all rows
+    for seed, empty, repeat in [(1, 0.4, False), (2, 0.0, True), (3, 0.7, True)]:
+        ids, weights = _choice(rows, E, k, seed, gpu_device, empty, repeat)
+        ids[rows // 2] = -1
+        got = ex(x, ids, weights)
+        _check_experts(got, x, ids, weights, values)
+        assert (got[rows // 2] == 0).all()
+    for only in (0, E - 1):
+        ids.fill_(only)
+        _check_experts(ex(x, ids, weights), x, ids, weights, values)
+    ids.fill_(-1)
+    weights.fill_(math.nan)
+    assert (ex(x, ids, weights) == 0).all()
+    ex.check_errors()
+
+
+@pytest.mark.parametrize("rows,E,k,H,I", LISTS)
+def test_experts_in_lists_of_16_hard_rows(gpu_device, rows, E, k, H, I):
+    """Ids outside the experts, values that are not finite, rows and places out of wider
+    tensors, and the C entry that adds into padded rows."""
+    import ctypes
+
+    from tilefoundry_amd import _lib
+    from tilefoundry_amd._lib import lib, ptr
+
+    assert _tile_rows(rows, E, k, H, I) == 16
+    ex, values = _experts(E, H, I, 73, gpu_device)
+    base = torch.full((rows, H + 64), math.nan, dtype=BF)
+    base[:, 16:16 + H] = torch.randn(rows, H, generator=_gen(74)).to(BF)
+    base[0, 20], base[3, 30] = math.nan, math.inf
+    x = base.to(gpu_device)[:, 16:16 + H]
+    ids, weights = _choice(2 * rows, E, k, 75, gpu_device)
+    ids, weights = ids[::2], weights[::2]
+    crowd = _crowded(ids)
+    got = ex(x, crowd, weights, dtype=F32)
+    keep = torch.tensor([r for r in range(rows) if r not in (0, 3)], device=gpu_device)
+    assert got[0].isnan().all() and not got[3].isfinite().any()
+    _check_experts(got[keep], x[keep], crowd[keep], weights[keep], values)
+    clean = x.clone()
+    clean[0], clean[3] = clean[1], clean[2]
+    for bad in (E, -2, 2 ** 31 - 1, -2 ** 31):
+        wrong = crowd.clone()
+        wrong[rows - 1, 1] = bad
+        _check_experts(ex(clean, wrong, weights), clean, wrong, weights, values)
+        with pytest.raises(RuntimeError, match="id outside"):
+            ex.check_errors()
+    wide_i = torch.full((rows, k + 2), 999, dtype=torch.int32, device=gpu_device)
+    wide_w = torch.full((rows, k + 2), math.nan, device=gpu_device)
+    wide_i[:, :k], wide_w[:, :k] = crowd, weights
+    need = lib().tfd_mx4_experts_work_bytes(rows, k, E, H, I)
+    work = torch.full((need + 256,), 255, dtype=torch.uint8, device=gpu_device)
+    for dtype, kind in ((BF, _lib.TYPE_BF16), (F32, _lib.TYPE_F32)):
+        for accumulate in (0, 1):
+            out = torch.randn(rows + 2, H + 6, generator=_gen(76)).to(dtype).to(gpu_device)
+            before = out.clone()
+            a = _lib.TfdMx4ExpertsArgs(ptr(clean), H, ptr(wide_i), ptr(wide_w), k + 2,
+                                       ptr(ex.w_gu), ptr(ex.w_down), rows, k, E, H, I, ptr(out),
+                                       H + 6, kind, accumulate, 0.22, ptr(work), need, None)
+            lib().tfd_mx4_experts(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream)
+            _check_experts(out[:rows, :H], clean, crowd, weights, values, mult=0.22,
+                           start=before[:rows, :H] if accumulate else None)
+            assert torch.equal(out[rows:], before[rows:])
+            assert torch.equal(out[:, H:], before[:, H:])
+            assert (work[need:] == 255).all()
+
+
+def test_experts_in_lists_of_16_replay(gpu_device):
+    """The same bits from two streams at once and from two graphs that share the handle."""
+    rows, E, k, H, I = LISTS[0]
+    assert _tile_rows(rows, E, k, H, I) == 16
+    ex, _ = _experts(E, H, I, 77, gpu_device)
+    xs = torch.randn(4, rows, H, generator=_gen(78)).to(BF).to(gpu_device)
+    picks = [_choice(rows, E, k, 79 + i, gpu_device) for i in range(4)]
+    want = [ex(x, *p) for x, p in zip(xs, picks)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ex(xs[i], *picks[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    graphs = []
+    for _ in range(2):
+        static = [xs[0].clone(), picks[0][0].clone(), picks[0][1].clone()]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ex(*static)
+        graphs.append((g, static, y))
+    for i in (1, 2, 3):
+        for g, static, y in graphs:
+            for t, v in zip(static, (xs[i], *picks[i])):
+                t.copy_(v)
+        torch.cuda.synchronize()
+        for (g, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[i]) for _, _, y in graphs)
+
+
+@pytest.mark.parametrize("tile,counts", [
+    (64, [20, 40, 60, 70, 100, 0, 1]), (128, [129, 170, 200, 250, 20, 50, 300, 120, 0, 300])])
+def test_experts_tiles_of_every_height(gpu_device, tile, counts):
+    """Experts' rows that make tiles of each number of sixteens: up to 64 of 20 to 64 rows, up
+    to 128 of 20, 49, 50 and 74 (five sixteens) to 128."""
+    rows, E, k, H, I = sum(counts), len(counts), 1, 160, 96
+    assert _tile_rows(rows, E, k, H, I) == tile
+    ex, values = _experts(E, H, I, 80, gpu_device)
+    x = torch.randn(rows, H, generator=_gen(81)).to(BF).to(gpu_device)
+    ids = torch.repeat_interleave(torch.arange(E), torch.tensor(counts))
+    ids = ids[torch.randperm(rows, generator=_gen(82))].to(torch.int32).unsqueeze(1).to(gpu_device)
+    weights = torch.randn(rows, k, generator=_gen(83)).to(gpu_device)
+    for dtype in (BF, F32):
+        _check_experts(ex(x, ids, weights, dtype=dtype), x, ids, weights, values)
+
+
+@pytest.mark.parametrize("R,E,k,H,I", [(17, 8, 4, 64, 512), (11, 14, 12, 256, 1024),
+                                       (90, 40, 3, 512, 64)])
+def test_experts_workspace_serves_fewer_rows(gpu_device, R, E, k, H, I):
+    """One workspace, of R rows: calls of any number up to that stay inside it."""
+    import ctypes
+
+    from tilefoundry_amd import _lib
+    from tilefoundry_amd._lib import lib, ptr
+
+    need = lib().tfd_mx4_experts_work_bytes(R, k, E, H, I)
+    work = torch.full((need + 4096,), 165, dtype=torch.uint8, device=gpu_device)
+    ex, values = _experts(E, H, I, 84, gpu_device)
+    for rows in (R, R - 1, 16, 10, 1):
+        if rows > R:
+            continue
+        x = torch.randn(rows, H, generator=_gen(85)).to(BF).to(gpu_device)
+        ids, weights = _choice(rows, E, k, 86, gpu_device)
+        out = torch.empty(rows, H, device=gpu_device)
+        a = _lib.TfdMx4ExpertsArgs(ptr(x), H, ptr(ids), ptr(weights), k, ptr(ex.w_gu),
+                                   ptr(ex.w_down), rows, k, E, H, I, ptr(out), H, _lib.TYPE_F32,
+                                   0, 1.0, ptr(work), need, None)
+        lib().tfd_mx4_experts(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream)
+        _check_experts(out, x, ids, weights, values)
+        assert (work[need:] == 165).all()

@@ -390,3 +390,24 @@ def test_forward_mode_inputs_are_refused():
             mx4.quantise(x)
     with pytest.raises(ValueError, match="gradients"):
         torch.func.jvp(mx4.quantise, (x,), (x,))
+
+
+def test_reference_route_ranks_groups_by_their_best_two():
+    """(0, 5) outranks (1, 1), and the masked pair has nothing: the first group, best first."""
+    logits = torch.tensor([[0.0, 5.0, -math.inf, math.nan, 1.0, 1.0]])
+    assert R.route(logits, None, k=2, score="softmax", groups=3, keep=1)[1].tolist() == [[1, 0]]
+
+
+def test_form_entries_refuse():
+    form = (ctypes.c_int32 * 4)()
+    for M, K, N in ((0, 64, 64), (-1, 64, 64), (4, 48, 64), (4, 0, 64), (4, 64, 0),
+                    (4, 64, 2 ** 24 + 1), (4, 2 ** 22 + 32, 64)):
+        with pytest.raises(TFDError):
+            lib().tfd_mx4_gemm_form(0, M, K, N, form)
+    with pytest.raises(TFDError):
+        lib().tfd_mx4_gemm_form(0, 4, 64, 64, None)
+    tile = lib().tfd_mx4_experts_tile_rows
+    for bad in ((0, 1, 1, 32, 32), (65536, 1, 1, 32, 32), (1, 0, 1, 32, 32), (1, 65, 1, 32, 32),
+                (1, 1, 0, 32, 32), (1, 1, 513, 32, 32), (1, 1, 1, 0, 32), (1, 1, 1, 32, 0)):
+        assert tile(*bad) == -1
+    assert tile(16, 8, 64, 64, 32) == 0 and tile(16, 9, 64, 64, 32) != 0

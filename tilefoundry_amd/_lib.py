@@ -13,7 +13,7 @@ from pathlib import Path
 
 from .build import LIB
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 
 PRO_PLAIN, PRO_NORM = 0, 1
 EPI_STORE, EPI_RESID, EPI_SWIGLU, EPI_LOGITS, EPI_RESID_F32 = 0, 1, 2, 3, 4
@@ -147,9 +147,11 @@ SIGNATURES: dict[str, list] = {
     "tfd_mx4_packed_bytes": [L, I],
     "tfd_mx4_pack": [P, P, P, P, L, I, P, P],
     "tfd_mx4_gemm_work_bytes": [I, I, I],
+    "tfd_mx4_gemm_form": [I, I, I, I, P],
     "tfd_mx4_gemm": [P, P],
     "tfd_route_experts": [P, P],
     "tfd_mx4_experts_work_bytes": [I, I, I, I, I],
+    "tfd_mx4_experts_tile_rows": [I, I, I, I, I],
     "tfd_mx4_experts": [P, P],
 }
 RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c_int64,
@@ -157,7 +159,7 @@ RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c
             "tfd_mx4_gemm_work_bytes": ctypes.c_int64,
             "tfd_mx4_experts_work_bytes": ctypes.c_int64}
 UNCHECKED = {"tfd_abi_version", "tfd_decode_persistent_grid", "tfd_panel_gemm_slices",
-             "tfd_panel_attn_rows"}
+             "tfd_panel_attn_rows", "tfd_mx4_experts_tile_rows"}
 
 
 class TfdLayer(ctypes.Structure):

@@ -1131,6 +1131,15 @@ extern "C" int64_t tfd_mx4_gemm_work_bytes(int M, int K, int N) {
   return s > 1 ? (int64_t)s * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
+extern "C" int tfd_mx4_gemm_form(int x_mx4, int M, int K, int N, int32_t form[4]) {
+  if (!form) return fail(kBadArg, "mx4_gemm_form: null form");
+  if (const int rc = job_checks("mx4_gemm_form", K, N)) return rc;
+  if (M <= 0) return fail(kBadShape, "mx4_gemm_form: M=%d", M);
+  const DensePlan p = dense_plan(x_mx4 != 0, M, K, N);
+  form[0] = p.rows, form[1] = p.cols, form[2] = p.slices, form[3] = p.rest;
+  return 0;
+}
+
 extern "C" int tfd_mx4_gemm(const TfdMx4GemmArgs* args, void* stream) {
   if (!args) return fail(kBadArg, "mx4_gemm: null args");
   const TfdMx4GemmArgs& a = *args;
@@ -1192,6 +1201,14 @@ extern "C" {
 int64_t tfd_mx4_experts_work_bytes(int rows, int k, int experts, int H, int I) {
   if (rows <= 0 || k <= 0 || experts <= 0 || H <= 0 || I <= 0) return 0;
   return experts_work(rows, k, experts, H, I);
+}
+
+int tfd_mx4_experts_tile_rows(int rows, int k, int experts, int H, int I) {
+  if (rows <= 0 || rows > 65535 || k < 1 || k > 64 || experts < 1 ||
+      experts > TFD_ROUTE_MAX_EXPERTS || H <= 0 || I <= 0)
+    return -1;
+  const Plan p = experts_plan(rows, k, experts, H, I);
+  return p.fused ? 0 : p.tile_rows;
 }
 
 int tfd_mx4_experts(const TfdMx4ExpertsArgs* args, void* stream) {
