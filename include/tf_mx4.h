@@ -71,6 +71,8 @@ typedef struct {
   void* work;
   int64_t work_bytes;
 } TfdMx4GemmArgs;
+/* up to so many rows K is never split: no work */
+#define TFD_MX4_WHOLE_ROWS 64
 int64_t tfd_mx4_gemm_work_bytes(int M, int K, int N);
 /* How a product of these sizes runs on the current device, for tests and measurements: form =
  * rows and columns of a block's outputs, parts of K (with work), and the last blocks that run

@@ -398,6 +398,30 @@ def test_reference_route_ranks_groups_by_their_best_two():
     assert R.route(logits, None, k=2, score="softmax", groups=3, keep=1)[1].tolist() == [[1, 0]]
 
 
+def _form(M, K, N, both=False):
+    form = (ctypes.c_int32 * 4)()
+    lib().tfd_mx4_gemm_form(int(both), M, K, N, form)
+    return list(form)
+
+
+def test_products_of_few_rows_have_no_work():
+    """mx4.Linear asks for work past MX4_WHOLE_ROWS alone: up to there K is never split, and the
+    header's number is the package's."""
+    from pathlib import Path
+
+    header = Path(__file__).resolve().parent.parent / "include" / "tf_mx4.h"
+    assert f"#define TFD_MX4_WHOLE_ROWS {_lib.MX4_WHOLE_ROWS}\n" in header.read_text()
+    work = lib().tfd_mx4_gemm_work_bytes
+    for M in (1, 16, 17, 33, _lib.MX4_WHOLE_ROWS):
+        for K in (32, 544, 2048, 6144, 65536, 1 << 22):
+            for N in (1, 17, 2048, 12288, 1 << 20):
+                assert work(M, K, N) == 0
+                assert _form(M, K, N)[2] == _form(M, K, N, True)[2] == 1
+    for M, K, N in ((65, 1184, 130), (66, 2176, 70), (128, 6144, 260), (300, 4128, 513)):
+        parts = max(_form(M, K, N)[2], _form(M, K, N, True)[2])
+        assert parts > 1 and work(M, K, N) == parts * M * (-(-N // 4) * 4) * 4
+
+
 def test_form_entries_refuse():
     form = (ctypes.c_int32 * 4)()
     for M, K, N in ((0, 64, 64), (-1, 64, 64), (4, 48, 64), (4, 0, 64), (4, 64, 0),

@@ -69,6 +69,7 @@ TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ROUTE_MAX_EXPERTS = 512
 MX4_BLOCK = 32
+MX4_WHOLE_ROWS = 64                          # products of up to so many rows never split K
 
 #: argtypes of every entry, in header order (restype is int unless named here)
 SIGNATURES: dict[str, list] = {

@@ -1062,7 +1062,7 @@ DensePlan dense_plan(bool mx, int M, int K, int N) {
     p.items = (int64_t)((M + rows - 1) / rows) * ((N + cols - 1) / cols);
   };
   if (M <= 16) return p;
-  if (M <= 64) {
+  if (M <= TFD_MX4_WHOLE_ROWS) {
     shape(32, 64);
     if (p.items < cus / 2) shape(32, 16);
     if (p.cols == 16 && K >= 2048 && (M + 15) / 16 * ((N + 15) / 16) <= cus) shape(16, 16);

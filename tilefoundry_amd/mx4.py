@@ -260,7 +260,7 @@ class Linear:
             raise ValueError(f"Linear: up to {MAX_ROWS} rows a call, got {rows}")
         L = lib()
         work, need = None, 0
-        if rows > 64:                        # (fewer never split K)
+        if rows > _lib.MX4_WHOLE_ROWS:
             need = L.tfd_mx4_gemm_work_bytes(rows, K, self.N)
             work = values.new_empty(need, dtype=U8) if need else None
         a = _lib.TfdMx4GemmArgs(ptr(values), row_stride(values), ptr(scales), ldxs,
