@@ -222,7 +222,8 @@ def _out_type(dtype, what: str) -> int:
 class Linear:
     """x -> x W^T by mx4 weights ``[N, K]``, kept in the layout the kernels read.
 
-    x: bf16 ``[..., K]`` (weights become bf16 on the way, exactly), or an ``Mx4`` of that
+    x: bf16 ``[..., K]`` (weights become bf16 on the way, exactly; an infinity where a scale byte
+    past 252, which ``quantise`` never gives, takes one over its range), or an ``Mx4`` of that
     shape (both operands stay in 4 bits).  Sums are f32; the output is bf16 or f32."""
 
     def __init__(self, weight: Mx4):
@@ -279,8 +280,8 @@ class Experts:
 
     Sums are f32, the output rounded once to bf16 or f32.  The hidden values are the down
     product's operands: rounded to bf16, or in calls of up to 16 rows and 128 places kept as
-    sums of two bf16 (2^-17).  Id -1 is an empty
-    place; any other id outside the experts is skipped and raises ``check_errors``.  An
+    sums of two bf16 (2^-17); a row's last bits so depend on its call's rows.  Id -1 is an empty
+    place; any other id outside the experts is skipped and makes ``check_errors`` raise.  An
     expert may come twice in a row.  A call takes up to 65,535 rows, whose x and hidden
     values are each below 2 GiB."""
 
@@ -342,4 +343,5 @@ class Experts:
         torch.cuda.synchronize(self.device)
         if int(self.err.item()):
             self.err.zero_()
+            torch.cuda.synchronize(self.device)      # before a call on another stream
             raise RuntimeError("mx4 experts: an id outside the experts (and not -1) was skipped")
