@@ -170,7 +170,7 @@ struct RowTile {
   }
 };
 
-// The row tiles that fit a list's head: what group_listed wrote after them.
+// The row tiles that fit a list's head, as k_mx4_group wrote it there.
 __device__ __forceinline__ int listed_room(const Job& a) { return a.groups[1]; }
 
 template <int kEpi>
@@ -392,20 +392,22 @@ __global__ __launch_bounds__(kWaves * kWave) void k_mx4_few(Job a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: the matrix cores bound it.  A block of four waves takes up to TM x 16 rows
-// by 4 x TN x 16 columns.  Its rows pass through LDS, a stage (128 k of bf16, 256 k of
-// codes) at a time in two buffers, in the order the matrix instruction takes them (a
-// wave's read is 1 KiB in a row, and a write's eight lanes are 128 bytes in a row: no bank
-// conflicts); each wave's own weights go straight to its registers, two blocks of 128 k
+// Many rows.  A block of four waves takes up to TM x 16 rows by 4 x TN x 16 columns.
+// Its rows pass through LDS, a stage (128 k of bf16, 256 k of codes) at a time in two
+// buffers, in the order the matrix instruction takes them (a wave's read is 1 KiB in a row,
+// and a write's eight lanes are 128 bytes in a row: no bank conflicts; those of microscaled
+// rows' scales, a byte a lane, are 18% of that product's LDS cycles); each wave's own weights go straight to its registers, two blocks of 128 k
 // ahead, and are converted there.  bf16 rows come in two halves, each loaded and written
 // beside the products of half a stage: with all in flight at once the kernel needs more
 // than the 256 registers at which two blocks share a compute unit.  (DMA into LDS needs
 // none, but every LDS read behind it waits for it.)
 // Measured: 4,001 x 2048 x 12288 of bf16 146 to 157 us (1,280 to 1,380 TFLOP/s; 4,096 x 8192 x
-// 8192 1,550; a large library product of bf16 reaches 1,413 here), 4,001 x 4096 x 8512 of
-// codes 92 us (3,000 TFLOP/s): there the matrix instructions fill a third of the time, and
-// the operands' way from L2 bounds it (narrower blocks, which read more, are slower in
-// proportion).
+// 8192 1,550; a large library product of bf16 reaches 1,413 here): the matrix cores, busy 57%
+// of a profiled launch, and the ends of a pipeline of 16 blocks of k.  4,001 x 4096 x
+// 8512 of codes 92 us (3,000 TFLOP/s): nothing is full there.  Matrix instructions take 31%
+// of the time, the VALU 26%, LDS 17%; L2 is asked every 2.4 cycles a channel (about 15 bytes
+// a cycle and compute unit, 86% hits).  Of the waves' time 46% waits to issue, 23% for loads,
+// LDS or barriers: the order of two waves a SIMD, not a rate, keeps it there.
 // ---------------------------------------------------------------------------
 template <int kX, int TM>
 struct ManyLds {
@@ -967,7 +969,8 @@ Plan experts_plan(int rows, int k, int E, int H, int I) {
   Plan p = {};
   p.fused = rows <= kHereRows && n <= kHereMax;
   // By the rows an expert has if all are picked alike (us, weights from memory): items of 16
-  // rows by the stream's kernel for few, the longer K the more (64 Granite rows, 9 an expert:
+  // rows by the stream's kernel for few, the longer gate/up's K the more (fitted to I < H;
+  // down's K, which is I, does not enter) (64 Granite rows, 9 an expert:
   // 95; tiles of 64 103; 128 rows 134 and 110; 64 Qwen3.5 rows, 2 an expert, 69 and 72; 250
   // rows, 8, 109 and 105); tiles of up to 64 (512 Granite rows 167; tiles of 128 184); of up
   // to 128 past as many (1,024 Granite rows 272; 64 286).
