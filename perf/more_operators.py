@@ -1,0 +1,507 @@
+"""Operators of decoding with more than one continuation, as measurable cases.
+
+* ``tree``: attention of drafted tokens, which form a tree, over a paged cache;
+* ``beam``: the choice of the best beams among all beams' next tokens;
+* ``reorder``: what each row of a batch owns, moved to the rows that continue it;
+* ``pages``: pages of a cache shared, copied before a write, freed and compacted
+  (``fork``, ``churn``), and accepted positions of drafted tokens moved together (``keep``).
+
+Sizes are those of this repository's models: Qwen3-1.7B (16 query and 8 key heads of 128, 28
+layers, vocabulary 151,936), Qwen3.5 (16 and 2 heads of 256, vocabulary 248,320, recurrent
+state 32 x 128 x 128 a layer) and Granite-4.0-H (32 and 8 heads of 128, vocabulary 100,352).
+A page holds 16 positions.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+
+BF, F32, F64, I32, I64 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.int64
+DEV = "cuda:0"
+TYPES = {"bf16": BF, "f32": F32, "f16": torch.float16}
+PAGE = 16
+
+
+# --------------------------------------------------------------------- the cases
+def listed():
+    return [
+        # one sequence's chat turn, 16 drafted tokens: latency
+        {"name": "tree 1 sequence", "kind": "tree", "rows": 1, "nodes": 16, "context": 700,
+         "heads": 16, "kv_heads": 8, "dim": 128},
+        # a batch of 32 over 4,096-token contexts, a few drafted tokens each
+        {"name": "tree batch", "kind": "tree", "rows": 32, "nodes": 7, "context": 4096,
+         "heads": 16, "kv_heads": 8, "dim": 128},
+        # long documents, wide trees
+        {"name": "tree long", "kind": "tree", "rows": 4, "nodes": 61, "context": 30000,
+         "heads": 32, "kv_heads": 8, "dim": 128},
+        # few key heads of 256
+        {"name": "tree wide heads", "kind": "tree", "rows": 8, "nodes": 23, "context": 5003,
+         "heads": 16, "kv_heads": 2, "dim": 256},
+        # one sequence, four beams: latency
+        {"name": "beam 4", "kind": "beam", "groups": 1, "beams": 4, "vocab": 151936,
+         "type": "f32", "penalty": 0.0, "done": False},
+        # a batch of translations: eight beams, some of them finished, ranked by length
+        {"name": "beam 8 of 4", "kind": "beam", "groups": 4, "beams": 8, "vocab": 248320,
+         "type": "f32", "penalty": 0.6, "done": True},
+        # many beams, bf16 logits (equal ones are common)
+        {"name": "beam 16 of 16", "kind": "beam", "groups": 16, "beams": 16, "vocab": 100352,
+         "type": "bf16", "penalty": 0.0, "done": True},
+        # token histories and counters of 32 rows: latency
+        {"name": "reorder histories", "kind": "reorder", "groups": 8, "beams": 4, "layers": 2,
+         "state": 2176, "conv": 16},
+        # recurrent states and conv windows of a Qwen3.5 batch of two sequences, four beams
+        {"name": "reorder states", "kind": "reorder", "groups": 2, "beams": 4, "layers": 30,
+         "state": 524288, "conv": 24576},
+        # a step of four beams over a Qwen3-1.7B cache
+        {"name": "pages fork", "kind": "pages", "what": "fork", "rows": 4, "beams": 4,
+         "context": 709, "layers": 28, "kv_heads": 8, "dim": 128},
+        # a drafted step's accepted tokens of 32 sequences moved together
+        {"name": "pages keep", "kind": "pages", "what": "keep", "rows": 32, "nodes": 16,
+         "context": 300, "layers": 28, "kv_heads": 8, "dim": 128},
+        # two turns of serving: half of the sequences end, the rest is compacted, others start
+        {"name": "pages churn", "kind": "pages", "what": "churn", "rows": 24, "context": 611,
+         "layers": 28, "kv_heads": 8, "dim": 128},
+    ]
+
+
+def _spread(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["tree", "tree", "tree", "beam", "beam", "reorder", "pages", "pages"])
+    if kind == "tree":
+        dim, group = rng.choice([64, 128, 128, 256]), rng.choice([1, 2, 4, 8])
+        kv_heads = rng.choice([1, 2, 4, 8])
+        rows, nodes = _spread(rng, 1, 32), _spread(rng, 1, 64)
+        most = 1_000_000_000 // (rows * kv_heads * dim * max(8, nodes * group // 4))
+        return {"kind": kind, "rows": rows, "nodes": nodes,
+                "context": _spread(rng, 1, max(2, min(30000, most))), "heads": kv_heads * group,
+                "kv_heads": kv_heads, "dim": dim}
+    if kind == "beam":
+        beams, vocab = _spread(rng, 1, 32), _spread(rng, 500, 250000)
+        most = max(1, min(32, 24_000_000 // (beams * vocab)))
+        return {"kind": kind, "groups": _spread(rng, 1, most), "beams": beams, "vocab": vocab,
+                "type": rng.choice(["f32", "f32", "bf16", "f16"]),
+                "penalty": rng.choice([0.0, 0.6, 1.0]), "done": rng.random() < 0.5}
+    if kind == "reorder":
+        beams, groups = rng.randint(1, 16), rng.randint(1, 8)
+        layers = rng.randint(1, 30)
+        most = 125_000_000 // (beams * groups * layers)
+        return {"kind": kind, "groups": groups, "beams": beams, "layers": layers,
+                "state": _spread(rng, 1, most), "conv": rng.randint(1, 9000)}
+    what = rng.choice(["fork", "fork", "keep", "churn"])
+    layers, kv_heads = rng.randint(1, 28), rng.choice([1, 2, 8])
+    dim = rng.choice([64, 128, 256])
+    beams = rng.randint(1, 8) if what == "fork" else 1
+    rows = beams * rng.randint(1, max(1, 24 // beams)) if what != "churn" else rng.randint(2, 24)
+    most = 380_000_000 // (layers * kv_heads * dim * rows)
+    return {"kind": kind, "what": what, "rows": rows, "beams": beams,
+            "nodes": rng.randint(2, 48), "context": _spread(rng, 1, min(6000, max(2, most))),
+            "layers": layers, "kv_heads": kv_heads, "dim": dim}
+
+
+# ------------------------------------------------------------------ drawn inputs
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _rn(g, *shape, s=1.0, dtype=F32):
+    return (torch.randn(*shape, generator=g, device=DEV) * s).to(dtype)
+
+
+def _rand(g, *shape):
+    return torch.rand(*shape, generator=g, device=DEV)
+
+
+def _noise(g, *shape):
+    """bf16 values of about unit size, made quickly."""
+    return torch.empty(*shape, device=DEV, dtype=BF).uniform_(-2, 2, generator=g)
+
+
+def _lengths(rows, context):
+    """Contexts of unlike lengths up to *context*, the same whatever the seed."""
+    return [max(1, context - (37 * r) % max(1, context // 8)) for r in range(rows)]
+
+
+def _ceil(a, b):
+    return -(-a // b)
+
+
+def _tree_inputs(case, seed):
+    g, B, T = _gen(seed), case["rows"], case["nodes"]
+    HQ, HKV, D = case["heads"], case["kv_heads"], case["dim"]
+    lens = _lengths(B, case["context"])
+    width = _ceil(max(lens) + T, PAGE)
+    total = B * width
+    # node t's parent is one of the four before it (the first is the root)
+    back = 1 + (_rand(g, B, T) * 4).long()
+    parents = torch.clamp(torch.arange(T, device=DEV) - back, min=0)
+    # a node sees itself and what its parent sees: steps upwards, as often as there are nodes
+    step = torch.eye(T, device=DEV) + torch.nn.functional.one_hot(parents, T).to(F32)
+    seen = torch.linalg.matrix_power(step, 64) > 0
+    bits = torch.ones(64, dtype=I64, device=DEV) << torch.arange(64, device=DEV)
+    masks = torch.zeros(B, T, 64, dtype=I64, device=DEV)
+    masks[:, :, :T] = seen.long()
+    return {
+        "q": _rn(g, B, T, HQ, D, dtype=BF),
+        "k": _rn(g, total, HKV, PAGE, D, dtype=BF), "v": _rn(g, total, HKV, PAGE, D, dtype=BF),
+        "table": torch.randperm(total, generator=g, device=DEV).to(I32).view(B, width),
+        "lengths": torch.tensor(lens, dtype=I32, device=DEV),
+        "masks": (masks * bits).sum(2, keepdim=True)}
+
+
+def _beam_inputs(case, seed):
+    g, G, K, V = _gen(seed), case["groups"], case["beams"], case["vocab"]
+    x = _rn(g, G * K, V, s=2.0)
+    # a few tokens of each row stand out, as they do behind a trained head
+    at = (_rand(g, G * K, 12) * V).long()
+    x.scatter_(1, at, 9.0 + _rn(g, G * K, 12, s=2.0))
+    done = _rand(g, G, K) < (0.2 if case["done"] else -1.0)
+    lengths = torch.where(done, 5 + (_rand(g, G, K) * 30).int(), torch.full((), 36, device=DEV))
+    return {"logits": x.to(TYPES[case["type"]]), "scores": -20 + _rn(g, G, K, s=1.5),
+            "lengths": lengths.to(I32), "done": done}
+
+
+def _parents(g, groups, beams):
+    """Each group's beams continue some of its beams, the better ones more often."""
+    u = torch.rand(groups, beams, generator=g, device=DEV)
+    mine = torch.clamp((u * u * beams).long(), max=beams - 1)
+    return (mine + beams * torch.arange(groups, device=DEV).unsqueeze(1)).flatten().to(I32)
+
+
+def _reorder_inputs(case, seed):
+    g, rows = _gen(seed), case["groups"] * case["beams"]
+    return {"parents": _parents(g, case["groups"], case["beams"]),
+            "states": [torch.rand(rows, n, generator=g, device=DEV).to(t) for n, t in
+                       ((case["state"], F32), (case["conv"], BF)) for _ in range(case["layers"])]}
+
+
+def _pages_inputs(case, seed):
+    g, what, B = _gen(seed), case["what"], case["rows"]
+    L, HKV, D = case["layers"], case["kv_heads"], case["dim"]
+    lens = _lengths(B, case["context"])
+    if what == "fork":            # a group's beams are equally long
+        lens = [lens[r // case["beams"]] for r in range(B)]
+    extra = {"fork": 1, "keep": case.get("nodes", 0), "churn": 0}[what]
+    width = _ceil(max(lens) + extra, PAGE) + 1
+    need = [_ceil(n + (extra if what == "keep" else 0), PAGE) for n in lens]
+    count = sum(need)
+    total = count + B * 2 + (max(sum(need[:B // 2]), sum(need[B // 2:])) if what == "churn" else 0)
+    half = sum(need[:B // 2])
+    if what == "churn":           # the first half's pages lie below the second half's
+        order = torch.cat((torch.randperm(half, generator=g, device=DEV),
+                           half + torch.randperm(count - half, generator=g, device=DEV)))
+    else:
+        order = torch.randperm(total, generator=g, device=DEV)[:count]
+    needs = torch.tensor(need, device=DEV)
+    places = torch.arange(width, device=DEV)
+    used = places < needs.unsqueeze(1)
+    table = torch.full((B, width), -1, dtype=I64, device=DEV)
+    table[used] = order
+    lengths = torch.tensor(lens, dtype=I32, device=DEV)
+    if what == "fork":            # a group's first half is one prompt
+        first = torch.arange(B, device=DEV) // case["beams"] * case["beams"]
+        shared = places < lengths.unsqueeze(1) // PAGE // 2
+        table = torch.where(shared, table[first], table)
+    refs = torch.zeros(total, dtype=I32, device=DEV)
+    flat = table.flatten()
+    refs.scatter_add_(0, flat.clamp(min=0), (flat >= 0).to(I32))
+    s = {"table": table.to(I32).contiguous(), "refs": refs, "lengths": lengths,
+         "k": _noise(g, L, total, HKV, PAGE, D), "v": _noise(g, L, total, HKV, PAGE, D)}
+    if what == "fork":
+        s["parents"] = _parents(g, B // case["beams"], case["beams"])
+    elif what == "keep":
+        T = case["nodes"]
+        counts = 1 + (_rand(g, B) * min(T, 6)).long()
+        # counts of the nodes in rising order, the root first
+        weight = _rand(g, B, T)
+        weight[:, 0] = -1
+        rank = torch.argsort(torch.argsort(weight, 1), 1)
+        at = torch.arange(T, device=DEV).expand(B, T)
+        chosen = torch.where(rank < counts.unsqueeze(1), at, torch.full_like(at, T))
+        path = torch.sort(chosen, 1).values
+        s["path"] = torch.where(path == T, -1, path).to(I32)
+        s["counts"] = counts.to(I32)
+    else:
+        second = torch.arange(B, device=DEV) >= B // 2
+        s["halves"] = [~second, second]
+        s["zeros"] = torch.zeros_like(lengths)
+        s["starts"] = [torch.where(m, lengths, torch.zeros_like(lengths)) for m in s["halves"]]
+    return s
+
+
+MAKE = {"tree": _tree_inputs, "beam": _beam_inputs, "reorder": _reorder_inputs,
+        "pages": _pages_inputs}
+EOS = 2
+
+
+def prepare(case, seed):
+    s = {"case": case, **MAKE[case["kind"]](case, seed)}
+    if own:                       # the handles that a serving program keeps
+        from tilefoundry_amd import beam, pages
+
+        if case["kind"] == "beam":
+            s["handle"] = beam.Beam(case["beams"], eos=EOS, length_penalty=case["penalty"])
+        elif case["kind"] == "reorder":
+            s["handle"] = beam.States(s["states"])
+        elif case["kind"] == "pages":
+            s["handle"] = pages.Pages([s["k"], s["v"]], table=s["table"], refs=s["refs"])
+    return s
+
+
+# ------------------------------------------------------------------ plain forms
+def _positions(pool, table, n):
+    """The first *n* positions of each row of *table*: f32 [rows, heads, n, dim]."""
+    x = pool[table[:, :_ceil(n, PAGE)].long()].to(F32)           # rows, pages, heads, 16, dim
+    return x.transpose(1, 2).flatten(2, 3)[:, :, :n]
+
+
+def _tree(case, s):
+    B, T, HQ, D = s["q"].shape
+    HKV = case["kv_heads"]
+    n = case["context"] + T
+    k, v = _positions(s["k"], s["table"], n), _positions(s["v"], s["table"], n)
+    q = s["q"].to(F32).unflatten(2, (HKV, HQ // HKV)).permute(0, 2, 1, 3, 4).flatten(2, 3)
+    x = q @ k.transpose(2, 3) * D ** -0.5                        # rows, kv heads, T group, n
+    at = torch.arange(n, device=DEV)
+    node = at - s["lengths"].unsqueeze(1)                        # rows, n
+    may = (s["masks"] >> node.clamp(0, 63).unsqueeze(1)) & 1     # rows, T, n
+    may = (node < 0).unsqueeze(1) | ((node < T).unsqueeze(1) & (may == 1))
+    may = may.repeat_interleave(HQ // HKV, 1).unsqueeze(1)
+    x = torch.where(may, x, torch.full_like(x, -math.inf))
+    p = torch.exp(x - x.amax(3, keepdim=True))
+    o = (p @ v) / p.sum(3, keepdim=True)
+    return o.unflatten(2, (T, HQ // HKV)).permute(0, 2, 1, 3, 4).flatten(2, 3).to(BF)
+
+
+def _beam(case, s):
+    G, K, V = case["groups"], case["beams"], case["vocab"]
+    x = s["logits"].to(F32)
+    # an f32's bits as an integer of the same order, equal ones by the lower token
+    i = (x + 0.0).view(I32)
+    i = (i ^ ((i >> 31) & 0x7fffffff)).to(I64)
+    keys = (i << 32) | (0xffffffff - torch.arange(V, device=DEV))
+    n = min(K, V)
+    tokens = 0xffffffff - (torch.topk(keys, n, dim=1).values & 0xffffffff)
+    x64 = x.to(F64)
+    top = x64.amax(1, keepdim=True)
+    lse = top + torch.log(torch.exp(x64 - top).sum(1, keepdim=True))
+    done, scores = s["done"].flatten().unsqueeze(1), s["scores"].flatten().to(F64).unsqueeze(1)
+    own_length = s["lengths"].flatten().unsqueeze(1)
+    value = scores + x64.gather(1, tokens) - lse
+    # a finished beam offers itself
+    first = torch.arange(n, device=DEV) == 0
+    value = torch.where(done, torch.where(first, scores, -math.inf), value)
+    tokens = torch.where(done, EOS, tokens)
+    length = torch.where(done, own_length, own_length + 1).expand(G * K, n)
+    rank = value / length.to(F64).clamp(min=1.0) ** case["penalty"]
+    order = torch.sort(rank.view(G, K * n), dim=1, descending=True, stable=True).indices[:, :K]
+    parents = order // n + K * torch.arange(G, device=DEV).unsqueeze(1)
+    picked = tokens.reshape(G, K * n).gather(1, order)
+    return (parents.to(I32), picked.to(I32), value.view(G, K * n).gather(1, order).to(F32),
+            length.reshape(G, K * n).gather(1, order).to(I32),
+            (picked == EOS) | done.view(G, K).gather(1, order // n))
+
+
+def _counted(refs, pages, by):
+    """refs, *by* more for each of *pages*, in place; -1 is no page."""
+    refs.scatter_add_(0, pages.clamp(min=0).long(), torch.where(pages >= 0, by, 0).to(I32))
+
+
+def _fork(s, parents, lengths):
+    table = s["table"]
+    old = table.clone()
+    whose = parents.clamp(min=0).long()
+    lengths = torch.where(parents >= 0, lengths[whose], 0)
+    place = torch.arange(table.shape[1], device=DEV)
+    kept = (place < ((lengths + PAGE - 1) // PAGE).unsqueeze(1)) | \
+        (parents == torch.arange(len(parents), device=DEV)).unsqueeze(1)
+    table.copy_(torch.where(kept & (parents >= 0).unsqueeze(1), old[whose], -1))
+    _counted(s["refs"], old.flatten(), -1)
+    _counted(s["refs"], table.flatten(), 1)
+    return lengths
+
+
+def _take(s, lengths, n):
+    """Pages for n positions behind lengths, each row's its own to write."""
+    table, refs = s["table"], s["refs"]
+    place = torch.arange(table.shape[1], device=DEV)
+    first = (lengths // PAGE).unsqueeze(1)
+    wanted = (place >= first) & (place < ((lengths + n + PAGE - 1) // PAGE).unsqueeze(1))
+    wanted &= (lengths + n > lengths).unsqueeze(1)
+    page = table.clamp(min=0).long()
+    has = wanted & (table >= 0)
+    at = torch.arange(table.numel(), device=DEV).view_as(table)
+    none = torch.full_like(at, table.numel())
+    writers = torch.zeros_like(refs).scatter_add_(0, page.flatten(), has.flatten().to(I32))
+    lowest = torch.full(refs.shape, table.numel(), dtype=I64, device=DEV)
+    lowest.scatter_reduce_(0, page.flatten(), torch.where(has, at, none).flatten(), "amin")
+    stays = has & ((refs[page] == 1) | ((writers[page] == refs[page]) & (lowest[page] == at)))
+    new = wanted & ~stays
+    rank = (torch.cumsum(new.flatten(), 0) - 1).view_as(table).clamp(min=0)
+    free = torch.sort((refs > 0).to(torch.uint8), stable=True).indices
+    fresh = torch.where(new, free[rank.clamp(max=len(free) - 1)].to(I32), -1)
+    # what a shared page holds below the new positions goes along
+    copied = new & has & (place == first) & (lengths % PAGE != 0).unsqueeze(1)
+    src, dst = table[copied].long(), fresh[copied].long()
+    s["k"][:, dst] = s["k"][:, src]
+    s["v"][:, dst] = s["v"][:, src]
+    _counted(refs, torch.where(new & has, table, -1).flatten(), -1)
+    _counted(refs, fresh.flatten(), 1)
+    table.copy_(torch.where(new, fresh, table))
+
+
+def _compact(s):
+    live = s["refs"] > 0
+    at = torch.arange(len(live), device=DEV)
+    n = live.sum()
+    src, dst = torch.nonzero(live & (at >= n)).flatten(), torch.nonzero(~live & (at < n)).flatten()
+    s["k"][:, dst] = s["k"][:, src]
+    s["v"][:, dst] = s["v"][:, src]
+    now = at.clone()
+    now[src] = dst
+    s["refs"][dst] = s["refs"][src]
+    s["refs"][src] = 0
+    table = s["table"]
+    table.copy_(torch.where(table >= 0, now[table.clamp(min=0).long()].to(I32), -1))
+    return n.to(I32)
+
+
+def _keep(s, lengths, path, counts):
+    r, i = torch.nonzero(torch.arange(path.shape[1], device=DEV) < counts.unsqueeze(1),
+                         as_tuple=True)
+    src, dst = lengths[r] + path[r, i], lengths[r] + i
+    for_src = s["table"][r, (src // PAGE).long()].long(), (src % PAGE).long()
+    for_dst = s["table"][r, (dst // PAGE).long()].long(), (dst % PAGE).long()
+    s["k"][:, for_dst[0], :, for_dst[1]] = s["k"][:, for_src[0], :, for_src[1]]
+    s["v"][:, for_dst[0], :, for_dst[1]] = s["v"][:, for_src[0], :, for_src[1]]
+    return lengths + counts
+
+
+def _bits(t):
+    return t.view(torch.int16 if t.element_size() == 2 else I32)
+
+
+def _cache(s):
+    return [_bits(s["k"]), _bits(s["v"]), s["table"], s["refs"]]
+
+
+def run(state):
+    s, case = state, state["case"]
+    kind = case["kind"]
+    if kind == "tree":
+        if own:
+            from tilefoundry_amd import tree
+
+            return tree.attention(s["q"], s["k"], s["v"], s["table"], s["lengths"], s["masks"])
+        return _tree(case, s)
+    if kind == "beam":
+        if own:
+            return tuple(s["handle"](s["logits"], s["scores"], s["lengths"], s["done"]))
+        return _beam(case, s)
+    if kind == "reorder":
+        if own:
+            s["handle"].reorder(s["parents"])
+        else:
+            rows = s["parents"].long()
+            [t.copy_(t[rows]) for t in s["states"]]
+        return [_bits(t) for t in s["states"]]
+    if case["what"] == "fork":
+        if own:
+            lengths = s["handle"].fork(s["parents"], s["lengths"])
+            s["handle"].take(lengths, 1)
+        else:
+            lengths = _fork(s, s["parents"], s["lengths"])
+            _take(s, lengths, 1)
+        return [*_cache(s), lengths]
+    if case["what"] == "keep":
+        if own:
+            lengths = s["handle"].keep(s["lengths"], s["path"], s["counts"])
+        else:
+            lengths = _keep(s, s["lengths"], s["path"], s["counts"])
+        return [*_cache(s), lengths]
+    return [*_cache(s), *(_turn(s, m, n) for m, n in zip(s["halves"], s["starts"]))]
+
+
+def _turn(s, ends, starts):
+    """Rows end, the rest is compacted, other sequences start in them."""
+    if own:
+        s["handle"].free(ends)
+        live = s["handle"].compact()
+        s["handle"].take(s["zeros"], starts)
+        return live
+    _fork(s, torch.where(ends, -1, torch.arange(len(ends), device=DEV)), s["lengths"])
+    live = _compact(s)
+    _take(s, s["zeros"], starts)
+    return live
+
+
+# ------------------------------------------------------------- work and exactness
+def work(case):
+    kind = case["kind"]
+    if kind == "tree":
+        lens = _lengths(case["rows"], case["context"])
+        T, D = case["nodes"], case["dim"]
+        seen = sum(n + T for n in lens)
+        return {"bytes": 4 * seen * case["kv_heads"] * D +
+                4 * case["rows"] * T * case["heads"] * D,
+                "flops": 4 * seen * T * case["heads"] * D}
+    if kind == "beam":
+        rows = case["groups"] * case["beams"]
+        size = 4 if case["type"] == "f32" else 2
+        return {"bytes": rows * (case["vocab"] * size + 30), "flops": 6 * rows * case["vocab"]}
+    if kind == "reorder":
+        rows = case["groups"] * case["beams"]
+        # about half of the rows change; what they take comes from fewer
+        return {"bytes": rows * case["layers"] * (4 * case["state"] + 2 * case["conv"]),
+                "flops": rows}
+    B, one = case["rows"], 4 * case["layers"] * case["kv_heads"] * case["dim"]
+    if case["what"] == "fork":    # about half of the rows write a page that another one keeps
+        return {"bytes": B * PAGE * one + 8 * B * (case["context"] // PAGE + 1), "flops": B}
+    if case["what"] == "keep":
+        return {"bytes": 2 * B * max(1, min(case["nodes"], 6) // 2) * one, "flops": B}
+    need = [_ceil(n, PAGE) for n in _lengths(B, case["context"])]
+    moved = min(sum(need[:B // 2]), sum(need[B // 2:]))
+    return {"bytes": 2 * 2 * moved * PAGE * one + 16 * sum(need), "flops": B}
+
+
+def exact(case, seed):
+    if case["kind"] == "tree":
+        s = _tree_inputs(case, seed)
+        B, T, HQ, D = s["q"].shape
+        g = HQ // case["kv_heads"]
+        out = torch.empty(B, T, HQ, D, dtype=F64, device=DEV)
+        for b, n in enumerate(s["lengths"].tolist()):
+            rows = s["table"][b, torch.arange(n + T, device=DEV) // PAGE].long()
+            off = torch.arange(n + T, device=DEV) % PAGE
+            seen = torch.ones(T, n + T, dtype=torch.bool, device=DEV)
+            seen[:, n:] = s["masks"][b].bitwise_right_shift(
+                torch.arange(T, device=DEV)).remainder(2) == 1
+            for h in range(case["kv_heads"]):
+                k, v = s["k"][rows, h, off].to(F64), s["v"][rows, h, off].to(F64)
+                for j in range(h * g, h * g + g):
+                    x = torch.matmul(s["q"][b, :, j].to(F64), k.t().contiguous()) / math.sqrt(D)
+                    out[b, :, j] = torch.matmul(
+                        torch.softmax(x.masked_fill(~seen, -math.inf), 1), v)
+        return out
+    if case["kind"] == "beam":
+        s, K, V = _beam_inputs(case, seed), case["beams"], case["vocab"]
+        scores = []
+        for g in range(case["groups"]):
+            at = slice(g * K, g * K + K)
+            lp = torch.log_softmax(s["logits"][at].to(F64), 1) + \
+                s["scores"][g].to(F64).unsqueeze(1)
+            length = (s["lengths"][g] + 1).to(F64)
+            for b in torch.nonzero(s["done"][g]).flatten().tolist():
+                lp[b] = -math.inf
+                lp[b, EOS] = s["scores"][g, b].to(F64)
+                length[b] -= 1
+            rank = (lp / length.pow(case["penalty"]).unsqueeze(1)).flatten()
+            best = torch.sort(rank, descending=True, stable=True).indices[:K]
+            scores.append(lp.flatten()[best])
+        return None, None, torch.stack(scores), None, None
+    return None                   # what is moved has no other value
