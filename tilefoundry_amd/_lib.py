@@ -13,7 +13,7 @@ from pathlib import Path
 
 from .build import LIB
 
-ABI_VERSION = 19
+ABI_VERSION = 20
 
 PRO_PLAIN, PRO_NORM = 0, 1
 EPI_STORE, EPI_RESID, EPI_SWIGLU, EPI_LOGITS, EPI_RESID_F32 = 0, 1, 2, 3, 4
@@ -70,6 +70,18 @@ SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 ROUTE_MAX_EXPERTS = 512
 MX4_BLOCK = 32
 MX4_WHOLE_ROWS = 64                          # products of up to so many rows never split K
+
+#: include/tf_search.h: device error bits, limits
+ERR_ROW_RANGE, ERR_NO_PAGES = 64, 128
+TREE_MAX_NODES = 256
+BEAM_MAX, BEAM_MAX_VOCAB = 64, 1 << 20
+PAGES_MAX_ROWS = 1024
+
+
+def pages_scratch(rows: int, max_pages: int, num_pages: int) -> int:
+    """int32 words of a page table's scratch (TFD_PAGES_SCRATCH)."""
+    return 3 * num_pages + rows * max_pages + 2 * rows + 16
+
 
 #: argtypes of every entry, in header order (restype is int unless named here)
 SIGNATURES: dict[str, list] = {
@@ -154,11 +166,27 @@ SIGNATURES: dict[str, list] = {
     "tfd_mx4_experts_work_bytes": [I, I, I, I, I],
     "tfd_mx4_experts_tile_rows": [I, I, I, I, I],
     "tfd_mx4_experts": [P, P],
+    # include/tf_search.h
+    "tfd_tree_masks": [P, P, I, I, P, P, P, P],
+    "tfd_tree_accept": [P, P, P, P, I, I, P, P, P, P],
+    "tfd_tree_attn_work_bytes": [I, I, I, I, I, I],
+    "tfd_tree_attn": [P, P],
+    "tfd_beam_work_bytes": [I, I, I],
+    "tfd_beam_select": [P, P],
+    "tfd_state_blocks": [P, L],
+    "tfd_reorder_states": [P, I, L, P, I, I, P, P],
+    "tfd_pages_fork": [P, P, P, P, P, P],
+    "tfd_pages_take": [P, P, P, I, P],
+    "tfd_pages_copy": [P, P, P, I, P],
+    "tfd_pages_keep": [P, P, P, P, I, P, P],
+    "tfd_pages_compact": [P, P, P],
 }
 RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c_int64,
             "tfd_mx4_packed_bytes": ctypes.c_int64,
             "tfd_mx4_gemm_work_bytes": ctypes.c_int64,
-            "tfd_mx4_experts_work_bytes": ctypes.c_int64}
+            "tfd_mx4_experts_work_bytes": ctypes.c_int64,
+            "tfd_tree_attn_work_bytes": ctypes.c_int64, "tfd_beam_work_bytes": ctypes.c_int64,
+            "tfd_state_blocks": ctypes.c_int64}
 UNCHECKED = {"tfd_abi_version", "tfd_decode_persistent_grid", "tfd_panel_gemm_slices",
              "tfd_panel_attn_rows", "tfd_mx4_experts_tile_rows"}
 
@@ -383,6 +411,52 @@ class TfdMx4ExpertsArgs(ctypes.Structure):
                 ("ldo", c_int64), ("out_type", c_int), ("accumulate", c_int),
                 ("mult", c_float), ("work", c_void_p), ("work_bytes", c_int64),
                 ("err", c_void_p)]
+
+
+class TfdTreeAttnArgs(ctypes.Structure):
+    """``TfdTreeAttnArgs`` of include/tf_search.h, field for field."""
+
+    _fields_ = [("q", c_void_p), *[(n, c_int64) for n in ("q_row", "q_node", "q_head")],
+                *[(n, c_void_p) for n in ("k_pool", "v_pool", "page_table", "lengths", "counts",
+                                          "masks")],
+                *[(n, c_int) for n in ("rows", "nodes", "heads", "kv_heads", "head_dim",
+                                       "max_pages", "num_pages")],
+                ("scale", c_float), ("out", c_void_p), ("out_panel", c_int),
+                ("work", c_void_p), ("work_bytes", c_int64), ("err", c_void_p)]
+
+
+class TfdBeamArgs(ctypes.Structure):
+    """``TfdBeamArgs`` of include/tf_search.h, field for field."""
+
+    _fields_ = [("logits", c_void_p), ("ldl", c_int64), ("type", c_int), ("scores", c_void_p),
+                ("lengths", c_void_p), ("done", c_void_p),
+                *[(n, c_int) for n in ("groups", "beams", "vocab", "eos")],
+                ("penalty", c_float),
+                *[(n, c_void_p) for n in ("parents", "tokens", "scores_out", "lengths_out",
+                                          "done_out", "work")],
+                ("work_bytes", c_int64)]
+
+
+class TfdState(ctypes.Structure):
+    """``TfdState`` of include/tf_search.h: one tensor whose rows move."""
+
+    _fields_ = [("base", c_void_p), ("row_bytes", c_int64), ("first_block", c_int64)]
+
+
+class TfdPool(ctypes.Structure):
+    """``TfdPool`` of include/tf_search.h: one tensor of pages."""
+
+    _fields_ = [("base", c_void_p), ("page_bytes", c_int64), ("heads", ctypes.c_int32),
+                ("row_bytes", ctypes.c_int32)]
+
+
+class TfdPages(ctypes.Structure):
+    """``TfdPages`` of include/tf_search.h, field for field."""
+
+    _fields_ = [("pools", c_void_p), ("n_pools", c_int), ("max_page_bytes", c_int64),
+                ("table", c_void_p), ("refs", c_void_p),
+                *[(n, c_int) for n in ("rows", "max_pages", "num_pages")],
+                ("scratch", c_void_p), ("err", c_void_p)]
 
 
 class TfdDecodeArgs(ctypes.Structure):

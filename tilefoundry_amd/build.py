@@ -22,7 +22,7 @@ ARCH = "gfx950"
 SOURCES = ["qwen3_decode.hip", "qwen3_xcd.hip", "qwen3_batch.hip", "hybrid.hip",
            "gqa_hybrid.hip", "twin_ops.hip", "hybrid_small.hip", "sample.hip",
            "prefill.hip", "prefill_hybrid.hip", "mx4.hip",
-           "mx4_products.hip", "route.hip"]
+           "mx4_products.hip", "route.hip", "tree.hip", "beam.hip", "pages.hip"]
 
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
