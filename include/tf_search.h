@@ -85,7 +85,7 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream);
  * eos was taken).  Places for which no candidate is left hold their own row as parent, token
  * -1, score -inf, and that row's length and done.  eos -1: no token finishes.
  * logits f32, bf16 or f16 [rows][ldl]; lengths NULL: zeros, done NULL: none (uint8).
- * vocab <= 2^20, groups <= 65535, beams <= 64, rows x vocab / 1024 below 2^24.  work:
+ * vocab <= 2^20, groups <= 65535, beams <= 64, rows x vocab / 1024 below 2^23.  work:
  * tfd_beam_work_bytes, 16-byte aligned, contents free, one call's at a time.  The outputs must
  * not be the inputs. */
 typedef struct {
@@ -111,15 +111,19 @@ int tfd_beam_select(const TfdBeamArgs* args, void* stream);
 /* Rows of `n` tensors moved to the rows that continue them, in place: row r becomes what row
  * parents[r] was.  Groups of `beams` rows (<= 64); a parent lies in its row's group (another one
  * raises TFD_ERR_ROW_RANGE and leaves the row as it is).  `states`: a device array; first_block
- * = the running sum of tfd_state_blocks of the tensors before, `blocks` the sum of all. */
+ * = the running sum of tfd_state_blocks of the tensors before, `blocks` the sum of all (below
+ * 2^24).  `pieces`: how many 4 KiB of a row a block takes one after another (fewer of tensors
+ * whose rows are no multiples of 16 bytes): 1 for small states, 4 where there are blocks
+ * enough all the same. */
 typedef struct {
   void* base;         /* [rows][row_bytes] */
   int64_t row_bytes;
   int64_t first_block;
 } TfdState;
-int64_t tfd_state_blocks(const void* base, int64_t row_bytes);
-int tfd_reorder_states(const TfdState* states, int n, int64_t blocks, const int32_t* parents,
-                       int groups, int beams, int32_t* err, void* stream);
+int64_t tfd_state_blocks(const void* base, int64_t row_bytes, int pieces);
+int tfd_reorder_states(const TfdState* states, int n, int pieces, int64_t blocks,
+                       const int32_t* parents, int groups, int beams, int32_t* err,
+                       void* stream);
 
 /* ---- pages -------------------------------------------------------------------------- */
 #define TFD_PAGES_MAX_ROWS 1024

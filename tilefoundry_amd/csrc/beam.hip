@@ -27,154 +27,247 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-__device__ __forceinline__ uint64_t lane_u64(uint64_t v, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)v, lane);
-  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(v >> 32), lane);
-  return ((uint64_t)hi << 32) | lo;
+template <int kCtrl>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, false);
 }
-__device__ __forceinline__ double lane_d(double v, int lane) {
-  return __builtin_bit_cast(double, lane_u64(__builtin_bit_cast(uint64_t, v), lane));
+__device__ __forceinline__ double pair_d(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
+template <int kCtrl>
+__device__ __forceinline__ double dpp_d(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return pair_d(dpp_u<kCtrl>((uint32_t)b), dpp_u<kCtrl>((uint32_t)(b >> 32)));
+}
+// Sums and conjunctions over a wave, in registers (DPP and lane swaps).
 __device__ __forceinline__ double wave_sum_d(double v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
-  return v;
+  v += dpp_d<kDppXor1>(v);
+  v += dpp_d<kDppXor2>(v);
+  v += dpp_d<kDppHalfMirror>(v);
+  v += dpp_d<kDppMirror>(v);
+  uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const auto l = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+  const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false,
+                                                  false);
+  v = pair_d(l[0], h[0]) + pair_d(l[1], h[1]);
+  b = __builtin_bit_cast(uint64_t, v);
+  const auto m = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+  const auto n = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false,
+                                                  false);
+  return pair_d(m[0], n[0]) + pair_d(m[1], n[1]);
+}
+__device__ __forceinline__ uint32_t wave_and(uint32_t v) {
+  v &= dpp_u<kDppXor1>(v);
+  v &= dpp_u<kDppXor2>(v);
+  v &= dpp_u<kDppHalfMirror>(v);
+  v &= dpp_u<kDppMirror>(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = a[0] & a[1];
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return __builtin_amdgcn_readfirstlane(b[0] & b[1]);
 }
 
-// exp(x) for x <= 0 to about an f32's last bit: the product with log2 e in two parts.
-__device__ __forceinline__ float exp_neg(float x) {
+// 2^(d log2 e) for d <= 0 to about an f32's last bit: log2 e in two parts.
+__device__ __forceinline__ float exp_neg(float d) {
   constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596303e-8f;
-  const float t = x * kHi;
-  const float rest = fmaf(x, kHi, -t) + x * kLo;
-  const float e = __builtin_amdgcn_exp2f(t);
-  return x < -100.f ? 0.f : fmaf(e, rest * 0.69314718055994530942f, e);
+  return __builtin_amdgcn_exp2f(fmaf(d, kHi, d * kLo));
+}
+
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);     // (-0 as +0)
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float float_of(uint32_t o) {
+  return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o);
+}
+
+// The largest of three, NaN left out (written out: fmaxf first makes its operands quiet).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
+// The largest t that at least k of the lanes' values reach (0: fewer are above 0), bit by bit
+// below the bits that all share; it may stop short where exactly k do.
+template <int kN>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[kN], int k) {
+  uint32_t all = v[0], any = v[0];
+#pragma unroll
+  for (int i = 1; i < kN; ++i) all &= v[i], any |= v[i];
+  all = wave_and(all), any = ~wave_and(~any);
+  uint32_t t = 0;
+  if (all == any) return all;                // (all equal)
+  const uint32_t top = 0x80000000u >> __builtin_clz(all ^ any);
+  t = any & ~(2 * top - 1);
+#pragma unroll 1
+  for (uint32_t bit = top; bit; bit >>= 1) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) n += __popcll(__ballot(v[i] >= (t | bit)));
+    if (n < k) continue;
+    t |= bit;
+    if (n == k) break;
+  }
+  return t;
 }
 
 struct BeamPlan {
-  int per, chunks;       // values of a thread, chunks of a row
+  int per, chunks;       // values of a lane, chunks (of a wave) of a row
 };
-constexpr int kScan = 256;
+constexpr int kNear = 256;                   // candidates a wave holds
 
-// What a row's chunk leaves: its largest logit, the sum of exp(x - that), and its `beams`
-// largest keys in falling order (0 where there are fewer).
+// What a wave's chunk of a row leaves: its largest logit, the sum of exp(x - that), and its
+// `beams` largest keys in falling order (0 where there are fewer).
 struct ChunkSum {
   double sum;
   float top;
   int pad;
 };
 
-// ---------------------------------------------------------------------------
-// A block per chunk of a row, its values in registers.  The beams-th largest of the threads'
-// best keys bounds the chunk's beams-th largest from below; what reaches it -- in at most
-// `beams` threads -- is collected and ranked by counting.
-// ---------------------------------------------------------------------------
 template <int kType>
 __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
-  float v;
-  if (kType == TFD_TYPE_F32) v = ((const float*)p)[i];
-  else if (kType == TFD_TYPE_BF16) v = bf2f(((const bf16*)p)[i]);
-  else v = (float)__builtin_bit_cast(_Float16, ((const uint16_t*)p)[i]);
-  return v;
+  if (kType == TFD_TYPE_F32) return ((const float*)p)[i];
+  if (kType == TFD_TYPE_BF16) return bf2f(((const bf16*)p)[i]);
+  return (float)__builtin_bit_cast(_Float16, ((const uint16_t*)p)[i]);
 }
 
+// ---------------------------------------------------------------------------
+// A wave per chunk of a row, its values in registers, no barrier.  The beams-th largest of
+// the lanes' best values bounds the chunk's beams-th largest from below: what reaches it,
+// hardly more than `beams` values, goes through LDS to be ranked by counting.  Where more do
+// than LDS holds (equal logits), the places are filled one by one, from memory.  Four values at a time
+// are tested by their largest.
+// ---------------------------------------------------------------------------
 template <int kType, int kPer, bool kVec>
-__global__ __launch_bounds__(kScan) void k_beam_scan(TfdBeamArgs a, int chunks,
-                                                     ChunkSum* __restrict__ sums,
-                                                     uint64_t* __restrict__ lists) {
-  constexpr int kWaves = kScan / kWave;
-  __shared__ uint64_t best_s[kScan];
-  __shared__ uint64_t found_s[kMaxBeams * kPer];
-  __shared__ float top_s[kWaves];
-  __shared__ double sum_s[kWaves];
-  __shared__ uint64_t bound_s;
-  __shared__ int n_s;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+__global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k_beam_scan(TfdBeamArgs a, int chunks, int waves,
+                                                      ChunkSum* __restrict__ sums,
+                                                      uint64_t* __restrict__ lists) {
+  constexpr float kInf = __builtin_huge_valf();
+  constexpr int kQuads = kPer / 4;
+  __shared__ uint64_t near_s[kWavesPerBlock][kNear];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int in_block = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int w = blockIdx.x * kWavesPerBlock + in_block;
+  if (w >= waves) return;
+  const int row = w / chunks, chunk = w % chunks;
   if (a.done && a.done[row]) return;               // (its lists are not read)
-  const int c0 = chunk * kScan * kPer, K = a.beams;
+  uint64_t* const near = near_s[in_block];
+  const int c0 = chunk * kWave * kPer, K = a.beams;
   const int64_t base = (int64_t)row * a.ldl;
   float x[kPer];
-  auto at = [&](int j) { return c0 + (j / 4) * 4 * kScan + 4 * tid + j % 4; };
-  if (kVec) {
+  // a lane's values come in runs of kRun, 16 bytes of memory
+  constexpr int kRun = kType == TFD_TYPE_F32 ? 4 : 8;
+  auto at = [&](int j) { return c0 + (j / kRun) * kRun * kWave + kRun * lane + j % kRun; };
+  auto put_run = [&](int j, const u32x4& v) {
 #pragma unroll
-    for (int j = 0; j < kPer; j += 4) {
-      const int i = min(at(j), a.vocab - 4);       // (vocab % 4 == 0)
-      if (kType == TFD_TYPE_F32) {
-        const u32x4 v = *(g_u32x4*)((const float*)a.logits + base + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[j + e] = __uint_as_float(v[e]);
-      } else {
-        const uint64_t v = *(const uint64_t*)((const uint16_t*)a.logits + base + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint16_t h = (uint16_t)(v >> (16 * e));
-          x[j + e] = kType == TFD_TYPE_BF16 ? bf2f(h) : (float)__builtin_bit_cast(_Float16, h);
-        }
-      }
+    for (int e = 0; e < kRun; ++e) {
+      if (kType == TFD_TYPE_F32) x[j + e] = __uint_as_float(v[e % 4]);
+      else if (kType == TFD_TYPE_BF16) x[j + e] = e % 2 ? bf_hi(v[e / 2]) : bf_lo(v[e / 2]);
+      else x[j + e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(v[e / 2] >> (16 * (e % 2))));
     }
+  };
+  const bool whole = c0 + kWave * kPer <= a.vocab;
+  if (kVec && whole) {
+    constexpr int kSize = kType == TFD_TYPE_F32 ? 4 : 2;
+    const uint8_t* const p = (const uint8_t*)a.logits + (base + c0) * kSize + lane * 16;
+#pragma unroll
+    for (int j = 0; j < kPer; j += kRun)
+      put_run(j, __builtin_nontemporal_load((g_u32x4*)(p + j * kWave * kSize)));
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = logit_at<kType>(a.logits, base + min(at(j), a.vocab - 1));
-  }
-  float top = -__builtin_huge_valf();
-  int where = 0;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    if (x[j] > 3.402823466e38f) x[j] = 3.402823466e38f;      // (NaN stays)
-    if (at(j) >= a.vocab) x[j] = -__builtin_huge_valf();
-    if (x[j] > top) top = x[j], where = j;
-  }
-  const uint64_t best = key_of(top, at(where));
-  if (tid == 0) n_s = 0, bound_s = 0;
-  best_s[tid] = best;
-  const float wt = wave_max(top);
-  if (lane == 0) top_s[wave] = wt;
-  __syncthreads();
-  float m = top_s[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) m = fmaxf(m, top_s[w]);
-  double sum = 0.0;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) sum += x[j] > -__builtin_huge_valf() ? exp_neg(x[j] - m) : 0.f;
-  sum = wave_sum_d(sum);
-  if (lane == 0) sum_s[wave] = sum;
-  int rank = 0;
-  for (int i = 0; i < kScan; i += 2) rank += (best_s[i] > best) + (best_s[i + 1] > best);
-  if (best && rank == K - 1) bound_s = best;
-  __syncthreads();
-  const uint64_t bound = bound_s;
-  if (best && best >= bound) {
-#pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const uint64_t k = key_of(x[j], at(j));
-      if (k && k >= bound) found_s[atomicAdd(&n_s, 1)] = k;
+      x[j] = logit_at<kType>(a.logits, base + min(at(j), a.vocab - 1));
+      if (at(j) >= a.vocab) x[j] = -kInf;
     }
   }
-  __syncthreads();
-  const int n = n_s;
-  uint64_t* const list = lists + (int64_t)blockIdx.x * K;
-  for (int i = tid; i < n; i += kScan) {
-    const uint64_t k = found_s[i];
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += found_s[j] > k;
-    if (r < K) list[r] = k;
-  }
-  for (int i = n + tid; i < K; i += kScan) list[i] = 0;
-  if (tid == 0) {
-    double t = 0.0;
+  // largest of four, of the lane, of the wave; the sum (once more with NaN and +inf put in
+  // their places where there are any: the sum shows them)
+  float top4[kQuads], best, m;
+  double sum;
+#pragma unroll 1
+  for (int again = 0; again < 2; ++again) {
+    best = -kInf;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) t += sum_s[w];
-    sums[blockIdx.x] = ChunkSum{t, m, 0};
+    for (int q = 0; q < kQuads; ++q)
+      top4[q] = max3(max3(x[4 * q], x[4 * q + 1], x[4 * q + 2]), x[4 * q + 3], -kInf);
+#pragma unroll
+    for (int q = 0; q < kQuads; q += 2) best = max3(best, top4[q], top4[q + 1]);
+    m = wave_max(best);
+    const float ref = m == -kInf ? 0.f : m;
+    sum = 0.0;
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = exp_neg(x[4 * q + i] - ref);
+      sum += (double)((e[0] + e[1]) + (e[2] + e[3]));
+    }
+    sum = wave_sum_d(sum);
+    if (sum < 1e30) break;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = fminf(fmaxf(x[j], -kInf), 3.402823466e38f);
   }
+  const uint32_t t = kth_largest<1>({best > -kInf ? order_of(best) : 0u}, K);
+  // what reaches it (t 0: every candidate)
+  const float bound = t ? float_of(t) : -3.402823466e38f;
+  int n = 0;
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    if (!__any(top4[q] >= bound)) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int j = 4 * q + e;
+      const uint64_t who = __ballot(x[j] >= bound);
+      if (!who) continue;
+      const int place = n + __builtin_amdgcn_mbcnt_hi(
+                                (uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      if (x[j] >= bound && place < kNear) near[place] = key_of(x[j], at(j));
+      n += __popcll(who);
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  uint64_t* const list = lists + (int64_t)w * K;
+  if (n <= kNear) {
+    for (int i = lane; i < n; i += kWave) {
+      const uint64_t k = near[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += near[j] > k;
+      if (r < K) list[r] = k;
+    }
+    if (n + lane < K) list[n + lane] = 0;          // (beams <= 64)
+  } else {
+    uint64_t last = ~0ull;
+#pragma unroll 1
+    for (int r = 0; r < K; ++r) {
+      uint64_t mine = 0;
+#pragma unroll 1
+      for (int i = c0 + lane; i < min(c0 + kWave * kPer, a.vocab); i += kWave) {
+        const uint64_t k = key_of(fminf(fmaxf(logit_at<kType>(a.logits, base + i), -kInf),
+                                        3.402823466e38f), i);
+        if (k < last && k > mine) mine = k;
+      }
+      for (int d = 1; d < kWave; d *= 2) {
+        const uint64_t o = __shfl_xor((unsigned long long)mine, d, kWave);
+        mine = o > mine ? o : mine;
+      }
+      if (lane == 0) list[r] = mine;               // (more than beams candidates are there)
+      last = mine;
+    }
+  }
+  if (lane == 0) sums[w] = ChunkSum{sum, m, 0};
 }
 
 // ---------------------------------------------------------------------------
 // A block per group.  Candidates in order: rank, then the lower row, then the key.  A wave's
 // beams-th best list head bounds the group's beams-th best candidate from below; what reaches
-// the largest such bound is collected and ranked by counting.  If more than the buffer holds
-// does (thousands of equal ranks), the places are filled one by one instead.
+// the largest such bound is collected and ranked by counting.  If more does than the buffer
+// holds (thousands of equal ranks), the places are filled one by one instead.  A thread holds
+// the first keys of a list from the start on, so that few loads wait for others.
 // ---------------------------------------------------------------------------
-constexpr int kMerge = 512, kMergeWaves = kMerge / kWave, kFound = 2048;
+constexpr int kMerge = 1024, kMergeWaves = kMerge / kWave, kFound = 2048;
+constexpr int kHeldKeys = 4, kHeldSums = 3, kHeads = 256;
 
 struct Cand {
   double rank;
@@ -182,101 +275,141 @@ struct Cand {
   int beam;
 };
 __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
-  if (a.rank != b.rank) return a.rank > b.rank;
-  if (a.beam != b.beam) return a.beam < b.beam;
-  return a.key > b.key;
+  return (a.rank > b.rank) |
+         ((a.rank == b.rank) & ((a.beam < b.beam) | ((a.beam == b.beam) & (a.key > b.key))));
 }
 
 __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks,
                                                        const ChunkSum* __restrict__ sums,
                                                        const uint64_t* __restrict__ lists) {
-  __shared__ double add_s[kMaxBeams], div_s[kMaxBeams];
+  __shared__ double add_s[kMaxBeams], inv_s[kMaxBeams];
   __shared__ float top_s[kMaxBeams];
-  __shared__ double bound_s[kMergeWaves];
+  __shared__ uint8_t done_s[kMaxBeams];
+  __shared__ int length_s[kMaxBeams];
+  __shared__ uint32_t bound_s[kMergeWaves];
   __shared__ double found_rank[kFound];
   __shared__ uint64_t found_key[kFound];
   __shared__ uint8_t found_beam[kFound];
+  __shared__ uint32_t head_s[kHeads];
   __shared__ Cand wave_s[kMergeWaves];
-  __shared__ int n_s;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const int K = a.beams, row0 = blockIdx.x * K;
-  if (tid == 0) n_s = 0;
-  // value = add + (logit - top), rank = value / div (the difference first: an infinite logit
+  __shared__ int n_s, heads_s, rank_s[kWave];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int K = a.beams, row0 = blockIdx.x * K, n_lists = K * chunks;
+  const uint64_t* const mine = lists + (int64_t)row0 * chunks * K;
+  uint64_t held[kHeldKeys];
+#pragma unroll
+  for (int i = 0; i < kHeldKeys; ++i)
+    held[i] = mine[(int64_t)min(tid, n_lists - 1) * K + min(i, K - 1)];
+  if (tid == 0) n_s = heads_s = 0;
+  if (tid < kWave) rank_s[tid] = 0;
+  // value = add + (logit - top), rank = value * inv (the difference first: an infinite logit
   // stands as 3.4e38); a row that offers nothing has add NaN
   for (int b = wave; b < K; b += kMergeWaves) {
     const int row = row0 + b;
+    const ChunkSum* const t = sums + (int64_t)row * chunks;
+    ChunkSum c[kHeldSums];
+#pragma unroll
+    for (int i = 0; i < kHeldSums; ++i) c[i] = t[min(lane + i * kWave, chunks - 1)];
     const float score = a.scores[row];
+    const int length = a.lengths ? a.lengths[row] : 0;
     const bool over = a.done && a.done[row], none = !(fabsf(score) < __builtin_huge_valf());
+    const double inv = a.penalty == 0.f ? 1.0
+                                        : 1.0 / pow((double)max(length + (over ? 0 : 1), 1),
+                                                    (double)a.penalty);
     double lse = 0.0;
     float m = -__builtin_huge_valf();
     if (!over) {
-      const ChunkSum* const t = sums + (int64_t)row * chunks;
-      for (int c = lane; c < chunks; c += kWave) m = fmaxf(m, t[c].top);
+#pragma unroll
+      for (int i = 0; i < kHeldSums; ++i) m = fmaxf(m, c[i].top);
+      for (int i = lane + kHeldSums * kWave; i < chunks; i += kWave) m = fmaxf(m, t[i].top);
       m = wave_max(m);
+      // (an f32 exponential: the largest chunk's is exactly one)
       double s = 0.0;
-      for (int c = lane; c < chunks; c += kWave)
-        if (t[c].top > -__builtin_huge_valf()) s += t[c].sum * exp((double)t[c].top - (double)m);
+#pragma unroll
+      for (int i = 0; i < kHeldSums; ++i)
+        if (c[i].sum > 0.0 && lane + i * kWave < chunks)
+          s += c[i].sum * (double)exp_neg(c[i].top - m);
+      for (int i = lane + kHeldSums * kWave; i < chunks; i += kWave)
+        if (t[i].sum > 0.0) s += t[i].sum * (double)exp_neg(t[i].top - m);
       lse = log(wave_sum_d(s));
     }
     if (lane == 0) {
-      const int len = (a.lengths ? a.lengths[row] : 0) + (over ? 0 : 1);
       top_s[b] = m;
+      done_s[b] = over;
+      length_s[b] = length;
       add_s[b] = none ? __builtin_nan("") : (double)score - lse;
-      div_s[b] = a.penalty == 0.f ? 1.0 : pow((double)max(len, 1), (double)a.penalty);
+      inv_s[b] = inv;
     }
   }
   __syncthreads();
-  const int n_lists = K * chunks;
   auto value_of = [&](const Cand& c) {
-    return add_s[c.beam] + ((double)logit_of(c.key) - (double)top_s[c.beam]);
+    return done_s[c.beam] ? add_s[c.beam]
+                          : add_s[c.beam] + ((double)logit_of(c.key) - (double)top_s[c.beam]);
   };
-  // entry i of a row's list; a finished row's only candidate lies in its first list
-  auto cand = [&](int list, int i) {
+  // entry i of a row's list, whose key (as far as there is one) is `key`; a finished row's
+  // only candidate lies in its first list
+  auto with_key = [&](int list, int i, uint64_t key) {
     Cand c;
     c.beam = list / chunks;
-    const int row = row0 + c.beam;
-    c.rank = kNone;
-    c.key = 0;
-    if (a.done && a.done[row]) {
-      if (list % chunks == 0 && i == 0) {
-        c.key = key_of(0.f, a.eos);
-        c.rank = add_s[c.beam] / div_s[c.beam];
-      }
-    } else {
-      c.key = lists[((int64_t)row * chunks + list % chunks) * K + i];
-      if (c.key) c.rank = value_of(c) / div_s[c.beam];
-    }
-    if (c.key && !(c.rank > kNone)) c.key = 0, c.rank = kNone;
+    c.key = !done_s[c.beam] ? key
+            : list == c.beam * chunks && i == 0 ? key_of(0.f, a.eos) : 0;
+    c.rank = c.key ? value_of(c) * inv_s[c.beam] : kNone;
+    if (!(c.rank > kNone)) c.key = 0, c.rank = kNone;
     return c;
   };
-  double best = kNone;
-  for (int l = tid; l < n_lists; l += kMerge) best = fmax(best, cand(l, 0).rank);
-  int rank = 0;
-  for (int i = 0; i < kWave; ++i) {
-    const double o = lane_d(best, i);
-    rank += o > best || (o == best && i < lane);
-  }
-  const uint64_t who = __ballot(rank == K - 1);
-  if (lane == 0) bound_s[wave] = lane_d(best, (int)__builtin_ctzll(who));
+  auto cand = [&](int list, int i) { return with_key(list, i, mine[(int64_t)list * K + i]); };
+  double best = tid < n_lists ? with_key(tid, 0, held[0]).rank : kNone;
+  for (int l = tid + kMerge; l < n_lists; l += kMerge) best = fmax(best, cand(l, 0).rank);
+  // in f32, rounded down: a bound all the same
+  const uint32_t head = best > kNone ? order_of(__double2float_rd(best)) : 0u;
+  const uint32_t t = kth_largest<1>({head}, K);
+  if (lane == 0) bound_s[wave] = t;
   __syncthreads();
-  double bound = bound_s[0];
-  for (int w = 1; w < kMergeWaves; ++w) bound = fmax(bound, bound_s[w]);
-  for (int l = tid; l < n_lists; l += kMerge)
-    for (int i = 0; i < K; ++i) {
-      const Cand c = cand(l, i);
-      if (!c.key || c.rank < bound) break;
-      const int at = atomicAdd(&n_s, 1);
-      if (at < kFound) found_rank[at] = c.rank, found_key[at] = c.key, found_beam[at] = c.beam;
-    }
+  uint32_t top = bound_s[0];
+#pragma unroll
+  for (int w = 1; w < kMergeWaves; ++w) top = max(top, bound_s[w]);
+  // the threads' heads that reach it bound it once more (every wave for itself)
+  if (head >= max(top, 1u)) {
+    const int at = atomicAdd(&heads_s, 1);
+    if (at < kHeads) head_s[at] = head;
+  }
+  __syncthreads();
+  if (heads_s > 2 * K && heads_s <= kHeads) {
+    uint32_t v[kHeads / kWave];
+#pragma unroll
+    for (int i = 0; i < kHeads / kWave; ++i)
+      v[i] = lane + i * kWave < heads_s ? head_s[lane + i * kWave] : 0u;
+    top = max(top, kth_largest(v, K));
+  }
+  const double bound = top ? (double)float_of(top) : kNone;
+  auto collect = [&](const Cand& c) {
+    if (!c.key || c.rank < bound) return false;
+    const int at = atomicAdd(&n_s, 1);
+    if (at < kFound) found_rank[at] = c.rank, found_key[at] = c.key, found_beam[at] = c.beam;
+    return true;
+  };
+  auto walk = [&](int l, int from) {
+    for (int i = from; i < K; ++i)
+      if (!collect(cand(l, i))) break;
+  };
+  if (tid < n_lists) {
+    bool more = true;
+#pragma unroll
+    for (int i = 0; i < kHeldKeys; ++i)
+      if (more && i < K) more = collect(with_key(tid, i, held[i]));
+    if (more) walk(tid, kHeldKeys);
+  }
+  for (int l = tid + kMerge; l < n_lists; l += kMerge) walk(l, 0);
   __syncthreads();
   const int n = n_s;
   auto put = [&](int place, const Cand& c) {
     const int row = row0 + c.beam, at = row0 + place;
-    const bool over = a.done && a.done[row];
-    const int token = token_of(c.key), len = a.lengths ? a.lengths[row] : 0;
+    const bool over = done_s[c.beam];
+    const int token = token_of(c.key), len = length_s[c.beam];
     a.parents[at] = row;
     a.tokens[at] = token;
-    a.scores_out[at] = over ? a.scores[row] : (float)value_of(c);
+    a.scores_out[at] = (float)value_of(c);
     a.lengths_out[at] = len + (over ? 0 : 1);
     a.done_out[at] = over || token == a.eos;
   };
@@ -285,9 +418,26 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     a.parents[at] = at;
     a.tokens[at] = -1;
     a.scores_out[at] = -__builtin_huge_valf();
-    a.lengths_out[at] = a.lengths ? a.lengths[at] : 0;
-    a.done_out[at] = a.done ? a.done[at] : 0;
+    a.lengths_out[at] = length_s[place];
+    a.done_out[at] = done_s[place];
   };
+  if (n <= kWave) {                          // a candidate per lane, the others shared by waves
+    if (lane < n) {
+      const Cand c{found_rank[lane], found_key[lane], found_beam[lane]};
+      int r = 0;
+      for (int j = wave; j < n; j += kMergeWaves)
+        r += better(Cand{found_rank[j], found_key[j], found_beam[j]}, c);
+      if (r) atomicAdd(&rank_s[lane], r);
+    }
+    __syncthreads();
+    if (tid < n) {
+      const int r = rank_s[tid];
+      if (r < K) put(r, Cand{found_rank[tid], found_key[tid], found_beam[tid]});
+    } else if (tid < K) {
+      put_none(tid);
+    }
+    return;
+  }
   if (n <= kFound) {
     for (int i = tid; i < n; i += kMerge) {
       const Cand c{found_rank[i], found_key[i], found_beam[i]};
@@ -295,8 +445,7 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
       for (int j = 0; j < n; ++j) r += better(Cand{found_rank[j], found_key[j], found_beam[j]}, c);
       if (r < K) put(r, c);
     }
-    for (int i = n + tid; i < K; i += kMerge) put_none(i);
-    return;
+    return;                                  // (more than K)
   }
   Cand last{__builtin_huge_val(), ~0ull, -1};
   for (int place = 0; place < K; ++place) {
@@ -328,25 +477,31 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   }
 }
 
-BeamPlan beam_plan(int rows, int vocab) {
+// Chunks as long as leave some waves for every compute unit and, for a group, no more lists
+// than the merging block has threads; longer where there are many waves all the same.
+BeamPlan beam_plan(int rows, int beams, int vocab) {
   BeamPlan p;
-  p.per = 4;
-  while (p.per < 32 && (int64_t)rows * ((vocab + kScan * p.per - 1) / (kScan * p.per)) > 1024)
-    p.per *= 2;
-  p.chunks = (vocab + kScan * p.per - 1) / (kScan * p.per);
+  p.per = 8;
+  auto chunks = [&] { return (vocab + kWave * p.per - 1) / (kWave * p.per); };
+  while (p.per < 32 && ((int64_t)rows * chunks() > 2048 || beams * chunks() > kMerge)) p.per *= 2;
+  if (p.per == 32 && (int64_t)rows * chunks() > 8192) p.per = 64;
+  p.chunks = chunks();
   return p;
 }
 
 bool beam_shape(int groups, int beams, int vocab) {
   return groups >= 0 && groups <= 65535 && beams >= 1 && beams <= kMaxBeams && vocab >= 1 &&
          vocab <= TFD_BEAM_MAX_VOCAB &&
-         (int64_t)groups * beams * ((vocab + 1023) / 1024) < (1 << 24);
+         (int64_t)groups * beams * ((vocab + 1023) / 1024) < (1 << 23);
 }
 
 // ---------------------------------------------------------------------------
 // Reorder.  A thread owns one place of all rows of a group: it reads every row that
 // another one becomes before it writes any, so nothing has to be kept twice.  Rows that stay
-// are neither read (but by others) nor written.
+// are neither read (but by others) nor written.  A wave knows the moves by itself -- lane b
+// holds row b's parent, a 64-bit mask the rows that move -- and finds its tensor by a
+// ballot, so nothing waits for a barrier; of the pieces that a block takes one after
+// another, the next one's loads are in flight behind the current one's stores.
 // ---------------------------------------------------------------------------
 constexpr int kUnits = 4;                    // small units per thread
 
@@ -354,72 +509,80 @@ __host__ __device__ inline int state_unit(const void* base, int64_t row_bytes) {
   const uint64_t both = (uint64_t)(uintptr_t)base | (uint64_t)row_bytes;
   return both % 16 == 0 ? 16 : both % 4 == 0 ? 4 : both % 2 == 0 ? 2 : 1;
 }
-inline int64_t state_blocks(const void* base, int64_t row_bytes) {
-  const int64_t per = kBlock * (state_unit(base, row_bytes) == 16 ? 1 : kUnits) *
-                      (int64_t)state_unit(base, row_bytes);
-  return (row_bytes + per - 1) / per;
+
+// The moves' sources, as many as there are, or their stores.
+template <typename T, int kN, int kMoves, bool kStore>
+__device__ __forceinline__ void each_move(T (&v)[kMoves][kN], T* p, int64_t units, int64_t u0,
+                                          uint64_t moved, int from) {
+#pragma unroll
+  for (int i = 0; i < kMoves; ++i) {
+    if (moved) {
+      const int to = (int)__builtin_ctzll(moved);
+      moved &= moved - 1;
+      T* const row = p + (kStore ? to : __builtin_amdgcn_readlane(from, to)) * units;
+#pragma unroll
+      for (int k = 0; k < kN; ++k) {
+        const int64_t u = u0 + k * kBlock;
+        if (!kStore) v[i][k] = row[min(u, units - 1)];
+        else if (u < units) row[u] = v[i][k];
+      }
+    }
+  }
 }
 
-template <typename T, int kN, int kBeams>
-__device__ __forceinline__ void move_rows(uint8_t* base, int64_t row_bytes, int64_t unit0,
-                                          const int* from_s, int beams) {
+template <typename T, int kN, int kMoves>
+__device__ __forceinline__ void move_rows(uint8_t* base, int64_t row_bytes, int64_t block,
+                                          int pieces, uint64_t moved, int from) {
+  constexpr int kBuffers = kMoves <= 16 ? 2 : 1;
   const int64_t units = row_bytes / (int64_t)sizeof(T);
   T* const p = reinterpret_cast<T*>(base);
-  T v[kBeams][kN];
+  int64_t u = block * pieces * (kBlock * kN) + threadIdx.x;
+  T v[kBuffers][kMoves][kN];
+  each_move<T, kN, kMoves, false>(v[0], p, units, u, moved, from);
+#pragma unroll 1
+  for (int i = 0; i < pieces; i += kBuffers) {
 #pragma unroll
-  for (int b = 0; b < kBeams; ++b) {
-    const int from = b < beams ? __builtin_amdgcn_readfirstlane(from_s[b]) : b;
-    if (from != b) {
-#pragma unroll
-      for (int k = 0; k < kN; ++k) {
-        const int64_t u = min(unit0 + k * kBlock + (int64_t)threadIdx.x, units - 1);
-        v[b][k] = p[from * units + u];
-      }
-    }
-  }
-#pragma unroll
-  for (int b = 0; b < kBeams; ++b) {
-    const int from = b < beams ? __builtin_amdgcn_readfirstlane(from_s[b]) : b;
-    if (from != b) {
-#pragma unroll
-      for (int k = 0; k < kN; ++k) {
-        const int64_t u = unit0 + k * kBlock + (int64_t)threadIdx.x;
-        if (u < units) p[b * units + u] = v[b][k];
-      }
+    for (int b = 0; b < kBuffers; ++b) {
+      const int64_t next = u + kBlock * kN;
+      const bool more = i + b + 1 < pieces && next - (int)threadIdx.x < units;
+      if (kBuffers > 1 && more)
+        each_move<T, kN, kMoves, false>(v[(b + 1) % kBuffers], p, units, next, moved, from);
+      each_move<T, kN, kMoves, true>(v[b], p, units, u, moved, from);
+      if (!more) return;
+      if (kBuffers == 1) each_move<T, kN, kMoves, false>(v[0], p, units, next, moved, from);
+      u = next;
     }
   }
 }
 
-template <int kBeams>
+template <int kMoves>
 __global__ __launch_bounds__(kBlock) void k_reorder(const TfdState* __restrict__ states, int n,
-                                                    const int* __restrict__ parents, int beams,
-                                                    int* err) {
-  __shared__ int from_s[kBeams];
-  const int g = blockIdx.y;
-  if ((int)threadIdx.x < beams) {
-    const int first = g * beams, from = parents[first + threadIdx.x];
-    const bool in = from >= first && from < first + beams;
-    if (!in) raise_error(err, TFD_ERR_ROW_RANGE);
-    from_s[threadIdx.x] = in ? from - first : (int)threadIdx.x;
+                                                    int pieces, const int* __restrict__ parents,
+                                                    int beams, int* err) {
+  const int lane = threadIdx.x & (kWave - 1), first = blockIdx.y * beams;
+  int from = lane;
+  if (lane < beams) from = parents[first + lane] - first;
+  const int64_t block = blockIdx.x;
+  int t = -1;
+  for (int i = 0; i < n; i += kWave)
+    t += __popcll(__ballot(i + lane < n && states[min(i + lane, n - 1)].first_block <= block));
+  if (from < 0 || from >= beams) {
+    if (lane < beams) raise_error(err, TFD_ERR_ROW_RANGE);
+    from = lane;
   }
-  int lo = 0, hi = n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (states[mid].first_block <= (int64_t)blockIdx.x) lo = mid;
-    else hi = mid;
-  }
-  const TfdState t = states[lo];
-  __syncthreads();
-  const int64_t block = (int64_t)blockIdx.x - t.first_block;
-  uint8_t* const base = (uint8_t*)t.base + g * beams * t.row_bytes;
-  const int unit = state_unit(t.base, t.row_bytes);
-  if (unit == 16) move_rows<u32x4, 1, kBeams>(base, t.row_bytes, block * kBlock, from_s, beams);
+  const uint64_t moved = __ballot(from != lane);
+  if (!moved) return;
+  const TfdState st = states[__builtin_amdgcn_readfirstlane(t)];
+  const int64_t at = block - st.first_block;
+  uint8_t* const base = (uint8_t*)st.base + first * st.row_bytes;
+  const int unit = state_unit(st.base, st.row_bytes);
+  if (unit == 16) move_rows<u32x4, 1, kMoves>(base, st.row_bytes, at, pieces, moved, from);
   else if (unit == 4)
-    move_rows<uint32_t, kUnits, kBeams>(base, t.row_bytes, block * kBlock * kUnits, from_s, beams);
+    move_rows<uint32_t, kUnits, kMoves>(base, st.row_bytes, at, pieces, moved, from);
   else if (unit == 2)
-    move_rows<uint16_t, kUnits, kBeams>(base, t.row_bytes, block * kBlock * kUnits, from_s, beams);
+    move_rows<uint16_t, kUnits, kMoves>(base, st.row_bytes, at, pieces, moved, from);
   else
-    move_rows<uint8_t, kUnits, kBeams>(base, t.row_bytes, block * kBlock * kUnits, from_s, beams);
+    move_rows<uint8_t, kUnits, kMoves>(base, st.row_bytes, at, pieces, moved, from);
 }
 
 }  // namespace
@@ -428,7 +591,7 @@ extern "C" {
 
 int64_t tfd_beam_work_bytes(int groups, int beams, int vocab) {
   if (!beam_shape(groups, beams, vocab)) return 0;
-  const BeamPlan p = beam_plan(groups * beams, vocab);
+  const BeamPlan p = beam_plan(groups * beams, beams, vocab);
   return (int64_t)groups * beams * p.chunks * ((int64_t)sizeof(ChunkSum) + 8 * beams);
 }
 
@@ -455,21 +618,22 @@ int tfd_beam_select(const TfdBeamArgs* args, void* stream) {
   if (!a.work || (uintptr_t)a.work % 16 ||
       a.work_bytes < tfd_beam_work_bytes(a.groups, a.beams, a.vocab))
     return fail(kBadArg, "beam_select: work of %lld bytes", (long long)a.work_bytes);
-  const BeamPlan p = beam_plan(rows, a.vocab);
+  const BeamPlan p = beam_plan(rows, a.beams, a.vocab);
   ChunkSum* const sums = (ChunkSum*)a.work;
   uint64_t* const lists = (uint64_t*)(sums + (int64_t)rows * p.chunks);
-  const bool vec = a.vocab % 4 == 0 && a.ldl % 4 == 0 && (uintptr_t)a.logits % (4 * size) == 0;
-  const unsigned grid = (unsigned)(rows * p.chunks);
+  const bool vec = a.ldl * size % 16 == 0 && (uintptr_t)a.logits % 16 == 0;
+  const int waves = rows * p.chunks;
+  const unsigned grid = (unsigned)((waves + kWavesPerBlock - 1) / kWavesPerBlock);
   auto s = (hipStream_t)stream;
 #define TFD_SCAN(T, P)                                                                   \
-  if (vec) k_beam_scan<T, P, true><<<grid, kScan, 0, s>>>(a, p.chunks, sums, lists);     \
-  else k_beam_scan<T, P, false><<<grid, kScan, 0, s>>>(a, p.chunks, sums, lists);
+  if (vec) k_beam_scan<T, P, true><<<grid, kBlock, 0, s>>>(a, p.chunks, waves, sums, lists); \
+  else k_beam_scan<T, P, false><<<grid, kBlock, 0, s>>>(a, p.chunks, waves, sums, lists);
 #define TFD_SCAN_TYPE(T)                         \
   {                                              \
-    if (p.per == 4) { TFD_SCAN(T, 4) }           \
-    else if (p.per == 8) { TFD_SCAN(T, 8) }      \
+    if (p.per == 8) { TFD_SCAN(T, 8) }           \
     else if (p.per == 16) { TFD_SCAN(T, 16) }    \
-    else { TFD_SCAN(T, 32) }                     \
+    else if (p.per == 32) { TFD_SCAN(T, 32) }    \
+    else { TFD_SCAN(T, 64) }                     \
   }
   if (a.type == TFD_TYPE_F32) TFD_SCAN_TYPE(TFD_TYPE_F32)
   else if (a.type == TFD_TYPE_BF16) TFD_SCAN_TYPE(TFD_TYPE_BF16)
@@ -480,25 +644,31 @@ int tfd_beam_select(const TfdBeamArgs* args, void* stream) {
   return launched("beam_select");
 }
 
-int64_t tfd_state_blocks(const void* base, int64_t row_bytes) {
-  return row_bytes > 0 ? state_blocks(base, row_bytes) : 0;
+int64_t tfd_state_blocks(const void* base, int64_t row_bytes, int pieces) {
+  if (row_bytes <= 0 || pieces < 1) return 0;
+  const int unit = state_unit(base, row_bytes);
+  const int64_t per = (int64_t)kBlock * pieces * (unit == 16 ? 16 : kUnits * unit);
+  return (row_bytes + per - 1) / per;
 }
 
-int tfd_reorder_states(const TfdState* states, int n, int64_t blocks, const int32_t* parents,
-                       int groups, int beams, int32_t* err, void* stream) {
-  if (n < 0 || groups < 0 || groups > 65535 || beams < 1 || beams > kMaxBeams || blocks < 0 ||
-      blocks >= (1ll << 24))
-    return fail(kBadShape, "reorder_states: n=%d groups=%d beams=%d (1..%d) blocks=%lld", n, groups,
-                beams, kMaxBeams, (long long)blocks);
+int tfd_reorder_states(const TfdState* states, int n, int pieces, int64_t blocks,
+                       const int32_t* parents, int groups, int beams, int32_t* err,
+                       void* stream) {
+  if (n < 0 || pieces < 1 || groups < 0 || groups > 65535 || beams < 1 || beams > kMaxBeams ||
+      blocks < 0 || blocks >= (1ll << 24))
+    return fail(kBadShape, "reorder_states: n=%d pieces=%d groups=%d beams=%d (1..%d) blocks=%lld",
+                n, pieces, groups, beams, kMaxBeams, (long long)blocks);
   if (n == 0 || groups == 0 || blocks == 0) return 0;
   if (!states || !parents) return fail(kBadArg, "reorder_states: null pointer");
   const dim3 grid((unsigned)blocks, groups);
   auto s = (hipStream_t)stream;
-  if (beams <= 4) k_reorder<4><<<grid, kBlock, 0, s>>>(states, n, parents, beams, err);
-  else if (beams <= 8) k_reorder<8><<<grid, kBlock, 0, s>>>(states, n, parents, beams, err);
-  else if (beams <= 16) k_reorder<16><<<grid, kBlock, 0, s>>>(states, n, parents, beams, err);
-  else if (beams <= 32) k_reorder<32><<<grid, kBlock, 0, s>>>(states, n, parents, beams, err);
-  else k_reorder<64><<<grid, kBlock, 0, s>>>(states, n, parents, beams, err);
+#define TFD_MOVES(M) k_reorder<M><<<grid, kBlock, 0, s>>>(states, n, pieces, parents, beams, err)
+  if (beams <= 4) TFD_MOVES(4);
+  else if (beams <= 8) TFD_MOVES(8);
+  else if (beams <= 16) TFD_MOVES(16);
+  else if (beams <= 32) TFD_MOVES(32);
+  else TFD_MOVES(64);
+#undef TFD_MOVES
   return launched("reorder_states");
 }
 

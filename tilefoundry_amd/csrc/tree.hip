@@ -112,20 +112,22 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // t G + g) with its n = L + count positions.  Everything is kept transposed, so that a lane
 // owns one query's softmax: S^T = K Q^T gives lane l the scores of query l % 16 at
 // positions 16 i + 4 (l / 16) + e, which is, packed, an operand of O^T += V^T P^T (a product's
-// k may be taken in any order that both operands share).
-//
-// A wave takes every (4 splits)-th tile of 32 positions (two pages) for 16 NQ columns:
-// its K goes from memory into registers as operands, its V through a private piece of LDS, from
-// which the transposing read gives V^T's operands.  No barrier until the waves' sums are
-// joined; the next tile's loads are in flight behind the current one's products.  V lies in
-// LDS by rows, its 32-byte pieces permuted by the row so that the 16 rows of a transposing read
-// take the fewest cycles.
+// k may be taken in any order that both operands share).  V lies in LDS by rows, and the
+// transposing read gives V^T's operands; its 32-byte pieces are permuted by the row so that the
+// 16 rows of such a read take the fewest cycles.
 //
 // Softmax with a running maximum, in f32; a rescale only where a maximum moved.  A
 // probability is the sum of two bf16, so that it is not the less exact operand.
+//
+// Two kernels.  Few columns (k_tree_few): the keys are what is waited for, so each wave
+// takes other tiles of 32 positions, its K straight into registers as operands and its V
+// through a private piece of LDS, and no barrier until the waves' sums are joined.  Many
+// columns (k_tree_many): the waves take 16 NQ columns each and share tiles in LDS, which come
+// in by way of registers a tile ahead, one barrier a tile.  Both may cut a row's positions into
+// splits, which k_tree_join adds.
 // ---------------------------------------------------------------------------
 typedef short i16x4 __attribute__((ext_vector_type(4)));
-constexpr int kTile = 32;                    // positions
+constexpr int kTile = 32;                    // positions of a wave's tile
 
 template <int D>
 __device__ __forceinline__ int v_swizzle(int row) {
@@ -136,21 +138,23 @@ template <int D>
 __device__ __forceinline__ int v_at(int row, int chunk) {
   return row * D * 2 + ((chunk ^ v_swizzle<D>(row)) << 5);
 }
-
-struct TreePlan {
-  int nq, mtiles, splits;
-};
-
-template <int D, int NQ>
-constexpr int tree_lds() {
-  const int v = 4 * kTile * D * 2, join = 4 * NQ * 1024;
-  return 16 * NQ * D * 2 + (v > join ? v : join);
+// byte of K[row][8 chunk]: 16 rows of a chunk lie in as many places of 256 bytes
+template <int D>
+__device__ __forceinline__ int k_at(int row, int chunk) {
+  return row * D * 2 + ((chunk ^ (D == 64 ? (row >> 1) & 7 : row & 15)) << 4);
 }
 
-// Blocks of a compute unit that the registers of a variant allow.
-template <int D, int NQ>
-constexpr int tree_blocks() {
-  return D * NQ <= 64 ? 4 : D * NQ <= 128 ? 3 : D * NQ <= 256 ? 2 : 1;
+// V^T's operand for dims 16 dt .. + 15 and the 32 positions at `v`.
+template <int D>
+__device__ __forceinline__ u32x4 v_operand(const uint8_t* v, int dt, int lane) {
+  i16x4 f[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    f[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) i16x4*)(v +
+            v_at<D>(16 * t + 4 * (lane >> 4) + ((lane & 15) >> 2), dt) + (lane & 3) * 8));
+  const u32x2 a = __builtin_bit_cast(u32x2, f[0]), b = __builtin_bit_cast(u32x2, f[1]);
+  return u32x4{a.x, a.y, b.x, b.y};
 }
 
 // Two bf16 with zeros in the place of infinities and NaN.
@@ -159,69 +163,184 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
   return w;
 }
+// 16 bytes of V at position j of a tile that reaches the drafted positions: zeros past the last
+// one, which holds anything, and in the place of drafted values that are not finite.
+__device__ __forceinline__ u32x4 clean_v(u32x4 v, int j, int L, int n, bool& odd) {
+  if (j >= n) v = u32x4{0u, 0u, 0u, 0u};
+  if (j >= L) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t f = finite_halves(v[w]);
+      odd |= f != v[w];
+      v[w] = f;
+    }
+  }
+  return v;
+}
 
-template <int D, int NQ>
-__global__ __launch_bounds__(kBlock, (tree_blocks<D, NQ>())) void k_tree_attn(
-    TfdTreeAttnArgs a, int splits, int mtiles,
-                                                      float* __restrict__ part_o,
-                                                      float* __restrict__ part_ml) {
+// One row's part of a call, as a block sees it.
+struct TreeRow {
+  const int* table;
+  const bf16 *k, *v;                         // of the kv head, page 0
+  const uint64_t* masks;
+  int64_t page_size;
+  int row, h, G, L, n, cols, first, words, last_page, num_pages;
+  bool bad_page;
+
+  __device__ __forceinline__ int page_at(int i) {
+    const int p = table[min(i, last_page)];
+    const bool ok = p >= 0 && p < num_pages;
+    bad_page |= !ok;
+    return ok ? p : 0;
+  }
+  __device__ __forceinline__ int node_of(int c) const { return (first + min(c, cols - 1)) / G; }
+  // bit i: column c sees position j0 + i, i < 32 (the context: every one)
+  __device__ __forceinline__ uint32_t seen(int c, int j0) const {
+    const uint64_t* const m = masks + (int64_t)node_of(c) * words;
+    const int from = j0 - L, w = max(from, 0) >> 6, sh = max(from, 0) & 63;
+    uint64_t bits = m[min(w, words - 1)] >> sh;
+    if (w >= words) bits = 0;
+    const uint64_t next = m[min(w + 1, words - 1)];
+    if (sh && w + 1 < words) bits |= next << (64 - sh);
+    if (from <= -kTile) bits = 0xffffffffu;
+    else if (from < 0) bits = (bits << -from) | ((1ull << -from) - 1);
+    const int left = n - j0;
+    if (left < kTile) bits = left > 0 ? bits & ((1ull << left) - 1) : 0;
+    return (uint32_t)bits;
+  }
+};
+
+// `unit` = (row, kv head, split); false: nothing to do.
+__device__ __forceinline__ bool tree_row(const TfdTreeAttnArgs& a, int unit, int splits, int first,
+                                         TreeRow& t) {
+  t.h = unit / splits % a.kv_heads;
+  t.row = unit / splits / a.kv_heads;
+  t.G = a.heads / a.kv_heads;
+  t.first = first;
+  const int count = row_nodes(a.counts, t.row, a.nodes);
+  t.cols = count * t.G - first;              // of this block on
+  if (t.cols <= 0) return false;
+  t.L = a.lengths[t.row];
+  t.n = t.L + count;
+  if (t.L < 0 || (int64_t)t.L + count > (int64_t)a.max_pages * kPage) {
+    if (threadIdx.x == 0) raise_error(a.err, kErrPosRange);
+    t.L = t.n = 0;
+  }
+  t.words = (a.nodes + 63) / 64;
+  t.table = a.page_table + (int64_t)t.row * a.max_pages;
+  t.masks = a.masks + (int64_t)t.row * a.nodes * t.words;
+  const int64_t head_size = kPage * a.head_dim;
+  t.page_size = a.kv_heads * head_size;
+  t.k = (const bf16*)a.k_pool + t.h * head_size;
+  t.v = (const bf16*)a.v_pool + t.h * head_size;
+  t.last_page = max(0, (t.n - 1) / kPage);
+  t.num_pages = a.num_pages;
+  t.bad_page = false;
+  return true;
+}
+
+// Eight probabilities' place in a column's softmax: the scores of 32 positions (this lane's
+// eight) become operands, maximum, sum and outputs follow.
+template <int DT, int NQ>
+__device__ __forceinline__ void tree_softmax(const f32x4 (&st)[2], float c2, float& mx, float& sum,
+                                             f32x4 (&o)[DT][NQ], int qt, u32x4& hi4, u32x4& lo4) {
+  float tm = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
+                   fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
+  float lo, hi;
+  pair16(tm, lo, hi);
+  tm = fmaxf(lo, hi);
+  pair32(tm, lo, hi);
+  const float m1 = fmaxf(mx, fmaxf(lo, hi));
+  const float ref = m1 == kPanelNegInf ? 0.f : m1 * c2;
+  if (__any(m1 != mx)) {
+    const float alpha = __builtin_amdgcn_exp2f(mx * c2 - ref);
+    mx = m1;
+    sum *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[dt][qt][e] *= alpha;
+  }
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4], c2, -ref));
+    sum += p[i];
+  }
+  hi4 = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] -= i % 2 ? bf_hi(hi4[i / 2]) : bf_lo(hi4[i / 2]);
+  lo4 = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
+}
+
+__device__ __forceinline__ float quad_sum(float v) {   // over a column's four lanes
+  float lo, hi;
+  pair16(v, lo, hi);
+  v = lo + hi;
+  pair32(v, lo, hi);
+  return lo + hi;
+}
+
+// A product would take a value that is not finite into every column (0 * inf): such values of
+// drafted nodes were left out of it and come in here, where they are seen.  y: dims 16 dt +
+// 4 kq .. + 3 of column c; positions j0 .. j1 - 1.
+__device__ __forceinline__ void add_odd(TreeRow& t, f32x4& y, int c, int d, int j0, int j1, int D) {
+  const uint64_t* const m = t.masks + (int64_t)t.node_of(c) * t.words;
+#pragma unroll 1
+  for (int j = max(j0, t.L); j < min(j1, t.n); ++j) {
+    const u32x2 x = *reinterpret_cast<const u32x2*>(
+        t.v + t.page_at(j / kPage) * t.page_size + (j % kPage) * D + d);
+    const bool see = (m[(j - t.L) >> 6] >> ((j - t.L) & 63)) & 1;
+    const uint32_t z[2] = {x.x, x.y};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = e % 2 ? bf_hi(z[e / 2]) : bf_lo(z[e / 2]);
+      if (see && !(fabsf(v) < __builtin_huge_valf())) y[e] += v;
+    }
+  }
+}
+
+__device__ __forceinline__ int64_t out_at(const TfdTreeAttnArgs& a, int64_t rr, int head, int d) {
+  return a.out_panel ? panel_off(rr, head * a.head_dim + d, a.heads * a.head_dim)
+                     : (rr * a.heads + head) * a.head_dim + d;
+}
+
+// The block's unit and tile of columns: blocks that read the same keys lie 8 apart, on one XCD.
+__device__ __forceinline__ void tree_block(int mtiles, int& unit, int& mt) {
+  const int per8 = 8 * mtiles;
+  unit = (int)(blockIdx.x / per8) * 8 + (int)(blockIdx.x % 8);
+  mt = (int)(blockIdx.x % per8) / 8;
+}
+
+// ------------------------------------------------------------------------ few columns
+template <int D, int NQ, int W>
+constexpr int few_lds() {
+  return 16 * NQ * D * 2 + W * kTile * D * 2;
+}
+
+template <int D, int NQ, int W>
+__global__ __launch_bounds__(W * kWave, D * NQ <= 64 ? 4 : D * NQ <= 128 ? 3 : 2)
+void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
+                float* __restrict__ part_ml) {
   constexpr int DS = D / 32, DT = D / 16, kCols = 16 * NQ;
   constexpr int kV = D / 16;                 // V loads of a tile: 1 KiB each
   constexpr int kRowsPerLoad = 512 / D;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float ml_s[2][kWavesPerBlock][kCols];
+  __shared__ float m_s[W][kCols], l_s[W][kCols], inv_s[kCols];
   uint8_t* const q_s = smem;                 // operand order: 1 KiB per (16 columns, 32 dims)
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 15, kq = lane >> 4;
   uint8_t* const v_s = smem + kCols * D * 2 + wave * kTile * D * 2;
-
-  // blocks that read the same keys lie 8 apart: one XCD's L2
-  const int per8 = 8 * mtiles;
-  const int unit = (int)(blockIdx.x / per8) * 8 + (int)(blockIdx.x % 8);
-  const int mt = (int)(blockIdx.x % per8) / 8;
-  if (unit >= a.rows * a.kv_heads * splits) return;
-  const int split = unit % splits, h = unit / splits % a.kv_heads, row = unit / splits / a.kv_heads;
-  const int G = a.heads / a.kv_heads;
-  const int count = row_nodes(a.counts, row, a.nodes);
-  const int cols = count * G - mt * kCols;   // of this block
-  if (cols <= 0) return;
-  int L = a.lengths[row];
-  const bool bad_length = L < 0 || (int64_t)L + count > (int64_t)a.max_pages * kPage;
-  if (bad_length) {
-    if (tid == 0) raise_error(a.err, kErrPosRange);
-    L = 0;
-  }
-  const int n = bad_length ? 0 : L + count;
-  const int tiles = (n + kTile - 1) / kTile, words = (a.nodes + 63) / 64;
-  const int* __restrict__ table = a.page_table + (int64_t)row * a.max_pages;
-  const int64_t head_size = kPage * D, page_size = (int64_t)a.kv_heads * head_size;
-  const bf16* const kp = (const bf16*)a.k_pool + h * head_size;
-  const bf16* const vp = (const bf16*)a.v_pool + h * head_size;
-  const int last_page = max(0, (n - 1) / kPage);
-
-  bool page_bad = false;
-  auto page_at = [&](int i) {
-    const int p = table[min(i, last_page)];
-    const bool ok = p >= 0 && p < a.num_pages;
-    page_bad |= !ok;
-    return ok ? p : 0;
-  };
-
-  // the block's queries
-  for (int i = tid; i < kCols * D / 8; i += kBlock) {
-    const int b = i / 64, l = i % 64;        // block b: columns 16 (b / DS), dims 32 (b % DS)
-    const int c = 16 * (b / DS) + (l & 15), d = 32 * (b % DS) + 8 * (l >> 4);
-    const int cc = mt * kCols + min(c, cols - 1);
-    const int node = cc / G, head = h * G + cc % G;
-    *reinterpret_cast<u32x4*>(q_s + i * 16) = load16(
-        (const bf16*)a.q + row * a.q_row + node * a.q_node + head * a.q_head + d);
-  }
+  const int unit = blockIdx.x, split = unit % splits;
+  TreeRow t;
+  if (!tree_row(a, unit, splits, 0, t)) return;
+  const int tiles = (t.n + kTile - 1) / kTile;
 
   u32x4 kr[2][DS], vr[kV];
   auto load_k = [&](int p0, int p1) {
-    const bf16* const k0 = kp + p0 * page_size + r * D + 8 * kq;
-    const bf16* const k1 = kp + p1 * page_size + r * D + 8 * kq;
+    const bf16* const k0 = t.k + p0 * t.page_size + r * D + 8 * kq;
+    const bf16* const k1 = t.k + p1 * t.page_size + r * D + 8 * kq;
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       kr[0][s] = load16(k0 + 32 * s);
@@ -229,8 +348,8 @@ __global__ __launch_bounds__(kBlock, (tree_blocks<D, NQ>())) void k_tree_attn(
     }
   };
   auto load_v = [&](int p0, int p1) {
-    const bf16* const v0 = vp + p0 * page_size + lane * 8;
-    const bf16* const v1 = vp + p1 * page_size + lane * 8;
+    const bf16* const v0 = t.v + p0 * t.page_size + lane * 8;
+    const bf16* const v1 = t.v + p1 * t.page_size + lane * 8;
 #pragma unroll
     for (int i = 0; i < kV / 2; ++i) {
       vr[i] = load16(v0 + i * 512);
@@ -249,43 +368,36 @@ __global__ __launch_bounds__(kBlock, (tree_blocks<D, NQ>())) void k_tree_attn(
     for (int dt = 0; dt < DT; ++dt) o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int slots = splits * kWavesPerBlock;
-  const int tile0 = split * kWavesPerBlock + wave;
+  const int slots = splits * W, tile0 = split * W + wave;
   int tile = tile0, p0 = 0, p1 = 0;
   bool odd = false;                          // a drafted value is not finite
   if (tile < tiles) {
-    p0 = page_at(2 * tile), p1 = page_at(2 * tile + 1);
+    p0 = t.page_at(2 * tile), p1 = t.page_at(2 * tile + 1);
     load_v(p0, p1);
     load_k(p0, p1);
-    p0 = page_at(2 * (tile + slots)), p1 = page_at(2 * (tile + slots) + 1);
+    p0 = t.page_at(2 * (tile + slots)), p1 = t.page_at(2 * (tile + slots) + 1);
+  }
+  for (int i = tid; i < kCols * D / 8; i += W * kWave) {
+    const int b = i / 64, l = i % 64;        // block b: columns 16 (b / DS), dims 32 (b % DS)
+    const int c = min(16 * (b / DS) + (l & 15), t.cols - 1), d = 32 * (b % DS) + 8 * (l >> 4);
+    *reinterpret_cast<u32x4*>(q_s + i * 16) =
+        load16((const bf16*)a.q + t.row * a.q_row + c / t.G * a.q_node +
+               (t.h * t.G + c % t.G) * a.q_head + d);
   }
   __syncthreads();                           // the queries are in place
 
   for (; tile < tiles; tile += slots) {
     const int j0 = tile * kTile;
-    const bool edge = j0 + kTile > L;        // drafted positions, or none, in this tile
-    // V into LDS; positions past the last hold anything and read as zeros, drafted values that
-    // are not finite too (below)
+    const bool edge = j0 + kTile > t.L;      // drafted positions, or none, in this tile
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
       const int rr = i * kRowsPerLoad + lane / (D / 8), c8 = lane % (D / 8);
       u32x4 v = vr[i];
-      if (edge) {
-        if (j0 + rr >= n) v = u32x4{0u, 0u, 0u, 0u};
-        if (j0 + rr >= L) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t f = finite_halves(v[w]);
-            odd |= f != v[w];
-            v[w] = f;
-          }
-        }
-      }
+      if (edge) v = clean_v(v, j0 + rr, t.L, t.n, odd);
       *reinterpret_cast<u32x4*>(v_s + v_at<D>(rr, c8 >> 1) + (c8 & 1) * 16) = v;
     }
     const bool more = tile + slots < tiles;
     if (more) load_v(p0, p1);
-
     u32x4 ph[NQ], pl[NQ];
 #pragma unroll
     for (int qt = 0; qt < NQ; ++qt) {
@@ -297,88 +409,35 @@ __global__ __launch_bounds__(kBlock, (tree_blocks<D, NQ>())) void k_tree_attn(
         st[1] = mfma(kr[1][s], qf, st[1]);
       }
       if (edge) {
-        // bit i: this column sees position j0 + i (the context: every one)
-        const int node = (mt * kCols + min(16 * qt + r, cols - 1)) / G, from = j0 - L;
-        const uint64_t* const mrow = a.masks + ((int64_t)row * a.nodes + node) * words;
-        const int w = max(from, 0) >> 6, sh = max(from, 0) & 63;
-        const uint64_t m0 = mrow[w], m1 = mrow[min(w + 1, words - 1)];
-        uint64_t bits = m0 >> sh;
-        if (sh && w + 1 < words) bits |= m1 << (64 - sh);
-        if (from < 0) bits = (bits << -from) | ((1ull << -from) - 1);
-        if (n - j0 < kTile) bits &= (1ull << (n - j0)) - 1;
-        const uint32_t see = (uint32_t)bits >> (4 * kq);
+        const uint32_t see = t.seen(16 * qt + r, j0) >> (4 * kq);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            st[t][e] = (see >> (16 * t + e)) & 1 ? st[t][e] : kPanelNegInf;
+        for (int i = 0; i < 8; ++i)
+          st[i / 4][i % 4] = (see >> (16 * (i / 4) + i % 4)) & 1 ? st[i / 4][i % 4] : kPanelNegInf;
       }
-      float tm = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
-                       fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
-      float lo, hi;
-      pair16(tm, lo, hi);
-      tm = fmaxf(lo, hi);
-      pair32(tm, lo, hi);
-      const float m1 = fmaxf(mx[qt], fmaxf(lo, hi));
-      const float ref = m1 == kPanelNegInf ? 0.f : m1 * c2;
-      if (__any(m1 != mx[qt])) {
-        const float alpha = __builtin_amdgcn_exp2f(mx[qt] * c2 - ref);
-        mx[qt] = m1;
-        sum[qt] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[dt][qt][e] *= alpha;
-      }
-      float p[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4], c2, -ref));
-        sum[qt] += p[i];
-      }
-      ph[qt] = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        p[i] -= i % 2 ? bf_hi(ph[qt][i / 2]) : bf_lo(ph[qt][i / 2]);
-      pl[qt] = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
-      if (NQ > 2) __builtin_amdgcn_sched_barrier(0);   // (else registers are spilled)
+      tree_softmax<DT, NQ>(st, c2, mx[qt], sum[qt], o, qt, ph[qt], pl[qt]);
     }
     if (more) {
       load_k(p0, p1);
-      p0 = page_at(2 * (tile + 2 * slots)), p1 = page_at(2 * (tile + 2 * slots) + 1);
+      p0 = t.page_at(2 * (tile + 2 * slots)), p1 = t.page_at(2 * (tile + 2 * slots) + 1);
     }
-
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      i16x4 f[2];
+      const u32x4 vf = v_operand<D>(v_s, dt, lane);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        f[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) i16x4*)(v_s +
-                v_at<D>(16 * t + 4 * kq + (r >> 2), dt) + (r & 3) * 8));
-      const u32x2 f0 = __builtin_bit_cast(u32x2, f[0]), f1 = __builtin_bit_cast(u32x2, f[1]);
-      const u32x4 vf = u32x4{f0.x, f0.y, f1.x, f1.y};
+      for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pl[qt], o[dt][qt]);
 #pragma unroll
-      for (int qt = 0; qt < NQ; ++qt) {
-        o[dt][qt] = mfma(vf, pl[qt], o[dt][qt]);
-        o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
-      }
-      if (NQ > 2 && dt % 2) __builtin_amdgcn_sched_barrier(0);
+      for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
     }
   }
   odd = __any(odd);
 
-  // join the waves: maxima and sums, then 16 dims of all columns at a time
+  // join the waves: maxima and sums, then DT / NQ times 16 dims of all columns at a time
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
-    float lo, hi, l = sum[qt];
-    pair16(l, lo, hi);
-    l = lo + hi;
-    pair32(l, lo, hi);
-    l = lo + hi;
+    sum[qt] = quad_sum(sum[qt]);
     if (kq == 0) {
-      ml_s[0][wave][16 * qt + r] = mx[qt];
-      ml_s[1][wave][16 * qt + r] = l;
+      m_s[wave][16 * qt + r] = mx[qt];
+      l_s[wave][16 * qt + r] = sum[qt];
     }
   }
   __syncthreads();                           // (V's pieces are free from here on)
@@ -386,131 +445,334 @@ __global__ __launch_bounds__(kBlock, (tree_blocks<D, NQ>())) void k_tree_attn(
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
     const int c = 16 * qt + r;
-    float m = ml_s[0][0][c];
+    float m = m_s[0][c], l = 0.f;
 #pragma unroll
-    for (int w = 1; w < kWavesPerBlock; ++w) m = fmaxf(m, ml_s[0][w][c]);
-    // a sum of NaN is one whatever its maximum
-    const float l = ml_s[1][wave][c];
-    scale[qt] = l != l ? l : mx[qt] == kPanelNegInf ? 0.f
-                                                    : __builtin_amdgcn_exp2f((mx[qt] - m) * c2);
-  }
-  // A product would take a value that is not finite into every column (0 * inf): such values
-  // of drafted nodes were left out of it and come in here, where they are seen.
-  auto add_odd = [&](f32x4& y, int dt, int qt) {
-    const int node = (mt * kCols + min(16 * qt + r, cols - 1)) / G;
-    const uint64_t* const mrow = a.masks + ((int64_t)row * a.nodes + node) * words;
-#pragma unroll 1
-    for (int t = tile0; t < tiles; t += slots)
-#pragma unroll 1
-      for (int j = max(t * kTile, L); j < min(t * kTile + kTile, n); ++j) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(
-            vp + page_at(j / kPage) * page_size + (j % kPage) * D + 16 * dt + 4 * kq);
-        const bool see = (mrow[(j - L) >> 6] >> ((j - L) & 63)) & 1;
-        const uint32_t z[2] = {x.x, x.y};
+    for (int w = 1; w < W; ++w) m = fmaxf(m, m_s[w][c]);
+    // (a wave that saw nothing: a sum of zero; a sum of NaN is one whatever its maximum)
+    scale[qt] = sum[qt] != sum[qt] ? sum[qt]
+                : mx[qt] == kPanelNegInf ? 0.f
+                                         : __builtin_amdgcn_exp2f((mx[qt] - m) * c2);
+    if (wave == 0 && kq == 0) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = e % 2 ? bf_hi(z[e / 2]) : bf_lo(z[e / 2]);
-          if (see && !(fabsf(v) < __builtin_huge_valf())) y[e] += v;
-        }
+      for (int w = 0; w < W; ++w)
+        l += l_s[w][c] * (m_s[w][c] == kPanelNegInf
+                              ? 1.f
+                              : __builtin_amdgcn_exp2f((m_s[w][c] - m) * c2));
+      inv_s[c] = l == 0.f ? 0.f : 1.f / l;
+      if (splits > 1 && c < t.cols) {
+        part_ml[((int64_t)unit * kCols + c) * 2] = m;
+        part_ml[((int64_t)unit * kCols + c) * 2 + 1] = l;
       }
-  };
+    }
+  }
   float* const join = reinterpret_cast<float*>(smem + kCols * D * 2);
-  const int64_t pcol = (int64_t)unit * mtiles * kCols + mt * kCols;
+  constexpr int kDims = DT / NQ;             // 16 dims each, of a pass
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    if (dt) __syncthreads();
+  for (int pass = 0; pass < NQ; ++pass) {
+    if (pass) __syncthreads();
 #pragma unroll
-    for (int qt = 0; qt < NQ; ++qt) {
-      f32x4 y = o[dt][qt] * scale[qt];
-      if (scale[qt] == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (odd) add_odd(y, dt, qt);
-      *reinterpret_cast<f32x4*>(join + (wave * NQ + qt) * 256 + r * 16 + kq * 4) = y;
-    }
-    __syncthreads();
+    for (int i = 0; i < kDims; ++i)
 #pragma unroll
-    for (int qt = 0; qt < NQ; ++qt) {
-      const int c = 16 * qt + tid / 16, d = 16 * dt + tid % 16;
-      float m = ml_s[0][0][c], l = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 1; w < kWavesPerBlock; ++w) m = fmaxf(m, ml_s[0][w][c]);
-#pragma unroll
-      for (int w = 0; w < kWavesPerBlock; ++w) {
-        y += join[(w * NQ + qt) * 256 + tid];
-        // (nothing seen: a sum of zero)
-        const float f = ml_s[0][w][c] == kPanelNegInf
-                            ? 1.f
-                            : __builtin_amdgcn_exp2f((ml_s[0][w][c] - m) * c2);
-        l += ml_s[1][w][c] * f;
+      for (int qt = 0; qt < NQ; ++qt) {
+        const int dt = pass * kDims + i;
+        f32x4 y = o[dt][qt] * scale[qt];
+        if (scale[qt] == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (odd)
+          for (int k = tile0; k < tiles; k += slots)
+            add_odd(t, y, 16 * qt + r, 16 * dt + 4 * kq, k * kTile, k * kTile + kTile, D);
+        *reinterpret_cast<f32x4*>(join + ((wave * NQ + qt) * kDims + i) * 256 + r * 16 + kq * 4) =
+            y;
       }
-      if (c >= cols) continue;
+    __syncthreads();
+    constexpr int kAll = NQ * kDims * 64;    // four values each
+    for (int i = tid; i < kAll; i += W * kWave) {
+      f32x4 y = *reinterpret_cast<const f32x4*>(join + i * 4);
+#pragma unroll
+      for (int w = 1; w < W; ++w)
+        y += *reinterpret_cast<const f32x4*>(join + (w * kAll + i) * 4);
+      const int c = 16 * (i / 64 / kDims) + i % 64 / 4;
+      const int d = 16 * (pass * kDims + i / 64 % kDims) + i % 4 * 4;
+      if (c >= t.cols) continue;
       if (splits == 1) {
-        const int cc = mt * kCols + c, node = cc / G, head = h * G + cc % G;
-        const float v = l == 0.f ? 0.f : y / l;
-        const int64_t rr = (int64_t)row * a.nodes + node;
-        const int64_t at = a.out_panel ? panel_off(rr, head * D + d, a.heads * D)
-                                       : (rr * a.heads + head) * D + d;
-        ((bf16*)a.out)[at] = f2bf(v);
+        const float f = inv_s[c];
+        if (f == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, (int64_t)t.row * a.nodes + c / t.G,
+                                                        t.h * t.G + c % t.G, d)) =
+            u32x2{pack2(y[0] * f, y[1] * f), pack2(y[2] * f, y[3] * f)};
       } else {
-        part_o[(pcol + c) * D + d] = y;
-        if (dt == 0 && tid % 16 == 0) {
-          part_ml[(pcol + c) * 2] = m;
-          part_ml[(pcol + c) * 2 + 1] = l;
-        }
+        *reinterpret_cast<f32x4*>(part_o + ((int64_t)unit * kCols + c) * D + d) = y;
       }
     }
   }
-  if (page_bad && lane == 0) raise_error(a.err, kErrPageRange);
+  if (t.bad_page && lane == 0) raise_error(a.err, kErrPageRange);
 }
 
-// The splits' sums joined: a wave per (row, node, head).
+// ----------------------------------------------------------------------- many columns
+template <int D>
+constexpr int many_tile() {                  // positions
+  return D <= 128 ? 64 : 32;
+}
+template <int D>
+constexpr int many_nq() {
+  return D <= 128 ? 2 : 1;
+}
+template <int D>
+constexpr int many_lds() {                   // two buffers of K and V
+  return 2 * 2 * many_tile<D>() * D * 2;
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles,
+                                                            float* __restrict__ part_o,
+                                                            float* __restrict__ part_ml) {
+  constexpr int NQ = many_nq<D>(), DS = D / 32, DT = D / 16, kPos = many_tile<D>();
+  constexpr int kCols = 16 * NQ * W, kBytes = kPos * D * 2;
+  constexpr int kLoads = kBytes / 16 / (W * kWave);    // of K, of V, by a thread
+  constexpr int kChunks = D / 8;             // 16 bytes each, of a position
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int odd_s;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int r = lane & 15, kq = lane >> 4;
+  int unit, mt;
+  tree_block(mtiles, unit, mt);
+  if (unit >= a.rows * a.kv_heads * splits) return;
+  const int split = unit % splits;
+  TreeRow t;
+  if (!tree_row(a, unit, splits, mt * kCols, t)) return;
+  const int c0 = wave * 16 * NQ;             // this wave's columns, within the block's
+
+  // this split's tiles
+  const int tiles = (t.n + kPos - 1) / kPos;
+  const int begin = (int)((int64_t)tiles * split / splits);
+  const int end = (int)((int64_t)tiles * (split + 1) / splits);
+
+  u32x4 kr[kLoads], vr[kLoads];
+  int pages[kLoads];                         // of the tile that is loaded next
+  auto next_pages = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      pages[i] = t.page_at(tile * (kPos / kPage) +
+                           (i * W + wave) * kWave / kChunks / kPage);
+  };
+  auto load_tile = [&]() {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int64_t at = pages[i] * t.page_size + (i * W * kWave + tid) % (kPage * kChunks) * 8;
+      kr[i] = load16(t.k + at);
+      vr[i] = load16(t.v + at);
+    }
+  };
+  bool odd = false;                          // a drafted value is not finite
+  auto store_tile = [&](uint8_t* buf, int tile) {
+    const bool edge = (tile + 1) * kPos > t.L;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = i * W * kWave + tid, rr = at / kChunks, c8 = at % kChunks;
+      *reinterpret_cast<u32x4*>(buf + k_at<D>(rr, c8)) = kr[i];
+      u32x4 v = vr[i];
+      if (edge) v = clean_v(v, tile * kPos + rr, t.L, t.n, odd);
+      *reinterpret_cast<u32x4*>(buf + kBytes + v_at<D>(rr, c8 >> 1) + (c8 & 1) * 16) = v;
+    }
+  };
+
+  if (begin < end) {
+    next_pages(begin);
+    load_tile();
+    next_pages(begin + 1);
+  }
+  u32x4 qf[NQ][DS];
+#pragma unroll
+  for (int qt = 0; qt < NQ; ++qt) {
+    const int c = t.first + min(c0 + 16 * qt + r, t.cols - 1);
+    const bf16* const q = (const bf16*)a.q + t.row * a.q_row + c / t.G * a.q_node +
+                          (t.h * t.G + c % t.G) * a.q_head + 8 * kq;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) qf[qt][s] = load16(q + 32 * s);
+  }
+  const float c2 = a.scale * 1.44269504088896340736f;
+  float mx[NQ], sum[NQ];
+  f32x4 o[DT][NQ];
+#pragma unroll
+  for (int qt = 0; qt < NQ; ++qt) {
+    mx[qt] = kPanelNegInf;
+    sum[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (tid == 0) odd_s = 0;
+  if (begin < end) {
+    store_tile(smem, begin);
+    if (begin + 1 < end) load_tile();
+    next_pages(begin + 2);
+  }
+  __syncthreads();
+
+  for (int tile = begin; tile < end; ++tile) {
+    uint8_t* const buf = smem + ((tile - begin) & 1) * 2 * kBytes;
+    uint8_t* const other = smem + ((tile - begin + 1) & 1) * 2 * kBytes;
+    if (tile + 1 < end) store_tile(other, tile + 1);   // (read by all before the last barrier)
+    if (tile + 2 < end) {
+      load_tile();
+      next_pages(tile + 3);
+    }
+    const bool edge = (tile + 1) * kPos > t.L;
+    if (c0 < t.cols) {
+#pragma unroll
+      for (int kk = 0; kk < kPos / kTile; ++kk) {
+        f32x4 st[NQ][2];
+#pragma unroll
+        for (int qt = 0; qt < NQ; ++qt)
+          st[qt][0] = st[qt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < DS; ++s)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const u32x4 kf = *reinterpret_cast<const u32x4*>(
+                buf + k_at<D>(kk * kTile + 16 * p + r, 4 * s + kq));
+#pragma unroll
+            for (int qt = 0; qt < NQ; ++qt) st[qt][p] = mfma(kf, qf[qt][s], st[qt][p]);
+          }
+        u32x4 ph[NQ], pl[NQ];
+#pragma unroll
+        for (int qt = 0; qt < NQ; ++qt) {
+          if (edge) {
+            const uint32_t see =
+                t.seen(c0 + 16 * qt + r, tile * kPos + kk * kTile) >> (4 * kq);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              st[qt][i / 4][i % 4] =
+                  (see >> (16 * (i / 4) + i % 4)) & 1 ? st[qt][i / 4][i % 4] : kPanelNegInf;
+          }
+          tree_softmax<DT, NQ>(st[qt], c2, mx[qt], sum[qt], o, qt, ph[qt], pl[qt]);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, lane);
+#pragma unroll
+          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pl[qt], o[dt][qt]);
+#pragma unroll
+          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
+        }
+      }
+    }
+    if (tile + 1 < end) __syncthreads();
+  }
+  if (odd) odd_s = 1;
+  __syncthreads();
+  odd = odd_s;
+
+  const int64_t pcol = ((int64_t)unit * mtiles + mt) * kCols;
+#pragma unroll
+  for (int qt = 0; qt < NQ; ++qt) {
+    const int c = c0 + 16 * qt + r;
+    const float l = quad_sum(sum[qt]), inv = l == 0.f ? 0.f : 1.f / l;
+    if (c >= t.cols) continue;
+    if (splits > 1 && kq == 0) {
+      part_ml[(pcol + c) * 2] = mx[qt];
+      part_ml[(pcol + c) * 2 + 1] = l;
+    }
+    const int cc = t.first + c;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const int d = 16 * dt + 4 * kq;
+      f32x4 y = o[dt][qt];
+      if (odd) add_odd(t, y, c, d, begin * kPos, end * kPos, D);
+      if (splits == 1) {
+        if (inv == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
+        *reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, (int64_t)t.row * a.nodes + cc / t.G,
+                                                        t.h * t.G + cc % t.G, d)) =
+            u32x2{pack2(y[0] * inv, y[1] * inv), pack2(y[2] * inv, y[3] * inv)};
+      } else {
+        *reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d) = y;
+      }
+    }
+  }
+  if (t.bad_page && lane == 0) raise_error(a.err, kErrPageRange);
+}
+
+// ---------------------------------------------------------------------------
+// The splits' sums joined: a wave per (row, node, head); lane s holds split s's maximum and
+// sum, so that all weights take one round of loads.
+// ---------------------------------------------------------------------------
+constexpr int kMaxSplits = kWave;
+
 template <int D>
 __global__ __launch_bounds__(kBlock) void k_tree_join(TfdTreeAttnArgs a, int splits, int pad_cols,
                                                       const float* __restrict__ part_o,
                                                       const float* __restrict__ part_ml) {
   constexpr int kPer = D / kWave;
   const int lane = threadIdx.x & (kWave - 1);
-  const int64_t i = (int64_t)blockIdx.x * kWavesPerBlock + threadIdx.x / kWave;
+  const int64_t i = (int64_t)blockIdx.x * kWavesPerBlock +
+                    __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   const int64_t rr = i / a.heads;
   const int head = (int)(i % a.heads), row = (int)(rr / a.nodes), node = (int)(rr % a.nodes);
   if (row >= a.rows || node >= row_nodes(a.counts, row, a.nodes)) return;
   const int G = a.heads / a.kv_heads, h = head / G, c = node * G + head % G;
   const float c2 = a.scale * 1.44269504088896340736f;
-  const int64_t first = ((int64_t)row * a.kv_heads + h) * splits;
-  float m = kPanelNegInf, l = 0.f, y[kPer];
+  const int64_t at0 = ((int64_t)row * a.kv_heads + h) * splits * pad_cols + c;
+  const int64_t mine = at0 + (int64_t)min(lane, splits - 1) * pad_cols;
+  const float ms = part_ml[mine * 2], ls = lane < splits ? part_ml[mine * 2 + 1] : 0.f;
+  // (a split that saw nothing: a sum of zero)
+  const float m = wave_max(ls == 0.f ? kPanelNegInf : ms);
+  const float w = ls == 0.f ? 0.f : ms == kPanelNegInf ? 1.f
+                                                       : __builtin_amdgcn_exp2f((ms - m) * c2);
+  const float l = wave_sum(ls * w);
+  float y[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) y[e] = 0.f;
-  for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[((first + s) * pad_cols + c) * 2]);
+#pragma unroll 4
   for (int s = 0; s < splits; ++s) {
-    const int64_t at = (first + s) * pad_cols + c;
-    const float ms = part_ml[at * 2];
-    const float ls = part_ml[at * 2 + 1];
-    if (ls == 0.f) continue;                 // it saw nothing
-    const float w = ms == kPanelNegInf ? 1.f : __builtin_amdgcn_exp2f((ms - m) * c2);
-    l += w * ls;
+    const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s));
+    const float* const p = part_o + (at0 + (int64_t)s * pad_cols) * D + lane * kPer;
+    float x[kPer];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) y[e] += w * part_o[at * D + lane * kPer + e];
+    for (int e = 0; e < kPer; ++e) x[e] = p[e];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) y[e] += f == 0.f ? 0.f : f * x[e];
   }
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) {
-    const int d = lane * kPer + e;
-    const int64_t at = a.out_panel ? panel_off(rr, head * D + d, a.heads * D)
-                                   : (rr * a.heads + head) * D + d;
-    ((bf16*)a.out)[at] = f2bf(l == 0.f ? 0.f : y[e] / l);
-  }
+  for (int e = 0; e < kPer; ++e)
+    ((bf16*)a.out)[out_at(a, rr, head, lane * kPer + e)] = f2bf(l == 0.f ? 0.f : y[e] / l);
 }
+
+// How a call runs.  Few columns (up to 32, 16 of 256 dims): blocks of four waves, or where a row's tiles are few
+// enough for one block of eight, that alone (no second launch).  Many: four or eight waves of
+// 32 columns (16 of 256 dims).  Splits: as many as fill the compute units' blocks once.
+struct TreePlan {
+  int nq, waves, mtiles, cols, splits;       // nq 0: many columns; cols: of a block
+};
 
 TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, int max_pages) {
   TreePlan p;
   const int cols = nodes * (heads / kv_heads);
-  p.nq = cols <= 16 ? 1 : cols <= 32 || head_dim == 256 ? 2 : 4;
-  p.mtiles = (cols + 16 * p.nq - 1) / (16 * p.nq);
-  const int64_t base = (int64_t)rows * kv_heads * p.mtiles;
-  const int64_t tiles = ((int64_t)max_pages + 1) / 2;
-  const int64_t want = (3 * (int64_t)compute_units() + base - 1) / base;
-  const int64_t most = (tiles + kWavesPerBlock - 1) / kWavesPerBlock;
-  p.splits = (int)(want < most ? want : most);
-  if (p.splits > 64) p.splits = 64;
-  if (p.splits < 1) p.splits = 1;
+  const int64_t tiles = ((int64_t)max_pages + 1) / 2, units = (int64_t)rows * kv_heads;
+  const int64_t cus = compute_units();
+  int64_t per_cu, most;                      // blocks of a compute unit, splits that have work
+  if (cols <= 16 || (cols <= 32 && head_dim <= 128)) {
+    p.nq = cols <= 16 ? 1 : 2;
+    p.waves = 4;
+    p.mtiles = 1;
+    p.cols = 16 * p.nq;
+    per_cu = head_dim * p.nq <= 64 ? 4 : head_dim * p.nq <= 128 ? 3 : 2;
+    most = (tiles + p.waves - 1) / p.waves;
+    if (tiles <= 8 * 8) {
+      p.waves = 8;
+      most = 1;
+    }
+  } else {
+    const int wave_cols = head_dim <= 128 ? 32 : 16;
+    p.nq = 0;
+    p.waves = cols <= 4 * wave_cols ? 4 : 8;
+    p.cols = p.waves * wave_cols;
+    p.mtiles = (cols + p.cols - 1) / p.cols;
+    per_cu = 8 / p.waves;
+    most = (tiles + 7) / 8;
+  }
+  const int64_t want = per_cu * cus / (units * p.mtiles > 0 ? units * p.mtiles : 1);
+  int64_t splits = want < most ? want : most;
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  p.splits = splits < 1 ? 1 : (int)splits;
   return p;
 }
 
@@ -553,7 +815,7 @@ int64_t tfd_tree_attn_work_bytes(int rows, int nodes, int heads, int kv_heads, i
   if (!tree_shape(rows, nodes, heads, kv_heads, head_dim, max_pages) || rows == 0) return 0;
   const TreePlan p = tree_plan(rows, nodes, heads, kv_heads, head_dim, max_pages);
   if (p.splits == 1) return 0;
-  return (int64_t)rows * kv_heads * p.splits * p.mtiles * 16 * p.nq * (head_dim + 2) * 4;
+  return (int64_t)rows * kv_heads * p.splits * p.mtiles * p.cols * (head_dim + 2) * 4;
 }
 
 int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
@@ -574,7 +836,7 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
       (uintptr_t)a.k_pool % 16 || (uintptr_t)a.v_pool % 16)
     return fail(kBadArg, "tree_attn: q and the pools must be 16-byte aligned");
   const TreePlan p = tree_plan(a.rows, a.nodes, a.heads, a.kv_heads, a.head_dim, a.max_pages);
-  const int64_t cols = (int64_t)a.rows * a.kv_heads * p.splits * p.mtiles * 16 * p.nq;
+  const int64_t cols = (int64_t)a.rows * a.kv_heads * p.splits * p.mtiles * p.cols;
   if (p.splits > 1 && (!a.work || (uintptr_t)a.work % 16 ||
                        a.work_bytes < cols * (a.head_dim + 2) * 4))
     return fail(kBadArg, "tree_attn: work of %lld bytes", (long long)a.work_bytes);
@@ -583,33 +845,47 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
     return fail(kUnsupported, "tree_attn: more than one launch holds");
   float* const po = (float*)a.work;
   float* const pml = po + cols * a.head_dim;
-  const dim3 grid((unsigned)(units * p.mtiles));
+  const unsigned few = (unsigned)((int64_t)a.rows * a.kv_heads * p.splits);
+  const unsigned many = (unsigned)(units * p.mtiles);
+  const int pad = p.mtiles * p.cols;
+  const unsigned joins =
+      (unsigned)(((int64_t)a.rows * a.nodes * a.heads + kWavesPerBlock - 1) / kWavesPerBlock);
   auto s = (hipStream_t)stream;
-#define TFD_TREE(D, NQ)                                                                       \
+  // (past 64 KiB of LDS a kernel has to be allowed)
+#define TFD_TREE_RUN(KERNEL, LDS, GRID, THREADS, ...)                                         \
   {                                                                                           \
-    constexpr int lds = tree_lds<D, NQ>();                                                    \
-    if (lds > 65536) {                                                                        \
-      const hipError_t e = hipFuncSetAttribute((const void*)k_tree_attn<D, NQ>,               \
+    constexpr int lds = LDS;                                                                  \
+    if (lds > 60000) {                                                                        \
+      const hipError_t e = hipFuncSetAttribute((const void*)KERNEL,                           \
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds); \
       if (e != hipSuccess) return fail((int)e, "tree_attn: %s", hipGetErrorString(e));        \
     }                                                                                         \
-    k_tree_attn<D, NQ><<<grid, kBlock, lds, s>>>(a, p.splits, p.mtiles, po, pml);             \
+    KERNEL<<<GRID, THREADS, lds, s>>>(__VA_ARGS__);                                           \
   }
+#define TFD_TREE_FEW(D, NQ, W) \
+  TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), few, W * kWave, a, p.splits, po, pml)
+#define TFD_TREE_MANY(D, W) \
+  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D>()), many, W * kWave, a, p.splits, p.mtiles, po, pml)
 #define TFD_TREE_DIM(D)                                                                       \
   {                                                                                           \
-    if (p.nq == 1) TFD_TREE(D, 1)                                                             \
-    else if (p.nq == 2) TFD_TREE(D, 2)                                                        \
-    else if constexpr (D <= 128) TFD_TREE(D, 4)                                               \
-    if (p.splits > 1)                                                                         \
-      k_tree_join<D><<<(unsigned)(((int64_t)a.rows * a.nodes * a.heads + kWavesPerBlock - 1) / \
-                                  kWavesPerBlock),                                            \
-                       kBlock, 0, s>>>(a, p.splits, p.mtiles * 16 * p.nq, po, pml);           \
+    if (p.nq == 1 && p.waves == 4) TFD_TREE_FEW(D, 1, 4)                                      \
+    else if (p.nq == 1) TFD_TREE_FEW(D, 1, 8)                                                 \
+    else if (p.nq == 2) {                                                                     \
+      if constexpr (D <= 128) {                                                               \
+        if (p.waves == 4) TFD_TREE_FEW(D, 2, 4)                                               \
+        else TFD_TREE_FEW(D, 2, 8)                                                            \
+      }                                                                                       \
+    } else if (p.waves == 4) TFD_TREE_MANY(D, 4)                                              \
+    else TFD_TREE_MANY(D, 8)                                                                  \
+    if (p.splits > 1) k_tree_join<D><<<joins, kBlock, 0, s>>>(a, p.splits, pad, po, pml);     \
   }
   if (a.head_dim == 64) TFD_TREE_DIM(64)
   else if (a.head_dim == 128) TFD_TREE_DIM(128)
   else TFD_TREE_DIM(256)
 #undef TFD_TREE_DIM
-#undef TFD_TREE
+#undef TFD_TREE_MANY
+#undef TFD_TREE_FEW
+#undef TFD_TREE_RUN
   return launched("tree_attn");
 }
 
