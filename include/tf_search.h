@@ -67,6 +67,11 @@ typedef struct {
 } TfdTreeAttnArgs;
 int64_t tfd_tree_attn_work_bytes(int rows, int nodes, int heads, int kv_heads, int head_dim,
                                  int max_pages);
+/* How a call of these sizes runs on the current device, for tests and measurements: form = 16s of
+ * columns that a wave with its own positions takes (0: waves share positions and each takes
+ * other columns), waves of a block, blocks for a row's columns, splits of its positions. */
+int tfd_tree_attn_form(int rows, int nodes, int heads, int kv_heads, int head_dim, int max_pages,
+                       int32_t form[4]);
 int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream);
 
 /* ---- beams -------------------------------------------------------------------------- */

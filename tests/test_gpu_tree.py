@@ -3,6 +3,7 @@ within one bf16 rounding of the output (2^-8 of its value, half a step of eight 
 error of its operands: a probability is a sum of two bf16 (2^-16 of it), scores are f32 sums of
 exact products (2^-24 of the sum of their sizes for each of dim additions, at most dim 2^-24
 times |q| |k| here), sums over n positions n 2^-24 of the sum of |p v|."""
+import ctypes
 import math
 
 import pytest
@@ -10,6 +11,7 @@ import torch
 
 from tests import _search_ref as R
 from tilefoundry_amd import _lib, tree
+from tilefoundry_amd._lib import lib
 
 pytestmark = pytest.mark.gpu
 
@@ -26,15 +28,18 @@ def _parents(g, rows, nodes):
     return p.to(I32)
 
 
-def _case(seed, rows, nodes, heads, kv_heads, dim, lengths, spare=3):
+def _case(seed, rows, nodes, heads, kv_heads, dim, lengths, spare=3, room=0):
+    """*room*: pages more that a row's table has place for (-1: none there)."""
     g = _gen(seed)
     width = max(-(-(n + nodes) // 16) for n in lengths) + 1
     pages = rows * width + spare
     perm = torch.randperm(pages, generator=g)[:rows * width]
+    table = torch.full((rows, width + room), -1, dtype=I32)
+    table[:, :width] = perm.view(rows, width)
     return {"q": torch.randn(rows, nodes, heads, dim, generator=g).to(BF),
             "k_pool": torch.randn(pages, kv_heads, 16, dim, generator=g).to(BF),
             "v_pool": torch.randn(pages, kv_heads, 16, dim, generator=g).to(BF),
-            "table": perm.view(rows, width).to(I32),
+            "table": table,
             "lengths": torch.tensor(lengths, dtype=I32),
             "masks": R.words(R.ancestors(_parents(g, rows, nodes))[0], nodes)}
 
@@ -111,6 +116,48 @@ def test_accept(gpu_device, rows, nodes):
 def test_attention(gpu_device, rows, nodes, heads, kv_heads, dim, lengths):
     c = _case(rows * 100 + nodes, rows, nodes, heads, kv_heads, dim, lengths)
     _check(c, gpu_device)
+
+
+FORMS = [  # (rows, nodes, heads, kv heads, dim, room), form: how such calls run
+    ((1, 7, 4, 2, 64, 9), (1, 16, 1, 1)), ((2, 20, 4, 2, 128, 9), (1, 12, 3, 1)),
+    ((1, 13, 8, 2, 256, 9), (1, 8, 4, 1)),
+    ((3, 7, 4, 2, 64, 400), (1, 4, 1, 51)), ((3, 7, 4, 2, 128, 400), (1, 4, 1, 51)),
+    ((3, 4, 8, 2, 256, 400), (1, 4, 1, 51)), ((64, 2, 16, 8, 64, 400), (1, 4, 1, 2)),
+    ((2, 16, 4, 2, 64, 400), (2, 4, 1, 51)), ((2, 11, 4, 2, 128, 400), (2, 4, 1, 51)),
+    ((36, 11, 16, 8, 128, 400), (2, 4, 1, 1)),
+    ((2, 21, 8, 2, 64, 400), (0, 4, 1, 26)), ((2, 21, 8, 2, 128, 400), (0, 4, 1, 26)),
+    ((2, 13, 8, 2, 256, 400), (0, 4, 1, 26)), ((1, 61, 8, 2, 128, 400), (0, 8, 1, 26)),
+    ((1, 61, 16, 2, 64, 400), (0, 8, 2, 26)), ((1, 23, 16, 2, 256, 400), (0, 8, 2, 26)),
+    ((33, 33, 16, 8, 128, 400), (0, 4, 1, 1)), ((33, 66, 16, 8, 64, 9), (0, 8, 1, 1)),
+    ((33, 10, 16, 8, 256, 100), (0, 4, 1, 1))]
+
+
+@pytest.mark.parametrize("shape,form", FORMS)
+def test_attention_forms(gpu_device, shape, form):
+    """Every way a call may run: with its rows' tables far longer than the rows; drafted values
+    that are not finite, absent nodes."""
+    rows, nodes, heads, kv_heads, dim, room = shape
+    lengths = [(71 * b + 13) % 210 if rows > 8 or b else 333 for b in range(rows)]
+    c = _case(sum(shape), rows, nodes, heads, kv_heads, dim, lengths, room=room)
+    got = (ctypes.c_int32 * 4)()
+    lib().tfd_tree_attn_form(rows, nodes, heads, kv_heads, dim, c["table"].shape[1], got)
+    base = (tuple(got)[:3], form[:3])
+    assert base[0] == base[1] and (got[3] > 1) == (form[3] > 1), tuple(got)
+    if rows > 8:                                     # the reference takes its time
+        few = torch.tensor([0, 7, rows - 1])
+        d = {k: v.to(gpu_device) for k, v in c.items()}
+        out = tree.attention(**d).cpu()[few]
+        part = {**c, **{k: c[k][few] for k in ("q", "table", "lengths", "masks")}}
+        want, size = R.attention(**part)
+        assert ((out.double() - want).abs() <= _bound(c, want, size, dim ** -0.5)).all()
+        return
+    _check(c, gpu_device)
+    counts = torch.tensor([nodes - 1, 0, nodes][:rows], dtype=I32)
+    c["masks"][0, nodes // 2:] &= ~2
+    at = 333 + 1                                     # node 1's value
+    c["v_pool"][c["table"][0, at // 16].long(), 0, at % 16, 5] = math.inf
+    c["v_pool"][c["table"][0, at // 16].long(), 0, at % 16, dim - 1] = math.nan
+    _check(c, gpu_device, counts=counts)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])

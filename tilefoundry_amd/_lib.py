@@ -170,6 +170,7 @@ SIGNATURES: dict[str, list] = {
     "tfd_tree_masks": [P, P, I, I, P, P, P, P],
     "tfd_tree_accept": [P, P, P, P, I, I, P, P, P, P],
     "tfd_tree_attn_work_bytes": [I, I, I, I, I, I],
+    "tfd_tree_attn_form": [I, I, I, I, I, I, P],
     "tfd_tree_attn": [P, P],
     "tfd_beam_work_bytes": [I, I, I],
     "tfd_beam_select": [P, P],

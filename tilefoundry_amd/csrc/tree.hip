@@ -184,29 +184,35 @@ struct TreeRow {
   const bf16 *k, *v;                         // of the kv head, page 0
   const uint64_t* masks;
   int64_t page_size;
-  int row, h, G, L, n, cols, first, words, last_page, num_pages;
+  int row, h, G, L, n, cols, first, words, last_page, num_pages, max_pages;
   bool bad_page;
 
+  // Entries past the last position's page need not be set: page 0 in their place (and they
+  // are read before that page is known: no load waits for the row's length).
   __device__ __forceinline__ int page_at(int i) {
-    const int p = table[min(i, last_page)];
+    const int p = table[min(i, max_pages - 1)];
     const bool ok = p >= 0 && p < num_pages;
-    bad_page |= !ok;
+    bad_page |= !ok && i <= last_page;
     return ok ? p : 0;
   }
   __device__ __forceinline__ int node_of(int c) const { return (first + min(c, cols - 1)) / G; }
-  // bit i: column c sees position j0 + i, i < 32 (the context: every one)
-  __device__ __forceinline__ uint32_t seen(int c, int j0) const {
-    const uint64_t* const m = masks + (int64_t)node_of(c) * words;
-    const int from = j0 - L, w = max(from, 0) >> 6, sh = max(from, 0) & 63;
-    uint64_t bits = m[min(w, words - 1)] >> sh;
-    if (w >= words) bits = 0;
-    const uint64_t next = m[min(w + 1, words - 1)];
-    if (sh && w + 1 < words) bits |= next << (64 - sh);
+  // bit i: a column that sees the nodes of m0 (and m1, the next word) from node `from` = j0 - L
+  // on, or from 0, sees position j0 + i, i < 32 (the context: every one)
+  __device__ __forceinline__ uint32_t seen(uint64_t m0, uint64_t m1, int j0) const {
+    const int from = j0 - L, sh = max(from, 0) & 63;
+    uint64_t bits = m0 >> sh;
+    if (sh) bits |= m1 << (64 - sh);
     if (from <= -kTile) bits = 0xffffffffu;
     else if (from < 0) bits = (bits << -from) | ((1ull << -from) - 1);
     const int left = n - j0;
     if (left < kTile) bits = left > 0 ? bits & ((1ull << left) - 1) : 0;
     return (uint32_t)bits;
+  }
+  __device__ __forceinline__ uint32_t seen_by(int c, int j0) const {
+    const uint64_t* const m = masks + (int64_t)node_of(c) * words;
+    const int w = max(j0 - L, 0) >> 6;
+    const uint64_t m0 = m[min(w, words - 1)], m1 = m[min(w + 1, words - 1)];
+    return seen(w < words ? m0 : 0, w + 1 < words ? m1 : 0, j0);
   }
 };
 
@@ -233,19 +239,21 @@ __device__ __forceinline__ bool tree_row(const TfdTreeAttnArgs& a, int unit, int
   t.page_size = a.kv_heads * head_size;
   t.k = (const bf16*)a.k_pool + t.h * head_size;
   t.v = (const bf16*)a.v_pool + t.h * head_size;
-  t.last_page = max(0, (t.n - 1) / kPage);
+  t.last_page = t.n > 0 ? (t.n - 1) / kPage : -1;
   t.num_pages = a.num_pages;
+  t.max_pages = a.max_pages;
   t.bad_page = false;
   return true;
 }
 
-// Eight probabilities' place in a column's softmax: the scores of 32 positions (this lane's
-// eight) become operands, maximum, sum and outputs follow.
-template <int DT, int NQ>
-__device__ __forceinline__ void tree_softmax(const f32x4 (&st)[2], float c2, float& mx, float& sum,
-                                             f32x4 (&o)[DT][NQ], int qt, u32x4& hi4, u32x4& lo4) {
-  float tm = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
-                   fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
+// A column's softmax goes on with the scores of kN x 16 positions (this lane's 4 kN): the
+// running maximum, and with it what was summed so far, ...
+template <int kN, int DT, int NQ>
+__device__ __forceinline__ float tree_maximum(const f32x4 (&st)[kN], float c2, float& mx, float& sum,
+                                              f32x4 (&o)[DT][NQ], int qt) {
+  float tm = st[0][0];
+#pragma unroll
+  for (int i = 1; i < 4 * kN; ++i) tm = fmaxf(tm, st[i / 4][i % 4]);
   float lo, hi;
   pair16(tm, lo, hi);
   tm = fmaxf(lo, hi);
@@ -261,10 +269,15 @@ __device__ __forceinline__ void tree_softmax(const f32x4 (&st)[2], float c2, flo
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[dt][qt][e] *= alpha;
   }
+  return ref;
+}
+// ... and the probabilities of 32 of them as operands.
+__device__ __forceinline__ void tree_weights(const f32x4& s0, const f32x4& s1, float c2, float ref,
+                                             float& sum, u32x4& hi4, u32x4& lo4) {
   float p[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    p[i] = __builtin_amdgcn_exp2f(fmaf(st[i / 4][i % 4], c2, -ref));
+    p[i] = __builtin_amdgcn_exp2f(fmaf(i < 4 ? s0[i % 4] : s1[i % 4], c2, -ref));
     sum += p[i];
   }
   hi4 = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
@@ -320,21 +333,25 @@ constexpr int few_lds() {
 
 template <int D, int NQ, int W>
 __global__ __launch_bounds__(W * kWave, D * NQ <= 64 ? 4 : D * NQ <= 128 ? 3 : 2)
-void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
+void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ part_o,
                 float* __restrict__ part_ml) {
   constexpr int DS = D / 32, DT = D / 16, kCols = 16 * NQ;
   constexpr int kV = D / 16;                 // V loads of a tile: 1 KiB each
   constexpr int kRowsPerLoad = 512 / D;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float m_s[W][kCols], l_s[W][kCols], inv_s[kCols];
+  __shared__ int odd_s;
   uint8_t* const q_s = smem;                 // operand order: 1 KiB per (16 columns, 32 dims)
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 15, kq = lane >> 4;
   uint8_t* const v_s = smem + kCols * D * 2 + wave * kTile * D * 2;
-  const int unit = blockIdx.x, split = unit % splits;
+  int unit, mt;
+  tree_block(mtiles, unit, mt);
+  if (unit >= a.rows * a.kv_heads * splits) return;
+  const int split = unit % splits;
   TreeRow t;
-  if (!tree_row(a, unit, splits, 0, t)) return;
+  if (!tree_row(a, unit, splits, mt * kCols, t)) return;
   const int tiles = (t.n + kTile - 1) / kTile;
 
   u32x4 kr[2][DS], vr[kV];
@@ -369,21 +386,25 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
   }
 
   const int slots = splits * W, tile0 = split * W + wave;
-  int tile = tile0, p0 = 0, p1 = 0;
+  int tile = tile0;
   bool odd = false;                          // a drafted value is not finite
+  int p0 = t.page_at(2 * tile), p1 = t.page_at(2 * tile + 1);
   if (tile < tiles) {
-    p0 = t.page_at(2 * tile), p1 = t.page_at(2 * tile + 1);
     load_v(p0, p1);
     load_k(p0, p1);
     p0 = t.page_at(2 * (tile + slots)), p1 = t.page_at(2 * (tile + slots) + 1);
   }
+  uint64_t see[NQ];                          // (up to 64 nodes)
+#pragma unroll
+  for (int qt = 0; qt < NQ; ++qt) see[qt] = t.masks[t.node_of(16 * qt + r)];
   for (int i = tid; i < kCols * D / 8; i += W * kWave) {
     const int b = i / 64, l = i % 64;        // block b: columns 16 (b / DS), dims 32 (b % DS)
-    const int c = min(16 * (b / DS) + (l & 15), t.cols - 1), d = 32 * (b % DS) + 8 * (l >> 4);
+    const int c = t.first + min(16 * (b / DS) + (l & 15), t.cols - 1), d = 32 * (b % DS) + 8 * (l >> 4);
     *reinterpret_cast<u32x4*>(q_s + i * 16) =
         load16((const bf16*)a.q + t.row * a.q_row + c / t.G * a.q_node +
                (t.h * t.G + c % t.G) * a.q_head + d);
   }
+  if (tid == 0) odd_s = 0;
   __syncthreads();                           // the queries are in place
 
   for (; tile < tiles; tile += slots) {
@@ -409,12 +430,13 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
         st[1] = mfma(kr[1][s], qf, st[1]);
       }
       if (edge) {
-        const uint32_t see = t.seen(16 * qt + r, j0) >> (4 * kq);
+        const uint32_t bits = t.seen(j0 - t.L < 64 ? see[qt] : 0, 0, j0) >> (4 * kq);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          st[i / 4][i % 4] = (see >> (16 * (i / 4) + i % 4)) & 1 ? st[i / 4][i % 4] : kPanelNegInf;
+          st[i / 4][i % 4] = (bits >> (16 * (i / 4) + i % 4)) & 1 ? st[i / 4][i % 4] : kPanelNegInf;
       }
-      tree_softmax<DT, NQ>(st, c2, mx[qt], sum[qt], o, qt, ph[qt], pl[qt]);
+      const float ref = tree_maximum<2, DT, NQ>(st, c2, mx[qt], sum[qt], o, qt);
+      tree_weights(st[0], st[1], c2, ref, sum[qt], ph[qt], pl[qt]);
     }
     if (more) {
       load_k(p0, p1);
@@ -429,9 +451,9 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
       for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
     }
   }
-  odd = __any(odd);
 
   // join the waves: maxima and sums, then DT / NQ times 16 dims of all columns at a time
+  if (odd) odd_s = 1;
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
     sum[qt] = quad_sum(sum[qt]);
@@ -441,32 +463,37 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
     }
   }
   __syncthreads();                           // (V's pieces are free from here on)
+  const int64_t pcol = ((int64_t)unit * mtiles + mt) * kCols;
   float scale[NQ];
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
     const int c = 16 * qt + r;
-    float m = m_s[0][c], l = 0.f;
+    float m = m_s[0][c];
 #pragma unroll
     for (int w = 1; w < W; ++w) m = fmaxf(m, m_s[w][c]);
     // (a wave that saw nothing: a sum of zero; a sum of NaN is one whatever its maximum)
     scale[qt] = sum[qt] != sum[qt] ? sum[qt]
                 : mx[qt] == kPanelNegInf ? 0.f
                                          : __builtin_amdgcn_exp2f((mx[qt] - m) * c2);
-    if (wave == 0 && kq == 0) {
+  }
+  if (tid < kCols) {
+    float m = m_s[0][tid], l = 0.f;
 #pragma unroll
-      for (int w = 0; w < W; ++w)
-        l += l_s[w][c] * (m_s[w][c] == kPanelNegInf
+    for (int w = 1; w < W; ++w) m = fmaxf(m, m_s[w][tid]);
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+      l += l_s[w][tid] * (m_s[w][tid] == kPanelNegInf
                               ? 1.f
-                              : __builtin_amdgcn_exp2f((m_s[w][c] - m) * c2));
-      inv_s[c] = l == 0.f ? 0.f : 1.f / l;
-      if (splits > 1 && c < t.cols) {
-        part_ml[((int64_t)unit * kCols + c) * 2] = m;
-        part_ml[((int64_t)unit * kCols + c) * 2 + 1] = l;
-      }
+                              : __builtin_amdgcn_exp2f((m_s[w][tid] - m) * c2));
+    inv_s[tid] = l == 0.f ? 0.f : 1.f / l;
+    if (splits > 1 && tid < t.cols) {
+      part_ml[(pcol + tid) * 2] = m;
+      part_ml[(pcol + tid) * 2 + 1] = l;
     }
   }
   float* const join = reinterpret_cast<float*>(smem + kCols * D * 2);
   constexpr int kDims = DT / NQ;             // 16 dims each, of a pass
+  constexpr int kAll = NQ * kDims * 64;      // values of a pass, in fours
 #pragma unroll
   for (int pass = 0; pass < NQ; ++pass) {
     if (pass) __syncthreads();
@@ -474,17 +501,13 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
     for (int i = 0; i < kDims; ++i)
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt) {
-        const int dt = pass * kDims + i;
-        f32x4 y = o[dt][qt] * scale[qt];
+        f32x4 y = o[pass * kDims + i][qt] * scale[qt];
         if (scale[qt] == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (odd)
-          for (int k = tile0; k < tiles; k += slots)
-            add_odd(t, y, 16 * qt + r, 16 * dt + 4 * kq, k * kTile, k * kTile + kTile, D);
         *reinterpret_cast<f32x4*>(join + ((wave * NQ + qt) * kDims + i) * 256 + r * 16 + kq * 4) =
             y;
       }
     __syncthreads();
-    constexpr int kAll = NQ * kDims * 64;    // four values each
+#pragma unroll 1
     for (int i = tid; i < kAll; i += W * kWave) {
       f32x4 y = *reinterpret_cast<const f32x4*>(join + i * 4);
 #pragma unroll
@@ -493,14 +516,18 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, float* __restrict__ part_o,
       const int c = 16 * (i / 64 / kDims) + i % 64 / 4;
       const int d = 16 * (pass * kDims + i / 64 % kDims) + i % 4 * 4;
       if (c >= t.cols) continue;
+      if (odd_s)
+        for (int k = t.L / kTile; k < tiles; ++k)
+          if (k / W % splits == split) add_odd(t, y, c, d, k * kTile, k * kTile + kTile, D);
       if (splits == 1) {
         const float f = inv_s[c];
         if (f == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
-        *reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, (int64_t)t.row * a.nodes + c / t.G,
-                                                        t.h * t.G + c % t.G, d)) =
+        const int cc = t.first + c, node = cc / t.G;
+        *reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, (int64_t)t.row * a.nodes + node,
+                                                        t.h * t.G + cc - node * t.G, d)) =
             u32x2{pack2(y[0] * f, y[1] * f), pack2(y[2] * f, y[3] * f)};
       } else {
-        *reinterpret_cast<f32x4*>(part_o + ((int64_t)unit * kCols + c) * D + d) = y;
+        *reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d) = y;
       }
     }
   }
@@ -618,34 +645,43 @@ __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, i
     }
     const bool edge = (tile + 1) * kPos > t.L;
     if (c0 < t.cols) {
+      f32x4 st[NQ][kPos / 16];
+#pragma unroll
+      for (int qt = 0; qt < NQ; ++qt)
+#pragma unroll
+        for (int p = 0; p < kPos / 16; ++p) st[qt][p] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DS; ++s)
+#pragma unroll
+        for (int p = 0; p < kPos / 16; ++p) {
+          const u32x4 kf =
+              *reinterpret_cast<const u32x4*>(buf + k_at<D>(16 * p + r, 4 * s + kq));
+#pragma unroll
+          for (int qt = 0; qt < NQ; ++qt) st[qt][p] = mfma(kf, qf[qt][s], st[qt][p]);
+        }
+      float ref[NQ];
+#pragma unroll
+      for (int qt = 0; qt < NQ; ++qt) {
+        if (edge) {
+#pragma unroll
+          for (int kk = 0; kk < kPos / kTile; ++kk) {
+            const uint32_t bits =
+                t.seen_by(c0 + 16 * qt + r, tile * kPos + kk * kTile) >> (4 * kq);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              f32x4& x = st[qt][2 * kk + i / 4];
+              x[i % 4] = (bits >> (16 * (i / 4) + i % 4)) & 1 ? x[i % 4] : kPanelNegInf;
+            }
+          }
+        }
+        ref[qt] = tree_maximum<kPos / 16, DT, NQ>(st[qt], c2, mx[qt], sum[qt], o, qt);
+      }
 #pragma unroll
       for (int kk = 0; kk < kPos / kTile; ++kk) {
-        f32x4 st[NQ][2];
-#pragma unroll
-        for (int qt = 0; qt < NQ; ++qt)
-          st[qt][0] = st[qt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < DS; ++s)
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const u32x4 kf = *reinterpret_cast<const u32x4*>(
-                buf + k_at<D>(kk * kTile + 16 * p + r, 4 * s + kq));
-#pragma unroll
-            for (int qt = 0; qt < NQ; ++qt) st[qt][p] = mfma(kf, qf[qt][s], st[qt][p]);
-          }
         u32x4 ph[NQ], pl[NQ];
 #pragma unroll
-        for (int qt = 0; qt < NQ; ++qt) {
-          if (edge) {
-            const uint32_t see =
-                t.seen(c0 + 16 * qt + r, tile * kPos + kk * kTile) >> (4 * kq);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              st[qt][i / 4][i % 4] =
-                  (see >> (16 * (i / 4) + i % 4)) & 1 ? st[qt][i / 4][i % 4] : kPanelNegInf;
-          }
-          tree_softmax<DT, NQ>(st[qt], c2, mx[qt], sum[qt], o, qt, ph[qt], pl[qt]);
-        }
+        for (int qt = 0; qt < NQ; ++qt)
+          tree_weights(st[qt][2 * kk], st[qt][2 * kk + 1], c2, ref[qt], sum[qt], ph[qt], pl[qt]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, lane);
@@ -672,19 +708,37 @@ __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, i
       part_ml[(pcol + c) * 2] = mx[qt];
       part_ml[(pcol + c) * 2 + 1] = l;
     }
-    const int cc = t.first + c;
+    const int cc = t.first + c, node = cc / t.G, head = t.h * t.G + cc - node * t.G;
+    const int64_t rr = (int64_t)t.row * a.nodes + node;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const int d = 16 * dt + 4 * kq;
       f32x4 y = o[dt][qt];
-      if (odd) add_odd(t, y, c, d, begin * kPos, end * kPos, D);
       if (splits == 1) {
         if (inv == 0.f) y = f32x4{0.f, 0.f, 0.f, 0.f};
-        *reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, (int64_t)t.row * a.nodes + cc / t.G,
-                                                        t.h * t.G + cc % t.G, d)) =
+        *reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, rr, head, d)) =
             u32x2{pack2(y[0] * inv, y[1] * inv), pack2(y[2] * inv, y[3] * inv)};
       } else {
         *reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d) = y;
+      }
+    }
+    // (what a lane has written it reads again)
+    if (odd) {
+#pragma unroll 1
+      for (int d = 4 * kq; d < D; d += 16) {
+        f32x4 y;
+        if (splits == 1) {
+          u32x2* const to = reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, rr, head, d));
+          const u32x2 w = *to;
+          y = f32x4{bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y)};
+          add_odd(t, y, c, d, begin * kPos, end * kPos, D);
+          *to = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+        } else {
+          f32x4* const to = reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d);
+          y = *to;
+          add_odd(t, y, c, d, begin * kPos, end * kPos, D);
+          *to = y;
+        }
       }
     }
   }
@@ -736,12 +790,17 @@ __global__ __launch_bounds__(kBlock) void k_tree_join(TfdTreeAttnArgs a, int spl
     ((bf16*)a.out)[out_at(a, rr, head, lane * kPer + e)] = f2bf(l == 0.f ? 0.f : y[e] / l);
 }
 
-// How a call runs.  Few columns (up to 32, 16 of 256 dims): blocks of four waves, or where a row's tiles are few
-// enough for one block of eight, that alone (no second launch).  Many: four or eight waves of
-// 32 columns (16 of 256 dims).  Splits: as many as fill the compute units' blocks once.
+// How a call runs.  A row's tiles that one block's waves can take in a few turns, and no more
+// blocks than compute units: that block alone, 16 columns a block, without a second launch.
+// Else few columns (up to 32, 16 of 256 dims): blocks of four waves; many: four or eight
+// waves of 32 columns (16 of 256 dims).  Splits: as many as fill the compute units' blocks once.
 struct TreePlan {
   int nq, waves, mtiles, cols, splits;       // nq 0: many columns; cols: of a block
 };
+
+// waves of a block that runs alone: what 16 columns' registers leave room for
+constexpr int alone_waves(int head_dim) { return head_dim == 64 ? 16 : head_dim == 128 ? 12 : 8; }
+constexpr int kAloneTurns = 5, kAloneCols = 64;
 
 TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, int max_pages) {
   TreePlan p;
@@ -749,26 +808,27 @@ TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, i
   const int64_t tiles = ((int64_t)max_pages + 1) / 2, units = (int64_t)rows * kv_heads;
   const int64_t cus = compute_units();
   int64_t per_cu, most;                      // blocks of a compute unit, splits that have work
-  if (cols <= 16 || (cols <= 32 && head_dim <= 128)) {
+  if (cols <= kAloneCols && nodes <= 64 && tiles <= kAloneTurns * alone_waves(head_dim) &&
+      units * ((cols + 15) / 16) <= cus) {
+    p.nq = 1;
+    p.waves = alone_waves(head_dim);
+    p.cols = 16;
+    per_cu = most = 1;
+  } else if (cols <= 16 || (cols <= 32 && head_dim <= 128)) {
     p.nq = cols <= 16 ? 1 : 2;
     p.waves = 4;
-    p.mtiles = 1;
     p.cols = 16 * p.nq;
     per_cu = head_dim * p.nq <= 64 ? 4 : head_dim * p.nq <= 128 ? 3 : 2;
     most = (tiles + p.waves - 1) / p.waves;
-    if (tiles <= 8 * 8) {
-      p.waves = 8;
-      most = 1;
-    }
   } else {
     const int wave_cols = head_dim <= 128 ? 32 : 16;
     p.nq = 0;
     p.waves = cols <= 4 * wave_cols ? 4 : 8;
     p.cols = p.waves * wave_cols;
-    p.mtiles = (cols + p.cols - 1) / p.cols;
     per_cu = 8 / p.waves;
     most = (tiles + 7) / 8;
   }
+  p.mtiles = (cols + p.cols - 1) / p.cols;
   const int64_t want = per_cu * cus / (units * p.mtiles > 0 ? units * p.mtiles : 1);
   int64_t splits = want < most ? want : most;
   if (splits > kMaxSplits) splits = kMaxSplits;
@@ -818,6 +878,20 @@ int64_t tfd_tree_attn_work_bytes(int rows, int nodes, int heads, int kv_heads, i
   return (int64_t)rows * kv_heads * p.splits * p.mtiles * p.cols * (head_dim + 2) * 4;
 }
 
+int tfd_tree_attn_form(int rows, int nodes, int heads, int kv_heads, int head_dim, int max_pages,
+                       int32_t form[4]) {
+  if (!form) return fail(kBadArg, "tree_attn_form: null pointer");
+  if (!tree_shape(rows, nodes, heads, kv_heads, head_dim, max_pages) || rows == 0)
+    return fail(kBadShape, "tree_attn_form: rows=%d nodes=%d heads=%d kv_heads=%d", rows, nodes,
+                heads, kv_heads);
+  const TreePlan p = tree_plan(rows, nodes, heads, kv_heads, head_dim, max_pages);
+  form[0] = p.nq;
+  form[1] = p.waves;
+  form[2] = p.mtiles;
+  form[3] = p.splits;
+  return 0;
+}
+
 int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
   if (!args) return fail(kBadArg, "tree_attn: null args");
   const TfdTreeAttnArgs& a = *args;
@@ -845,8 +919,7 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
     return fail(kUnsupported, "tree_attn: more than one launch holds");
   float* const po = (float*)a.work;
   float* const pml = po + cols * a.head_dim;
-  const unsigned few = (unsigned)((int64_t)a.rows * a.kv_heads * p.splits);
-  const unsigned many = (unsigned)(units * p.mtiles);
+  const unsigned blocks = (unsigned)(units * p.mtiles);
   const int pad = p.mtiles * p.cols;
   const unsigned joins =
       (unsigned)(((int64_t)a.rows * a.nodes * a.heads + kWavesPerBlock - 1) / kWavesPerBlock);
@@ -863,18 +936,16 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
     KERNEL<<<GRID, THREADS, lds, s>>>(__VA_ARGS__);                                           \
   }
 #define TFD_TREE_FEW(D, NQ, W) \
-  TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), few, W * kWave, a, p.splits, po, pml)
+  TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), blocks, W * kWave, a, p.splits, p.mtiles, po, \
+               pml)
 #define TFD_TREE_MANY(D, W) \
-  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D>()), many, W * kWave, a, p.splits, p.mtiles, po, pml)
+  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D>()), blocks, W * kWave, a, p.splits, p.mtiles, po, pml)
 #define TFD_TREE_DIM(D)                                                                       \
   {                                                                                           \
     if (p.nq == 1 && p.waves == 4) TFD_TREE_FEW(D, 1, 4)                                      \
-    else if (p.nq == 1) TFD_TREE_FEW(D, 1, 8)                                                 \
+    else if (p.nq == 1) TFD_TREE_FEW(D, 1, alone_waves(D))                                    \
     else if (p.nq == 2) {                                                                     \
-      if constexpr (D <= 128) {                                                               \
-        if (p.waves == 4) TFD_TREE_FEW(D, 2, 4)                                               \
-        else TFD_TREE_FEW(D, 2, 8)                                                            \
-      }                                                                                       \
+      if constexpr (D <= 128) TFD_TREE_FEW(D, 2, 4)                                           \
     } else if (p.waves == 4) TFD_TREE_MANY(D, 4)                                              \
     else TFD_TREE_MANY(D, 8)                                                                  \
     if (p.splits > 1) k_tree_join<D><<<joins, kBlock, 0, s>>>(a, p.splits, pad, po, pml);     \
