@@ -116,14 +116,15 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // transposing read gives V^T's operands; its 32-byte pieces are permuted by the row so that the
 // 16 rows of such a read take the fewest cycles.
 //
-// Softmax with a running maximum, in f32; a rescale only where a maximum moved.  A
+// Softmax against a running reference, in f32.  A
 // probability is the sum of two bf16, so that it is not the less exact operand.
 //
 // Two kernels.  Few columns (k_tree_few): the keys are what is waited for, so each wave
 // takes other tiles of 32 positions, its K straight into registers as operands and its V
 // through a private piece of LDS, and no barrier until the waves' sums are joined.  Many
-// columns (k_tree_many): the waves take 16 NQ columns each and share tiles in LDS, which come
-// in by way of registers a tile ahead, one barrier a tile.  Both may cut a row's positions into
+// columns (k_tree_many): the waves take 16 NQ columns each and share tiles in LDS, loaded
+// straight to it three tiles ahead (from pages anywhere a load takes some 3 us), one barrier a
+// tile.  Both may cut a row's positions into
 // splits, which k_tree_join adds.
 // ---------------------------------------------------------------------------
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -178,6 +179,10 @@ __device__ __forceinline__ u32x4 clean_v(u32x4 v, int j, int L, int n, bool& odd
   return v;
 }
 
+// What all lanes read alike and no kernel here writes, through the scalar cache.
+typedef const __attribute__((address_space(4))) int c_int;
+__device__ __forceinline__ c_int* uniform(const int* p) { return (c_int*)(uintptr_t)p; }
+
 // One row's part of a call, as a block sees it.
 struct TreeRow {
   const int* table;
@@ -223,10 +228,11 @@ __device__ __forceinline__ bool tree_row(const TfdTreeAttnArgs& a, int unit, int
   t.row = unit / splits / a.kv_heads;
   t.G = a.heads / a.kv_heads;
   t.first = first;
-  const int count = row_nodes(a.counts, t.row, a.nodes);
+  const int count =
+      a.counts ? max(0, min(uniform(a.counts)[t.row], a.nodes)) : a.nodes;
   t.cols = count * t.G - first;              // of this block on
   if (t.cols <= 0) return false;
-  t.L = a.lengths[t.row];
+  t.L = uniform(a.lengths)[t.row];
   t.n = t.L + count;
   if (t.L < 0 || (int64_t)t.L + count > (int64_t)a.max_pages * kPage) {
     if (threadIdx.x == 0) raise_error(a.err, kErrPosRange);
@@ -247,7 +253,11 @@ __device__ __forceinline__ bool tree_row(const TfdTreeAttnArgs& a, int unit, int
 }
 
 // A column's softmax goes on with the scores of kN x 16 positions (this lane's 4 kN): the
-// running maximum, and with it what was summed so far, ...
+// reference that exponents count from, and with it what was summed so far, ...  It follows the
+// maximum only when that has risen by 2^kMaxRise: probabilities up to 256 are as exact as up
+// to 1 (both operands have eight exponent bits), and a rescale of all outputs then is rare.
+constexpr float kMaxRise = 8.f;
+
 template <int kN, int DT, int NQ>
 __device__ __forceinline__ float tree_maximum(const f32x4 (&st)[kN], float c2, float& mx, float& sum,
                                               f32x4 (&o)[DT][NQ], int qt) {
@@ -259,8 +269,8 @@ __device__ __forceinline__ float tree_maximum(const f32x4 (&st)[kN], float c2, f
   tm = fmaxf(lo, hi);
   pair32(tm, lo, hi);
   const float m1 = fmaxf(mx, fmaxf(lo, hi));
-  const float ref = m1 == kPanelNegInf ? 0.f : m1 * c2;
-  if (__any(m1 != mx)) {
+  if (__any(m1 * c2 > mx * c2 + kMaxRise || (mx == kPanelNegInf && m1 > mx))) {
+    const float ref = m1 == kPanelNegInf ? 0.f : m1 * c2;
     const float alpha = __builtin_amdgcn_exp2f(mx * c2 - ref);
     mx = m1;
     sum *= alpha;
@@ -269,9 +279,10 @@ __device__ __forceinline__ float tree_maximum(const f32x4 (&st)[kN], float c2, f
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[dt][qt][e] *= alpha;
   }
-  return ref;
+  return mx == kPanelNegInf ? 0.f : mx * c2;
 }
-// ... and the probabilities of 32 of them as operands.
+// ... and the probabilities of 32 of them as operands: bf16, and with kTwo what that leaves out.
+template <bool kTwo>
 __device__ __forceinline__ void tree_weights(const f32x4& s0, const f32x4& s1, float c2, float ref,
                                              float& sum, u32x4& hi4, u32x4& lo4) {
   float p[8];
@@ -281,6 +292,7 @@ __device__ __forceinline__ void tree_weights(const f32x4& s0, const f32x4& s1, f
     sum += p[i];
   }
   hi4 = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
+  if constexpr (!kTwo) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) p[i] -= i % 2 ? bf_hi(hi4[i / 2]) : bf_lo(hi4[i / 2]);
   lo4 = u32x4{pack2(p[0], p[1]), pack2(p[2], p[3]), pack2(p[4], p[5]), pack2(p[6], p[7])};
@@ -388,11 +400,20 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
   const int slots = splits * W, tile0 = split * W + wave;
   int tile = tile0;
   bool odd = false;                          // a drafted value is not finite
-  int p0 = t.page_at(2 * tile), p1 = t.page_at(2 * tile + 1);
+  // lane l holds the page of half l % 2 of this wave's next l / 2-th tile: a scalar load of two
+  // would be waited for with the next LDS read
+  int ids = 0;
+  auto refill = [&](int from) {
+    ids = t.page_at(2 * (from + (lane >> 1) * slots) + (lane & 1));
+  };
+  auto page = [&](int turn, int half) {
+    return __builtin_amdgcn_readlane(ids, 2 * (turn % 32) + half);
+  };
+  refill(tile0);
+  int turn = 0, p0 = page(0, 0), p1 = page(0, 1);
   if (tile < tiles) {
     load_v(p0, p1);
     load_k(p0, p1);
-    p0 = t.page_at(2 * (tile + slots)), p1 = t.page_at(2 * (tile + slots) + 1);
   }
   uint64_t see[NQ];                          // (up to 64 nodes)
 #pragma unroll
@@ -418,6 +439,8 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
       *reinterpret_cast<u32x4*>(v_s + v_at<D>(rr, c8 >> 1) + (c8 & 1) * 16) = v;
     }
     const bool more = tile + slots < tiles;
+    if (++turn % 32 == 0) refill(tile + slots);
+    p0 = page(turn, 0), p1 = page(turn, 1);
     if (more) load_v(p0, p1);
     u32x4 ph[NQ], pl[NQ];
 #pragma unroll
@@ -436,12 +459,9 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
           st[i / 4][i % 4] = (bits >> (16 * (i / 4) + i % 4)) & 1 ? st[i / 4][i % 4] : kPanelNegInf;
       }
       const float ref = tree_maximum<2, DT, NQ>(st, c2, mx[qt], sum[qt], o, qt);
-      tree_weights(st[0], st[1], c2, ref, sum[qt], ph[qt], pl[qt]);
+      tree_weights<true>(st[0], st[1], c2, ref, sum[qt], ph[qt], pl[qt]);
     }
-    if (more) {
-      load_k(p0, p1);
-      p0 = t.page_at(2 * (tile + 2 * slots)), p1 = t.page_at(2 * (tile + 2 * slots) + 1);
-    }
+    if (more) load_k(p0, p1);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const u32x4 vf = v_operand<D>(v_s, dt, lane);
@@ -531,31 +551,49 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
       }
     }
   }
-  if (t.bad_page && lane == 0) raise_error(a.err, kErrPageRange);
+  if (t.bad_page) raise_error(a.err, kErrPageRange);
 }
 
 // ----------------------------------------------------------------------- many columns
-template <int D>
-constexpr int many_tile() {                  // positions
-  return D <= 128 ? 64 : 32;
+template <int D, int W>
+constexpr int many_tile() {                  // positions: 32 KiB of LDS a tile, 16 of small blocks
+  return D <= 128 && W == 8 ? 64 : 32;
 }
-template <int D>
-constexpr int many_nq() {
-  return D <= 128 ? 2 : 1;
+constexpr int kManyNq = 2;                   // 16s of columns of a wave
+constexpr int kStages = 4;                   // tiles of K and V in LDS
+template <int D, int W>
+constexpr int many_lds() {
+  return kStages * 2 * many_tile<D, W>() * D * 2;
 }
-template <int D>
-constexpr int many_lds() {                   // two buffers of K and V
-  return 2 * 2 * many_tile<D>() * D * 2;
+
+// 16 bytes a lane from `base` + `at` straight to LDS, 1 KiB from byte `to` on.  Written out: the
+// compiler waits for all such loads before it reads any LDS, where here three tiles' stay in
+// flight.  There is no register that they write, and what they have written is read behind
+// landed() and a barrier.
+__device__ __forceinline__ void load_to_lds(const bf16* base, uint32_t at, uint32_t to) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(to), "v"(at), "s"(base)
+      : "memory", "m0");
+}
+// All but the last kN of this wave's loads have landed.
+template <int kN>
+__device__ __forceinline__ void landed() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kN) : "memory");
 }
 
 template <int D, int W>
 __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles,
                                                             float* __restrict__ part_o,
                                                             float* __restrict__ part_ml) {
-  constexpr int NQ = many_nq<D>(), DS = D / 32, DT = D / 16, kPos = many_tile<D>();
+  constexpr int NQ = kManyNq, DS = D / 32, DT = D / 16, kPos = many_tile<D, W>();
   constexpr int kCols = 16 * NQ * W, kBytes = kPos * D * 2;
-  constexpr int kLoads = kBytes / 16 / (W * kWave);    // of K, of V, by a thread
+  constexpr int kLoads = kBytes / 1024 / W;  // of K, of V, by a wave: 1 KiB each
   constexpr int kChunks = D / 8;             // 16 bytes each, of a position
+  constexpr int kRows = kWave / kChunks;     // positions of a load
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int odd_s;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
@@ -574,40 +612,38 @@ __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, i
   const int begin = (int)((int64_t)tiles * split / splits);
   const int end = (int)((int64_t)tiles * (split + 1) / splits);
 
-  u32x4 kr[kLoads], vr[kLoads];
-  int pages[kLoads];                         // of the tile that is loaded next
-  auto next_pages = [&](int tile) {
+  // Load i of this wave takes positions kRows (i W + wave) .. of a tile; a lane's place in LDS
+  // follows from its number, so it loads the 16 bytes that belong there.
+  uint32_t k_from[kLoads], v_from[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      pages[i] = t.page_at(tile * (kPos / kPage) +
-                           (i * W + wave) * kWave / kChunks / kPage);
+  for (int i = 0; i < kLoads; ++i) {
+    const int row = (i * W + wave) * kRows + lane / kChunks, slot = lane % kChunks;
+    const int kc = slot ^ (k_at<D>(row, 0) - row * D * 2) / 16;
+    const int vc = slot ^ (v_at<D>(row, 0) - row * D * 2) / 16;
+    k_from[i] = (uint32_t)(row % kPage * D + kc * 8) * 2;
+    v_from[i] = (uint32_t)(row % kPage * D + vc * 8) * 2;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  // Pages of the next kPages / kPagesOf tiles, in LDS: a scalar load of some would be waited for
+  // with the next LDS read, a vector load behind all tiles' loads.
+  constexpr int kPagesOf = kPos / kPage, kPages = 1024;
+  __shared__ int page_s[kPages];
+  auto fill_pages = [&](int tile) {
+    for (int i = tid; i < kPages; i += W * kWave) page_s[i] = t.page_at(tile * kPagesOf + i);
   };
-  auto load_tile = [&]() {
+  auto load_tile = [&](int tile) {
+    const int n = tile - begin;
+    const uint32_t buf = lds0 + (uint32_t)(n % kStages) * 2 * kBytes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int64_t at = pages[i] * t.page_size + (i * W * kWave + tid) % (kPage * kChunks) * 8;
-      kr[i] = load16(t.k + at);
-      vr[i] = load16(t.v + at);
-    }
-  };
-  bool odd = false;                          // a drafted value is not finite
-  auto store_tile = [&](uint8_t* buf, int tile) {
-    const bool edge = (tile + 1) * kPos > t.L;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = i * W * kWave + tid, rr = at / kChunks, c8 = at % kChunks;
-      *reinterpret_cast<u32x4*>(buf + k_at<D>(rr, c8)) = kr[i];
-      u32x4 v = vr[i];
-      if (edge) v = clean_v(v, tile * kPos + rr, t.L, t.n, odd);
-      *reinterpret_cast<u32x4*>(buf + kBytes + v_at<D>(rr, c8 >> 1) + (c8 & 1) * 16) = v;
+      const int page = __builtin_amdgcn_readfirstlane(
+          page_s[n * kPagesOf % kPages + (i * W + wave) * kRows / kPage]);
+      const uint32_t to = buf + (uint32_t)(i * W + wave) * 1024;
+      load_to_lds(t.k + page * t.page_size, k_from[i], to);
+      load_to_lds(t.v + page * t.page_size, v_from[i], to + kBytes);
     }
   };
 
-  if (begin < end) {
-    next_pages(begin);
-    load_tile();
-    next_pages(begin + 1);
-  }
   u32x4 qf[NQ][DS];
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
@@ -628,20 +664,48 @@ __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, i
     for (int dt = 0; dt < DT; ++dt) o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   if (tid == 0) odd_s = 0;
-  if (begin < end) {
-    store_tile(smem, begin);
-    if (begin + 1 < end) load_tile();
-    next_pages(begin + 2);
-  }
+  fill_pages(begin);
+  // (the queries are waited for here: else a tile's products would do it, and so wait for the
+  // loads of the tiles behind)
+#pragma unroll
+  for (int qt = 0; qt < NQ; ++qt)
+#pragma unroll
+    for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(qf[qt][s]));
   __syncthreads();
-
+#pragma unroll
+  for (int i = 0; i + 1 < kStages; ++i)
+    if (begin + i < end) load_tile(begin + i);
+  constexpr int kTileLoads = 2 * kLoads;     // of a wave
+  // tile's loads have landed, those of the tiles behind it may be in flight
+  auto wait_for = [&](int tile) {
+    if (tile + 2 < end) landed<2 * kTileLoads>();
+    else if (tile + 1 < end) landed<kTileLoads>();
+    else landed<0>();
+  };
+  static_assert(kStages == 4, "wait_for counts two tiles behind the one that is read next");
+  if (begin < end) wait_for(begin);
+  __syncthreads();
   for (int tile = begin; tile < end; ++tile) {
-    uint8_t* const buf = smem + ((tile - begin) & 1) * 2 * kBytes;
-    uint8_t* const other = smem + ((tile - begin + 1) & 1) * 2 * kBytes;
-    if (tile + 1 < end) store_tile(other, tile + 1);   // (read by all before the last barrier)
-    if (tile + 2 < end) {
-      load_tile();
-      next_pages(tile + 3);
+    uint8_t* const buf = smem + (tile - begin) % kStages * 2 * kBytes;
+    // (into the buffer of the tile before, which all have read)
+    const int ahead = tile + kStages - 1;
+    if (ahead < end) {
+      if ((ahead - begin) * kPagesOf % kPages == 0) {
+        fill_pages(ahead);
+        __syncthreads();
+      }
+      load_tile(ahead);
+    }
+    if ((tile + 1) * kPos > t.L) {           // drafted positions, or none: clean V
+      bool odd = false;                      // a drafted value is not finite
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int at = (i * W + wave) * kWave + lane, row = at / kChunks;
+        u32x4* const v = reinterpret_cast<u32x4*>(buf + kBytes + at * 16);
+        *v = clean_v(*v, tile * kPos + row, t.L, t.n, odd);
+      }
+      if (odd) odd_s = 1;
+      __syncthreads();
     }
     const bool edge = (tile + 1) * kPos > t.L;
     if (c0 < t.cols) {
@@ -678,25 +742,25 @@ __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, i
       }
 #pragma unroll
       for (int kk = 0; kk < kPos / kTile; ++kk) {
-        u32x4 ph[NQ], pl[NQ];
+        u32x4 pr[NQ], none;
 #pragma unroll
         for (int qt = 0; qt < NQ; ++qt)
-          tree_weights(st[qt][2 * kk], st[qt][2 * kk + 1], c2, ref[qt], sum[qt], ph[qt], pl[qt]);
+          tree_weights<false>(st[qt][2 * kk], st[qt][2 * kk + 1], c2, ref[qt], sum[qt], pr[qt],
+                              none);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, lane);
 #pragma unroll
-          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pl[qt], o[dt][qt]);
-#pragma unroll
-          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
+          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pr[qt], o[dt][qt]);
         }
       }
     }
-    if (tile + 1 < end) __syncthreads();
+    if (tile + 1 < end) {
+      wait_for(tile + 1);
+      __syncthreads();
+    }
   }
-  if (odd) odd_s = 1;
-  __syncthreads();
-  odd = odd_s;
+  const bool odd = odd_s;                    // (set before the last tile's barrier)
 
   const int64_t pcol = ((int64_t)unit * mtiles + mt) * kCols;
 #pragma unroll
@@ -742,7 +806,7 @@ __global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, i
       }
     }
   }
-  if (t.bad_page && lane == 0) raise_error(a.err, kErrPageRange);
+  if (t.bad_page) raise_error(a.err, kErrPageRange);
 }
 
 // ---------------------------------------------------------------------------
@@ -821,9 +885,9 @@ TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, i
     per_cu = head_dim * p.nq <= 64 ? 4 : head_dim * p.nq <= 128 ? 3 : 2;
     most = (tiles + p.waves - 1) / p.waves;
   } else {
-    const int wave_cols = head_dim <= 128 ? 32 : 16;
+    const int wave_cols = 16 * kManyNq;
     p.nq = 0;
-    p.waves = cols <= 4 * wave_cols ? 4 : 8;
+    p.waves = cols <= 4 * wave_cols && head_dim <= 128 ? 4 : 8;
     p.cols = p.waves * wave_cols;
     per_cu = 8 / p.waves;
     most = (tiles + 7) / 8;
@@ -939,15 +1003,16 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
   TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), blocks, W * kWave, a, p.splits, p.mtiles, po, \
                pml)
 #define TFD_TREE_MANY(D, W) \
-  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D>()), blocks, W * kWave, a, p.splits, p.mtiles, po, pml)
+  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D, W>()), blocks, W * kWave, a, p.splits, p.mtiles, po, pml)
 #define TFD_TREE_DIM(D)                                                                       \
   {                                                                                           \
     if (p.nq == 1 && p.waves == 4) TFD_TREE_FEW(D, 1, 4)                                      \
     else if (p.nq == 1) TFD_TREE_FEW(D, 1, alone_waves(D))                                    \
     else if (p.nq == 2) {                                                                     \
       if constexpr (D <= 128) TFD_TREE_FEW(D, 2, 4)                                           \
-    } else if (p.waves == 4) TFD_TREE_MANY(D, 4)                                              \
-    else TFD_TREE_MANY(D, 8)                                                                  \
+    } else if (p.waves == 4) {                                                                \
+      if constexpr (D <= 128) TFD_TREE_MANY(D, 4)                                             \
+    } else TFD_TREE_MANY(D, 8)                                                                \
     if (p.splits > 1) k_tree_join<D><<<joins, kBlock, 0, s>>>(a, p.splits, pad, po, pml);     \
   }
   if (a.head_dim == 64) TFD_TREE_DIM(64)
