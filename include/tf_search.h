@@ -36,12 +36,23 @@ int tfd_tree_accept(const int32_t* tokens, const int32_t* parents, const int32_t
                     const int32_t* counts, int rows, int nodes, int32_t* path,
                     int32_t* accepted, int32_t* next, void* stream);
 
+/* tf_decode.h's tfd_panel_qkv_append for drafted nodes: row m is rotated to position pos[m] (that
+ * of its depth), and its key and value go to position slot[m] of sequence seq[m]'s pages; a
+ * row with slot[m] < 0 is not there. */
+int tfd_tree_qkv_append(const float* part, int slices, int M, int heads, int kv_heads,
+                        int head_dim, const void* gamma_q, const void* gamma_k,
+                        const void* cos_table, const void* sin_table, int rope_rows,
+                        const int32_t* pos, const int32_t* slot, const int32_t* seq,
+                        const int32_t* page_table, int max_pages, void* k_pool, void* v_pool,
+                        int num_pages, float scale, float eps, void* q_out, int32_t* err,
+                        void* stream);
 /* Attention of drafted nodes.  Row b's nodes have their keys and values at positions
  * lengths[b] + t of its pages.  Node t attends to every position below lengths[b] and to node n
  * where bit n of masks[b][t] is set and n < counts[b]:
  *   out = sum_j softmax_j(scale q . k_j) v_j,
- * scores and sums in f32, the probabilities (a product's operands) as sums of two bf16, one rounding of
- * the output.  A node that sees nothing gets zeros.  What a node does not see takes no part,
+ * scores and sums in f32, one rounding of the output.  The probabilities, a product's operands,
+ * are sums of two bf16 (2^-16 of each) where few columns, nodes x heads / kv_heads, share a kv
+ * head, and one bf16 (2^-8) where tfd_tree_attn_form says many.  A node that sees nothing gets zeros.  What a node does not see takes no part,
  * values that are not finite included.  q bf16, rows / nodes / heads q_row / q_node / q_head
  * elements apart (multiples of 8, 16-byte aligned).  out: [rows][nodes][heads][head_dim], or
  * with out_panel the rows x nodes rows of tf_decode.h's panel order.  Nodes from counts[b] on

@@ -22,6 +22,10 @@ the whole vocabulary at temperature 1.0 (``examples/granite_4_0_h_small-cuda/
 run.py:21-28``) -- which ``--temperature``, ``--top-k`` (0: the whole
 vocabulary), ``--top-p`` and ``--sample-seed`` override.  Qwen3 (greedy only in
 its reference) samples through the batched engine with one sequence.
+
+Two searches of Qwen3's batched engine: ``--beams K`` prints the best of K continuations by
+beam search (``--length-penalty``, ``--eos``), ``--draft N`` checks up to N drafted tokens a
+pass, taken from where the text repeats itself; its tokens are the greedy ones.
 """
 from __future__ import annotations
 
@@ -157,6 +161,24 @@ def build(args, model: str, device: str):
                 return r.tokens[0], r.seconds, r.prefill_seconds
 
             return make_batch, run_batch, cfg.vocab_size, "batch, sampled"
+        if args.beams or args.draft:
+            from tilefoundry_amd.qwen3.batch_engine import BatchEngine
+
+            def make_search(prompt_len):
+                return BatchEngine(cfg, w, batch=args.beams or 1, device=device,
+                                   max_new=args.max_new_tokens,
+                                   prompt_room=max(room, prompt_len + 8))
+
+            def run_search(eng, prompt):
+                if args.draft:
+                    r = eng.speculate([prompt], args.max_new_tokens, nodes=args.draft)
+                    return r.tokens[0], r.seconds, r.prefill_seconds
+                r = eng.beam_search([prompt], args.max_new_tokens, beams=args.beams, eos=args.eos,
+                                    length_penalty=args.length_penalty)
+                return r.tokens[0][0], r.seconds, r.prefill_seconds
+
+            return make_search, run_search, cfg.vocab_size, \
+                f"batch, {args.beams} beams" if args.beams else f"batch, {args.draft} drafted"
         mode = args.mode or ("xcd" if xcd_fits(cfg, device) else "persistent")
 
         def make(prompt_len):
@@ -242,7 +264,20 @@ def main(argv: list[str] | None = None) -> int:
     ap.add_argument("--top-p", type=float, default=None,
                     help="--sample: nucleus mass inside the top k")
     ap.add_argument("--sample-seed", type=int, default=0, help="--sample: seed of the draws")
+    ap.add_argument("--beams", type=int, default=0, metavar="K",
+                    help="Qwen3: the best of K continuations by beam search (1..32)")
+    ap.add_argument("--eos", type=int, default=None, help="--beams: the token that ends one")
+    ap.add_argument("--length-penalty", type=float, default=0.0,
+                    help="--beams: compare scores over length ** this (default 0: their sums)")
+    ap.add_argument("--draft", type=int, default=0, metavar="N",
+                    help="Qwen3: check up to N drafted tokens a pass (1..256)")
     args = ap.parse_args(argv)
+    if not 0 <= args.beams <= 32 or not 0 <= args.draft <= 256:
+        raise SystemExit("--beams takes 1..32, --draft 1..256")
+    if args.beams and args.draft or (args.beams or args.draft) and args.sample:
+        raise SystemExit("--beams, --draft and --sample exclude each other")
+    if not args.beams and (args.eos is not None or args.length_penalty):
+        raise SystemExit("--eos / --length-penalty need --beams")
     if not args.sample and any(v is not None for v in (args.temperature, args.top_k,
                                                        args.top_p)):
         raise SystemExit("--temperature / --top-k / --top-p need --sample")
@@ -253,6 +288,8 @@ def main(argv: list[str] | None = None) -> int:
     model = model_of(args)
     if args.experts is not None and model != "granite":
         raise SystemExit("--experts is for granite")
+    if (args.beams or args.draft) and (model != "qwen3" or args.mode):
+        raise SystemExit("--beams / --draft are for qwen3, without --mode")
 
     tokenizer = None
     if args.ckpt is not None and args.prompt is not None:

@@ -169,6 +169,8 @@ SIGNATURES: dict[str, list] = {
     # include/tf_search.h
     "tfd_tree_masks": [P, P, I, I, P, P, P, P],
     "tfd_tree_accept": [P, P, P, P, I, I, P, P, P, P],
+    "tfd_tree_qkv_append": [P, I, I, I, I, I, P, P, P, P, I, P, P, P, P, I, P, P, I, F, F, P, P,
+                            P],
     "tfd_tree_attn_work_bytes": [I, I, I, I, I, I],
     "tfd_tree_attn_form": [I, I, I, I, I, I, P],
     "tfd_tree_attn": [P, P],
@@ -186,7 +188,7 @@ RESTYPES = {"tfd_last_error": ctypes.c_char_p, "tfd_sample_work_bytes": ctypes.c
             "tfd_mx4_packed_bytes": ctypes.c_int64,
             "tfd_mx4_gemm_work_bytes": ctypes.c_int64,
             "tfd_mx4_experts_work_bytes": ctypes.c_int64,
-            "tfd_tree_attn_work_bytes": ctypes.c_int64, "tfd_beam_work_bytes": ctypes.c_int64,
+        "tfd_tree_attn_work_bytes": ctypes.c_int64, "tfd_beam_work_bytes": ctypes.c_int64,
             "tfd_state_blocks": ctypes.c_int64}
 UNCHECKED = {"tfd_abi_version", "tfd_decode_persistent_grid", "tfd_panel_gemm_slices",
              "tfd_panel_attn_rows", "tfd_mx4_experts_tile_rows"}

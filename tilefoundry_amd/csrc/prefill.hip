@@ -21,6 +21,7 @@
 #include "panel.h"
 #include "tf_decode.h"
 #include "tf_hybrid.h"
+#include "tf_search.h"
 
 using namespace tfd;
 using namespace tfd_host;
@@ -202,24 +203,27 @@ __global__ __launch_bounds__(kBlock, 2) void k_gemm_panels(const bf16* __restric
 // ---------------------------------------------------------------------------
 // After the q/k/v projection (model.py:172-190, 339-352): per head RMSNorm and
 // RoPE of the queries (times the score scale) and keys, keys and values appended
-// at the row's position of its sequence's pages.  A wave per (row, head vector).
+// at the row's position of its sequence's pages (or, drafted nodes, at `slot`; below 0: the
+// row is not there).  A wave per (row, head vector).
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ __launch_bounds__(kBlock) void k_panel_qkv(
     const float* __restrict__ part, int slices, int M, int heads, int kv_heads,
     const bf16* __restrict__ gq, const bf16* __restrict__ gk, const bf16* __restrict__ cos_t,
     const bf16* __restrict__ sin_t, int rope_rows, const int* __restrict__ pos,
-    const int* __restrict__ seq, const int* __restrict__ page_table, int max_pages,
-    bf16* __restrict__ kpool, bf16* __restrict__ vpool, int num_pages, float scale, float eps,
-    bf16* __restrict__ q_out, int* err) {
+    const int* __restrict__ slot, const int* __restrict__ seq,
+    const int* __restrict__ page_table, int max_pages, bf16* __restrict__ kpool,
+    bf16* __restrict__ vpool, int num_pages, float scale, float eps, bf16* __restrict__ q_out,
+    int* err) {
   constexpr int kHalf = D / 2;
   const int m = blockIdx.x, lane = threadIdx.x & (kWave - 1);
   const int v = blockIdx.y * kWavesPerBlock + threadIdx.x / kWave;
   if (v >= heads + 2 * kv_heads) return;
   const int N = (heads + 2 * kv_heads) * D;
-  const int P = pos[m];
+  const int P = pos[m], S = slot ? slot[m] : P;
   const bool isq = v < heads, isv = v >= heads + kv_heads;
-  if (P < 0 || P >= rope_rows || P >= max_pages * kPage) {
+  if (slot && S < 0) return;
+  if (P < 0 || P >= rope_rows || S < 0 || S >= max_pages * kPage) {
     if (lane == 0) raise_error(err, kErrPosRange);
     return;
   }
@@ -249,14 +253,14 @@ __global__ __launch_bounds__(kBlock) void k_panel_qkv(
     q[li + kHalf] = f2bf(o1 * scale);
     return;
   }
-  const int page = page_table[(int64_t)seq[m] * max_pages + P / kPage];
+  const int page = page_table[(int64_t)seq[m] * max_pages + S / kPage];
   if (page < 0 || page >= num_pages) {
     if (lane == 0) raise_error(err, kErrPageRange);
     return;
   }
   const int h = isv ? v - heads - kv_heads : v - heads;
   bf16* pool = isv ? vpool : kpool;
-  bf16* o = pool + (((int64_t)page * kv_heads + h) * kPage + P % kPage) * D;
+  bf16* o = pool + (((int64_t)page * kv_heads + h) * kPage + S % kPage) * D;
   o[li] = f2bf(o0);
   o[li + kHalf] = f2bf(o1);
 }
@@ -1001,10 +1005,11 @@ int tfd_panel_add_norm(const float* part, int slices, const void* resid, void* h
   return launched("panel_add_norm");
 }
 
-int tfd_panel_qkv_append(const float* part, int slices, int M, int heads, int kv_heads,
-                         int head_dim, const void* gamma_q, const void* gamma_k,
+static int qkv_append(const float* part, int slices, int M, int heads, int kv_heads, int head_dim,
+                      const void* gamma_q, const void* gamma_k,
                          const void* cos_table, const void* sin_table, int rope_rows,
-                         const int32_t* pos, const int32_t* seq, const int32_t* page_table,
+                         const int32_t* pos, const int32_t* slot, const int32_t* seq,
+                         const int32_t* page_table,
                          int max_pages, void* k_pool, void* v_pool, int num_pages, float scale,
                          float eps, void* q_out, int32_t* err, void* stream) {
   if (!part || !gamma_q || !gamma_k || !cos_table || !sin_table || !pos || !seq || !page_table ||
@@ -1019,12 +1024,35 @@ int tfd_panel_qkv_append(const float* part, int slices, int M, int heads, int kv
 #define TFD_PANEL_QKV(D)                                                                        \
   hipLaunchKernelGGL((k_panel_qkv<D>), grid, dim3(kBlock), 0, s, part, slices, M, heads, kv_heads, \
                      (const bf16*)gamma_q, (const bf16*)gamma_k, (const bf16*)cos_table,        \
-                     (const bf16*)sin_table, rope_rows, pos, seq, page_table, max_pages,        \
+                     (const bf16*)sin_table, rope_rows, pos, slot, seq, page_table, max_pages,        \
                      (bf16*)k_pool, (bf16*)v_pool, num_pages, scale, eps, (bf16*)q_out, err)
   if (head_dim == 128) TFD_PANEL_QKV(128);
   else TFD_PANEL_QKV(64);
 #undef TFD_PANEL_QKV
   return launched("panel_qkv_append");
+}
+
+int tfd_panel_qkv_append(const float* part, int slices, int M, int heads, int kv_heads,
+                         int head_dim, const void* gamma_q, const void* gamma_k,
+                         const void* cos_table, const void* sin_table, int rope_rows,
+                         const int32_t* pos, const int32_t* seq, const int32_t* page_table,
+                         int max_pages, void* k_pool, void* v_pool, int num_pages, float scale,
+                         float eps, void* q_out, int32_t* err, void* stream) {
+  return qkv_append(part, slices, M, heads, kv_heads, head_dim, gamma_q, gamma_k, cos_table,
+                    sin_table, rope_rows, pos, nullptr, seq, page_table, max_pages, k_pool, v_pool,
+                    num_pages, scale, eps, q_out, err, stream);
+}
+
+int tfd_tree_qkv_append(const float* part, int slices, int M, int heads, int kv_heads,
+                         int head_dim, const void* gamma_q, const void* gamma_k,
+                         const void* cos_table, const void* sin_table, int rope_rows,
+                         const int32_t* pos, const int32_t* slot, const int32_t* seq, const int32_t* page_table,
+                         int max_pages, void* k_pool, void* v_pool, int num_pages, float scale,
+                         float eps, void* q_out, int32_t* err, void* stream) {
+  if (!slot) return fail(kBadArg, "tree_qkv_append: null pointer");
+  return qkv_append(part, slices, M, heads, kv_heads, head_dim, gamma_q, gamma_k, cos_table,
+                    sin_table, rope_rows, pos, slot, seq, page_table, max_pages, k_pool, v_pool,
+                    num_pages, scale, eps, q_out, err, stream);
 }
 
 int tfd_panel_attn_rows(int group) { return group > 0 && group <= 8 ? 64 / group : 0; }

@@ -116,8 +116,13 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // transposing read gives V^T's operands; its 32-byte pieces are permuted by the row so that the
 // 16 rows of such a read take the fewest cycles.
 //
-// Softmax against a running reference, in f32.  A
-// probability is the sum of two bf16, so that it is not the less exact operand.
+// Softmax against a running reference, in f32.  The
+// probabilities have to become bf16 for the second product.
+// By few columns, which wait for keys, they stay a sum of two bf16 (2^-16 of each).  By many they
+// are one bf16: the second product of a second half costs a seventh to a third of the call (253
+// to 180 us at 2 rows of 32,760 positions, 64 nodes of 16 heads over 8), and what it buys is
+// small beside the output's own rounding (2^-8 of a probability, and they average: 1.4 times the
+// error of an attention in f32 that rounds its output, against 1.0).
 //
 // Two kernels.  Few columns (k_tree_few): the keys are what is waited for, so each wave
 // takes other tiles of 32 positions, its K straight into registers as operands and its V

@@ -30,6 +30,7 @@ from .config import Qwen3Config
 from .engine import bf16_scale, scatter_cache
 from .prefill import (Prefill, attention_splits, gate_up_panels, in_vocab, int32_ids,
                       token_array)
+from .search import BeamSearch, NgramDraft, Speculation
 from .weights import head_rows, pack_layer, validate
 
 MAX_BATCH = 32
@@ -251,15 +252,23 @@ class BatchEngine:
             self._gemm(self.xn, w["w_gu"], H, 2 * I, _lib.EPI_SWIGLU, None, self.hmid, 0, s)
         self._project(self.hmid, w["w_down"], I, self.h1, x_out, gamma, s)
 
-    def _step(self):
-        s = self._stream()
-        L, B, H = self._lib, self.B, self.H
+    def _forward(self, s: int):
+        """Every layer and the head for the staged embeddings: the sequences' logits."""
         self._norm(self.hid, self.layers[0]["gamma_in"], s)
         for i in range(self.L):
             self._layer(i, s)
-        self._gemm(self.xn, self.w_head, H, self.V, _lib.EPI_LOGITS, None, self.logits,
+        self._gemm(self.xn, self.w_head, self.H, self.V, _lib.EPI_LOGITS, None, self.logits,
                    self.V, s)
+
+    def _step(self):
+        s = self._stream()
+        self._forward(s)
         self.picker(self.logits, self.V, self.pick, self.pos, s)
+        self._finalize(s)
+
+    def _finalize(self, s: int):
+        """Picks recorded, positions advanced, the next tokens' embeddings staged."""
+        L, B, H = self._lib, self.B, self.H
         L.tfd_finalize_rows(ptr(self.pick), B, ptr(self.inp), self.nsteps, ptr(self.plen),
                             ptr(self.ids), ptr(self.pos), ptr(self.sam), self.nsteps,
                             self.nsteps, ptr(self.w_embed), ptr(self.hid), H, H, self.V,
@@ -336,20 +345,42 @@ class BatchEngine:
         self._lib.tfd_embed_rows_bf16(ptr(self.w_embed), ptr(self.ids), ptr(self.hid), self.H,
                                       self.B, self.H, self.V, ptr(self.err), self._stream())
 
+    def _prompt_pass(self) -> Prefill:
+        if getattr(self, "_prefiller", None) is None:
+            self._prefiller = Prefill(weakref.ref(self), packed=True)
+        return self._prefiller
+
     def prefill(self, prompts: list[list[int]]):
         """Fill sequence b's cache at positions 0 .. len(prompts[b]) - 2 in batched
         passes (``qwen3.prefill``, through b's page-table row), so that the next
         step decodes every prompt's last token at its own position."""
         if len(prompts) != self.B or any(len(p) < 1 for p in prompts):
             raise ValueError(f"need {self.B} non-empty prompts")
-        if getattr(self, "_prefiller", None) is None:
-            self._prefiller = Prefill(weakref.ref(self), packed=True)
         self._load_prompts(prompts)
-        self._prefiller.run_many([(p[:-1], 0, b) for b, p in enumerate(prompts) if len(p) > 1])
+        self._prompt_pass().run_many([(p[:-1], 0, b) for b, p in enumerate(prompts) if len(p) > 1])
         self.pos.copy_(torch.tensor([len(p) - 1 for p in prompts], dtype=torch.int32))
         self.ids.copy_(torch.tensor([int(p[-1]) for p in prompts], dtype=torch.int64))
         self._lib.tfd_embed_rows_bf16(ptr(self.w_embed), ptr(self.ids), ptr(self.hid), self.H,
                                       self.B, self.H, self.V, ptr(self.err), self._stream())
+
+    def beam_search(self, prompts: list[list[int]], max_new: int, *, beams: int,
+                    eos: int | None = None, length_penalty: float = 0.0):
+        """The *beams* best continuations of each prompt by beam search
+        (``qwen3.search.BeamSearch``): prompts times beams fill the batch."""
+        key = (beams, eos, float(length_penalty))
+        known = self.__dict__.setdefault("_beam_searches", {})
+        if key not in known:
+            known[key] = BeamSearch(weakref.ref(self), *key)
+        return known[key].run(prompts, max_new)
+
+    def speculate(self, prompts: list[list[int]], max_new: int, *, nodes: int = 8, draft=None):
+        """``generate``, greedy, several tokens a pass: a draft's tree of up to *nodes* tokens is
+        checked at once and the agreeing ones are kept (``qwen3.search.Speculation``; draft:
+        ``qwen3.search.NgramDraft`` unless given)."""
+        known = self.__dict__.setdefault("_speculations", {})
+        if nodes not in known:
+            known[nodes] = Speculation(weakref.ref(self), nodes)
+        return known[nodes].run(prompts, max_new, NgramDraft() if draft is None else draft)
 
     def check_errors(self):
         e = int(self.err.item())

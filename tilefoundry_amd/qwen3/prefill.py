@@ -231,6 +231,21 @@ class Prefill:
                                       s)
         return self._slices(M, K, N)
 
+    def _gate_up(self, w, M, s):
+        """hmid = SwiGLU of the gate/up projection of xn (model.py:227-234)."""
+        L, H, I = self._lib, self.H, self.I
+        slices = self._slices(M, H, 2 * I)
+        if M <= 16 or not (slices > 1 or gate_up_panels(M, I, self.cus)):
+            L.tfd_gemm_skinny_bf16(ptr(self.xn), ptr(w["w_gu"]), M, H, 2 * I, _lib.EPI_SWIGLU,
+                                   None, 0, ptr(self.hmid), 0, ptr(self.work),
+                                   self.work.numel(), s)
+        elif slices == 1:
+            L.tfd_panel_gemm_bf16(ptr(self.xn), ptr(w["w_gu"]), M, H, 2 * I, _lib.PANEL_SWIGLU,
+                                  ptr(self.hmid), s)
+        else:
+            sl = self._gemm(self.xn, w["w_gu"], M, H, 2 * I, s)
+            L.tfd_panel_swiglu(ptr(self.part), sl, M, 2 * I, ptr(self.hmid), s)
+
     def _layer(self, i, M, pos, seq, tiles, ntiles, s):
         """One decoder layer (model.py:236-266) for M prompt rows; xn holds its
         normalised input.  The last layer stops at its keys and values."""
@@ -251,17 +266,7 @@ class Prefill:
         sl = self._gemm(self.attn, w["w_o"], M, self.QD, H, s)
         L.tfd_panel_add_norm(ptr(self.part), sl, ptr(self.hid), ptr(self.h1),
                              ptr(w["gamma_post"]), ptr(self.xn), M, H, self.eps, s)
-        slices = self._slices(M, H, 2 * I)
-        if M <= 16 or not (slices > 1 or gate_up_panels(M, I, self.cus)):
-            L.tfd_gemm_skinny_bf16(ptr(self.xn), ptr(w["w_gu"]), M, H, 2 * I, _lib.EPI_SWIGLU,
-                                   None, 0, ptr(self.hmid), 0, ptr(self.work),
-                                   self.work.numel(), s)
-        elif slices == 1:
-            L.tfd_panel_gemm_bf16(ptr(self.xn), ptr(w["w_gu"]), M, H, 2 * I, _lib.PANEL_SWIGLU,
-                                  ptr(self.hmid), s)
-        else:
-            sl = self._gemm(self.xn, w["w_gu"], M, H, 2 * I, s)
-            L.tfd_panel_swiglu(ptr(self.part), sl, M, 2 * I, ptr(self.hmid), s)
+        self._gate_up(w, M, s)
         sl = self._gemm(self.hmid, w["w_down"], M, I, H, s)
         L.tfd_panel_add_norm(ptr(self.part), sl, ptr(self.h1), ptr(self.hid),
                              ptr(self.layers[i + 1]["gamma_in"]), ptr(self.xn), M, H, self.eps, s)
