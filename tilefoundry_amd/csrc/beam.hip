@@ -67,10 +67,12 @@ __device__ __forceinline__ uint32_t wave_and(uint32_t v) {
   return __builtin_amdgcn_readfirstlane(b[0] & b[1]);
 }
 
+constexpr float kLog2e = 1.44269502162933349609375f;
+
 // 2^(d log2 e) for d <= 0 to about an f32's last bit: log2 e in two parts.
 __device__ __forceinline__ float exp_neg(float d) {
-  constexpr float kHi = 1.44269502162933349609375f, kLo = 1.92596303e-8f;
-  return __builtin_amdgcn_exp2f(fmaf(d, kHi, d * kLo));
+  constexpr float kLo = 1.92596303e-8f;
+  return __builtin_amdgcn_exp2f(fmaf(d, kLog2e, d * kLo));
 }
 
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -112,10 +114,29 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&v)[kN], int k) 
   return t;
 }
 
+// A lane's place behind the n before, of the lanes of `who`.
+__device__ __forceinline__ int placed_at(uint64_t who, int n) {
+  return n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                            __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+}
+
 struct BeamPlan {
   int per, chunks;       // values of a lane, chunks (of a wave) of a row
 };
-constexpr int kNear = 256;                   // candidates a wave holds
+
+// What a wave holds of its chunk's candidates: values by fours (each four consecutive tokens)
+// in which one reaches the bound, and those that do.
+constexpr int kFours = 64, kAtOnce = 8;
+typedef float f4 __attribute__((ext_vector_type(4)));
+struct alignas(16) Near {
+  float x[4 * kFours];
+  uint64_t near[4 * kFours + kAtOnce];
+  int token[kFours];
+};
+// Up to so many beams the bound comes from the lanes' best values: that leaves
+// 64 ln(64 / (64 - beams)) fours, 30 of 24 beams; above it from all fours' best, which leaves as many as
+// there are beams, for one ballot a four and bit.
+constexpr int kFewBeams = 24;
 
 // What a wave's chunk of a row leaves: its largest logit, the sum of exp(x - that), and its
 // `beams` largest keys in falling order (0 where there are fewer).
@@ -135,9 +156,9 @@ __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
 // ---------------------------------------------------------------------------
 // A wave per chunk of a row, its values in registers, no barrier.  The beams-th largest of
 // the lanes' best values bounds the chunk's beams-th largest from below: what reaches it,
-// hardly more than `beams` values, goes through LDS to be ranked by counting.  Where more do
-// than LDS holds (equal logits), the places are filled one by one, from memory.  Four values at a time
-// are tested by their largest.
+// hardly more than `beams` values, goes through LDS to be ranked by counting.  Four values at a
+// time are tested by their largest and moved together.  Where more do than LDS holds (equal
+// logits), the places are filled one by one, from memory.
 // ---------------------------------------------------------------------------
 template <int kType, int kPer, bool kVec>
 __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k_beam_scan(TfdBeamArgs a, int chunks, int waves,
@@ -145,14 +166,14 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
                                                       uint64_t* __restrict__ lists) {
   constexpr float kInf = __builtin_huge_valf();
   constexpr int kQuads = kPer / 4;
-  __shared__ uint64_t near_s[kWavesPerBlock][kNear];
+  __shared__ Near near_s[kWavesPerBlock];
   const int lane = threadIdx.x & (kWave - 1);
   const int in_block = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   const int w = blockIdx.x * kWavesPerBlock + in_block;
   if (w >= waves) return;
   const int row = w / chunks, chunk = w % chunks;
   if (a.done && a.done[row]) return;               // (its lists are not read)
-  uint64_t* const near = near_s[in_block];
+  Near& mine_s = near_s[in_block];
   const int c0 = chunk * kWave * kPer, K = a.beams;
   const int64_t base = (int64_t)row * a.ldl;
   float x[kPer];
@@ -181,12 +202,13 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
       if (at(j) >= a.vocab) x[j] = -kInf;
     }
   }
-  // largest of four, of the lane, of the wave; the sum (once more with NaN and +inf put in
-  // their places where there are any: the sum shows them)
+  // Largest of four, of the lane, of the wave, and the sum of 2^(x log2 e - c), c = m log2 e rounded:
+  // one fused multiply-add a value, and what c's rounding left out (exactly fma's remainder) is
+  // put right in the sum.  log2 e as one f32 is 1.3e-8 of x - m off: 1.1e-7 of a sum over
+  // 4,096 equal values, half of an f32's last place at one, where the scores that go out
+  // are themselves f32 of at least ln 4096.
   float top4[kQuads], best, m;
-  double sum;
-#pragma unroll 1
-  for (int again = 0; again < 2; ++again) {
+  auto tops = [&] {
     best = -kInf;
 #pragma unroll
     for (int q = 0; q < kQuads; ++q)
@@ -194,46 +216,81 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
 #pragma unroll
     for (int q = 0; q < kQuads; q += 2) best = max3(best, top4[q], top4[q + 1]);
     m = wave_max(best);
-    const float ref = m == -kInf ? 0.f : m;
-    sum = 0.0;
+  };
+  auto added = [&](auto term) {
+    double sum = 0.0;
 #pragma unroll
     for (int q = 0; q < kQuads; ++q) {
       float e[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) e[i] = exp_neg(x[4 * q + i] - ref);
+      for (int i = 0; i < 4; ++i) e[i] = term(x[4 * q + i]);
       sum += (double)((e[0] + e[1]) + (e[2] + e[3]));
     }
-    sum = wave_sum_d(sum);
-    if (sum < 1e30) break;
+    return wave_sum_d(sum);
+  };
+  tops();
+  const float c = -m * kLog2e;
+  double sum = added([&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, kLog2e, c)); }) *
+               (double)__builtin_amdgcn_exp2f(-fmaf(m, kLog2e, c));
+  // NaN or +inf among the values, none above -inf, or a reference so large that its remainder
+  // is: with the first two put in their places (NaN as -inf, +inf as the largest number),
+  // differences first
+  if (!(fabsf(m) <= 1048576.f && sum < 1e30)) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = fminf(fmaxf(x[j], -kInf), 3.402823466e38f);
+    for (int j = 0; j < kPer; ++j) {
+      asm volatile("" : "+v"(x[j]));         // (or it is done for every chunk, to be chosen from)
+      x[j] = fminf(fmaxf(x[j], -kInf), 3.402823466e38f);
+    }
+    tops();
+    const float ref = m == -kInf ? 0.f : m;
+    sum = added([&](float v) { return exp_neg(v - ref); });
   }
-  const uint32_t t = kth_largest<1>({best > -kInf ? order_of(best) : 0u}, K);
-  // what reaches it (t 0: every candidate)
+  uint32_t t;
+  if (K <= kFewBeams) {
+    t = kth_largest<1>({best > -kInf ? order_of(best) : 0u}, K);
+  } else {
+    uint32_t o[kQuads];
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) o[q] = top4[q] > -kInf ? order_of(top4[q]) : 0u;
+    t = kth_largest(o, K);
+  }
+  // the fours that reach it (t 0: every one that has a candidate)
   const float bound = t ? float_of(t) : -3.402823466e38f;
-  int n = 0;
+  int fours = 0;
 #pragma unroll
   for (int q = 0; q < kQuads; ++q) {
-    if (!__any(top4[q] >= bound)) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = 4 * q + e;
-      const uint64_t who = __ballot(x[j] >= bound);
-      if (!who) continue;
-      const int place = n + __builtin_amdgcn_mbcnt_hi(
-                                (uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-      if (x[j] >= bound && place < kNear) near[place] = key_of(x[j], at(j));
+    const uint64_t who = __ballot(top4[q] >= bound);
+    if (!who) continue;
+    const int place = placed_at(who, fours);
+    if (top4[q] >= bound && place < kFours) {
+      *reinterpret_cast<f4*>(mine_s.x + 4 * place) =
+          f4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+      mine_s.token[place] = at(4 * q);
+    }
+    fours += __popcll(who);
+  }
+  auto wrote = [] {                          // (this wave's LDS operations run in order)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  wrote();
+  uint64_t* const list = lists + (int64_t)w * K;
+  if (fours <= kFours) {
+    int n = 0;
+    for (int i = lane; i - lane < 4 * fours; i += kWave) {
+      const float v = i < 4 * fours ? mine_s.x[i] : -kInf;
+      const uint64_t who = __ballot(v >= bound);
+      if (v >= bound) mine_s.near[placed_at(who, n)] = key_of(v, mine_s.token[i / 4] + i % 4);
       n += __popcll(who);
     }
-  }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  uint64_t* const list = lists + (int64_t)w * K;
-  if (n <= kNear) {
+    if (lane < kAtOnce) mine_s.near[n + lane] = 0;
+    wrote();
     for (int i = lane; i < n; i += kWave) {
-      const uint64_t k = near[i];
+      const uint64_t k = mine_s.near[i];
       int r = 0;
-      for (int j = 0; j < n; ++j) r += near[j] > k;
+      for (int j = 0; j < n; j += kAtOnce)
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e) r += mine_s.near[j + e] > k;
       if (r < K) list[r] = k;
     }
     if (n + lane < K) list[n + lane] = 0;          // (beams <= 64)
@@ -267,7 +324,7 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
 // the first keys of a list from the start on, so that few loads wait for others.
 // ---------------------------------------------------------------------------
 constexpr int kMerge = 1024, kMergeWaves = kMerge / kWave, kFound = 2048;
-constexpr int kHeldKeys = 4, kHeldSums = 3, kHeads = 256;
+constexpr int kHeldKeys = 4, kHeldSums = 3, kHeads = 256, kFewHeads = 32;
 
 struct Cand {
   double rank;
@@ -292,7 +349,7 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   __shared__ uint8_t found_beam[kFound];
   __shared__ uint32_t head_s[kHeads];
   __shared__ Cand wave_s[kMergeWaves];
-  __shared__ int n_s, heads_s, rank_s[kWave];
+  __shared__ int n_s, heads_s;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int K = a.beams, row0 = blockIdx.x * K, n_lists = K * chunks;
@@ -302,7 +359,6 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   for (int i = 0; i < kHeldKeys; ++i)
     held[i] = mine[(int64_t)min(tid, n_lists - 1) * K + min(i, K - 1)];
   if (tid == 0) n_s = heads_s = 0;
-  if (tid < kWave) rank_s[tid] = 0;
   // value = add + (logit - top), rank = value * inv (the difference first: an infinite logit
   // stands as 3.4e38); a row that offers nothing has add NaN
   for (int b = wave; b < K; b += kMergeWaves) {
@@ -314,9 +370,9 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     const float score = a.scores[row];
     const int length = a.lengths ? a.lengths[row] : 0;
     const bool over = a.done && a.done[row], none = !(fabsf(score) < __builtin_huge_valf());
-    const double inv = a.penalty == 0.f ? 1.0
-                                        : 1.0 / pow((double)max(length + (over ? 0 : 1), 1),
-                                                    (double)a.penalty);
+    const double inv = a.penalty == 0.f
+                           ? 1.0
+                           : exp(-(double)a.penalty * log((double)max(length + (over ? 0 : 1), 1)));
     double lse = 0.0;
     float m = -__builtin_huge_valf();
     if (!over) {
@@ -369,17 +425,24 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   uint32_t top = bound_s[0];
 #pragma unroll
   for (int w = 1; w < kMergeWaves; ++w) top = max(top, bound_s[w]);
-  // the threads' heads that reach it bound it once more (every wave for itself)
-  if (head >= max(top, 1u)) {
-    const int at = atomicAdd(&heads_s, 1);
-    if (at < kHeads) head_s[at] = head;
+  // the threads' heads that reach it; where they are many, they bound it once more (every wave for
+  // itself)
+  const uint64_t reach = __ballot(head >= max(top, 1u));
+  if (reach) {
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&heads_s, __popcll(reach));
+    at = placed_at(reach, __builtin_amdgcn_readfirstlane(at));
+    if (head >= max(top, 1u) && at < kHeads) head_s[at] = head;
   }
   __syncthreads();
-  if (heads_s > 2 * K && heads_s <= kHeads) {
+  const int heads = heads_s;
+  if (heads > kFewHeads && heads <= kWave) {
+    top = max(top, kth_largest<1>({lane < heads ? head_s[lane] : 0u}, K));
+  } else if (heads > kWave && heads <= kHeads) {
     uint32_t v[kHeads / kWave];
 #pragma unroll
     for (int i = 0; i < kHeads / kWave; ++i)
-      v[i] = lane + i * kWave < heads_s ? head_s[lane + i * kWave] : 0u;
+      v[i] = lane + i * kWave < heads ? head_s[lane + i * kWave] : 0u;
     top = max(top, kth_largest(v, K));
   }
   const double bound = top ? (double)float_of(top) : kNone;
@@ -421,21 +484,14 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     a.lengths_out[at] = length_s[place];
     a.done_out[at] = done_s[place];
   };
-  if (n <= kWave) {                          // a candidate per lane, the others shared by waves
-    if (lane < n) {
-      const Cand c{found_rank[lane], found_key[lane], found_beam[lane]};
-      int r = 0;
-      for (int j = wave; j < n; j += kMergeWaves)
-        r += better(Cand{found_rank[j], found_key[j], found_beam[j]}, c);
-      if (r) atomicAdd(&rank_s[lane], r);
-    }
-    __syncthreads();
-    if (tid < n) {
-      const int r = rank_s[tid];
-      if (r < K) put(r, Cand{found_rank[tid], found_key[tid], found_beam[tid]});
-    } else if (tid < K) {
-      put_none(tid);
-    }
+  if (n <= kWave) {                          // a candidate per lane of one wave
+    if (wave > 0) return;
+    const Cand c = lane < n ? Cand{found_rank[lane], found_key[lane], found_beam[lane]} : Cand{};
+    int r = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) r += better(Cand{found_rank[j], found_key[j], found_beam[j]}, c);
+    if (lane < n && r < K) put(r, c);
+    if (lane >= n && lane < K) put_none(lane);
     return;
   }
   if (n <= kFound) {

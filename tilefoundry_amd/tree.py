@@ -123,18 +123,19 @@ def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table
     if q.dim() != 4:
         raise ValueError(f"q must be [rows, nodes, heads, dim], got {tuple(q.shape)}")
     rows, nodes, heads, dim = q.shape
-    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or \
-            k_pool.shape[2:] != (_lib.PAGE_SIZE, dim):
+    pool = k_pool.shape
+    if len(pool) != 4 or pool != v_pool.shape or pool[2] != _lib.PAGE_SIZE or pool[3] != dim:
         raise ValueError(f"pools must be [pages, kv_heads, {_lib.PAGE_SIZE}, {dim}], got "
                          f"{tuple(k_pool.shape)} and {tuple(v_pool.shape)}")
-    pages, kv_heads = k_pool.shape[:2]
+    pages, kv_heads = pool[0], pool[1]
     if dim not in HEAD_DIMS:
         raise ValueError(f"head dimension {dim} is none of {', '.join(map(str, HEAD_DIMS))}")
     if not 1 <= nodes <= MAX_NODES or rows > MAX_ROWS:
         raise ValueError(f"1 to {MAX_NODES} nodes of up to {MAX_ROWS} rows, got {nodes} of {rows}")
     if not 1 <= kv_heads <= heads <= 65535 or heads % kv_heads or pages < 1:
         raise ValueError(f"{heads} heads over {kv_heads} kv heads in {pages} pages")
-    if table.dim() != 2 or table.shape[0] != rows or not 1 <= table.shape[1] <= 1 << 22:
+    width = table.shape[1] if table.dim() == 2 else 0
+    if not 1 <= width <= 1 << 22 or table.shape[0] != rows:
         raise ValueError(f"table must be [{rows}, 1..2^22], got {tuple(table.shape)}")
     if lengths.shape != (rows,):
         raise ValueError(f"lengths must be [{rows}], got {tuple(lengths.shape)}")
@@ -150,18 +151,22 @@ def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table
             k_pool.data_ptr() % 16 or v_pool.data_ptr() % 16:
         raise ValueError("pools must be contiguous and 16-byte aligned")
     check_device(q.device, k_pool, v_pool, table, lengths, masks)
-    counts = _counts(counts, rows, q.device)
-    _err(err, q.device)
-    if q.stride(3) != 1 or q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:3]):
+    if counts is not None:
+        counts = _counts(counts, rows, q.device)
+    if err is not None:
+        _err(err, q.device)
+    of_row, of_node, of_head, of_dim = q.stride()
+    if of_dim != 1 or q.data_ptr() % 16 or (of_row | of_node | of_head) % 8:
         q = q.clone(memory_format=torch.contiguous_format)
+        of_row, of_node, of_head, of_dim = q.stride()
     table, lengths, masks = table.contiguous(), lengths.contiguous(), masks.contiguous()
     out = q.new_empty((rows, nodes, heads, dim))
-    L, width = lib(), table.shape[1]
+    L = lib()
     need = L.tfd_tree_attn_work_bytes(rows, nodes, heads, kv_heads, dim, width)
     # of the stream that uses it, like the output: calls on several streams and captured
     # graphs share nothing
     work = q.new_empty(need, dtype=torch.uint8) if need else None
-    a = _lib.TfdTreeAttnArgs(ptr(q), *q.stride()[:3], ptr(k_pool), ptr(v_pool), ptr(table),
+    a = _lib.TfdTreeAttnArgs(ptr(q), of_row, of_node, of_head, ptr(k_pool), ptr(v_pool), ptr(table),
                              ptr(lengths), ptr(counts), ptr(masks), rows, nodes, heads, kv_heads,
                              dim, width, pages, scale, ptr(out), 0, ptr(work), need, ptr(err))
     launch(q.get_device(), L.tfd_tree_attn, ctypes.addressof(a))
