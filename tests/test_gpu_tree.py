@@ -131,13 +131,15 @@ def test_attention(gpu_device, rows, nodes, heads, kv_heads, dim, lengths):
 FORMS = [  # (rows, nodes, heads, kv heads, dim, room), form: how such calls run
     ((1, 7, 4, 2, 64, 9), (1, 16, 1, 1)), ((2, 20, 4, 2, 128, 9), (1, 12, 3, 1)),
     ((1, 13, 8, 2, 256, 9), (1, 8, 4, 1)),
-    ((3, 7, 4, 2, 64, 400), (1, 4, 1, 51)), ((3, 7, 4, 2, 128, 400), (1, 4, 1, 51)),
-    ((3, 4, 8, 2, 256, 400), (1, 4, 1, 51)), ((64, 2, 16, 8, 64, 400), (1, 4, 1, 2)),
-    ((2, 16, 4, 2, 64, 400), (2, 4, 1, 51)), ((2, 11, 4, 2, 128, 400), (2, 4, 1, 51)),
-    ((36, 11, 16, 8, 128, 400), (2, 4, 1, 1)),
-    ((2, 21, 8, 2, 64, 400), (0, 4, 1, 26)), ((2, 21, 8, 2, 128, 400), (0, 4, 1, 26)),
-    ((2, 13, 8, 2, 256, 400), (0, 8, 1, 26)), ((1, 61, 8, 2, 128, 400), (0, 8, 1, 26)),
-    ((1, 61, 16, 2, 64, 400), (0, 8, 2, 26)), ((1, 39, 16, 2, 256, 400), (0, 8, 2, 26)),
+    ((1, 31, 8, 2, 64, 90), (1, 16, 8, 3)), ((2, 11, 4, 2, 128, 400), (1, 12, 2, 17)),
+    ((2, 9, 8, 2, 256, 60), (1, 8, 3, 4)),
+    ((3, 7, 4, 2, 64, 100), (1, 4, 1, 13)), ((3, 7, 4, 2, 128, 100), (1, 4, 1, 13)),
+    ((3, 4, 8, 2, 256, 100), (1, 4, 1, 13)), ((64, 2, 16, 8, 64, 400), (1, 4, 1, 1)),
+    ((6, 16, 16, 8, 64, 400), (2, 4, 1, 5)), ((6, 16, 16, 8, 128, 400), (2, 4, 1, 5)),
+    ((36, 11, 16, 8, 64, 400), (2, 4, 1, 1)), ((36, 31, 16, 8, 128, 40), (2, 4, 2, 1)),
+    ((2, 21, 8, 2, 64, 400), (0, 4, 1, 25)), ((2, 21, 8, 2, 128, 400), (0, 8, 1, 25)),
+    ((2, 13, 8, 2, 256, 400), (0, 8, 1, 25)), ((1, 61, 8, 2, 128, 400), (0, 8, 1, 25)),
+    ((1, 61, 16, 2, 64, 400), (0, 8, 2, 25)), ((1, 39, 16, 2, 256, 400), (0, 8, 2, 25)),
     ((33, 33, 16, 8, 128, 400), (0, 4, 1, 1)), ((33, 66, 16, 8, 64, 9), (0, 8, 1, 1)),
     ((33, 10, 16, 8, 256, 100), (0, 8, 1, 1))]
 
@@ -160,7 +162,7 @@ def test_attention_forms(gpu_device, shape, form):
         assert ((out.double() - want).abs() <= _bound(c, want, size, dim ** -0.5)).all()
         return
     _check(c, gpu_device)
-    counts = torch.tensor([nodes - 1, 0, nodes][:rows], dtype=I32)
+    counts = torch.tensor(([nodes - 1, 0, nodes] * 3)[:rows], dtype=I32)
     c["masks"][0, nodes // 2:] &= ~2
     at = 333 + 1                                     # node 1's value
     c["v_pool"][c["table"][0, at // 16].long(), 0, at % 16, 5] = math.inf

@@ -1,4 +1,6 @@
 // Drafted tokens that form a tree: masks, acceptance, and attention over a paged cache.
+#include <algorithm>
+
 #include "host_common.h"
 #include "panel.h"
 #include "tf_search.h"
@@ -859,49 +861,65 @@ __global__ __launch_bounds__(kBlock) void k_tree_join(TfdTreeAttnArgs a, int spl
     ((bf16*)a.out)[out_at(a, rr, head, lane * kPer + e)] = f2bf(l == 0.f ? 0.f : y[e] / l);
 }
 
-// How a call runs.  A row's tiles that one block's waves can take in a few turns, and no more
-// blocks than compute units: that block alone, 16 columns a block, without a second launch.
-// Else few columns (up to 32, 16 of 256 dims): blocks of four waves; many: four or eight
-// waves of 32 columns (16 of 256 dims).  Splits: as many as fill the compute units' blocks once.
+// How a call runs (all times: one call in a captured graph, 16 heads over 8, 128 dims).
+//
+// Short: where every wave needs one tile of 32 positions, with 16 columns a block and no more
+// blocks than compute units, blocks of as many waves as their registers leave room for.  Two
+// tiles a wave instead of two splits save the join's launch and take the same (13.5 us of 1 row of
+// 700 positions by 16 nodes, 13.2 with the join).  1 row of 6,000 by 16 nodes: 18.3 us, by blocks of
+// four waves of 32 columns 24.1; by 8 nodes 16.7 and 19.7.  16 columns whose tiles blocks
+// of four waves hold at once too are faster by those (700 positions, 8 nodes: 11.4 us, 13.2),
+// down to what a single block holds (200: 10.1, 9.0).
+//
+// Few: up to 64 columns, 16 of 256 dims, in blocks of four waves of up to 32 (2 rows of 32,000 by 32
+// nodes: 60.0 us, by the kernel for many 68.6; 32 rows of 4,096: 118 both; 48 nodes 185 and 125).
+// One block a compute unit: what the splits leave is read again, and four waves' loads are
+// enough in flight (32 rows of 4,096 by 7 nodes: 97.6 us, with three a unit 104.1; 1 of 6,000 by 8:
+// 19.7 and 25.0).
+//
+// Many: eight waves of 32 columns, whose longer tiles cost less a position (32 rows of 4,096 by 60
+// nodes: 122 us, by two blocks of four waves 132); up to 128 columns four waves of 64 dims
+// (8 rows of 8,000: 48.9 us, by eight 51.0), or where there are more row heads than compute units (33
+// rows of 400 by 33: 30.6 us, 37.1).  Splits fill the compute units once (twice as many: 4 rows
+// of 30,000 by 61 nodes of 32 heads 177 us, 161 so, half as many 254).
 struct TreePlan {
   int nq, waves, mtiles, cols, splits;       // nq 0: many columns; cols: of a block
 };
 
-// waves of a block that runs alone: what 16 columns' registers leave room for
-constexpr int alone_waves(int head_dim) { return head_dim == 64 ? 16 : head_dim == 128 ? 12 : 8; }
-constexpr int kAloneTurns = 5, kAloneCols = 64;
+constexpr int short_waves(int head_dim) { return head_dim == 64 ? 16 : head_dim == 128 ? 12 : 8; }
+constexpr int kFewWaves = 4, kFewNodes = 64;
 
 TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, int max_pages) {
   TreePlan p;
   const int cols = nodes * (heads / kv_heads);
   const int64_t tiles = ((int64_t)max_pages + 1) / 2, units = (int64_t)rows * kv_heads;
-  const int64_t cus = compute_units();
-  int64_t per_cu, most;                      // blocks of a compute unit, splits that have work
-  if (cols <= kAloneCols && nodes <= 64 && tiles <= kAloneTurns * alone_waves(head_dim) &&
-      units * ((cols + 15) / 16) <= cus) {
+  const int64_t cus = compute_units(), mtiles = (cols + 15) / 16, wide = short_waves(head_dim);
+  // blocks a row head and 16 columns have to have for one tile a wave
+  const int64_t turns = std::min<int64_t>((tiles + wide - 1) / wide, kMaxSplits);
+  const int64_t by_four = std::min<int64_t>(cus / std::max<int64_t>(units, 1), kMaxSplits) * kFewWaves;
+  int64_t per_cu = 1, most;                  // blocks of a compute unit, splits that have work
+  if (cols <= 128 && nodes <= kFewNodes && units * mtiles * turns <= cus &&
+      (cols > 16 || turns == 1 || tiles > by_four)) {
     p.nq = 1;
-    p.waves = alone_waves(head_dim);
+    p.waves = (int)wide;
     p.cols = 16;
-    per_cu = most = 1;
-  } else if (cols <= 16 || (cols <= 32 && head_dim <= 128)) {
+    most = turns == 2 && cols > 16 ? 1 : turns;
+  } else if (cols <= 16 || (cols <= 64 && head_dim <= 128)) {
     p.nq = cols <= 16 ? 1 : 2;
-    p.waves = 4;
+    p.waves = kFewWaves;
     p.cols = 16 * p.nq;
-    per_cu = head_dim * p.nq <= 64 ? 4 : head_dim * p.nq <= 128 ? 3 : 2;
     most = (tiles + p.waves - 1) / p.waves;
   } else {
-    const int wave_cols = 16 * kManyNq;
+    const bool four = cols <= 4 * 16 * kManyNq && (head_dim == 64 || (head_dim == 128 && units > cus));
     p.nq = 0;
-    p.waves = cols <= 4 * wave_cols && head_dim <= 128 ? 4 : 8;
-    p.cols = p.waves * wave_cols;
+    p.waves = four ? 4 : 8;
+    p.cols = p.waves * 16 * kManyNq;
     per_cu = 8 / p.waves;
     most = (tiles + 7) / 8;
   }
   p.mtiles = (cols + p.cols - 1) / p.cols;
-  const int64_t want = per_cu * cus / (units * p.mtiles > 0 ? units * p.mtiles : 1);
-  int64_t splits = want < most ? want : most;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  p.splits = splits < 1 ? 1 : (int)splits;
+  const int64_t want = per_cu * cus / std::max<int64_t>(units * p.mtiles, 1);
+  p.splits = (int)std::max<int64_t>(std::min({want, most, (int64_t)kMaxSplits}), 1);
   return p;
 }
 
@@ -1011,10 +1029,10 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
   TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D, W>()), blocks, W * kWave, a, p.splits, p.mtiles, po, pml)
 #define TFD_TREE_DIM(D)                                                                       \
   {                                                                                           \
-    if (p.nq == 1 && p.waves == 4) TFD_TREE_FEW(D, 1, 4)                                      \
-    else if (p.nq == 1) TFD_TREE_FEW(D, 1, alone_waves(D))                                    \
+    if (p.nq == 1 && p.waves == kFewWaves) TFD_TREE_FEW(D, 1, kFewWaves)                      \
+    else if (p.nq == 1) TFD_TREE_FEW(D, 1, short_waves(D))                                    \
     else if (p.nq == 2) {                                                                     \
-      if constexpr (D <= 128) TFD_TREE_FEW(D, 2, 4)                                           \
+      if constexpr (D <= 128) TFD_TREE_FEW(D, 2, kFewWaves)                                   \
     } else if (p.waves == 4) {                                                                \
       if constexpr (D <= 128) TFD_TREE_MANY(D, 4)                                             \
     } else TFD_TREE_MANY(D, 8)                                                                \
