@@ -128,18 +128,15 @@ int tfd_beam_select(const TfdBeamArgs* args, void* stream);
  * parents[r] was.  Groups of `beams` rows (<= 64); a parent lies in its row's group (another one
  * raises TFD_ERR_ROW_RANGE and leaves the row as it is).  `states`: a device array; first_block
  * = the running sum of tfd_state_blocks of the tensors before, `blocks` the sum of all (below
- * 2^24).  `pieces`: how many 4 KiB of a row a block takes one after another (fewer of tensors
- * whose rows are no multiples of 16 bytes): 1 for small states, 4 where there are blocks
- * enough all the same. */
+ * 2^24; a block takes 4 KiB of a row, fewer of tensors whose rows are no multiples of 16 bytes). */
 typedef struct {
   void* base;         /* [rows][row_bytes] */
   int64_t row_bytes;
   int64_t first_block;
 } TfdState;
-int64_t tfd_state_blocks(const void* base, int64_t row_bytes, int pieces);
-int tfd_reorder_states(const TfdState* states, int n, int pieces, int64_t blocks,
-                       const int32_t* parents, int groups, int beams, int32_t* err,
-                       void* stream);
+int64_t tfd_state_blocks(const void* base, int64_t row_bytes);
+int tfd_reorder_states(const TfdState* states, int n, int64_t blocks, const int32_t* parents,
+                       int groups, int beams, int32_t* err, void* stream);
 
 /* ---- pages -------------------------------------------------------------------------- */
 #define TFD_PAGES_MAX_ROWS 1024

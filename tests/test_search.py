@@ -254,12 +254,12 @@ def test_beam_work_and_empty_calls():
     L = lib()
     assert L.tfd_beam_work_bytes(2, 4, 100) > 0 and L.tfd_beam_work_bytes(2, 65, 100) == 0
     assert L.tfd_beam_select(ctypes.addressof(_beam_args(groups=0)), 0) == 0
-    assert L.tfd_reorder_states(PTR, 0, 1, 0, PTR, 1, 4, 0, 0) == 0
-    assert L.tfd_state_blocks(PTR, 4096, 1) == 1 and L.tfd_state_blocks(PTR, 4097, 1) == 5
-    assert L.tfd_state_blocks(PTR, 4097, 4) == 2 and L.tfd_state_blocks(PTR, 0, 1) == 0
-    for bad in [(PTR, -1, 1, 0, PTR, 1, 4), (PTR, 1, 1, 1, PTR, 1, 65), (PTR, 1, 1, 1, PTR, 1, 0),
-                (PTR, 1, 1, 1 << 24, PTR, 1, 4), (0, 1, 1, 1, PTR, 1, 4),
-                (PTR, 1, 1, 1, 0, 1, 4), (PTR, 1, 0, 1, PTR, 1, 4)]:
+    assert L.tfd_reorder_states(PTR, 0, 0, PTR, 1, 4, 0, 0) == 0
+    assert L.tfd_state_blocks(PTR, 4096) == 1 and L.tfd_state_blocks(PTR, 4097) == 5
+    assert L.tfd_state_blocks(PTR, 0) == 0
+    for bad in [(PTR, -1, 0, PTR, 1, 4), (PTR, 1, 1, PTR, 1, 65), (PTR, 1, 1, PTR, 1, 0),
+                (PTR, 1, 1 << 24, PTR, 1, 4), (0, 1, 1, PTR, 1, 4),
+                (PTR, 1, 1, 0, 1, 4)]:
         with pytest.raises(TFDError):
             L.tfd_reorder_states(*bad, 0, 0)
 

@@ -176,8 +176,8 @@ SIGNATURES: dict[str, list] = {
     "tfd_tree_attn": [P, P],
     "tfd_beam_work_bytes": [I, I, I],
     "tfd_beam_select": [P, P],
-    "tfd_state_blocks": [P, L, I],
-    "tfd_reorder_states": [P, I, I, L, P, I, I, P, P],
+    "tfd_state_blocks": [P, L],
+    "tfd_reorder_states": [P, I, L, P, I, I, P, P],
     "tfd_pages_fork": [P, P, P, P, P, P],
     "tfd_pages_take": [P, P, P, I, P],
     "tfd_pages_copy": [P, P, P, I, P],

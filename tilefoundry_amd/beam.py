@@ -137,12 +137,10 @@ class States:
             raise ValueError(f"States: up to {MAX_GROUPS} groups, got {self.rows // self.beams}")
         L, blocks, entries = lib(), 0, []
         sizes = [t.numel() // self.rows * t.element_size() for t in self.tensors]
-        # blocks of 4 KiB of a row, or of 16 where that leaves 1,024 of them
-        self.pieces = 4 if sum(sizes) * (self.rows // self.beams) >= 1 << 24 else 1
         for t, size in zip(self.tensors, sizes):
             if size:
                 entries.append(_lib.TfdState(ptr(t), size, blocks))
-                blocks += L.tfd_state_blocks(ptr(t), size, self.pieces)
+                blocks += L.tfd_state_blocks(ptr(t), size)
         if blocks >= 1 << 24:
             raise ValueError("States: rows of up to 64 GiB in all")
         self.blocks, self.n = blocks, len(entries)
@@ -163,8 +161,8 @@ class States:
         if parents.get_device() != self.index:
             raise ValueError(f"States: parents on {parents.device}, tensors on {self.device}")
         parents = parents.contiguous()
-        launch(self.index, lib().tfd_reorder_states, ptr(self._entries), self.n, self.pieces,
-               self.blocks, ptr(parents), self.rows // self.beams, self.beams, ptr(self.err))
+        launch(self.index, lib().tfd_reorder_states, ptr(self._entries), self.n, self.blocks,
+               ptr(parents), self.rows // self.beams, self.beams, ptr(self.err))
 
     def check_errors(self) -> None:
         """Raises if a call since the last check met a parent outside its row's group (waits

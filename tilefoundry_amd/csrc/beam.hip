@@ -126,11 +126,11 @@ struct BeamPlan {
 
 // What a wave holds of its chunk's candidates: values by fours (each four consecutive tokens)
 // in which one reaches the bound, and those that do.
-constexpr int kFours = 64, kAtOnce = 8;
+constexpr int kFours = 128, kNear = 128, kAtOnce = 8;
 typedef float f4 __attribute__((ext_vector_type(4)));
 struct alignas(16) Near {
   float x[4 * kFours];
-  uint64_t near[4 * kFours + kAtOnce];
+  uint64_t near[kNear + kAtOnce];
   int token[kFours];
 };
 // Up to so many beams the bound comes from the lanes' best values: that leaves
@@ -275,14 +275,15 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
   };
   wrote();
   uint64_t* const list = lists + (int64_t)w * K;
-  if (fours <= kFours) {
-    int n = 0;
-    for (int i = lane; i - lane < 4 * fours; i += kWave) {
-      const float v = i < 4 * fours ? mine_s.x[i] : -kInf;
-      const uint64_t who = __ballot(v >= bound);
-      if (v >= bound) mine_s.near[placed_at(who, n)] = key_of(v, mine_s.token[i / 4] + i % 4);
-      n += __popcll(who);
-    }
+  int n = fours <= kFours ? 0 : kNear + 1;
+  for (int i = lane; n <= kNear && i - lane < 4 * fours; i += kWave) {
+    const float v = i < 4 * fours ? mine_s.x[i] : -kInf;
+    const uint64_t who = __ballot(v >= bound);
+    const int place = placed_at(who, n);
+    if (v >= bound && place < kNear) mine_s.near[place] = key_of(v, mine_s.token[i / 4] + i % 4);
+    n += __popcll(who);
+  }
+  if (n <= kNear) {
     if (lane < kAtOnce) mine_s.near[n + lane] = 0;
     wrote();
     for (int i = lane; i < n; i += kWave) {
@@ -319,12 +320,14 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
 // ---------------------------------------------------------------------------
 // A block per group.  Candidates in order: rank, then the lower row, then the key.  A wave's
 // beams-th best list head bounds the group's beams-th best candidate from below; what reaches
-// the largest such bound is collected and ranked by counting.  If more does than the buffer
-// holds (thousands of equal ranks), the places are filled one by one instead.  A thread holds
-// the first keys of a list from the start on, so that few loads wait for others.
+// the largest such bound is collected and ranked by counting by one wave, after another bound
+// where there are many.  If more does than the buffer holds (thousands of equal ranks), the
+// places are filled one by one instead.  A thread holds the first keys of a list from the start
+// on, so that few loads wait for others.  Bound by latency: 6.5 us for 4 beams of 151,936 logits
+// (4.5 of them until the lists, which other dies wrote, have come), 11.6 for 16 of 16.
 // ---------------------------------------------------------------------------
 constexpr int kMerge = 1024, kMergeWaves = kMerge / kWave, kFound = 2048;
-constexpr int kHeldKeys = 4, kHeldSums = 3, kHeads = 256, kFewHeads = 32;
+constexpr int kHeldKeys = 4, kHeldSums = 3, kFewHeads = 32;
 
 struct Cand {
   double rank;
@@ -347,9 +350,10 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   __shared__ double found_rank[kFound];
   __shared__ uint64_t found_key[kFound];
   __shared__ uint8_t found_beam[kFound];
-  __shared__ uint32_t head_s[kHeads];
+  __shared__ uint32_t head_s[kMerge];
   __shared__ Cand wave_s[kMergeWaves];
   __shared__ int n_s, heads_s;
+  __shared__ float least_s;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int K = a.beams, row0 = blockIdx.x * K, n_lists = K * chunks;
@@ -432,18 +436,25 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     int at = 0;
     if (lane == 0) at = atomicAdd(&heads_s, __popcll(reach));
     at = placed_at(reach, __builtin_amdgcn_readfirstlane(at));
-    if (head >= max(top, 1u) && at < kHeads) head_s[at] = head;
+    if (head >= max(top, 1u)) head_s[at] = head;
   }
   __syncthreads();
   const int heads = heads_s;
-  if (heads > kFewHeads && heads <= kWave) {
-    top = max(top, kth_largest<1>({lane < heads ? head_s[lane] : 0u}, K));
-  } else if (heads > kWave && heads <= kHeads) {
-    uint32_t v[kHeads / kWave];
+  auto again = [&](auto& v) {
 #pragma unroll
-    for (int i = 0; i < kHeads / kWave; ++i)
+    for (int i = 0; i < (int)(sizeof(v) / 4); ++i)
       v[i] = lane + i * kWave < heads ? head_s[lane + i * kWave] : 0u;
     top = max(top, kth_largest(v, K));
+  };
+  if (heads > 4 * kWave) {
+    uint32_t v[kMergeWaves];
+    again(v);
+  } else if (heads > kWave) {
+    uint32_t v[4];
+    again(v);
+  } else if (heads > kFewHeads) {
+    uint32_t v[1];
+    again(v);
   }
   const double bound = top ? (double)float_of(top) : kNone;
   auto collect = [&](const Cand& c) {
@@ -452,9 +463,16 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     if (at < kFound) found_rank[at] = c.rank, found_key[at] = c.key, found_beam[at] = c.beam;
     return true;
   };
-  auto walk = [&](int l, int from) {
-    for (int i = from; i < K; ++i)
-      if (!collect(cand(l, i))) break;
+  auto walk = [&](int l, int from) {         // kHeldKeys at a time: each load would be waited for
+    bool more = true;
+    for (int i0 = from; more && i0 < K; i0 += kHeldKeys) {
+      uint64_t keys[kHeldKeys];
+#pragma unroll
+      for (int i = 0; i < kHeldKeys; ++i) keys[i] = mine[(int64_t)l * K + min(i0 + i, K - 1)];
+#pragma unroll
+      for (int i = 0; i < kHeldKeys; ++i)
+        if (more && i0 + i < K) more = collect(with_key(l, i0 + i, keys[i]));
+    }
   };
   if (tid < n_lists) {
     bool more = true;
@@ -465,7 +483,7 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   }
   for (int l = tid + kMerge; l < n_lists; l += kMerge) walk(l, 0);
   __syncthreads();
-  const int n = n_s;
+  int n = n_s;
   auto put = [&](int place, const Cand& c) {
     const int row = row0 + c.beam, at = row0 + place;
     const bool over = done_s[c.beam];
@@ -484,6 +502,49 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     a.lengths_out[at] = length_s[place];
     a.done_out[at] = done_s[place];
   };
+  // many (a row far ahead of the others, whose lists' first keys are fewer than the beams): the
+  // beams-th best of them bounds them again, and what reaches that moves to the front
+  if (n > kWave && n <= kFound) {
+    if (wave == 0) {
+      auto bounded = [&](auto& v) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(v) / 4); ++i) {
+          const int j = lane + i * kWave;
+          v[i] = j < n ? order_of(__double2float_rd(found_rank[j])) : 0u;
+        }
+        least_s = float_of(kth_largest(v, K));
+      };
+      if (n <= 4 * kWave) {
+        uint32_t v[4];
+        bounded(v);
+      } else if (n <= 16 * kWave) {
+        uint32_t v[16];
+        bounded(v);
+      } else {
+        uint32_t v[kFound / kWave];
+        bounded(v);
+      }
+    }
+    __syncthreads();
+    const double least = (double)least_s;
+    Cand kept[kFound / kMerge];
+#pragma unroll
+    for (int i = 0; i < kFound / kMerge; ++i) {
+      const int j = min(tid + i * kMerge, n - 1);
+      kept[i] = Cand{found_rank[j], found_key[j], found_beam[j]};
+      if (tid + i * kMerge >= n || kept[i].rank < least) kept[i].key = 0;
+    }
+    if (tid == 0) n_s = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kFound / kMerge; ++i) {
+      if (!kept[i].key) continue;
+      const int at = atomicAdd(&n_s, 1);
+      found_rank[at] = kept[i].rank, found_key[at] = kept[i].key, found_beam[at] = kept[i].beam;
+    }
+    __syncthreads();
+    n = n_s;
+  }
   if (n <= kWave) {                          // a candidate per lane of one wave
     if (wave > 0) return;
     const Cand c = lane < n ? Cand{found_rank[lane], found_key[lane], found_beam[lane]} : Cand{};
@@ -534,13 +595,16 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
 }
 
 // Chunks as long as leave some waves for every compute unit and, for a group, no more lists
-// than the merging block has threads; longer where there are many waves all the same.
+// than the merging block has threads; longer where there are many waves all the same.  The scan
+// takes the same either way (8 beams of 4 groups over 248,320 f32 logits 10.9 us by 32 values a
+// lane, 11.0 by 64; 16 of 16 over 100,352 in bf16 20.4 and 20.5, 15 of them as its loads take), the
+// merge gains by fewer lists (11.7 and 10.9; 14.7 and 12.9).
 BeamPlan beam_plan(int rows, int beams, int vocab) {
   BeamPlan p;
   p.per = 8;
   auto chunks = [&] { return (vocab + kWave * p.per - 1) / (kWave * p.per); };
   while (p.per < 32 && ((int64_t)rows * chunks() > 2048 || beams * chunks() > kMerge)) p.per *= 2;
-  if (p.per == 32 && (int64_t)rows * chunks() > 8192) p.per = 64;
+  if (p.per == 32 && ((int64_t)rows * chunks() > 8192 || beams * chunks() > kMerge)) p.per = 64;
   p.chunks = chunks();
   return p;
 }
@@ -556,8 +620,9 @@ bool beam_shape(int groups, int beams, int vocab) {
 // another one becomes before it writes any, so nothing has to be kept twice.  Rows that stay
 // are neither read (but by others) nor written.  A wave knows the moves by itself -- lane b
 // holds row b's parent, a 64-bit mask the rows that move -- and finds its tensor by a
-// ballot, so nothing waits for a barrier; of the pieces that a block takes one after
-// another, the next one's loads are in flight behind the current one's stores.
+// ballot, so nothing waits for a barrier.  Bound by memory: 8 rows in groups of 4 of 30 states of
+// 2 MiB, 5 of them moved, 109 us; a block that took four pieces in turn, the next one's loads
+// behind the stores of the last, 127.
 // ---------------------------------------------------------------------------
 constexpr int kUnits = 4;                    // small units per thread
 
@@ -588,33 +653,19 @@ __device__ __forceinline__ void each_move(T (&v)[kMoves][kN], T* p, int64_t unit
 
 template <typename T, int kN, int kMoves>
 __device__ __forceinline__ void move_rows(uint8_t* base, int64_t row_bytes, int64_t block,
-                                          int pieces, uint64_t moved, int from) {
-  constexpr int kBuffers = kMoves <= 16 ? 2 : 1;
+                                          uint64_t moved, int from) {
   const int64_t units = row_bytes / (int64_t)sizeof(T);
+  const int64_t u = block * (kBlock * kN) + threadIdx.x;
   T* const p = reinterpret_cast<T*>(base);
-  int64_t u = block * pieces * (kBlock * kN) + threadIdx.x;
-  T v[kBuffers][kMoves][kN];
-  each_move<T, kN, kMoves, false>(v[0], p, units, u, moved, from);
-#pragma unroll 1
-  for (int i = 0; i < pieces; i += kBuffers) {
-#pragma unroll
-    for (int b = 0; b < kBuffers; ++b) {
-      const int64_t next = u + kBlock * kN;
-      const bool more = i + b + 1 < pieces && next - (int)threadIdx.x < units;
-      if (kBuffers > 1 && more)
-        each_move<T, kN, kMoves, false>(v[(b + 1) % kBuffers], p, units, next, moved, from);
-      each_move<T, kN, kMoves, true>(v[b], p, units, u, moved, from);
-      if (!more) return;
-      if (kBuffers == 1) each_move<T, kN, kMoves, false>(v[0], p, units, next, moved, from);
-      u = next;
-    }
-  }
+  T v[kMoves][kN];
+  each_move<T, kN, kMoves, false>(v, p, units, u, moved, from);
+  each_move<T, kN, kMoves, true>(v, p, units, u, moved, from);
 }
 
 template <int kMoves>
-__global__ __launch_bounds__(kBlock) void k_reorder(const TfdState* __restrict__ states, int n,
-                                                    int pieces, const int* __restrict__ parents,
-                                                    int beams, int* err) {
+__global__ __launch_bounds__(kBlock, kMoves <= 4 ? 8 : kMoves <= 16 ? 5 : 1) void k_reorder(const TfdState* __restrict__ states, int n,
+                                                    const int* __restrict__ parents, int beams,
+                                                    int* err) {
   const int lane = threadIdx.x & (kWave - 1), first = blockIdx.y * beams;
   int from = lane;
   if (lane < beams) from = parents[first + lane] - first;
@@ -632,13 +683,13 @@ __global__ __launch_bounds__(kBlock) void k_reorder(const TfdState* __restrict__
   const int64_t at = block - st.first_block;
   uint8_t* const base = (uint8_t*)st.base + first * st.row_bytes;
   const int unit = state_unit(st.base, st.row_bytes);
-  if (unit == 16) move_rows<u32x4, 1, kMoves>(base, st.row_bytes, at, pieces, moved, from);
+  if (unit == 16) move_rows<u32x4, 1, kMoves>(base, st.row_bytes, at, moved, from);
   else if (unit == 4)
-    move_rows<uint32_t, kUnits, kMoves>(base, st.row_bytes, at, pieces, moved, from);
+    move_rows<uint32_t, kUnits, kMoves>(base, st.row_bytes, at, moved, from);
   else if (unit == 2)
-    move_rows<uint16_t, kUnits, kMoves>(base, st.row_bytes, at, pieces, moved, from);
+    move_rows<uint16_t, kUnits, kMoves>(base, st.row_bytes, at, moved, from);
   else
-    move_rows<uint8_t, kUnits, kMoves>(base, st.row_bytes, at, pieces, moved, from);
+    move_rows<uint8_t, kUnits, kMoves>(base, st.row_bytes, at, moved, from);
 }
 
 }  // namespace
@@ -700,27 +751,25 @@ int tfd_beam_select(const TfdBeamArgs* args, void* stream) {
   return launched("beam_select");
 }
 
-int64_t tfd_state_blocks(const void* base, int64_t row_bytes, int pieces) {
-  if (row_bytes <= 0 || pieces < 1) return 0;
+int64_t tfd_state_blocks(const void* base, int64_t row_bytes) {
+  if (row_bytes <= 0) return 0;
   const int unit = state_unit(base, row_bytes);
-  const int64_t per = (int64_t)kBlock * pieces * (unit == 16 ? 16 : kUnits * unit);
+  const int64_t per = (int64_t)kBlock * (unit == 16 ? 16 : kUnits * unit);
   return (row_bytes + per - 1) / per;
 }
 
-int tfd_reorder_states(const TfdState* states, int n, int pieces, int64_t blocks,
-                       const int32_t* parents, int groups, int beams, int32_t* err,
-                       void* stream) {
-  if (n < 0 || pieces < 1 || groups < 0 || groups > 65535 || beams < 1 || beams > kMaxBeams ||
-      blocks < 0 || blocks >= (1ll << 24))
-    return fail(kBadShape, "reorder_states: n=%d pieces=%d groups=%d beams=%d (1..%d) blocks=%lld",
-                n, pieces, groups, beams, kMaxBeams, (long long)blocks);
+int tfd_reorder_states(const TfdState* states, int n, int64_t blocks, const int32_t* parents,
+                       int groups, int beams, int32_t* err, void* stream) {
+  if (n < 0 || groups < 0 || groups > 65535 || beams < 1 || beams > kMaxBeams || blocks < 0 ||
+      blocks >= (1ll << 24))
+    return fail(kBadShape, "reorder_states: n=%d groups=%d beams=%d (1..%d) blocks=%lld", n, groups,
+                beams, kMaxBeams, (long long)blocks);
   if (n == 0 || groups == 0 || blocks == 0) return 0;
   if (!states || !parents) return fail(kBadArg, "reorder_states: null pointer");
   const dim3 grid((unsigned)blocks, groups);
   auto s = (hipStream_t)stream;
-#define TFD_MOVES(M) k_reorder<M><<<grid, kBlock, 0, s>>>(states, n, pieces, parents, beams, err)
+#define TFD_MOVES(M) k_reorder<M><<<grid, kBlock, 0, s>>>(states, n, parents, beams, err)
   if (beams <= 4) TFD_MOVES(4);
-  else if (beams <= 8) TFD_MOVES(8);
   else if (beams <= 16) TFD_MOVES(16);
   else if (beams <= 32) TFD_MOVES(32);
   else TFD_MOVES(64);
