@@ -99,6 +99,49 @@ def test_beam_masks_infinities_and_nan(gpu_device):
     _check(gpu_device, Beam(K, eos=4), x, s, lengths, done)
 
 
+@pytest.mark.parametrize("groups,beams,vocab,dtype", [
+    (1, 64, 151936, BF), (2, 64, 40000, F32), (4, 32, 100352, F32), (3, 16, 100352, BF),
+    (2, 24, 20000, F16), (2, 25, 20000, F16)])
+def test_beam_rows_that_offer_much(gpu_device, groups, beams, vocab, dtype):
+    """Many beams; one row far ahead, whose lists hold more candidates than there are lists; all
+    rows alike but for their logits."""
+    x, s, _ = _draw(vocab - beams, groups, beams, vocab, dtype)
+    _check(gpu_device, Beam(beams), x, s)
+    s[:, beams // 2] += 30
+    _check(gpu_device, Beam(beams), x, s)
+    s[:] = -1.5
+    _check(gpu_device, Beam(beams), x, s)
+
+
+@pytest.mark.parametrize("beams", [4, 16, 64])
+def test_beam_thousands_of_equal_logits(gpu_device, beams):
+    x = torch.zeros(beams, 30000)
+    s = -torch.arange(float(beams)).view(1, beams)
+    _check(gpu_device, Beam(beams), x, s)            # a row's lowest tokens first
+    x[:] = -3e38                                     # masked but for three tokens a row
+    x[:, [17, 9000, 29999]] = torch.tensor([1.0, 2.0, 0.5])
+    s = s * 0.25
+    # Rows r and r + 2 differ by the half that logits 1.0 and 0.5 do: their candidates are equal
+    # in exact arithmetic (-r / 4 + 0.5 = -(r + 2) / 4 + 1.0), and which of two such is
+    # larger in 64 bits hangs on where the sum with lse was rounded (2^-53).  Their order is
+    # left open; values, the candidates' own values and that each comes once are not.
+    got = Beam(beams)(x.to(gpu_device), s.to(gpu_device))
+    want = R.beam(x, s, None, None)[2]
+    assert ((got.scores.cpu().double() - want).abs() <= want.abs() * 2.0 ** -24 + 2.0 ** -22).all()
+    p, t = got.parents.cpu()[0].long(), got.tokens.cpu()[0].long()
+    own = s[0, p].double() + torch.log_softmax(x.double(), 1)[p, t]
+    assert ((own - want[0]).abs() <= 2.0 ** -40).all()
+    assert len(set(zip(p.tolist(), t.tolist()))) == beams
+
+
+@pytest.mark.parametrize("scale", [1e4, 9e5, 3e6, 1e30])
+def test_beam_large_logits(gpu_device, scale):
+    """A reference whose product with log2 e is rounded by as much as the differences are."""
+    x, s, _ = _draw(8, 2, 4, 9001)
+    _check(gpu_device, Beam(4), x + scale, s)
+    _check(gpu_device, Beam(4), x - scale, s)
+
+
 def test_beam_adversarial_places(gpu_device):
     """The best logits side by side, all in one thread's or one chunk's values."""
     for at in (0, 4, 1021, 9000):

@@ -144,6 +144,13 @@ def test_speculation_gives_the_greedy_tokens(gpu_device, weights, nodes):
     assert e.generate(prompts, 30, prefill=True).tokens == want
 
 
+def test_speculation_with_room_for_many_nodes(gpu_device, weights):
+    prompts = [_prompt(n, SMALL.vocab_size, seed=40 + n) for n in (16, 3, 33)]
+    e = _engine(weights, gpu_device, 3)
+    want = e.generate(prompts, 30, prefill=True).tokens
+    assert e.speculate(prompts, 30, nodes=200, draft=_Known(prompts, want, True)).tokens == want
+
+
 def _same_to_a_near_tie(want, logits, got):
     assert len(want) == len(got)
     differ = [i for i, (a, b) in enumerate(zip(want, got)) if a != b]
@@ -215,5 +222,7 @@ def test_searches_refuse(gpu_device, weights):
              "before it")):
         with pytest.raises(ValueError, match=match):
             call()
+    with pytest.raises(ValueError, match="pass"):
+        _engine(weights, gpu_device, 17).speculate([p] * 17, 4, nodes=256)
     with pytest.raises(ValueError, match="greedy"):
         _engine(weights, gpu_device, 1, sampling=Sampling(top_k=4)).speculate([p], 4)

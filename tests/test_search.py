@@ -264,6 +264,17 @@ def test_beam_work_and_empty_calls():
             L.tfd_reorder_states(*bad, 0, 0)
 
 
+@pytest.mark.parametrize("at,value", [(0, 0), (1, 0), (2, -1), (3, 3), (4, 0), (5, 100), (6, 0),
+                                      (11, 0), (12, 0), (13, 0), (14, 0), (15, 0), (16, 0),
+                                      (18, 0), (21, 0)])
+def test_tree_qkv_append_refuses(at, value):
+    args = [PTR, 1, 4, 4, 2, 64, PTR, PTR, PTR, PTR, 64, PTR, PTR, PTR, PTR, 4, PTR, PTR, 8, 1.0,
+            1e-6, PTR, 0, 0]
+    args[at] = value
+    with pytest.raises(TFDError):
+        lib().tfd_tree_qkv_append(*args)
+
+
 def test_tree_entries_refuse():
     L = lib()
     assert L.tfd_tree_masks(0, 0, 0, 5, 0, 0, 0, 0) == 0

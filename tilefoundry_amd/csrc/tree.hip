@@ -118,21 +118,25 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // transposing read gives V^T's operands; its 32-byte pieces are permuted by the row so that the
 // 16 rows of such a read take the fewest cycles.
 //
-// Softmax against a running reference, in f32.  The
-// probabilities have to become bf16 for the second product.
-// By few columns, which wait for keys, they stay a sum of two bf16 (2^-16 of each).  By many they
-// are one bf16: the second product of a second half costs a seventh to a third of the call (253
-// to 180 us at 2 rows of 32,760 positions, 64 nodes of 16 heads over 8), and what it buys is
-// small beside the output's own rounding (2^-8 of a probability, and they average: 1.4 times the
-// error of an attention in f32 that rounds its output, against 1.0).
+// Softmax against a running reference, in f32.  The probabilities have to become bf16 for the
+// second product.  By few columns, which wait for keys, they stay a sum of two bf16 (2^-16 of
+// each).  By many they are one bf16: the product with a second half costs a fifth to a third of
+// the call (220 to 173 us at 4 rows to 30,000 positions, 61 nodes of 32 heads over 8), and
+// what it buys is small beside the output's own rounding (2^-8 of a probability, and they
+// average: 1.4 times the error of an attention in f32 that rounds its output).
 //
 // Two kernels.  Few columns (k_tree_few): the keys are what is waited for, so each wave
 // takes other tiles of 32 positions, its K straight into registers as operands and its V
 // through a private piece of LDS, and no barrier until the waves' sums are joined.  Many
 // columns (k_tree_many): the waves take 16 NQ columns each and share tiles in LDS, loaded
 // straight to it three tiles ahead (from pages anywhere a load takes some 3 us), one barrier a
-// tile.  Both may cut a row's positions into
-// splits, which k_tree_join adds.
+// tile.  Both may cut a row's positions into splits, which k_tree_join adds.
+//
+// Few columns are bound by memory (32 rows to 4,096 positions by 7 nodes: 93 us, 5.5 TB/s) or, by
+// one row, by latency (700 positions: 14 us).  Many: MFMA (35% of the time at 61 nodes of 32
+// heads), LDS, VALU and loads take turns, since registers leave room for two waves a SIMD (159 us,
+// 756 TFLOP/s); of 256 dims (8 rows to 5,003, 23 nodes of 16 heads over 2: 42 us) also by the
+// partial sums of its splits, which the join reads again (10 us).
 // ---------------------------------------------------------------------------
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 32;                    // positions of a wave's tile

@@ -26,7 +26,7 @@ from .. import _lib, tree
 from .._lib import ptr
 from ..beam import Beam, States
 from ..pages import Pages
-from .prefill import Prefill, in_vocab, token_array
+from .prefill import MAX_PASS, Prefill, in_vocab, token_array
 
 I32 = torch.int32
 
@@ -287,6 +287,8 @@ class Speculation:
         e = engine()
         if not 1 <= nodes <= tree.MAX_NODES:
             raise ValueError(f"nodes must lie in 1..{tree.MAX_NODES}, got {nodes}")
+        if e.B * nodes > MAX_PASS:
+            raise ValueError(f"{nodes} nodes of {e.B} sequences exceed a pass of {MAX_PASS} rows")
         self._engine, self.nodes = engine, nodes
         self.step = TreePass(engine, nodes)
         self.cache = Pages([e.kpool, e.vpool], table=e.page_table)
