@@ -52,9 +52,10 @@ int tfd_tree_qkv_append(const float* part, int slices, int M, int heads, int kv_
  *   out = sum_j softmax_j(scale q . k_j) v_j,
  * scores and sums in f32, one rounding of the output.  The probabilities, a product's operands,
  * are sums of two bf16 (2^-16 of each) where few columns, nodes x heads / kv_heads, share a kv
- * head, and one bf16 (2^-8) where tfd_tree_attn_form says many.  A node that sees nothing gets zeros.  What a node does not see takes no part,
- * values that are not finite included.  q bf16, rows / nodes / heads q_row / q_node / q_head
- * elements apart (multiples of 8, 16-byte aligned).  out: [rows][nodes][heads][head_dim], or
+ * head, and one bf16 (2^-8) where tfd_tree_attn_form says many.  A node that sees nothing gets
+ * zeros.  What a node does not see takes no part, values that are not finite included.  q bf16,
+ * rows / nodes / heads q_row / q_node / q_head elements apart (multiples of 8; q, the pools and
+ * out 16-byte aligned).  out: [rows][nodes][heads][head_dim], or
  * with out_panel the rows x nodes rows of tf_decode.h's panel order.  Nodes from counts[b] on
  * are not written.  head_dim 64, 128 or 256; heads a multiple of kv_heads; nodes <= 256; up to
  * 2^26 positions a row.  work: tfd_tree_attn_work_bytes, 16-byte aligned, contents free, one
@@ -148,8 +149,8 @@ typedef struct {
   int32_t heads, row_bytes;
 } TfdPool;
 /* A cache's pages: table int32 [rows][max_pages], -1 for no page, and refs int32 [num_pages],
- * the table entries that name a page (0: free).  scratch: int32 [TFD_PAGES_SCRATCH], zero before the
- * first call and left ready by each.  Calls on one cache are stream-ordered. */
+ * the table entries that name a page (0: free).  scratch: int32 [TFD_PAGES_SCRATCH], zero before
+ * the first call and left ready by each.  Calls on one cache are stream-ordered. */
 #define TFD_PAGES_SCRATCH(rows, max_pages, num_pages) \
   (3 * (int64_t)(num_pages) + (int64_t)(rows) * (max_pages) + 2 * (int64_t)(rows) + 16)
 typedef struct {

@@ -101,7 +101,7 @@ def test_beam_masks_infinities_and_nan(gpu_device):
 
 @pytest.mark.parametrize("groups,beams,vocab,dtype", [
     (1, 64, 151936, BF), (2, 64, 40000, F32), (4, 32, 100352, F32), (3, 16, 100352, BF),
-    (2, 24, 20000, F16), (2, 25, 20000, F16)])
+    (2, 24, 20000, F16), (2, 25, 20000, F16), (1, 64, 40001, F32), (1, 64, 40001, BF)])
 def test_beam_rows_that_offer_much(gpu_device, groups, beams, vocab, dtype):
     """Many beams; one row far ahead, whose lists hold more candidates than there are lists; all
     rows alike but for their logits."""

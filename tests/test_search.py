@@ -215,7 +215,8 @@ def _tree_args(**kw):
     ({"num_pages": 0}, -2, "num_pages"), ({"rows": -1}, -2, "rows"),
     ({"scale": 0.0}, -1, "scale"), ({"scale": math.nan}, -1, "scale"), ({"q": 0}, -1, "null"),
     ({"out": 0}, -1, "null"), ({"q": PTR + 2}, -1, "aligned"), ({"q_head": 68}, -1, "aligned"),
-    ({"k_pool": PTR + 8}, -1, "aligned"), ({"max_pages": 4000}, -1, "work"),
+    ({"k_pool": PTR + 8}, -1, "aligned"), ({"out": PTR + 8}, -1, "aligned"),
+    ({"max_pages": 4000}, -1, "work"),
     ({"max_pages": 4000, "work": PTR, "work_bytes": 16}, -1, "work")])
 def test_tree_attn_entry_refuses(kw, code, match):
     _refused("tfd_tree_attn", _tree_args(**kw), code, match)

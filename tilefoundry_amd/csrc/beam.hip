@@ -134,8 +134,8 @@ struct alignas(16) Near {
   int token[kFours];
 };
 // Up to so many beams the bound comes from the lanes' best values: that leaves
-// 64 ln(64 / (64 - beams)) fours, 30 of 24 beams; above it from all fours' best, which leaves as many as
-// there are beams, for one ballot a four and bit.
+// 64 ln(64 / (64 - beams)) fours, 30 of 24 beams; above it from all fours' best, which leaves as
+// many as there are beams, for one ballot a four and bit.
 constexpr int kFewBeams = 24;
 
 // What a wave's chunk of a row leaves: its largest logit, the sum of exp(x - that), and its
@@ -161,9 +161,9 @@ __device__ __forceinline__ float logit_at(const void* p, int64_t i) {
 // logits), the places are filled one by one, from memory.
 // ---------------------------------------------------------------------------
 template <int kType, int kPer, bool kVec>
-__global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k_beam_scan(TfdBeamArgs a, int chunks, int waves,
-                                                      ChunkSum* __restrict__ sums,
-                                                      uint64_t* __restrict__ lists) {
+__global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8)
+void k_beam_scan(TfdBeamArgs a, int chunks, int waves, ChunkSum* __restrict__ sums,
+                 uint64_t* __restrict__ lists) {
   constexpr float kInf = __builtin_huge_valf();
   constexpr int kQuads = kPer / 4;
   __shared__ Near near_s[kWavesPerBlock];
@@ -202,8 +202,8 @@ __global__ __launch_bounds__(kBlock, kPer == 64 ? 4 : kPer == 32 ? 6 : 8) void k
       if (at(j) >= a.vocab) x[j] = -kInf;
     }
   }
-  // Largest of four, of the lane, of the wave, and the sum of 2^(x log2 e - c), c = m log2 e rounded:
-  // one fused multiply-add a value, and what c's rounding left out (exactly fma's remainder) is
+  // Largest of four, of the lane, of the wave, and the sum of 2^(x log2 e + c), c = -m log2 e
+  // rounded: one fused multiply-add a value, and what c's rounding left out (exactly fma's remainder) is
   // put right in the sum.  log2 e as one f32 is 1.3e-8 of x - m off: 1.1e-7 of a sum over
   // 4,096 equal values, half of an f32's last place at one, where the scores that go out
   // are themselves f32 of at least ln 4096.
@@ -663,9 +663,9 @@ __device__ __forceinline__ void move_rows(uint8_t* base, int64_t row_bytes, int6
 }
 
 template <int kMoves>
-__global__ __launch_bounds__(kBlock, kMoves <= 4 ? 8 : kMoves <= 16 ? 5 : 1) void k_reorder(const TfdState* __restrict__ states, int n,
-                                                    const int* __restrict__ parents, int beams,
-                                                    int* err) {
+__global__ __launch_bounds__(kBlock, kMoves <= 4 ? 8 : kMoves <= 16 ? 5 : 1)
+void k_reorder(const TfdState* __restrict__ states, int n, const int* __restrict__ parents,
+               int beams, int* err) {
   const int lane = threadIdx.x & (kWave - 1), first = blockIdx.y * beams;
   int from = lane;
   if (lane < beams) from = parents[first + lane] - first;

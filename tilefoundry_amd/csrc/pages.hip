@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kOne) void k_pages_take(TfdPages p, const int* __re
 // ---------------------------------------------------------------------------
 // Copies: a block takes 32 KiB of one page of one pool at a time, all its loads before its
 // stores; the blocks walk the items, whose number (of pairs) may lie on the device.  Bound by
-// memory: 3.2 GB in 310 us a half, 5.1 TB/s; a page of each of 8 rows 4.4 us.
+// memory: 1.6 GB in 310 us, 5.1 TB/s; a page of each of 8 rows 4.4 us.
 // ---------------------------------------------------------------------------
 constexpr int kCopyLoads = 8;
 constexpr int64_t kCopyBytes = kBlock * 16 * kCopyLoads;
@@ -287,8 +287,8 @@ __global__ __launch_bounds__(kBlock) void k_pages_keep(TfdPages p, const int* __
       raise_error(p.err, kErrPage);
       return nullptr;
     }
-    return (uint8_t*)t.base + page * t.page_bytes + ((int64_t)h * kPage + pos % kPage) * t.row_bytes +
-           c * 16;
+    return (uint8_t*)t.base + page * t.page_bytes +
+           ((int64_t)h * kPage + pos % kPage) * t.row_bytes + c * 16;
   };
   for (int i = tid; i < t.heads * per; i += kBlock) {
     const int h = i / per, c = i % per;

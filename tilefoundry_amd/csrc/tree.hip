@@ -270,8 +270,8 @@ __device__ __forceinline__ bool tree_row(const TfdTreeAttnArgs& a, int unit, int
 constexpr float kMaxRise = 8.f;
 
 template <int kN, int DT, int NQ>
-__device__ __forceinline__ float tree_maximum(const f32x4 (&st)[kN], float c2, float& mx, float& sum,
-                                              f32x4 (&o)[DT][NQ], int qt) {
+__device__ __forceinline__ float tree_maximum(const f32x4 (&st)[kN], float c2, float& mx,
+                                              float& sum, f32x4 (&o)[DT][NQ], int qt) {
   float tm = st[0][0];
 #pragma unroll
   for (int i = 1; i < 4 * kN; ++i) tm = fmaxf(tm, st[i / 4][i % 4]);
@@ -431,7 +431,8 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
   for (int qt = 0; qt < NQ; ++qt) see[qt] = t.masks[t.node_of(16 * qt + r)];
   for (int i = tid; i < kCols * D / 8; i += W * kWave) {
     const int b = i / 64, l = i % 64;        // block b: columns 16 (b / DS), dims 32 (b % DS)
-    const int c = t.first + min(16 * (b / DS) + (l & 15), t.cols - 1), d = 32 * (b % DS) + 8 * (l >> 4);
+    const int c = t.first + min(16 * (b / DS) + (l & 15), t.cols - 1);
+    const int d = 32 * (b % DS) + 8 * (l >> 4);
     *reinterpret_cast<u32x4*>(q_s + i * 16) =
         load16((const bf16*)a.q + t.row * a.q_row + c / t.G * a.q_node +
                (t.h * t.G + c % t.G) * a.q_head + d);
@@ -597,9 +598,9 @@ __device__ __forceinline__ void landed() {
 }
 
 template <int D, int W>
-__global__ __launch_bounds__(W * kWave, 2) void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles,
-                                                            float* __restrict__ part_o,
-                                                            float* __restrict__ part_ml) {
+__global__ __launch_bounds__(W * kWave, 2)
+void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ part_o,
+                 float* __restrict__ part_ml) {
   constexpr int NQ = kManyNq, DS = D / 32, DT = D / 16, kPos = many_tile<D, W>();
   constexpr int kCols = 16 * NQ * W, kBytes = kPos * D * 2;
   constexpr int kLoads = kBytes / 1024 / W;  // of K, of V, by a wave: 1 KiB each
@@ -870,21 +871,21 @@ __global__ __launch_bounds__(kBlock) void k_tree_join(TfdTreeAttnArgs a, int spl
 // Short: where every wave needs one tile of 32 positions, with 16 columns a block and no more
 // blocks than compute units, blocks of as many waves as their registers leave room for.  Two
 // tiles a wave instead of two splits save the join's launch and take the same (13.5 us of 1 row of
-// 700 positions by 16 nodes, 13.2 with the join).  1 row of 6,000 by 16 nodes: 18.3 us, by blocks of
-// four waves of 32 columns 24.1; by 8 nodes 16.7 and 19.7.  16 columns whose tiles blocks
+// 700 positions by 16 nodes, 13.2 with the join).  1 row of 6,000 by 16 nodes: 18.3 us, by blocks
+// of four waves of 32 columns 24.1; by 8 nodes 16.7 and 19.7.  16 columns whose tiles blocks
 // of four waves hold at once too are faster by those (700 positions, 8 nodes: 11.4 us, 13.2),
 // down to what a single block holds (200: 10.1, 9.0).
 //
-// Few: up to 64 columns, 16 of 256 dims, in blocks of four waves of up to 32 (2 rows of 32,000 by 32
-// nodes: 60.0 us, by the kernel for many 68.6; 32 rows of 4,096: 118 both; 48 nodes 185 and 125).
+// Few: up to 64 columns, 16 of 256 dims, in blocks of four waves of up to 32 (2 rows of 32,000 by
+// 32 nodes: 60.0 us, by the kernel for many 68.6; 32 rows of 4,096: 118 both; 48 nodes 185 and 125).
 // One block a compute unit: what the splits leave is read again, and four waves' loads are
 // enough in flight (32 rows of 4,096 by 7 nodes: 97.6 us, with three a unit 104.1; 1 of 6,000 by 8:
 // 19.7 and 25.0).
 //
 // Many: eight waves of 32 columns, whose longer tiles cost less a position (32 rows of 4,096 by 60
 // nodes: 122 us, by two blocks of four waves 132); up to 128 columns four waves of 64 dims
-// (8 rows of 8,000: 48.9 us, by eight 51.0), or where there are more row heads than compute units (33
-// rows of 400 by 33: 30.6 us, 37.1).  Splits fill the compute units once (twice as many: 4 rows
+// (8 rows of 8,000: 48.9 us, by eight 51.0), or where there are more row heads than compute units
+// (33 rows of 400 by 33: 30.6 us, 37.1).  Splits fill the compute units once (twice as many: 4 rows
 // of 30,000 by 61 nodes of 32 heads 177 us, 161 so, half as many 254).
 struct TreePlan {
   int nq, waves, mtiles, cols, splits;       // nq 0: many columns; cols: of a block
@@ -900,7 +901,8 @@ TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, i
   const int64_t cus = compute_units(), mtiles = (cols + 15) / 16, wide = short_waves(head_dim);
   // blocks a row head and 16 columns have to have for one tile a wave
   const int64_t turns = std::min<int64_t>((tiles + wide - 1) / wide, kMaxSplits);
-  const int64_t by_four = std::min<int64_t>(cus / std::max<int64_t>(units, 1), kMaxSplits) * kFewWaves;
+  const int64_t by_four =
+      std::min<int64_t>(cus / std::max<int64_t>(units, 1), kMaxSplits) * kFewWaves;
   int64_t per_cu = 1, most;                  // blocks of a compute unit, splits that have work
   if (cols <= 128 && nodes <= kFewNodes && units * mtiles * turns <= cus &&
       (cols > 16 || turns == 1 || tiles > by_four)) {
@@ -914,7 +916,8 @@ TreePlan tree_plan(int rows, int nodes, int heads, int kv_heads, int head_dim, i
     p.cols = 16 * p.nq;
     most = (tiles + p.waves - 1) / p.waves;
   } else {
-    const bool four = cols <= 4 * 16 * kManyNq && (head_dim == 64 || (head_dim == 128 && units > cus));
+    const bool four = cols <= 4 * 16 * kManyNq &&
+                      (head_dim == 64 || (head_dim == 128 && units > cus));
     p.nq = 0;
     p.waves = four ? 4 : 8;
     p.cols = p.waves * 16 * kManyNq;
@@ -998,8 +1001,8 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
   if (!a.q || !a.k_pool || !a.v_pool || !a.page_table || !a.lengths || !a.masks || !a.out)
     return fail(kBadArg, "tree_attn: null pointer");
   if ((uintptr_t)a.q % 16 || a.q_row % 8 || a.q_node % 8 || a.q_head % 8 ||
-      (uintptr_t)a.k_pool % 16 || (uintptr_t)a.v_pool % 16)
-    return fail(kBadArg, "tree_attn: q and the pools must be 16-byte aligned");
+      (uintptr_t)a.k_pool % 16 || (uintptr_t)a.v_pool % 16 || (uintptr_t)a.out % 16)
+    return fail(kBadArg, "tree_attn: q, the pools and out must be 16-byte aligned");
   const TreePlan p = tree_plan(a.rows, a.nodes, a.heads, a.kv_heads, a.head_dim, a.max_pages);
   const int64_t cols = (int64_t)a.rows * a.kv_heads * p.splits * p.mtiles * p.cols;
   if (p.splits > 1 && (!a.work || (uintptr_t)a.work % 16 ||
@@ -1027,10 +1030,11 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
     KERNEL<<<GRID, THREADS, lds, s>>>(__VA_ARGS__);                                           \
   }
 #define TFD_TREE_FEW(D, NQ, W) \
-  TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), blocks, W * kWave, a, p.splits, p.mtiles, po, \
-               pml)
+  TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), blocks, W * kWave, a, p.splits, \
+               p.mtiles, po, pml)
 #define TFD_TREE_MANY(D, W) \
-  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D, W>()), blocks, W * kWave, a, p.splits, p.mtiles, po, pml)
+  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D, W>()), blocks, W * kWave, a, p.splits,     \
+               p.mtiles, po, pml)
 #define TFD_TREE_DIM(D)                                                                       \
   {                                                                                           \
     if (p.nq == 1 && p.waves == kFewWaves) TFD_TREE_FEW(D, 1, kFewWaves)                      \

@@ -37,9 +37,9 @@ BOOL = (torch.bool, torch.uint8)
 class Pages:
     """See the module docstring.
 
-    *pools*: tensors ``[pages, heads, 16, dim]``, or ``[layers, pages, heads, 16, dim]``, contiguous,
-    rows of a multiple of 16 bytes, all of one number of pages; they are kept.  *table* int32
-    ``[rows, max_pages]`` (-1: no page) and *refs* int32 ``[pages]`` are used in place if given;
+    *pools*: tensors ``[pages, heads, 16, dim]``, or ``[layers, pages, heads, 16, dim]``,
+    contiguous, rows of a multiple of 16 bytes, all of one number of pages; they are kept.
+    *table* int32 ``[rows, max_pages]`` (-1: no page) and *refs* int32 ``[pages]`` are used in place if given;
     without *table* it starts empty, without *refs* the table's entries are counted."""
 
     def __init__(self, pools, *, rows: int | None = None, max_pages: int | None = None,
@@ -157,8 +157,8 @@ class Pages:
         launch(self.index, lib().tfd_pages_take, self._at, ptr(lengths), ptr(counts), one)
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        """Page ``dst[i]`` of every pool becomes page ``src[i]`` (int32 ``[n]``).  No page may be in both
-        lists or twice in *dst*.  Table and references stay as they are."""
+        """Page ``dst[i]`` of every pool becomes page ``src[i]`` (int32 ``[n]``).  No page may be in
+        both lists or twice in *dst*.  Table and references stay as they are."""
         check_input(src, "src", INT32)
         if src.dim() != 1:
             raise ValueError(f"src must be [n], got {tuple(src.shape)}")
@@ -167,8 +167,8 @@ class Pages:
 
     def keep(self, lengths: torch.Tensor, path: torch.Tensor, counts: torch.Tensor
              ) -> torch.Tensor:
-        """Positions ``lengths[r] + path[r, i]`` move to ``lengths[r] + i`` for i < ``counts[r]``, in
-        every pool; -> ``lengths + counts``.  path (int32 ``[rows, nodes]``) rises along a row;
+        """Positions ``lengths[r] + path[r, i]`` move to ``lengths[r] + i`` for i < ``counts[r]``,
+        in every pool; -> ``lengths + counts``.  path (int32 ``[rows, nodes]``) rises along a row;
         a row where it does not keeps its positions and length (``check_errors``)."""
         check_input(path, "path", INT32)
         if path.dim() != 2 or path.shape[0] != self.rows or path.shape[1] < 1:

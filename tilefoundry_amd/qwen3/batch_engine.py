@@ -34,6 +34,7 @@ from .search import BeamSearch, NgramDraft, Speculation
 from .weights import head_rows, pack_layer, validate
 
 MAX_BATCH = 32
+MAX_SEARCHES = 4            # rules of beam searches whose graphs an engine keeps
 
 
 def _round_up(n: int, m: int) -> int:
@@ -370,6 +371,8 @@ class BatchEngine:
         key = (beams, eos, float(length_penalty))
         known = self.__dict__.setdefault("_beam_searches", {})
         if key not in known:
+            if len(known) == MAX_SEARCHES:           # (each keeps a captured graph)
+                known.pop(next(iter(known)))
             known[key] = BeamSearch(weakref.ref(self), *key)
         return known[key].run(prompts, max_new)
 
@@ -379,6 +382,7 @@ class BatchEngine:
         ``qwen3.search.NgramDraft`` unless given)."""
         known = self.__dict__.setdefault("_speculations", {})
         if nodes not in known:
+            known.clear()                            # (logits of batch x nodes rows)
             known[nodes] = Speculation(weakref.ref(self), nodes)
         return known[nodes].run(prompts, max_new, NgramDraft() if draft is None else draft)
 
