@@ -144,11 +144,49 @@ def test_speculation_gives_the_greedy_tokens(gpu_device, weights, nodes):
     assert e.generate(prompts, 30, prefill=True).tokens == want
 
 
+def test_speculation_without_graphs(gpu_device, weights):
+    """The captured pass and its launches one by one give the same, again and again."""
+    prompts = [_prompt(n, SMALL.vocab_size, seed=80 + n) for n in (21, 6)]
+    plain = _engine(weights, gpu_device, 2, graph=False)
+    e = _engine(weights, gpu_device, 2)
+    for nodes in (6, 9, 6):
+        want = plain.speculate(prompts, 30, nodes=nodes)
+        for _ in range(3):
+            got = e.speculate(prompts, 30, nodes=nodes)
+            assert got.tokens == want.tokens and got.passes == want.passes
+            e.generate(prompts, 5, prefill=True)     # eager work and the step's graph between
+
+
 def test_speculation_with_room_for_many_nodes(gpu_device, weights):
     prompts = [_prompt(n, SMALL.vocab_size, seed=40 + n) for n in (16, 3, 33)]
     e = _engine(weights, gpu_device, 3)
     want = e.generate(prompts, 30, prefill=True).tokens
     assert e.speculate(prompts, 30, nodes=200, draft=_Known(prompts, want, True)).tokens == want
+
+
+def test_prompts_of_one_token_and_one_new(gpu_device, weights):
+    e = _engine(weights, gpu_device, 2)
+    for prompts in ([[5], [9]], [[5], [9, 3]]):
+        want = e.generate(prompts, 6).tokens
+        assert e.speculate(prompts, 6, nodes=4).tokens == want
+        assert [b[0] for b in e.beam_search(prompts, 6, beams=1).tokens] == want
+        assert [len(t) for t in e.speculate(prompts, 1).tokens] == [1, 1]
+    two = e.beam_search([[5]], 1, beams=2)
+    assert two.tokens[0][0] == e.generate([[5], [9]], 1).tokens[0] and len(two.tokens[0][1]) == 1
+
+
+def test_searches_up_to_the_last_position(gpu_device, weights):
+    """Prompt and new tokens fill the engine's steps: the last node's slot is the last one."""
+    e = _engine(weights, gpu_device, 2, max_new=14, prompt_room=20)
+    prompts = [_prompt(20, SMALL.vocab_size, seed=n) for n in (60, 61)]
+    run = e.generate(prompts, 14, prefill=True, record_logits=True)
+    for draft in (NgramDraft(), _Known2(prompts, run.tokens)):
+        got = e.speculate(prompts, 14, nodes=16, draft=draft)
+        for b in range(2):
+            _same_to_a_near_tie(run.tokens[b], run.logits[b], got.tokens[b])
+    got = e.beam_search(prompts, 14, beams=1)
+    for b in range(2):
+        _same_to_a_near_tie(run.tokens[b], run.logits[b], got.tokens[b][0])
 
 
 def _same_to_a_near_tie(want, logits, got):

@@ -292,10 +292,32 @@ class Speculation:
         self._engine, self.nodes = engine, nodes
         self.step = TreePass(engine, nodes)
         self.cache = Pages([e.kpool, e.vpool], table=e.page_table)
+        # what a pass reads: tokens, parents and, in the first place of a row, its nodes
+        self.rows = torch.zeros(3, e.B, nodes, dtype=I32, device=e.device)
+        self.lengths = torch.zeros(e.B, dtype=I32, device=e.device)
+        self.graph = self.found = None
+
+    def _pass(self) -> torch.Tensor:
+        """One pass over ``rows``: each sequence's path, how many it holds and the token behind."""
+        tokens, parents, counts = self.rows.unbind(0)
+        counts = counts[:, 0].contiguous()
+        picks = self.step.picks_of(tokens, parents, counts, self.lengths)
+        path, accepted, after = tree.accept(tokens, parents, picks, counts)
+        self.lengths.copy_(self.cache.keep(self.lengths, path, accepted))
+        return torch.cat((path, accepted.unsqueeze(1), after.unsqueeze(1)), 1)
+
+    def _capture(self):
+        torch.cuda.synchronize(self._engine().device)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            self.found = self._pass()
+        self.graph = graph
 
     def run(self, prompts, max_new: int, draft) -> Speculated:
         e, T = self._engine(), self.nodes
         prompts = _checked(e, prompts, e.B, max_new)
+        if self.graph is None and e.graph is not None:
+            self._capture()
         torch.cuda.synchronize(e.device)
         t0 = perf_counter()
         e.prefill(prompts)
@@ -303,7 +325,7 @@ class Speculation:
         t1 = perf_counter()
         history = [p.tolist() for p in prompts]
         start = [len(p) for p in prompts]
-        lengths = e.pos.clone()
+        self.lengths.copy_(e.pos)
         passes = 0
         while True:
             # a draft reaches no further than what is still wanted (node 0 gives one token too)
@@ -326,14 +348,14 @@ class Speculation:
                 if not in_vocab(np.asarray(tokens, dtype=np.int64), e.V):
                     raise ValueError(f"draft: token ids must lie in [0, {e.V})")
                 rows[0, b, :n], rows[1, b, :n], rows[2, b, 0] = tokens, parents, n
-            tokens, parents, counts = torch.from_numpy(rows).to(e.device).unbind(0)
-            counts = counts[:, 0].contiguous()
-            picks = self.step.picks_of(tokens, parents, counts, lengths)
-            path, accepted, after = tree.accept(tokens, parents, picks, counts)
-            lengths = self.cache.keep(lengths, path, accepted)
-            got = torch.cat((path, accepted.unsqueeze(1), after.unsqueeze(1)), 1).tolist()
+            self.rows.copy_(torch.from_numpy(rows))
+            if self.graph is not None:
+                self.graph.replay()
+                found = self.found
+            else:
+                found = self._pass()
             passes += 1
-            for b, r in enumerate(got):
+            for b, r in enumerate(found.tolist()):
                 n = r[T]
                 history[b] += [int(rows[0, b, t]) for t in r[1:n]] + ([r[T + 1]] if n else [])
         t2 = perf_counter()
