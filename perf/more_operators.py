@@ -247,7 +247,7 @@ def prepare(case, seed):
         if case["kind"] == "beam":
             s["handle"] = beam.Beam(case["beams"], eos=EOS, length_penalty=case["penalty"])
         elif case["kind"] == "reorder":
-            s["handle"] = beam.States(s["states"])
+            s["handle"] = beam.States(s["states"], case["beams"])
         elif case["kind"] == "pages":
             s["handle"] = pages.Pages([s["k"], s["v"]], table=s["table"], refs=s["refs"])
     return s
