@@ -50,10 +50,9 @@ int tfd_tree_qkv_append(const float* part, int slices, int M, int heads, int kv_
  * lengths[b] + t of its pages.  Node t attends to every position below lengths[b] and to node n
  * where bit n of masks[b][t] is set and n < counts[b]:
  *   out = sum_j softmax_j(scale q . k_j) v_j,
- * scores and sums in f32, one rounding of the output.  The probabilities, a product's operands,
- * are sums of two bf16 (2^-16 of each) where few columns, nodes x heads / kv_heads, share a kv
- * head, and one bf16 (2^-8) where tfd_tree_attn_form says many.  A node that sees nothing gets
- * zeros.  What a node does not see takes no part, values that are not finite included.  q bf16,
+ * scores and sums in f32, one rounding of the output; the probabilities, a product's operands,
+ * are sums of two bf16 (2^-16 of each).  With `rounded` they may be one bf16 (2^-8), for speed,
+ * where tfd_tree_attn_form says many.  A node that sees nothing gets zeros.  What a node does not see takes no part, values that are not finite included.  q bf16,
  * rows / nodes / heads q_row / q_node / q_head elements apart (multiples of 8; q, the pools and
  * out 16-byte aligned).  out: [rows][nodes][heads][head_dim], or
  * with out_panel the rows x nodes rows of tf_decode.h's panel order.  Nodes from counts[b] on
@@ -76,6 +75,7 @@ typedef struct {
   void* work;
   int64_t work_bytes;
   int32_t* err;
+  int rounded;
 } TfdTreeAttnArgs;
 int64_t tfd_tree_attn_work_bytes(int rows, int nodes, int heads, int kv_heads, int head_dim,
                                  int max_pages);

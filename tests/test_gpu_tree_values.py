@@ -1,0 +1,102 @@
+"""Tree attention where its values, pages and lengths are unusual, by every way a call may run,
+against the definition in 64 bits.
+
+The bound is that of a probability as a sum of two bf16 in every form: what two of them leave out
+is 2^-8 of the second, itself 2^-8 of the first (half steps of eight bits), so 2^-16 of it; one
+bf16 rounding of the output, 2^-8 of its value; scores are f32 sums of exact products, dim 2^-24
+times |q| |k|, and the exponential's argument 2^-22; sums over n positions n 2^-24 of the sum of
+|p v|."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from tests import _search_ref as R
+from tests.test_gpu_tree import BF, FORMS, I32, _case, _form, _gen
+from tilefoundry_amd import _lib, tree
+from tilefoundry_amd._lib import lib, ptr
+
+pytestmark = pytest.mark.gpu
+
+MANY = [f for f in FORMS if f[1][0] == 0]
+
+
+def _lengths(rows):
+    return [(71 * b + 13) % 210 if rows > 8 or b else 333 for b in range(rows)]
+
+
+def _shape(shape, **kw):
+    rows, nodes, heads, kv_heads, dim, room = shape
+    return _case(sum(shape), rows, nodes, heads, kv_heads, dim, _lengths(rows), room=room, **kw)
+
+
+def _place(c, b, pos):
+    return c["table"][b, pos // 16].long(), pos % 16
+
+
+def _node(c, b, t):
+    """(f64 output of node t of row b [heads, dim], the sum of |p v|); a position whose page is
+    none of the pool's is left out."""
+    pages, kv_heads = c["k_pool"].shape[:2]
+    nodes, heads, dim = c["q"].shape[1:]
+    L = int(c["lengths"][b])
+    see = [j for j in range(nodes) if (int(c["masks"][b, t, j // 64]) >> (j % 64)) & 1]
+    at = torch.cat((torch.arange(L), torch.tensor(see, dtype=torch.int64) + L))
+    page = c["table"][b, at // 16].long()
+    held = (page >= 0) & (page < pages)
+    page, at = page[held], at[held]
+    if not len(at):
+        return torch.zeros(heads, dim).double(), torch.zeros(heads, dim).double()
+    k, v = (c[p][page, :, at % 16].double() for p in ("k_pool", "v_pool"))
+    out, size = (torch.empty(heads, dim, dtype=torch.float64) for _ in range(2))
+    for h in range(heads):
+        g = h // (heads // kv_heads)
+        p = torch.softmax(dim ** -0.5 * (k[:, g] @ c["q"][b, t, h].double()), 0).unsqueeze(1)
+        out[h], size[h] = (p * v[:, g]).sum(0), (p * v[:, g]).abs().sum(0)
+    return out, size
+
+
+def _bound(c, want, size, operand=2.0 ** -16):
+    dim = c["q"].shape[3]
+    n = int(c["lengths"].max()) + c["q"].shape[1]
+    kn = c["k_pool"].float()
+    kn = kn[torch.isfinite(kn).all(3)].norm(dim=1).max().double()
+    score = dim ** -0.5 * c["q"].double().norm(dim=3).max() * kn * (dim + 8) * 2.0 ** -24 + \
+        2.0 ** -22
+    return want.abs() * 2.0 ** -8 + size * (2 * score + operand + (n + 8) * 2.0 ** -24) + 1e-30
+
+
+def _check(c, dev, at, err=None, **kw):
+    """*at*: pairs of a row and a node."""
+    out = tree.attention(**{k: v.to(dev) for k, v in c.items()}, err=err, **kw).cpu().double()
+    operand = 2.0 ** (-8 if kw.get("rounded") else -16)
+    for b, t in at:
+        want, size = _node(c, b, t)
+        got, far = out[b, t], ~torch.isfinite(want)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), (b, t)
+        there = far & ~torch.isnan(want)
+        assert torch.equal(got[there], want[there]), (b, t)
+        off = (got - want).abs()[~far]
+        assert (off <= _bound(c, want, size, operand)[~far]).all(), (b, t, off.max())
+
+
+def _some(rows, nodes):
+    return sorted({(b, t) for b in (0, rows // 2, rows - 1) for t in
+                   (0, nodes // 3, nodes // 2, nodes - 2, nodes - 1) if t >= 0})
+
+
+@pytest.mark.parametrize("shape,form", MANY)
+def test_every_form_holds_probabilities_to_16_bits(gpu_device, shape, form):
+    c = _shape(shape)
+    assert _form(c)[0] == 0
+    _check(c, gpu_device, _some(*shape[:2]))
+
+
+@pytest.mark.parametrize("shape,form", FORMS)
+def test_probabilities_rounded_to_8_bits_where_asked(gpu_device, shape, form):
+    """By many columns alone: by few there is nothing to gain and nothing changes."""
+    c = _shape(shape)
+    _check(c, gpu_device, _some(*shape[:2]), rounded=True)
+    d = {k: v.to(gpu_device) for k, v in c.items()}
+    assert torch.equal(tree.attention(**d, rounded=True), tree.attention(**d)) == (form[0] > 0)

@@ -13,7 +13,7 @@ from pathlib import Path
 
 from .build import LIB
 
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 PRO_PLAIN, PRO_NORM = 0, 1
 EPI_STORE, EPI_RESID, EPI_SWIGLU, EPI_LOGITS, EPI_RESID_F32 = 0, 1, 2, 3, 4
@@ -425,7 +425,8 @@ class TfdTreeAttnArgs(ctypes.Structure):
                 *[(n, c_int) for n in ("rows", "nodes", "heads", "kv_heads", "head_dim",
                                        "max_pages", "num_pages")],
                 ("scale", c_float), ("out", c_void_p), ("out_panel", c_int),
-                ("work", c_void_p), ("work_bytes", c_int64), ("err", c_void_p)]
+                ("work", c_void_p), ("work_bytes", c_int64), ("err", c_void_p),
+                ("rounded", c_int)]
 
 
 class TfdBeamArgs(ctypes.Structure):

@@ -119,11 +119,10 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // 16 rows of such a read take the fewest cycles.
 //
 // Softmax against a running reference, in f32.  The probabilities have to become bf16 for the
-// second product.  By few columns, which wait for keys, they stay a sum of two bf16 (2^-16 of
-// each).  By many they are one bf16: the product with a second half costs a fifth to a third of
-// the call (220 to 173 us at 4 rows to 30,000 positions, 61 nodes of 32 heads over 8), and
-// what it buys is small beside the output's own rounding (2^-8 of a probability, and they
-// average: 1.4 times the error of an attention in f32 that rounds its output).
+// second product: they stay a sum of two bf16 (2^-16 of each), however many columns there are.
+// By many, a caller may ask for one (2^-8; they average: 1.4 times the error of an attention in
+// f32 that rounds its output), which saves a third of the products and half of what VALU does for
+// a probability: 215 to 161 us at 4 rows to 30,000 positions, 61 nodes of 32 heads over 8.
 //
 // Two kernels.  Few columns (k_tree_few): the keys are what is waited for, so each wave
 // takes other tiles of 32 positions, its K straight into registers as operands and its V
@@ -597,7 +596,7 @@ __device__ __forceinline__ void landed() {
   asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kN) : "memory");
 }
 
-template <int D, int W>
+template <int D, int W, bool kTwo>
 __global__ __launch_bounds__(W * kWave, 2)
 void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ part_o,
                  float* __restrict__ part_ml) {
@@ -752,18 +751,25 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
         }
         ref[qt] = tree_maximum<kPos / 16, DT, NQ>(st[qt], c2, mx[qt], sum[qt], o, qt);
       }
+      // (V's places are worked out for every tile: 256 dims leave no registers to hold them)
+      int vlane = lane;
+      if (D == 256) asm volatile("" : "+v"(vlane));
 #pragma unroll
       for (int kk = 0; kk < kPos / kTile; ++kk) {
-        u32x4 pr[NQ], none;
+        u32x4 ph[NQ], pl[NQ];
 #pragma unroll
         for (int qt = 0; qt < NQ; ++qt)
-          tree_weights<false>(st[qt][2 * kk], st[qt][2 * kk + 1], c2, ref[qt], sum[qt], pr[qt],
-                              none);
+          tree_weights<kTwo>(st[qt][2 * kk], st[qt][2 * kk + 1], c2, ref[qt], sum[qt], ph[qt],
+                             pl[qt]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, lane);
+          const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, vlane);
+          if constexpr (kTwo) {
 #pragma unroll
-          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pr[qt], o[dt][qt]);
+            for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pl[qt], o[dt][qt]);
+          }
+#pragma unroll
+          for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
         }
       }
     }
@@ -1032,9 +1038,13 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
 #define TFD_TREE_FEW(D, NQ, W) \
   TFD_TREE_RUN((k_tree_few<D, NQ, W>), (few_lds<D, NQ, W>()), blocks, W * kWave, a, p.splits, \
                p.mtiles, po, pml)
-#define TFD_TREE_MANY(D, W) \
-  TFD_TREE_RUN((k_tree_many<D, W>), (many_lds<D, W>()), blocks, W * kWave, a, p.splits,     \
-               p.mtiles, po, pml)
+#define TFD_TREE_MANY(D, W)                                                                 \
+  if (a.rounded)                                                                            \
+    TFD_TREE_RUN((k_tree_many<D, W, false>), (many_lds<D, W>()), blocks, W * kWave, a,      \
+                 p.splits, p.mtiles, po, pml)                                               \
+  else                                                                                      \
+    TFD_TREE_RUN((k_tree_many<D, W, true>), (many_lds<D, W>()), blocks, W * kWave, a,       \
+                 p.splits, p.mtiles, po, pml)
 #define TFD_TREE_DIM(D)                                                                       \
   {                                                                                           \
     if (p.nq == 1 && p.waves == kFewWaves) TFD_TREE_FEW(D, 1, kFewWaves)                      \
@@ -1042,8 +1052,10 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream) {
     else if (p.nq == 2) {                                                                     \
       if constexpr (D <= 128) TFD_TREE_FEW(D, 2, kFewWaves)                                   \
     } else if (p.waves == 4) {                                                                \
-      if constexpr (D <= 128) TFD_TREE_MANY(D, 4)                                             \
-    } else TFD_TREE_MANY(D, 8)                                                                \
+      if constexpr (D <= 128) { TFD_TREE_MANY(D, 4) }                                         \
+    } else {                                                                                  \
+      TFD_TREE_MANY(D, 8)                                                                     \
+    }                                                                                         \
     if (p.splits > 1) k_tree_join<D><<<joins, kBlock, 0, s>>>(a, p.splits, pad, po, pml);     \
   }
   if (a.head_dim == 64) TFD_TREE_DIM(64)

@@ -105,7 +105,8 @@ def accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor,
 
 def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table: torch.Tensor,
               lengths: torch.Tensor, masks: torch.Tensor, counts: torch.Tensor | None = None, *,
-              scale: float | None = None, err: torch.Tensor | None = None) -> torch.Tensor:
+              scale: float | None = None, err: torch.Tensor | None = None,
+              rounded: bool = False) -> torch.Tensor:
     """Attention of drafted nodes over a paged cache, bf16 ``[rows, nodes, heads, dim]``.
 
     q: bf16 of that shape, any strides.  Pools: bf16 ``[pages, kv_heads, 16, dim]``; table: int32
@@ -113,7 +114,10 @@ def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table
     Row b's nodes have their keys and values at positions ``lengths[b] + t``.  Node t attends to
     the positions below ``lengths[b]`` and to the nodes of ``masks[b, t]`` (``ancestors``, or any
     other bits); one that sees nothing gets zeros.  Of a row with ``counts[b]`` nodes the others
-    are not there and their outputs are not written.  Scale: dim^-1/2 unless given."""
+    are not there and their outputs are not written.  Scale: dim^-1/2 unless given.
+
+    Probabilities are held to 2^-16 in the product with the values.  *rounded* lets them be bf16
+    (2^-8) where many nodes and heads share a kv head, which is up to a quarter faster there."""
     check_input(q, "q", BF16)
     check_input(k_pool, "k_pool", BF16)
     check_input(v_pool, "v_pool", BF16)
@@ -168,6 +172,7 @@ def attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, table
     work = q.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.TfdTreeAttnArgs(ptr(q), of_row, of_node, of_head, ptr(k_pool), ptr(v_pool), ptr(table),
                              ptr(lengths), ptr(counts), ptr(masks), rows, nodes, heads, kv_heads,
-                             dim, width, pages, scale, ptr(out), 0, ptr(work), need, ptr(err))
+                             dim, width, pages, scale, ptr(out), 0, ptr(work), need, ptr(err),
+                             1 if rounded else 0)
     launch(q.get_device(), L.tfd_tree_attn, ctypes.addressof(a))
     return out
