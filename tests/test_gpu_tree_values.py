@@ -100,3 +100,37 @@ def test_probabilities_rounded_to_8_bits_where_asked(gpu_device, shape, form):
     _check(c, gpu_device, _some(*shape[:2]), rounded=True)
     d = {k: v.to(gpu_device) for k, v in c.items()}
     assert torch.equal(tree.attention(**d, rounded=True), tree.attention(**d)) == (form[0] > 0)
+
+
+@pytest.mark.parametrize("shape,form", FORMS)
+def test_cached_values_that_are_not_finite(gpu_device, shape, form):
+    """In the first, a middle and the last cached positions, in dims and heads of their own, both
+    infinities in one dim, and beside drafted ones."""
+    c = _shape(shape)
+    rows, nodes, heads, kv_heads, dim, _ = shape
+    for b in (0, rows - 1):
+        L = int(c["lengths"][b])
+        for pos, h, d, x in ((0, 0, 3, math.inf), (L // 2, 0, 8, -math.inf),
+                             (L - 1, kv_heads - 1, dim - 1, math.nan), (L - 1, 0, 20, math.inf),
+                             (L // 3, kv_heads - 1, 33, math.inf),
+                             (L // 2, kv_heads - 1, 33, -math.inf),
+                             (L // 4, 0, 50, -1e30), (L // 2, 0, 51, math.inf),
+                             (L + nodes - 1, 0, 51, -math.inf), (L + nodes - 1, 0, 52, -math.inf)):
+            page, off = _place(c, b, pos)
+            c["v_pool"][page, h, off, d] = x
+    _check(c, gpu_device, _some(rows, nodes))
+
+
+@pytest.mark.parametrize("nodes", [3, 80])
+def test_infinite_values_of_little_weight(gpu_device, nodes):
+    """The weight of an infinite value is far below an f32's smallest number, in its own wave, split
+    or tile and in others: it is above zero all the same."""
+    for at in (0, 700, 1399):
+        c = _case(at + nodes, 1, nodes, 2, 1, 128, [1400])
+        c["q"] *= 8
+        page, off = _place(c, 0, at)
+        c["k_pool"][page, :, off] = c["q"][0, 0, 0] * 0.5
+        for pos, d in ((3, 1), (690, 2), (710, 3), (1390, 4)):
+            page, off = _place(c, 0, pos)
+            c["v_pool"][page, 0, off, d] = math.inf if d % 2 else -math.inf
+        _check(c, gpu_device, [(0, 0), (0, nodes - 1)])

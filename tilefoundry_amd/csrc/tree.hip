@@ -335,6 +335,49 @@ __device__ __forceinline__ void add_odd(TreeRow& t, f32x4& y, int c, int d, int 
   }
 }
 
+// So do the context's, which every column sees: a dim of the output in which the product came
+// out not finite is what those values make it, since each has a weight above zero, however small.
+// They are looked for then alone: 3 bits of `odd` a dim (D / 8 words in LDS, 8 dims each), +inf,
+// -inf and NaN.  All threads of the block; positions j0 .. j1 - 1.
+template <int D>
+__device__ __forceinline__ void find_odd(TreeRow& t, uint32_t* odd, int j0, int j1) {
+  constexpr int kChunks = D / 8;
+  const int chunk = threadIdx.x % kChunks, step = blockDim.x / kChunks;
+  const int end = min(j1, t.L);
+  uint32_t found = 0;
+#pragma unroll 4
+  for (int j = j0 + (int)threadIdx.x / kChunks; j < end; j += step) {
+    const u32x4 x = load16(t.v + t.page_at(j / kPage) * t.page_size + (j % kPage) * D + 8 * chunk);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t h = e % 2 ? x[e / 2] >> 16 : x[e / 2] & 0xffffu;
+      if ((h & 0x7f80u) == 0x7f80u)
+        found |= (h & 0x7fu ? 4u : h >> 15 ? 2u : 1u) << (3 * e);
+    }
+  }
+  if (found) atomicOr(&odd[chunk], found);
+}
+// ... and put in their dims' places: 4 dims from d on.
+__device__ __forceinline__ void put_odd(f32x4& y, const uint32_t* odd, int d) {
+  const uint32_t bits = odd[d / 8] >> (3 * (d % 8));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t b = bits >> (3 * e) & 7;
+    if (b) y[e] = b == 1 ? __builtin_huge_valf() : b == 2 ? -__builtin_huge_valf()
+                                                         : __builtin_nanf("");
+  }
+}
+// Whether a column's sums may hold such values' products: not finite, of finite probabilities.
+template <int DT, int NQ>
+__device__ __forceinline__ bool lost(const f32x4 (&o)[DT][NQ], int qt, float sum) {
+  float z[4] = {0.f, 0.f, 0.f, 0.f};         // (0 times what is not finite is NaN)
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = fmaf(o[dt][qt][e], 0.f, z[e]);
+  return !((z[0] + z[1]) + (z[2] + z[3]) == 0.f) && sum == sum;
+}
+
 __device__ __forceinline__ int64_t out_at(const TfdTreeAttnArgs& a, int64_t rr, int head, int d) {
   return a.out_panel ? panel_off(rr, head * a.head_dim + d, a.heads * a.head_dim)
                      : (rr * a.heads + head) * a.head_dim + d;
@@ -362,7 +405,8 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
   constexpr int kRowsPerLoad = 512 / D;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float m_s[W][kCols], l_s[W][kCols], inv_s[kCols];
-  __shared__ int odd_s;
+  __shared__ uint32_t far_s[D / 8];
+  __shared__ int odd_s, lost_s;
   uint8_t* const q_s = smem;                 // operand order: 1 KiB per (16 columns, 32 dims)
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -436,7 +480,8 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
         load16((const bf16*)a.q + t.row * a.q_row + c / t.G * a.q_node +
                (t.h * t.G + c % t.G) * a.q_head + d);
   }
-  if (tid == 0) odd_s = 0;
+  if (tid == 0) odd_s = lost_s = 0;
+  if (tid < D / 8) far_s[tid] = 0;
   __syncthreads();                           // the queries are in place
 
   for (; tile < tiles; tile += slots) {
@@ -488,12 +533,19 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
     sum[qt] = quad_sum(sum[qt]);
+    if (lost(o, qt, sum[qt])) lost_s = 1;
     if (kq == 0) {
       m_s[wave][16 * qt + r] = mx[qt];
       l_s[wave][16 * qt + r] = sum[qt];
     }
   }
   __syncthreads();                           // (V's pieces are free from here on)
+  const bool far = lost_s;
+  if (far) {
+    for (int k = split * W; k < tiles; k += slots)
+      find_odd<D>(t, far_s, k * kTile, (k + W) * kTile);
+    __syncthreads();
+  }
   const int64_t pcol = ((int64_t)unit * mtiles + mt) * kCols;
   float scale[NQ];
 #pragma unroll
@@ -547,6 +599,7 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
       const int c = 16 * (i / 64 / kDims) + i % 64 / 4;
       const int d = 16 * (pass * kDims + i / 64 % kDims) + i % 4 * 4;
       if (c >= t.cols) continue;
+      if (far) put_odd(y, far_s, d);
       if (odd_s)
         for (int k = t.L / kTile; k < tiles; ++k)
           if (k / W % splits == split) add_odd(t, y, c, d, k * kTile, k * kTile + kTile, D);
@@ -606,7 +659,8 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
   constexpr int kChunks = D / 8;             // 16 bytes each, of a position
   constexpr int kRows = kWave / kChunks;     // positions of a load
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int odd_s;
+  __shared__ uint32_t far_s[D / 8];
+  __shared__ int odd_s, lost_s;
   const int tid = threadIdx.x, lane = tid & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int r = lane & 15, kq = lane >> 4;
@@ -674,7 +728,8 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt][qt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (tid == 0) odd_s = 0;
+  if (tid == 0) odd_s = lost_s = 0;
+  if (tid < D / 8) far_s[tid] = 0;
   fill_pages(begin);
   // (the queries are waited for here: else a tile's products would do it, and so wait for the
   // loads of the tiles behind)
@@ -720,6 +775,9 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
     }
     const bool edge = (tile + 1) * kPos > t.L;
     if (c0 < t.cols) {
+      // (operands' places are worked out for every tile: 256 dims leave no registers to hold them)
+      int at = lane;
+      if (D == 256) asm volatile("" : "+v"(at));
       f32x4 st[NQ][kPos / 16];
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt)
@@ -730,7 +788,7 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
 #pragma unroll
         for (int p = 0; p < kPos / 16; ++p) {
           const u32x4 kf =
-              *reinterpret_cast<const u32x4*>(buf + k_at<D>(16 * p + r, 4 * s + kq));
+              *reinterpret_cast<const u32x4*>(buf + k_at<D>(16 * p + (at & 15), 4 * s + (at >> 4)));
 #pragma unroll
           for (int qt = 0; qt < NQ; ++qt) st[qt][p] = mfma(kf, qf[qt][s], st[qt][p]);
         }
@@ -751,9 +809,6 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
         }
         ref[qt] = tree_maximum<kPos / 16, DT, NQ>(st[qt], c2, mx[qt], sum[qt], o, qt);
       }
-      // (V's places are worked out for every tile: 256 dims leave no registers to hold them)
-      int vlane = lane;
-      if (D == 256) asm volatile("" : "+v"(vlane));
 #pragma unroll
       for (int kk = 0; kk < kPos / kTile; ++kk) {
         u32x4 ph[NQ], pl[NQ];
@@ -763,7 +818,7 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
                              pl[qt]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, vlane);
+          const u32x4 vf = v_operand<D>(buf + kBytes + kk * kTile * D * 2, dt, at);
           if constexpr (kTwo) {
 #pragma unroll
             for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, pl[qt], o[dt][qt]);
@@ -779,12 +834,17 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
     }
   }
   const bool odd = odd_s;                    // (set before the last tile's barrier)
+#pragma unroll
+  for (int qt = 0; qt < NQ; ++qt) {
+    sum[qt] = quad_sum(sum[qt]);
+    if (lost(o, qt, sum[qt])) lost_s = 1;
+  }
 
   const int64_t pcol = ((int64_t)unit * mtiles + mt) * kCols;
 #pragma unroll
   for (int qt = 0; qt < NQ; ++qt) {
     const int c = c0 + 16 * qt + r;
-    const float l = quad_sum(sum[qt]), inv = l == 0.f ? 0.f : 1.f / l;
+    const float l = sum[qt], inv = l == 0.f ? 0.f : 1.f / l;
     if (c >= t.cols) continue;
     if (splits > 1 && kq == 0) {
       part_ml[(pcol + c) * 2] = mx[qt];
@@ -804,23 +864,29 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
         *reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d) = y;
       }
     }
-    // (what a lane has written it reads again)
-    if (odd) {
+  }
+  __syncthreads();
+  const bool far = lost_s;
+  if (far) {
+    find_odd<D>(t, far_s, begin * kPos, end * kPos);
+    __syncthreads();
+  }
+  if (far || odd) {                          // what a lane has written it reads again
+#pragma unroll 1
+    for (int c = c0 + r; c < min(c0 + 16 * NQ, t.cols); c += 16) {
+      const int cc = t.first + c, node = cc / t.G, head = t.h * t.G + cc - node * t.G;
+      const int64_t rr = (int64_t)t.row * a.nodes + node;
 #pragma unroll 1
       for (int d = 4 * kq; d < D; d += 16) {
+        u32x2* const to = reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, rr, head, d));
+        f32x4* const part = reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d);
         f32x4 y;
-        if (splits == 1) {
-          u32x2* const to = reinterpret_cast<u32x2*>((bf16*)a.out + out_at(a, rr, head, d));
-          const u32x2 w = *to;
-          y = f32x4{bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y)};
-          add_odd(t, y, c, d, begin * kPos, end * kPos, D);
-          *to = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
-        } else {
-          f32x4* const to = reinterpret_cast<f32x4*>(part_o + (pcol + c) * D + d);
-          y = *to;
-          add_odd(t, y, c, d, begin * kPos, end * kPos, D);
-          *to = y;
-        }
+        if (splits == 1) y = f32x4{bf_lo(to->x), bf_hi(to->x), bf_lo(to->y), bf_hi(to->y)};
+        else y = *part;
+        if (far) put_odd(y, far_s, d);
+        if (odd) add_odd(t, y, c, d, begin * kPos, end * kPos, D);
+        if (splits == 1) *to = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+        else *part = y;
       }
     }
   }
@@ -865,7 +931,8 @@ __global__ __launch_bounds__(kBlock) void k_tree_join(TfdTreeAttnArgs a, int spl
 #pragma unroll
     for (int e = 0; e < kPer; ++e) x[e] = p[e];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) y[e] += f == 0.f ? 0.f : f * x[e];
+    for (int e = 0; e < kPer; ++e)
+      y[e] += fabsf(x[e]) < __builtin_huge_valf() ? f * x[e] : x[e];
   }
 #pragma unroll
   for (int e = 0; e < kPer; ++e)
