@@ -52,9 +52,11 @@ int tfd_tree_qkv_append(const float* part, int slices, int M, int heads, int kv_
  *   out = sum_j softmax_j(scale q . k_j) v_j,
  * scores and sums in f32, one rounding of the output; the probabilities, a product's operands,
  * are sums of two bf16 (2^-16 of each).  With `rounded` they may be one bf16 (2^-8), for speed,
- * where tfd_tree_attn_form says many.  A node that sees nothing gets zeros.  What a node does not see takes no part, values that are not finite included.  q bf16,
- * rows / nodes / heads q_row / q_node / q_head elements apart (multiples of 8; q, the pools and
- * out 16-byte aligned).  out: [rows][nodes][heads][head_dim], or
+ * where tfd_tree_attn_form says many.  A node that sees nothing gets zeros.  What a node does not
+ * see takes no part, values that are not finite included, nor do positions of a page that is none
+ * of the pool's (TFD_ERR_PAGE_RANGE).  q bf16, rows / nodes / heads q_row / q_node / q_head
+ * elements apart (multiples of 8; q, the pools and out 16-byte aligned).  out:
+ * [rows][nodes][heads][head_dim], or
  * with out_panel the rows x nodes rows of tf_decode.h's panel order.  Nodes from counts[b] on
  * are not written.  head_dim 64, 128 or 256; heads a multiple of kv_heads; nodes <= 256; up to
  * 2^26 positions a row.  work: tfd_tree_attn_work_bytes, 16-byte aligned, contents free, one

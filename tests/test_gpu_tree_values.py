@@ -134,3 +134,30 @@ def test_infinite_values_of_little_weight(gpu_device, nodes):
             page, off = _place(c, 0, pos)
             c["v_pool"][page, 0, off, d] = math.inf if d % 2 else -math.inf
         _check(c, gpu_device, [(0, 0), (0, nodes - 1)])
+
+
+@pytest.mark.parametrize("shape,form", FORMS)
+def test_positions_in_pages_out_of_range_take_no_part(gpu_device, shape, form):
+    """No page, one past the pool and a negative one, in the first, middle and last places of rows,
+    drafted positions among them; the pool's first page, which no row has, holds NaN."""
+    c = _shape(shape)
+    rows, nodes = shape[:2]
+    spare = set(range(c["k_pool"].shape[0])) - set(c["table"].flatten().tolist())
+    if 0 not in spare:
+        page = spare.pop()
+        c["k_pool"][page], c["v_pool"][page] = c["k_pool"][0], c["v_pool"][0]
+        c["table"][c["table"] == 0] = page
+    c["k_pool"][0] = c["v_pool"][0] = math.nan
+    pages = c["k_pool"].shape[0]
+    bad = [-1, pages, -7, 2 ** 31 - 1]
+    for b, width in ((0, 333 + nodes), (rows - 1, int(c["lengths"][rows - 1]) + nodes)):
+        last = (width - 1) // 16
+        for i, place in enumerate({0, 1, 2, last // 2, last - 1, last}):
+            if 0 <= place <= last and (i + b) % 3 != 2:
+                c["table"][b, place] = bad[(i + b) % 4]
+    err = torch.zeros(1, dtype=I32, device=gpu_device)
+    _check(c, gpu_device, _some(rows, nodes), err)
+    assert err.item() == _lib.ERR_PAGE_RANGE
+    c["table"][0] = -1
+    d = {k: v.to(gpu_device) for k, v in c.items()}
+    assert not tree.attention(**d)[0].any()

@@ -174,10 +174,11 @@ __device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
   if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
   return w;
 }
-// 16 bytes of V at position j of a tile that reaches the drafted positions: zeros past the last
-// one, which holds anything, and in the place of drafted values that are not finite.
-__device__ __forceinline__ u32x4 clean_v(u32x4 v, int j, int L, int n, bool& odd) {
-  if (j >= n) v = u32x4{0u, 0u, 0u, 0u};
+// 16 bytes of V at position j of a tile that reaches the drafted positions or a page that is not
+// there: zeros in that page and past the last position, which hold anything, and in the place of
+// drafted values that are not finite.
+__device__ __forceinline__ u32x4 clean_v(u32x4 v, int j, int L, int n, bool held, bool& odd) {
+  if (j >= n || !held) v = u32x4{0u, 0u, 0u, 0u};
   if (j >= L) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
@@ -202,13 +203,14 @@ struct TreeRow {
   int row, h, G, L, n, cols, first, words, last_page, num_pages, max_pages;
   bool bad_page;
 
-  // Entries past the last position's page need not be set: page 0 in their place (and they
-  // are read before that page is known: no load waits for the row's length).
+  // A page, -1 for one that is none: its positions take no part, and loads take page 0 in its
+  // place.  Entries past the last position's page need not be set (and they are read before that
+  // page is known: no load waits for the row's length).
   __device__ __forceinline__ int page_at(int i) {
     const int p = table[min(i, max_pages - 1)];
     const bool ok = p >= 0 && p < num_pages;
     bad_page |= !ok && i <= last_page;
-    return ok ? p : 0;
+    return ok ? p : -1;
   }
   __device__ __forceinline__ int node_of(int c) const { return (first + min(c, cols - 1)) / G; }
   // bit i: a column that sees the nodes of m0 (and m1, the next word) from node `from` = j0 - L
@@ -323,8 +325,10 @@ __device__ __forceinline__ void add_odd(TreeRow& t, f32x4& y, int c, int d, int 
   const uint64_t* const m = t.masks + (int64_t)t.node_of(c) * t.words;
 #pragma unroll 1
   for (int j = max(j0, t.L); j < min(j1, t.n); ++j) {
-    const u32x2 x = *reinterpret_cast<const u32x2*>(
-        t.v + t.page_at(j / kPage) * t.page_size + (j % kPage) * D + d);
+    const int page = t.page_at(j / kPage);
+    if (page < 0) continue;
+    const u32x2 x =
+        *reinterpret_cast<const u32x2*>(t.v + page * t.page_size + (j % kPage) * D + d);
     const bool see = (m[(j - t.L) >> 6] >> ((j - t.L) & 63)) & 1;
     const uint32_t z[2] = {x.x, x.y};
 #pragma unroll
@@ -347,11 +351,12 @@ __device__ __forceinline__ void find_odd(TreeRow& t, uint32_t* odd, int j0, int 
   uint32_t found = 0;
 #pragma unroll 4
   for (int j = j0 + (int)threadIdx.x / kChunks; j < end; j += step) {
-    const u32x4 x = load16(t.v + t.page_at(j / kPage) * t.page_size + (j % kPage) * D + 8 * chunk);
+    const int page = t.page_at(j / kPage);
+    const u32x4 x = load16(t.v + max(page, 0) * t.page_size + (j % kPage) * D + 8 * chunk);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t h = e % 2 ? x[e / 2] >> 16 : x[e / 2] & 0xffffu;
-      if ((h & 0x7f80u) == 0x7f80u)
+      if (page >= 0 && (h & 0x7f80u) == 0x7f80u)
         found |= (h & 0x7fu ? 4u : h >> 15 ? 2u : 1u) << (3 * e);
     }
   }
@@ -422,8 +427,8 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
 
   u32x4 kr[2][DS], vr[kV];
   auto load_k = [&](int p0, int p1) {
-    const bf16* const k0 = t.k + p0 * t.page_size + r * D + 8 * kq;
-    const bf16* const k1 = t.k + p1 * t.page_size + r * D + 8 * kq;
+    const bf16* const k0 = t.k + max(p0, 0) * t.page_size + r * D + 8 * kq;
+    const bf16* const k1 = t.k + max(p1, 0) * t.page_size + r * D + 8 * kq;
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       kr[0][s] = load16(k0 + 32 * s);
@@ -431,8 +436,8 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
     }
   };
   auto load_v = [&](int p0, int p1) {
-    const bf16* const v0 = t.v + p0 * t.page_size + lane * 8;
-    const bf16* const v1 = t.v + p1 * t.page_size + lane * 8;
+    const bf16* const v0 = t.v + max(p0, 0) * t.page_size + lane * 8;
+    const bf16* const v1 = t.v + max(p1, 0) * t.page_size + lane * 8;
 #pragma unroll
     for (int i = 0; i < kV / 2; ++i) {
       vr[i] = load16(v0 + i * 512);
@@ -486,12 +491,14 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
 
   for (; tile < tiles; tile += slots) {
     const int j0 = tile * kTile;
-    const bool edge = j0 + kTile > t.L;      // drafted positions, or none, in this tile
+    const uint32_t held = (p0 < 0 ? 0u : 0xffffu) | (p1 < 0 ? 0u : 0xffff0000u);
+    // drafted positions, or none, in this tile
+    const bool edge = j0 + kTile > t.L || held != 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
       const int rr = i * kRowsPerLoad + lane / (D / 8), c8 = lane % (D / 8);
       u32x4 v = vr[i];
-      if (edge) v = clean_v(v, j0 + rr, t.L, t.n, odd);
+      if (edge) v = clean_v(v, j0 + rr, t.L, t.n, (i < kV / 2 ? p0 : p1) >= 0, odd);
       *reinterpret_cast<u32x4*>(v_s + v_at<D>(rr, c8 >> 1) + (c8 & 1) * 16) = v;
     }
     const bool more = tile + slots < tiles;
@@ -509,7 +516,7 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
         st[1] = mfma(kr[1][s], qf, st[1]);
       }
       if (edge) {
-        const uint32_t bits = t.seen(j0 - t.L < 64 ? see[qt] : 0, 0, j0) >> (4 * kq);
+        const uint32_t bits = (t.seen(j0 - t.L < 64 ? see[qt] : 0, 0, j0) & held) >> (4 * kq);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           st[i / 4][i % 4] = (bits >> (16 * (i / 4) + i % 4)) & 1 ? st[i / 4][i % 4] : kPanelNegInf;
@@ -701,8 +708,8 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
     const uint32_t buf = lds0 + (uint32_t)(n % kStages) * 2 * kBytes;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int page = __builtin_amdgcn_readfirstlane(
-          page_s[n * kPagesOf % kPages + (i * W + wave) * kRows / kPage]);
+      const int page = max(0, __builtin_amdgcn_readfirstlane(
+          page_s[n * kPagesOf % kPages + (i * W + wave) * kRows / kPage]));
       const uint32_t to = buf + (uint32_t)(i * W + wave) * 1024;
       load_to_lds(t.k + page * t.page_size, k_from[i], to);
       load_to_lds(t.v + page * t.page_size, v_from[i], to + kBytes);
@@ -737,7 +744,8 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
   for (int qt = 0; qt < NQ; ++qt)
 #pragma unroll
     for (int s = 0; s < DS; ++s) asm volatile("" : "+v"(qf[qt][s]));
-  __syncthreads();
+  // whether any of the pages is not there: then every tile looks for itself which are
+  bool gaps = __syncthreads_or(t.bad_page);
 #pragma unroll
   for (int i = 0; i + 1 < kStages; ++i)
     if (begin + i < end) load_tile(begin + i);
@@ -758,22 +766,31 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
     if (ahead < end) {
       if ((ahead - begin) * kPagesOf % kPages == 0) {
         fill_pages(ahead);
-        __syncthreads();
+        gaps = __syncthreads_or(t.bad_page);
       }
       load_tile(ahead);
     }
-    if ((tile + 1) * kPos > t.L) {           // drafted positions, or none: clean V
+    const bool edge = (tile + 1) * kPos > t.L || gaps;
+    uint32_t held[kPos / kTile];
+#pragma unroll
+    for (int kk = 0; kk < kPos / kTile; ++kk) {
+      held[kk] = 0xffffffffu;
+      if (!gaps) continue;
+      const int i = tile * kPagesOf + 2 * kk;
+      held[kk] = (t.page_at(i) < 0 ? 0u : 0xffffu) | (t.page_at(i + 1) < 0 ? 0u : 0xffff0000u);
+    }
+    if (edge) {                              // drafted positions, or none: clean V
       bool odd = false;                      // a drafted value is not finite
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int at = (i * W + wave) * kWave + lane, row = at / kChunks;
         u32x4* const v = reinterpret_cast<u32x4*>(buf + kBytes + at * 16);
-        *v = clean_v(*v, tile * kPos + row, t.L, t.n, odd);
+        const uint32_t bits = kPos == kTile || row < kTile ? held[0] : held[kPos / kTile - 1];
+        *v = clean_v(*v, tile * kPos + row, t.L, t.n, bits >> row % kTile & 1, odd);
       }
       if (odd) odd_s = 1;
       __syncthreads();
     }
-    const bool edge = (tile + 1) * kPos > t.L;
     if (c0 < t.cols) {
       // (operands' places are worked out for every tile: 256 dims leave no registers to hold them)
       int at = lane;
@@ -799,7 +816,7 @@ void k_tree_many(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ 
 #pragma unroll
           for (int kk = 0; kk < kPos / kTile; ++kk) {
             const uint32_t bits =
-                t.seen_by(c0 + 16 * qt + r, tile * kPos + kk * kTile) >> (4 * kq);
+                (t.seen_by(c0 + 16 * qt + r, tile * kPos + kk * kTile) & held[kk]) >> (4 * kq);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               f32x4& x = st[qt][2 * kk + i / 4];
