@@ -396,6 +396,13 @@ __device__ __forceinline__ void tree_block(int mtiles, int& unit, int& mt) {
 }
 
 // ------------------------------------------------------------------------ few columns
+// What a wave's lanes hand each other through LDS lies in order: its LDS operations run in theirs,
+// and the compiler moves none past this.
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 template <int D, int NQ, int W>
 constexpr int few_lds() {
   return 16 * NQ * D * 2 + W * kTile * D * 2;
@@ -501,6 +508,7 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
       if (edge) v = clean_v(v, j0 + rr, t.L, t.n, (i < kV / 2 ? p0 : p1) >= 0, odd);
       *reinterpret_cast<u32x4*>(v_s + v_at<D>(rr, c8 >> 1) + (c8 & 1) * 16) = v;
     }
+    wave_lds();
     const bool more = tile + slots < tiles;
     if (++turn % 32 == 0) refill(tile + slots);
     p0 = page(turn, 0), p1 = page(turn, 1);
@@ -533,6 +541,7 @@ void k_tree_few(TfdTreeAttnArgs a, int splits, int mtiles, float* __restrict__ p
 #pragma unroll
       for (int qt = 0; qt < NQ; ++qt) o[dt][qt] = mfma(vf, ph[qt], o[dt][qt]);
     }
+    wave_lds();                              // (the next tile's V goes to the same place)
   }
 
   // join the waves: maxima and sums, then DT / NQ times 16 dims of all columns at a time
