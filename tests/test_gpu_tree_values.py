@@ -161,3 +161,89 @@ def test_positions_in_pages_out_of_range_take_no_part(gpu_device, shape, form):
     c["table"][0] = -1
     d = {k: v.to(gpu_device) for k, v in c.items()}
     assert not tree.attention(**d)[0].any()
+
+
+def _long(rows, nodes, heads, kv_heads, dim, lengths, far):
+    """Rows of *lengths*, those of *far* by shuffled pages; the others have pages of their own up
+    to theirs."""
+    g = _gen(sum(lengths))
+    need = [-(-(n + nodes) // 16) for n in lengths]
+    pages = sum(need) + 1
+    order, width = torch.randperm(pages, generator=g).to(I32), max(need)
+    table, at = torch.full((rows, width), -1, dtype=I32), 0
+    for b, n in enumerate(need):
+        table[b, :n] = order[at:at + n]
+        at += n
+    parents = torch.clamp(torch.arange(nodes) - 1 - torch.arange(nodes) % 3, min=-1)
+    masks = R.words(R.ancestors(parents.view(1, nodes))[0], nodes).repeat(rows, 1, 1)
+    pools = [torch.randn(pages, kv_heads, 16, dim, generator=g, dtype=torch.float32).to(BF)
+             for _ in range(2)]
+    return {"q": torch.randn(rows, nodes, heads, dim, generator=g).to(BF), "k_pool": pools[0],
+            "v_pool": pools[1], "table": table, "lengths": torch.tensor(lengths, dtype=I32),
+            "masks": masks}
+
+
+@pytest.mark.parametrize("rows,heads,dim,long", [
+    (64, 16, 64, (4095, 4097, 8190)), (64, 16, 128, (4090, 4100, 8300)),
+    (40, 32, 128, (4096, 4120, 4200)), (64, 16, 256, (4100, 4099, 8200))])
+def test_few_columns_past_the_pages_a_wave_holds(gpu_device, rows, heads, dim, long):
+    """A wave of four holds the pages of 32 tiles of 32 positions: 4,096 of a row that is one
+    split."""
+    lengths = [13 + b % 40 for b in range(rows)]
+    far = (0, rows // 2, rows - 1)
+    for b, n in zip(far, long):
+        lengths[b] = n
+    c = _long(rows, 3, heads, 8, dim, lengths, far)
+    form = _form(c)
+    assert form[:2] == (1, 4) and form[3] == 1, form
+    _check(c, gpu_device, [(b, t) for b in far for t in range(3)])
+    c["table"][far[2], 257] = -1                     # behind the refill
+    _check(c, gpu_device, [(far[2], t) for t in range(3)])
+
+
+@pytest.mark.parametrize("rows,nodes,heads,dim,long,waves", [
+    (17, 66, 16, 64, (16390, 16384, 17000), 8), (17, 65, 16, 128, (16320, 16500, 32900), 8),
+    (33, 17, 32, 64, (16384, 16450, 16400), 4), (17, 40, 32, 256, (16300, 16390, 16900), 8)])
+def test_many_columns_past_the_pages_a_block_holds(gpu_device, rows, nodes, heads, dim, long,
+                                                   waves):
+    """A block holds 1,024 pages: 16,384 positions of a row that is one split."""
+    lengths = [13 + b % 40 for b in range(rows)]
+    far = (0, rows // 2, rows - 1)
+    for b, n in zip(far, long):
+        lengths[b] = n
+    c = _long(rows, nodes, heads, 8, dim, lengths, far)
+    form = _form(c)
+    assert form[:2] == (0, waves) and form[3] == 1, form
+    _check(c, gpu_device, [(b, t) for b in far for t in (0, nodes // 2, nodes - 1)])
+    c["table"][far[2], 1026] = -1                    # behind the refill
+    _check(c, gpu_device, [(far[2], t) for t in (0, nodes - 1)])
+
+
+@pytest.mark.parametrize("shape,form", FORMS)
+def test_nodes_that_are_not_there_are_not_written(gpu_device, shape, form):
+    """Rows with one node, half of theirs, whole and without: the others' outputs hold what
+    they held."""
+    c = _shape(shape)
+    rows, nodes, heads, kv_heads, dim, _ = shape
+    counts = torch.tensor([(nodes, 0, 1, nodes // 2)[(b + 3 - (rows > 1)) % 4] for b in range(rows)],
+                          dtype=I32)
+    d = {k: v.to(gpu_device) for k, v in c.items()}
+    held = torch.full_like(d["q"], 777.0)
+    counts_d = counts.to(gpu_device)
+    need = lib().tfd_tree_attn_work_bytes(rows, nodes, heads, kv_heads, dim, c["table"].shape[1])
+    work = torch.empty(max(need, 16), dtype=torch.uint8, device=gpu_device)
+    whole = tree.attention(**d, counts=counts_d)
+    a = _lib.TfdTreeAttnArgs(
+        ptr(d["q"]), *d["q"].stride()[:3], ptr(d["k_pool"]), ptr(d["v_pool"]), ptr(d["table"]),
+        ptr(d["lengths"]), ptr(counts_d), ptr(d["masks"]), rows, nodes, heads, kv_heads, dim,
+        c["table"].shape[1], c["k_pool"].shape[0], dim ** -0.5, ptr(held), 0, ptr(work), need, 0)
+    lib().tfd_tree_attn(ctypes.addressof(a), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    there = (torch.arange(nodes) < counts.unsqueeze(1)).to(gpu_device)
+    assert (held[~there] == 777.0).all() and (~there).any()
+    assert torch.equal(held[there], whole[there])
+    for b in {0, rows // 2, rows - 1}:
+        for t in {0, int(counts[b]) - 1}:
+            if 0 <= t < counts[b]:                   # (a node's ancestors lie before it)
+                want, size = _node(c, b, t)
+                assert ((held[b, t].cpu().double() - want).abs() <= _bound(c, want, size)).all()
