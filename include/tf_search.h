@@ -179,7 +179,8 @@ int tfd_pages_fork(const TfdPages* pages, const int32_t* parents, const uint8_t*
  * TFD_ERR_NO_PAGES is raised; positions past max_pages raise TFD_ERR_POS_RANGE. */
 int tfd_pages_take(const TfdPages* pages, const int32_t* lengths, const int32_t* counts,
                    int n_all, void* stream);
-/* Page dst[i] of every pool becomes page src[i]; no page is in both lists or twice in dst. */
+/* Page dst[i] of every pool becomes page src[i]; no page is in both lists or twice in dst.  A pair
+ * with a number outside the pools raises TFD_ERR_PAGE_RANGE and is left out. */
 int tfd_pages_copy(const TfdPages* pages, const int32_t* src, const int32_t* dst, int n,
                    void* stream);
 /* Positions lengths[r] + path[r][i] move to lengths[r] + i, i < counts[r], in every pool, and

@@ -233,3 +233,14 @@ def test_calls_in_a_graph(gpu_device):
         for x, y in zip(a.d, b.d):
             assert torch.equal(x, y)
     a.gpu.check_errors()
+
+
+def test_copy_of_no_page_is_reported(gpu_device):
+    """-1 names no page, as any other number outside the pool: the others are copied."""
+    for src, dst in (((-1, 3), (2, 1)), ((0, 3), (-1, 1)), ((-7, 3), (2, 1))):
+        b = Both(gpu_device, 1, 1, 12)
+        b.gpu.copy(ints(*src).to(gpu_device), ints(*dst).to(gpu_device))
+        b.cpu.failed = True
+        for p in b.cpu.pools:
+            p[1] = p[3]
+        b.same()

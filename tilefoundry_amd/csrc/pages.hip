@@ -214,12 +214,14 @@ __global__ __launch_bounds__(kOne) void k_pages_take(TfdPages p, const int* __re
 
 // ---------------------------------------------------------------------------
 // Copies: a block takes 32 KiB of one page of one pool at a time, all its loads before its
-// stores; the blocks walk the items, whose number (of pairs) may lie on the device.  Bound by
-// memory: 1.6 GB in 310 us, 5.1 TB/s; a page of each of 8 rows 4.4 us.
+// stores; the blocks walk the items, whose number (of pairs) may lie on the device.  kHoles: -1
+// in src is a place without a copy (take's list, a place for every row).  Bound by memory: 1.6 GB
+// in 310 us, 5.1 TB/s; a page of each of 8 rows 4.4 us.
 // ---------------------------------------------------------------------------
 constexpr int kCopyLoads = 8;
 constexpr int64_t kCopyBytes = kBlock * 16 * kCopyLoads;
 
+template <bool kHoles>
 __global__ __launch_bounds__(kBlock) void k_pages_copy(TfdPages p, const int* __restrict__ src,
                                                        const int* __restrict__ dst, int n,
                                                        const int* __restrict__ n_dev,
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(kBlock) void k_pages_copy(TfdPages p, const int* __
   for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
     const uint32_t pair = it / per, pool = it % per / pieces, piece = it % pieces;
     const int a = src[pair];
-    if (a == -1) continue;
+    if (kHoles && a == -1) continue;
     const int b = dst[pair];
     if (a < 0 || a >= p.num_pages || b < 0 || b >= p.num_pages) {
       if (threadIdx.x == 0) raise_error(p.err, kErrPage);
@@ -393,6 +395,7 @@ unsigned walk_blocks(int64_t items) {
 }
 
 // Up to n pairs (n_dev: their number on the device) of the lists copied in every pool.
+template <bool kHoles>
 int copy_pairs(const TfdPages& p, const int* src, const int* dst, int n, const int* n_dev,
                hipStream_t s) {
   if (n == 0 || p.n_pools == 0) return 0;
@@ -400,7 +403,7 @@ int copy_pairs(const TfdPages& p, const int* src, const int* dst, int n, const i
   const int64_t items = n * pieces * p.n_pools;
   if (pieces > (1 << 20) || items >= (1ll << 31))
     return fail(kUnsupported, "pages: %lld copies in one call", (long long)items);
-  k_pages_copy<<<walk_blocks(items), kBlock, 0, s>>>(p, src, dst, n, n_dev, (int)pieces);
+  k_pages_copy<kHoles><<<walk_blocks(items), kBlock, 0, s>>>(p, src, dst, n, n_dev, (int)pieces);
   return 0;
 }
 
@@ -428,7 +431,7 @@ int tfd_pages_take(const TfdPages* pages, const int32_t* lengths, const int32_t*
   auto s = (hipStream_t)stream;
   k_pages_take<<<1, kOne, 0, s>>>(p, lengths, counts, n_all);
   const Scratch t = scratch_of(p);
-  if (const int rc = copy_pairs(p, t.src, t.dst, p.rows, nullptr, s)) return rc;
+  if (const int rc = copy_pairs<true>(p, t.src, t.dst, p.rows, nullptr, s)) return rc;
   return launched("pages_take");
 }
 
@@ -439,7 +442,7 @@ int tfd_pages_copy(const TfdPages* pages, const int32_t* src, const int32_t* dst
   const TfdPages& p = *pages;
   if (n == 0 || p.n_pools == 0) return 0;
   if (!src || !dst) return fail(kBadArg, "pages_copy: null pointer");
-  if (const int rc = copy_pairs(p, src, dst, n, nullptr, (hipStream_t)stream)) return rc;
+  if (const int rc = copy_pairs<false>(p, src, dst, n, nullptr, (hipStream_t)stream)) return rc;
   return launched("pages_copy");
 }
 
@@ -463,7 +466,7 @@ int tfd_pages_compact(const TfdPages* pages, int32_t* live, void* stream) {
   auto s = (hipStream_t)stream;
   k_pages_pair<<<1, kOne, 0, s>>>(p, live);
   const int most = (p.num_pages + 1) / 2;    // pairs
-  if (const int rc = copy_pairs(p, t.first, t.list, most, t.head, s)) return rc;
+  if (const int rc = copy_pairs<false>(p, t.first, t.list, most, t.head, s)) return rc;
   const int64_t entries = (int64_t)p.rows * p.max_pages;
   k_pages_rename<<<(unsigned)((entries + kBlock - 1) / kBlock), kBlock, 0, s>>>(p);
   k_pages_settle<<<(most + kBlock - 1) / kBlock, kBlock, 0, s>>>(p);

@@ -158,7 +158,8 @@ class Pages:
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page ``dst[i]`` of every pool becomes page ``src[i]`` (int32 ``[n]``).  No page may be in
-        both lists or twice in *dst*.  Table and references stay as they are."""
+        both lists or twice in *dst*; a pair with a number outside the pools is left out
+        (``check_errors``).  Table and references stay as they are."""
         check_input(src, "src", INT32)
         if src.dim() != 1:
             raise ValueError(f"src must be [n], got {tuple(src.shape)}")
