@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from tests import _search_ref as R
+from tilefoundry_amd._lib import TFDError
 from tilefoundry_amd.pages import Pages
 
 pytestmark = pytest.mark.gpu
@@ -244,3 +245,23 @@ def test_copy_of_no_page_is_reported(gpu_device):
         for p in b.cpu.pools:
             p[1] = p[3]
         b.same()
+
+
+def test_refused_copies_leave_everything_as_it_was(gpu_device):
+    """Pages too large to be copied in one call are refused before anything is decided; the calls
+    after that are as ever."""
+    b = Both(gpu_device, rows=3, max_pages=3, num_pages=9)
+    b.call("take", ints(0, 0, 0), ints(20, 0, 18))
+    lengths = b.call("fork", ints(0, 0, 2), ints(20, 0, 18))
+    b.call("free", torch.tensor([True, False, False]))
+    size, scratch = b.gpu._args.max_page_bytes, b.gpu._scratch.clone()
+    b.gpu._args.max_page_bytes = 1 << 50
+    for call in (lambda: b.gpu.take(lengths.to(gpu_device), 1), b.gpu.compact,
+                 lambda: b.gpu.copy(ints(1).to(gpu_device), ints(8).to(gpu_device))):
+        with pytest.raises(TFDError, match="copies"):
+            call()
+        b.same()
+        assert torch.equal(b.gpu._scratch, scratch)
+    b.gpu._args.max_page_bytes = size
+    b.call("compact")
+    b.call("take", lengths, 1)

@@ -394,17 +394,25 @@ unsigned walk_blocks(int64_t items) {
   return (unsigned)(items < most ? items < 1 ? 1 : items : most);
 }
 
+int64_t copy_pieces(const TfdPages& p) { return (p.max_page_bytes + kCopyBytes - 1) / kCopyBytes; }
+
+// Refused before a call's first launch: what a call has decided it also copies.
+int check_copies(const TfdPages& p, int n) {
+  const int64_t pieces = copy_pieces(p);
+  if (pieces > (1 << 20) || n * pieces * p.n_pools >= (1ll << 31))
+    return fail(kUnsupported, "pages: copies of %d pages of %lld bytes in %d pools in one call", n,
+                (long long)p.max_page_bytes, p.n_pools);
+  return 0;
+}
+
 // Up to n pairs (n_dev: their number on the device) of the lists copied in every pool.
 template <bool kHoles>
-int copy_pairs(const TfdPages& p, const int* src, const int* dst, int n, const int* n_dev,
-               hipStream_t s) {
-  if (n == 0 || p.n_pools == 0) return 0;
-  const int64_t pieces = (p.max_page_bytes + kCopyBytes - 1) / kCopyBytes;
-  const int64_t items = n * pieces * p.n_pools;
-  if (pieces > (1 << 20) || items >= (1ll << 31))
-    return fail(kUnsupported, "pages: %lld copies in one call", (long long)items);
-  k_pages_copy<kHoles><<<walk_blocks(items), kBlock, 0, s>>>(p, src, dst, n, n_dev, (int)pieces);
-  return 0;
+void copy_pairs(const TfdPages& p, const int* src, const int* dst, int n, const int* n_dev,
+                hipStream_t s) {
+  if (n == 0 || p.n_pools == 0) return;
+  const int64_t pieces = copy_pieces(p);
+  k_pages_copy<kHoles><<<walk_blocks(n * pieces * p.n_pools), kBlock, 0, s>>>(p, src, dst, n, n_dev,
+                                                                              (int)pieces);
 }
 
 }  // namespace
@@ -428,10 +436,11 @@ int tfd_pages_take(const TfdPages* pages, const int32_t* lengths, const int32_t*
   if (const int rc = check_pages(pages, "pages_take")) return rc;
   if (!lengths) return fail(kBadArg, "pages_take: null pointer");
   const TfdPages& p = *pages;
+  if (const int rc = check_copies(p, p.rows)) return rc;
   auto s = (hipStream_t)stream;
   k_pages_take<<<1, kOne, 0, s>>>(p, lengths, counts, n_all);
   const Scratch t = scratch_of(p);
-  if (const int rc = copy_pairs<true>(p, t.src, t.dst, p.rows, nullptr, s)) return rc;
+  copy_pairs<true>(p, t.src, t.dst, p.rows, nullptr, s);
   return launched("pages_take");
 }
 
@@ -442,7 +451,8 @@ int tfd_pages_copy(const TfdPages* pages, const int32_t* src, const int32_t* dst
   const TfdPages& p = *pages;
   if (n == 0 || p.n_pools == 0) return 0;
   if (!src || !dst) return fail(kBadArg, "pages_copy: null pointer");
-  if (const int rc = copy_pairs<false>(p, src, dst, n, nullptr, (hipStream_t)stream)) return rc;
+  if (const int rc = check_copies(p, n)) return rc;
+  copy_pairs<false>(p, src, dst, n, nullptr, (hipStream_t)stream);
   return launched("pages_copy");
 }
 
@@ -462,11 +472,12 @@ int tfd_pages_keep(const TfdPages* pages, const int32_t* lengths, const int32_t*
 int tfd_pages_compact(const TfdPages* pages, int32_t* live, void* stream) {
   if (const int rc = check_pages(pages, "pages_compact")) return rc;
   const TfdPages& p = *pages;
+  const int most = (p.num_pages + 1) / 2;    // pairs
+  if (const int rc = check_copies(p, most)) return rc;
   const Scratch t = scratch_of(p);
   auto s = (hipStream_t)stream;
   k_pages_pair<<<1, kOne, 0, s>>>(p, live);
-  const int most = (p.num_pages + 1) / 2;    // pairs
-  if (const int rc = copy_pairs<false>(p, t.first, t.list, most, t.head, s)) return rc;
+  copy_pairs<false>(p, t.first, t.list, most, t.head, s);
   const int64_t entries = (int64_t)p.rows * p.max_pages;
   k_pages_rename<<<(unsigned)((entries + kBlock - 1) / kBlock), kBlock, 0, s>>>(p);
   k_pages_settle<<<(most + kBlock - 1) / kBlock, kBlock, 0, s>>>(p);
