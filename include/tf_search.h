@@ -97,7 +97,9 @@ int tfd_tree_attn(const TfdTreeAttnArgs* args, void* stream);
  *              or -inf is no candidate and not in the sum, +inf counts as the largest f32; a
  *              row whose score is NaN or infinite offers nothing;
  *   rank       the candidate's score / max(length, 1) ^ penalty, length = lengths[r] + 1 (a
- *              finished row: lengths[r]), in 64 bits;
+ *              finished row: lengths[r]), in 64 bits.  The sum in a score's logarithm is one of
+ *              f32 exponentials, up to 2^-22 of it off: two rows' candidates that lie closer
+ *              than that may come in either order, a row's own and equal rows' never;
  *   beams      the best of a group's candidates, in falling rank; equal ones by the lower row,
  *              in a row by the larger logit, then the lower token.
  * Out, per place: parents (row numbers), tokens, scores (f32), lengths and done (a parent's, or
@@ -115,7 +117,7 @@ typedef struct {
   const int32_t* lengths;
   const uint8_t* done;
   int groups, beams, vocab, eos;
-  float penalty;
+  double penalty;
   int32_t* parents;
   int32_t* tokens;
   float* scores_out;

@@ -248,3 +248,42 @@ def test_reorder_rows_past_4_gib(gpu_device):
     assert x[0, -3:].tolist() == [2.0] * 3 and x[1, -3:].tolist() == [1.0] * 3
     assert x[0, 5].item() == 7.0 and x[1, 5].item() == 0.0
     assert _lib.BEAM_MAX == 64
+
+
+@pytest.mark.parametrize("penalty", [0.5, 1.0, 2.0])
+@pytest.mark.parametrize("beams", [4, 32, 64])
+def test_beam_equal_ranks_of_unlike_lengths(gpu_device, beams, penalty):
+    """Finished beams whose scores over length ** penalty are the same number, exactly: the lower
+    row first.  (Scores, lengths and their powers are whole numbers here.)"""
+    n = 1 + torch.randperm(90, generator=torch.Generator().manual_seed(beams))[:beams]
+    lengths = n * n if penalty == 0.5 else n
+    scores = -3.0 * (n * n if penalty == 2.0 else n).float()
+    got = _check(gpu_device, Beam(beams, eos=1, length_penalty=penalty), torch.zeros(beams, 9),
+                 scores.view(1, -1), lengths.to(I32).view(1, -1),
+                 torch.ones(1, beams, dtype=torch.bool))
+    assert got.parents.cpu()[0].tolist() == list(range(beams))
+
+
+@pytest.mark.parametrize("penalty", [0.6, 0.7, 1.1])
+def test_beam_penalty_is_not_rounded(gpu_device, penalty):
+    """Finished beams, of 3 and 2^20 tokens, whose order is one thing by the penalty and another
+    by its nearest f32."""
+    rounded = float(torch.tensor(penalty, dtype=F32))
+    long = torch.tensor(-1000.0)
+    short = (long.double() * (3 / 2 ** 20) ** penalty).float()
+    ranks = [lambda p, s: float(s.double()) / 3 ** p, lambda p, s: float(long) / (2 ** 20) ** p]
+    step = short
+    for _ in range(40):                              # (f32 neighbours on both sides)
+        step = torch.nextafter(step, torch.tensor(-math.inf))
+    for _ in range(80):
+        step = torch.nextafter(step, torch.tensor(math.inf))
+        gap = [ranks[0](p, step) - ranks[1](p, step) for p in (penalty, rounded)]
+        if gap[0] * gap[1] < 0 and abs(gap[0]) > 1e-12:
+            break
+    else:
+        raise AssertionError("no such pair")
+    for scores in ((step, long), (long, step)):
+        _check(gpu_device, Beam(2, eos=1, length_penalty=penalty), torch.zeros(2, 9),
+               torch.stack(scores).view(1, 2),
+               torch.tensor([[3 if s is step else 2 ** 20 for s in scores]], dtype=I32),
+               torch.ones(1, 2, dtype=torch.bool))

@@ -7,13 +7,13 @@ returns non-zero raises ``TFDError`` carrying the library's own message.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_void_p
 from functools import lru_cache
 from pathlib import Path
 
 from .build import LIB
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 PRO_PLAIN, PRO_NORM = 0, 1
 EPI_STORE, EPI_RESID, EPI_SWIGLU, EPI_LOGITS, EPI_RESID_F32 = 0, 1, 2, 3, 4
@@ -435,7 +435,7 @@ class TfdBeamArgs(ctypes.Structure):
     _fields_ = [("logits", c_void_p), ("ldl", c_int64), ("type", c_int), ("scores", c_void_p),
                 ("lengths", c_void_p), ("done", c_void_p),
                 *[(n, c_int) for n in ("groups", "beams", "vocab", "eos")],
-                ("penalty", c_float),
+                ("penalty", c_double),
                 *[(n, c_void_p) for n in ("parents", "tokens", "scores_out", "lengths_out",
                                           "done_out", "work")],
                 ("work_bytes", c_int64)]

@@ -339,10 +339,21 @@ __device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
          ((a.rank == b.rank) & ((a.beam < b.beam) | ((a.beam == b.beam) & (a.key > b.key))));
 }
 
+// n ^ p.  Halves of whole numbers by products and a root, which are exact where the result is a
+// whole number (pow is off in its last place there, and orders equal ranks).
+__device__ __forceinline__ double length_power(int n, double p) {
+  const double twice = 2.0 * p;
+  if (twice != floor(twice)) return pow((double)n, p);
+  double y = (int)twice & 1 ? sqrt((double)n) : 1.0, b = n;
+  for (int k = (int)twice / 2; k; k /= 2, b *= b)
+    if (k & 1) y *= b;
+  return y;
+}
+
 __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks,
                                                        const ChunkSum* __restrict__ sums,
                                                        const uint64_t* __restrict__ lists) {
-  __shared__ double add_s[kMaxBeams], inv_s[kMaxBeams];
+  __shared__ double add_s[kMaxBeams], size_s[kMaxBeams];
   __shared__ float top_s[kMaxBeams];
   __shared__ uint8_t done_s[kMaxBeams];
   __shared__ int length_s[kMaxBeams];
@@ -363,8 +374,9 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
   for (int i = 0; i < kHeldKeys; ++i)
     held[i] = mine[(int64_t)min(tid, n_lists - 1) * K + min(i, K - 1)];
   if (tid == 0) n_s = heads_s = 0;
-  // value = add + (logit - top), rank = value * inv (the difference first: an infinite logit
-  // stands as 3.4e38); a row that offers nothing has add NaN
+  // value = add + (logit - top), rank = value / size (the difference first: an infinite logit
+  // stands as 3.4e38); a row that offers nothing has add NaN.  Divided, as the definition says: a
+  // product with the reciprocal orders ranks that are equal (-3 of length 3, -2 of 2) otherwise.
   for (int b = wave; b < K; b += kMergeWaves) {
     const int row = row0 + b;
     const ChunkSum* const t = sums + (int64_t)row * chunks;
@@ -374,9 +386,8 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     const float score = a.scores[row];
     const int length = a.lengths ? a.lengths[row] : 0;
     const bool over = a.done && a.done[row], none = !(fabsf(score) < __builtin_huge_valf());
-    const double inv = a.penalty == 0.f
-                           ? 1.0
-                           : exp(-(double)a.penalty * log((double)max(length + (over ? 0 : 1), 1)));
+    const double size =
+        a.penalty == 0.0 ? 1.0 : length_power(max(length + (over ? 0 : 1), 1), a.penalty);
     double lse = 0.0;
     float m = -__builtin_huge_valf();
     if (!over) {
@@ -399,7 +410,7 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
       done_s[b] = over;
       length_s[b] = length;
       add_s[b] = none ? __builtin_nan("") : (double)score - lse;
-      inv_s[b] = inv;
+      size_s[b] = size;
     }
   }
   __syncthreads();
@@ -414,7 +425,8 @@ __global__ __launch_bounds__(kMerge) void k_beam_merge(TfdBeamArgs a, int chunks
     c.beam = list / chunks;
     c.key = !done_s[c.beam] ? key
             : list == c.beam * chunks && i == 0 ? key_of(0.f, a.eos) : 0;
-    c.rank = c.key ? value_of(c) * inv_s[c.beam] : kNone;
+    c.rank = c.key ? value_of(c) : kNone;
+    if (a.penalty != 0.0) c.rank /= size_s[c.beam];
     if (!(c.rank > kNone)) c.key = 0, c.rank = kNone;
     return c;
   };
@@ -712,7 +724,7 @@ int tfd_beam_select(const TfdBeamArgs* args, void* stream) {
                 kMaxBeams, a.vocab);
   if (a.eos < -1 || a.eos >= a.vocab)
     return fail(kBadArg, "beam_select: eos %d outside -1..%d", a.eos, a.vocab - 1);
-  if (!(a.penalty >= 0.f) || a.penalty > 100.f)
+  if (!(a.penalty >= 0.0) || a.penalty > 100.0)
     return fail(kBadArg, "beam_select: penalty must lie in 0..100");
   if (a.groups == 0) return 0;
   if (!a.logits || !a.scores || !a.parents || !a.tokens || !a.scores_out || !a.lengths_out ||
