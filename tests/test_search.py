@@ -360,3 +360,19 @@ def test_structs_and_constants_match_the_header(tmp_path):
     subprocess.run(["gcc", str(tmp_path / "probe.c"), "-o", str(tmp_path / "probe")], check=True)
     out = subprocess.run([str(tmp_path / "probe")], capture_output=True, text=True, check=True)
     assert [int(v) for v in out.stdout.split()] == want
+
+
+def test_tensors_that_share_memory_are_refused():
+    """What one block of a call moves another would move again."""
+    x = torch.zeros(6, 2, 16, 16)
+    whole = torch.zeros(3, 6, 2, 16, 16)
+    for pools in ([x, x], [x, x.view(6, 1, 32, 16)[:, :, :16].contiguous(), x.view(6, 2, 16, 16)],
+                  [whole, whole[1]], [whole[:2], whole[1:]]):
+        with pytest.raises(ValueError, match="overlap"):
+            pages.Pages(pools, rows=2, max_pages=2)
+        with pytest.raises(ValueError, match="overlap|one number"):
+            beam.States(pools)
+    with pytest.raises(ValueError, match="GPU"):     # (side by side, or nothing in them)
+        pages.Pages([whole[0], whole[1], x], rows=2, max_pages=2)
+    with pytest.raises(ValueError, match="GPU"):
+        beam.States([x, x[:, :0], x[:, :0], torch.zeros_like(x)])

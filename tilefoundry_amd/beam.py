@@ -26,8 +26,8 @@ import torch
 
 from . import _lib
 from ._lib import lib, ptr
-from .mx4 import (FLOAT32, INT32, TYPES, _settle, check_device, check_input, launch, row_stride,
-                  rows_of)
+from .mx4 import (FLOAT32, INT32, TYPES, _settle, check_apart, check_device, check_input, launch,
+                  row_stride, rows_of)
 
 BOOL = (torch.bool, torch.uint8)
 MAX_GROUPS = 65535
@@ -112,8 +112,8 @@ class Beam:
 class States:
     """Tensors whose rows follow the beams: recurrent states, conv windows, token histories.
 
-    Each is contiguous ``[rows, ...]`` of any type, all of one number of rows, on one GPU; they
-    are kept.  Rows move within groups of *beams* (default: all rows, up to 64)."""
+    Each is contiguous ``[rows, ...]`` of any type, all of one number of rows, on one GPU, no two
+    in the same memory; they are kept.  Rows move within groups of *beams* (default: all rows, up to 64)."""
 
     def __init__(self, tensors, beams: int | None = None):
         self.tensors = list(tensors)
@@ -127,6 +127,7 @@ class States:
             if t.dim() < 1 or t.shape[0] != first.shape[0] or not t.is_contiguous():
                 raise ValueError(f"States: contiguous tensors of one number of rows, got "
                                  f"{tuple(t.shape)} beside {tuple(first.shape)}")
+        check_apart(self.tensors, "States")
         check_device(first.device, *self.tensors)
         self.rows, self.device = first.shape[0], first.device
         self.beams = beams if beams is not None else self.rows

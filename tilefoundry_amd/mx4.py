@@ -63,6 +63,14 @@ def check_device(device, *others) -> None:
             raise ValueError(f"tensors on {device} and on {t.device}")
 
 
+def check_apart(tensors, what: str) -> None:
+    """Contiguous tensors that a call writes side by side share no memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                   for t in tensors if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError(f"{what}: two of the tensors overlap in memory")
+
+
 # what the C entries take as 32-bit integers (ctypes would cut a larger one to its low bits)
 LONGEST = (1 << 31) - 1                      # values of a row
 MAX_K, MAX_N = 1 << 22, 1 << 24              # of a product

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import lib, ptr
-from .mx4 import INT32, _settle, check_device, check_input, launch
+from .mx4 import INT32, _settle, check_apart, check_device, check_input, launch
 
 PAGE = _lib.PAGE_SIZE
 MAX_ROWS = _lib.PAGES_MAX_ROWS
@@ -38,7 +38,8 @@ class Pages:
     """See the module docstring.
 
     *pools*: tensors ``[pages, heads, 16, dim]``, or ``[layers, pages, heads, 16, dim]``,
-    contiguous, rows of a multiple of 16 bytes, all of one number of pages; they are kept.
+    contiguous, rows of a multiple of 16 bytes, all of one number of pages, no two in the same
+    memory; they are kept.
     *table* int32 ``[rows, max_pages]`` (-1: no page) and *refs* int32 ``[pages]`` are used in place if given;
     without *table* it starts empty, without *refs* the table's entries are counted."""
 
@@ -58,6 +59,7 @@ class Pages:
             parts += list(t) if t.dim() == 5 else [t]
         if not parts:
             raise ValueError("Pages: pools without layers")
+        check_apart(self.pools, "Pages")
         self.device, self.num_pages = parts[0].device, parts[0].shape[0]
         check_device(self.device, *parts)
         entries = []
