@@ -264,3 +264,57 @@ def test_searches_refuse(gpu_device, weights):
         _engine(weights, gpu_device, 17).speculate([p] * 17, 4, nodes=256)
     with pytest.raises(ValueError, match="greedy"):
         _engine(weights, gpu_device, 1, sampling=Sampling(top_k=4)).speculate([p], 4)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("groups,beams", [(1, 4), (2, 3)])
+def test_beam_steps_take_their_own_pages(gpu_device, weights, monkeypatch, groups, beams, graph):
+    """Nothing but the step takes pages: its table is looked at between its take and its fork (one
+    by one), and every row's cache behind the fork is its parent's with what was written for that,
+    also where the captured step is replayed."""
+    e = _engine(weights, gpu_device, groups * beams, graph=graph)
+    prompts = [_prompt(n, SMALL.vocab_size, seed=n) for n in (9, 30)[:groups]]
+    e.beam_search(prompts, 1, beams=beams)
+    search = e._beam_searches[(beams, None, 0.0)]
+    assert (search.graph is not None) == graph
+    table, taken = e.page_table.clone(), torch.zeros_like(e.page_table)
+    chosen = torch.zeros(e.B, dtype=torch.int32, device=e.device)
+    forward, fork = e._forward, search.cache.fork
+
+    def look(s):
+        taken.copy_(e.page_table)
+        forward(s)
+
+    def follow(parents, lengths):
+        chosen.copy_(parents)
+        return fork(parents, lengths)
+
+    monkeypatch.setattr(e, "_forward", look)
+    monkeypatch.setattr(search.cache, "fork", follow)
+    if graph:
+        search._capture()                            # (with what looks at it in it)
+    search._begin(prompts)
+    n = [len(p) - 1 for p in prompts for _ in range(beams)]
+    kept, shared = [_row(e, r, n[r]) for r in range(e.B)], 0
+    for _ in range(36):
+        shared += int((search.cache.refs > 1).sum())
+        if graph:
+            search.graph.replay()
+        else:
+            search._step()
+        after, parents = e.page_table.clone(), chosen.tolist()
+        e.page_table.copy_(taken)
+        rows = [_row(e, r, n[r] + 1) for r in range(e.B)]
+        last = [int(taken[r, n[r] // 16]) for r in range(e.B)]
+        assert len(set(last)) == e.B                 # a page of one's own to write
+        e.page_table.copy_(after)
+        for r in range(e.B):
+            assert torch.equal(rows[r][:, :n[r]], kept[r]), r
+        n = [v + 1 for v in n]
+        assert e.pos.tolist() == n
+        kept = [rows[p] for p in parents]
+        for r in range(e.B):
+            assert torch.equal(_row(e, r, n[r]), kept[r]), r
+    assert shared > 0
+    search.cache.check_errors()
+    e.page_table.copy_(table)
