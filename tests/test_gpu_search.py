@@ -318,3 +318,22 @@ def test_beam_steps_take_their_own_pages(gpu_device, weights, monkeypatch, group
     assert shared > 0
     search.cache.check_errors()
     e.page_table.copy_(table)
+
+
+def test_a_refused_search_costs_no_other(gpu_device, weights):
+    """An engine's searches stay where another one is refused."""
+    e = _engine(weights, gpu_device, 4)
+    rules = [(1, None), (2, None), (4, None), (4, 5)]
+    for beams, eos in rules:
+        e.beam_search([[1, 2]] * (4 // beams), 2, beams=beams, eos=eos)
+    known = dict(e._beam_searches)
+    for kw in ({"beams": 3}, {"beams": 0}, {"beams": 4, "eos": SMALL.vocab_size},
+               {"beams": 2, "length_penalty": -1.0}):
+        with pytest.raises(ValueError):
+            e.beam_search([[1, 2]], 2, **kw)
+    assert e._beam_searches == known
+    e.speculate([[1, 2]] * 4, 2, nodes=3)
+    one = e._speculations[3]
+    with pytest.raises(ValueError):
+        e.speculate([[1, 2]] * 4, 2, nodes=0)
+    assert e._speculations == {3: one}

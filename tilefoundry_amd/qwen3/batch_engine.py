@@ -371,9 +371,10 @@ class BatchEngine:
         key = (beams, eos, float(length_penalty))
         known = self.__dict__.setdefault("_beam_searches", {})
         if key not in known:
+            search = BeamSearch(weakref.ref(self), *key)
             if len(known) == MAX_SEARCHES:           # (each keeps a captured graph)
                 known.pop(next(iter(known)))
-            known[key] = BeamSearch(weakref.ref(self), *key)
+            known[key] = search
         return known[key].run(prompts, max_new)
 
     def speculate(self, prompts: list[list[int]], max_new: int, *, nodes: int = 8, draft=None):
@@ -382,6 +383,7 @@ class BatchEngine:
         ``qwen3.search.NgramDraft`` unless given)."""
         known = self.__dict__.setdefault("_speculations", {})
         if nodes not in known:
+            Speculation.check(self, nodes)
             known.clear()                            # (logits of batch x nodes rows)
             known[nodes] = Speculation(weakref.ref(self), nodes)
         return known[nodes].run(prompts, max_new, NgramDraft() if draft is None else draft)

@@ -283,12 +283,16 @@ class Speculated:
 class Speculation:
     """Greedy decoding by checked drafts on a batch engine (a weak reference to it)."""
 
-    def __init__(self, engine, nodes: int):
-        e = engine()
+    @staticmethod
+    def check(e, nodes: int):
         if not 1 <= nodes <= tree.MAX_NODES:
             raise ValueError(f"nodes must lie in 1..{tree.MAX_NODES}, got {nodes}")
         if e.B * nodes > MAX_PASS:
             raise ValueError(f"{nodes} nodes of {e.B} sequences exceed a pass of {MAX_PASS} rows")
+
+    def __init__(self, engine, nodes: int):
+        e = engine()
+        self.check(e, nodes)
         self._engine, self.nodes = engine, nodes
         self.step = TreePass(engine, nodes)
         self.cache = Pages([e.kpool, e.vpool], table=e.page_table)
