@@ -323,8 +323,8 @@ void k_beam_scan(TfdBeamArgs a, int chunks, int waves, ChunkSum* __restrict__ su
 // the largest such bound is collected and ranked by counting by one wave, after another bound
 // where there are many.  If more does than the buffer holds (thousands of equal ranks), the
 // places are filled one by one instead.  A thread holds the first keys of a list from the start
-// on, so that few loads wait for others.  Bound by latency: 6.5 us for 4 beams of 151,936 logits
-// (4.5 of them until the lists, which other dies wrote, have come), 11.6 for 16 of 16.
+// on, so that few loads wait for others.  Bound by latency: 6.7 us for 4 beams of 151,936 logits
+// (4.5 of them until the lists, which other dies wrote, have come), 11.8 for 16 of 16.
 // ---------------------------------------------------------------------------
 constexpr int kMerge = 1024, kMergeWaves = kMerge / kWave, kFound = 2048;
 constexpr int kHeldKeys = 4, kHeldSums = 3, kFewHeads = 32;
@@ -633,8 +633,9 @@ bool beam_shape(int groups, int beams, int vocab) {
 // are neither read (but by others) nor written.  A wave knows the moves by itself -- lane b
 // holds row b's parent, a 64-bit mask the rows that move -- and finds its tensor by a
 // ballot, so nothing waits for a barrier.  Bound by memory: 8 rows in groups of 4 of 30 states of
-// 2 MiB, 5 of them moved, 109 us; a block that took four pieces in turn, the next one's loads
-// behind the stores of the last, 127.
+// 2 MiB and as many windows of 48 KiB, 5 rows moved from 4, 106 us, 6 from 6 148, all from all 190:
+// 5.2 to 5.5 TB/s.  A block that took four pieces in turn, the next one's loads behind the stores
+// of the last, was a sixth slower.
 // ---------------------------------------------------------------------------
 constexpr int kUnits = 4;                    // small units per thread
 

@@ -122,7 +122,7 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // second product: they stay a sum of two bf16 (2^-16 of each), however many columns there are.
 // By many, a caller may ask for one (2^-8; they average: 1.4 times the error of an attention in
 // f32 that rounds its output), which saves a third of the products and half of what VALU does for
-// a probability: 215 to 161 us at 4 rows to 30,000 positions, 61 nodes of 32 heads over 8.
+// a probability: 211 to 161 us at 4 rows to 30,000 positions, 61 nodes of 32 heads over 8.
 //
 // Two kernels.  Few columns (k_tree_few): the keys are what is waited for, so each wave
 // takes other tiles of 32 positions, its K straight into registers as operands and its V
@@ -132,10 +132,11 @@ __global__ __launch_bounds__(kWave) void k_tree_accept(
 // tile.  Both may cut a row's positions into splits, which k_tree_join adds.
 //
 // Few columns are bound by memory (32 rows to 4,096 positions by 7 nodes: 93 us, 5.5 TB/s) or, by
-// one row, by latency (700 positions: 14 us).  Many: MFMA (35% of the time at 61 nodes of 32
-// heads), LDS, VALU and loads take turns, since registers leave room for two waves a SIMD (159 us,
-// 756 TFLOP/s); of 256 dims (8 rows to 5,003, 23 nodes of 16 heads over 2: 42 us) also by the
-// partial sums of its splits, which the join reads again (10 us).
+// one row, by latency (700 positions: 14 us).  Many: MFMA (40% of the time at 61 nodes of 32
+// heads), LDS, VALU and loads take turns, since registers leave room for two waves a SIMD (203 us
+// and the join's 8, 590 TFLOP/s of the definition's products, whose second takes two); of 256 dims
+// (8 rows to 5,003, 23 nodes of 16 heads over 2: 50 us) also by the partial sums of its splits,
+// which the join reads again (10 us).
 // ---------------------------------------------------------------------------
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 32;                    // positions of a wave's tile
@@ -969,23 +970,26 @@ __global__ __launch_bounds__(kBlock) void k_tree_join(TfdTreeAttnArgs a, int spl
 //
 // Short: where every wave needs one tile of 32 positions, with 16 columns a block and no more
 // blocks than compute units, blocks of as many waves as their registers leave room for.  Two
-// tiles a wave instead of two splits save the join's launch and take the same (13.5 us of 1 row of
-// 700 positions by 16 nodes, 13.2 with the join).  1 row of 6,000 by 16 nodes: 18.3 us, by blocks
-// of four waves of 32 columns 24.1; by 8 nodes 16.7 and 19.7.  16 columns whose tiles blocks
+// tiles a wave instead of two splits save the join's launch: 1 row of 560 positions by 16 nodes
+// 11.4 us and 13.2 with the join, of 700, where nearly all waves take a second tile, 13.9 and 14.2;
+// 64 dims, 900 by 40 nodes, 10.4 and 11.9; 32 heads over 8, 600 by 8, 11.2 and 13.0; 256 dims,
+// whose tiles take longest, 300 by 13, 16.7 and 16.2.  1 row of 6,000 by 16 nodes: 18.0 us, by
+// blocks of four waves of 32 columns 24.1; by 8 nodes 16.7 and 19.7.  16 columns whose tiles blocks
 // of four waves hold at once too are faster by those (700 positions, 8 nodes: 11.4 us, 13.2),
 // down to what a single block holds (200: 10.1, 9.0).
 //
 // Few: up to 64 columns, 16 of 256 dims, in blocks of four waves of up to 32 (2 rows of 32,000 by
-// 32 nodes: 60.0 us, by the kernel for many 68.6; 32 rows of 4,096: 118 both; 48 nodes 185 and 125).
+// 32 nodes: 71 us, by the kernel for many 78; 32 rows of 4,096 by 30: 117 and 134; by 48 nodes
+// 185 and 137).
 // One block a compute unit: what the splits leave is read again, and four waves' loads are
 // enough in flight (32 rows of 4,096 by 7 nodes: 97.6 us, with three a unit 104.1; 1 of 6,000 by 8:
 // 19.7 and 25.0).
 //
 // Many: eight waves of 32 columns, whose longer tiles cost less a position (32 rows of 4,096 by 60
-// nodes: 122 us, by two blocks of four waves 132); up to 128 columns four waves of 64 dims
-// (8 rows of 8,000: 48.9 us, by eight 51.0), or where there are more row heads than compute units
-// (33 rows of 400 by 33: 30.6 us, 37.1).  Splits fill the compute units once (twice as many: 4 rows
-// of 30,000 by 61 nodes of 32 heads 177 us, 161 so, half as many 254).
+// nodes: 145 us, by two blocks of four waves 153); up to 128 columns four waves of 64 dims
+// (8 rows of 8,000: 58.2 us, by eight 59.6), or where there are more row heads than compute units
+// (33 rows of 400 by 33: 33.0 us, 43.1).  Splits fill the compute units once (twice as many: 4 rows
+// of 30,000 by 61 nodes of 32 heads 233 us for 211, 8 of 5,003 by 256 dims 85 for 55).
 struct TreePlan {
   int nq, waves, mtiles, cols, splits;       // nq 0: many columns; cols: of a block
 };
